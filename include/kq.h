@@ -257,6 +257,162 @@ int kq_attention_decode(kq_ctx* ctx, uint64_t out, uint64_t q, uint64_t k_cache,
 uint64_t kq_attention_workspace(kq_ctx* ctx, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim,
                                 uint32_t len);
 
+/* ---- Drafted tokens: rotary positions, a quantised paged cache, attention over it ------------
+ *
+ * A step that checks T drafted tokens at once (speculative decoding; T = 1 is a plain decode step)
+ * runs its projections as batches of T vectors. Between them it rotates every token's query and key
+ * heads by that token's own position, writes the keys and values into a paged cache held in 16, 8
+ * or 4 bits, and lets every drafted token attend over its sequence's cache and over the drafts above
+ * it in the tree. When some drafts are accepted, their rows move to the end of the kept context.
+ * kernite has no rotary embedding, no cache and no drafted tokens; the attention itself follows its
+ * microgpt example (examples/microgpt/src/gpu.rs:130-230). Positions, slots and lengths are read on
+ * the device (a captured graph serves every step). What the host cannot check there, the kernels
+ * do: a slot, page or length out of range is skipped and recorded in the ctx's device error word
+ * (kq_device_error), never followed. */
+
+/* Element types of activations (GGML's type numbers). */
+enum { KQ_TYPE_F32 = 0, KQ_TYPE_F16 = 1, KQ_TYPE_BF16 = 30 };
+
+/* Which elements of a head form pair i: (2i, 2i+1), or (i, i + rot_dim / 2). */
+enum { KQ_ROPE_PAIRS = 0, KQ_ROPE_HALVES = 1 };
+
+/* Pair i turns by position * f_i radians, f_i = base^(-2i / rot_dim) / freq_factors[i], and
+ * (x_a, x_b) becomes gain * (x_a cos - x_b sin, x_a sin + x_b cos). Long contexts: f_i is
+ * multiplied by freq_scale (< 1: positions interpolated), or, with ext_factor e > 0, by
+ * freq_scale * (1 - m_i) + m_i, m_i = e * (1 - ramp_i), ramp_i rising from 0 to 1 between the pairs
+ * that turn beta_fast and beta_slow times in orig_ctx positions, and the gain is then
+ * attn_factor * (1 + 0.1 ln(1 / freq_scale)) ("by parts", Peng et al., YaRN); else attn_factor. */
+typedef struct kq_rope_params {
+    uint32_t rot_dim;      /* the first rot_dim elements of a head are rotated: even, 2..256 */
+    uint32_t layout;       /* KQ_ROPE_* */
+    double base;           /* > 1 */
+    double freq_scale;     /* > 0; 1: none */
+    double ext_factor;     /* 0: none */
+    double attn_factor;    /* 1: none */
+    double beta_fast, beta_slow;
+    uint32_t orig_ctx;     /* needed with ext_factor */
+    uint32_t reserved;
+    const float* freq_factors; /* host, rot_dim / 2 values > 0; NULL: none */
+} kq_rope_params;
+
+/* The rotation's table, made once by kq_rope_init (host) and given to the calls below. */
+typedef struct kq_rope {
+    uint32_t rot_dim, layout;
+    float gain;
+    uint32_t reserved;
+    double turns[128];     /* pair i's turns (angle / 2 pi) per position */
+} kq_rope;
+int kq_rope_init(const kq_rope_params* params, kq_rope* out);
+
+/* y = x with the heads rotated, tokens x heads x head_dim elements of one type. Token t and head h
+ * of x start at x + t * x_token + h * x_head elements (0: dense, heads * head_dim and head_dim);
+ * y likewise. y == x with the same strides rotates in place; other overlaps are not allowed.
+ * positions: i32[tokens] on the device, negative ones turn backwards (a gradient goes through the
+ * rotation of -position, with the same gain). head_dim 1..1024, >= rot_dim. */
+typedef struct kq_rope_desc {
+    const kq_rope* rope;
+    uint64_t x, y, positions;
+    uint32_t type, tokens, heads, head_dim;
+    uint64_t x_token, x_head, y_token, y_head;
+} kq_rope_desc;
+int kq_rope_apply(kq_ctx* ctx, const kq_rope_desc* desc, kq_stream stream);
+
+/* A paged cache: two device arrays (k, v) of n_pages pages, each page_size positions (16, 32, 64,
+ * 128 or 256) of n_kv heads. KQ_CACHE_F16 holds 16-bit values; Q8 and Q4 hold blocks of 32 elements
+ * as codes c (-127..127 or -7..7) and one scale byte b: the scale is the f16 with bits b << 7 (5
+ * exponent, 3 fraction bits), the smallest one with scale * 127 (or 7) >= the block's largest
+ * magnitude, c = the nearest integer to x / scale (ties to even), the value c * scale, which f16
+ * holds exactly. Magnitudes above 65024 (Q8) or 64512 (Q4) saturate; a block with an infinity or a
+ * NaN reads back as NaN.
+ * Layout: [page][kv head][record]; a record is page_size rows of row_bytes codes, then (Q8, Q4)
+ * page_size x pitch / 32 scale bytes. pitch = head_dim rounded up to 64, 128 or 256 (elements past
+ * head_dim are zero), row_bytes = pitch * 2, pitch or pitch / 2. Q8 codes are stored + 128; Q4 codes
+ * + 8, eight consecutive elements in a 32-bit word at nibbles 0,4,1,5,2,6,3,7. The 16-byte unit l of
+ * a record's codes (row-major) lies at l ^ s(p), p its position in the page, s(p) = p mod 8 for
+ * row_bytes >= 128, 2 * ((p / 2) mod 4) for 64, 4 * ((p / 4) mod 2) for 32: the order in which the
+ * attention's shared-memory reads meet no bank twice, so pages are copied as they are.
+ * head_dim: a multiple of 32, 32..256. k, v 16-byte aligned. */
+enum { KQ_CACHE_F16 = 0, KQ_CACHE_Q8 = 1, KQ_CACHE_Q4 = 2 };
+typedef struct kq_cache {
+    uint32_t type, n_kv, head_dim, page_size;
+    uint32_t n_pages, reserved;
+    uint64_t k, v;
+} kq_cache;
+/* Bytes of each of k and v (k, v are not looked at); 0 when the cache is not a valid one. */
+uint64_t kq_cache_bytes(const kq_cache* cache);
+
+/* For each token: q_out <- its query heads rotated, the cache's slot slots[t] <- its key heads
+ * rotated and its value heads. Slot = page * page_size + position in the page; a negative slot writes
+ * nothing (q_out is still written). No two tokens may have the same slot. Heads of a token are dense
+ * (head_dim apart); token strides in elements, 0 = (n_heads + 2 n_kv) * head_dim for q, k, v (one
+ * q|k|v row) and n_heads * head_dim for q_out. q, k, v, q_out have one type; q_out may be q. q == 0:
+ * no queries; rope == NULL: no rotation (positions unused). The rotation is rounded once, to f32,
+ * before a key is quantised. */
+typedef struct kq_cache_write_desc {
+    const kq_cache* cache;
+    const kq_rope* rope;
+    uint64_t q, k, v, q_out;
+    uint64_t positions;    /* i32[tokens] */
+    uint64_t slots;        /* i64[tokens] */
+    uint64_t q_token, k_token, v_token, q_out_token;
+    uint32_t type, tokens, n_heads, reserved;
+} kq_cache_write_desc;
+int kq_cache_write(kq_ctx* ctx, const kq_cache_write_desc* desc, kq_stream stream);
+
+/* k_out, v_out (either may be 0) row i <- the values of slot slots[i], n_kv * head_dim elements of
+ * `type`, rows token_stride elements apart (0: dense). A negative slot gives a row of zeros. */
+typedef struct kq_cache_read_desc {
+    const kq_cache* cache;
+    uint64_t k_out, v_out;
+    uint64_t slots;        /* i64[count] */
+    uint64_t token_stride;
+    uint32_t type, count;
+} kq_cache_read_desc;
+int kq_cache_read(kq_ctx* ctx, const kq_cache_read_desc* desc, kq_stream stream);
+
+/* Rows move between slots as they are: within group g, moves starts[g] .. starts[g + 1) - 1 (at most
+ * 64) read every src before any dst is written, so a path's rows may slide over one another.
+ * Different groups may not touch one another's slots. A negative src or dst skips the move. */
+typedef struct kq_cache_move_desc {
+    const kq_cache* cache;
+    uint64_t src, dst;     /* i64[moves] */
+    uint64_t starts;       /* i32[groups + 1] */
+    uint32_t groups, moves;
+} kq_cache_move_desc;
+int kq_cache_move(kq_ctx* ctx, const kq_cache_move_desc* desc, kq_stream stream);
+
+/* Attention of drafted tokens. Sequence s has the tokens starts[s] .. starts[s + 1) - 1 (0..64), its
+ * drafts; its cache holds prefix[s] positions before them and the drafts' own rows at positions
+ * prefix[s] + 0, 1, ... (written before this call), position p in page pages[s * max_pages + p /
+ * page_size]. Token t attends over every position below prefix[s] and over the drafts u with bit u
+ * of mask[t] set (itself only if its bit is set); mask == 0: over the drafts up to itself. Query
+ * head h reads key/value head h / (n_heads / n_kv):
+ *   out[t][h] = sum_p w_p v_p, w = softmax_p(q[t][h] . k_p * scale).
+ * A token that sees no position gets zeros. A masked position's key and value are not looked at,
+ * infinities and NaNs included. q and out: `type`, heads dense, tokens q_token / out_token elements
+ * apart (0: n_heads * head_dim); q and out 16-byte aligned, strides multiples of 16 bytes; out may
+ * not overlap q. scale 0: 1 / sqrt(head_dim). Products: q and the weights enter the tensor cores as
+ * f16 (f32 activations: as the sum of two f16, about 22 bits), sums and softmax in f32; the order of
+ * the sums depends on the lengths and the GPU alone, so equal calls give equal bits.
+ * max_drafts, max_len: no sequence has more drafts, or prefix + drafts positions (max_len sizes the
+ * launch; a longer sequence is still served). n_heads / n_kv 1..64. */
+typedef struct kq_tree_desc {
+    const kq_cache* cache;
+    uint64_t q, out;
+    uint64_t q_token, out_token;
+    uint64_t starts, prefix; /* i32[n_seq + 1], i32[n_seq] */
+    uint64_t pages;          /* i32[n_seq][max_pages] */
+    uint64_t mask;           /* u64[tokens], or 0 */
+    uint64_t workspace, workspace_bytes; /* device, 16-byte aligned, nothing kept in it */
+    uint32_t type, n_heads, n_seq, tokens;
+    uint32_t max_drafts, max_len, max_pages;
+    float scale;
+} kq_tree_desc;
+int kq_attention_tree(kq_ctx* ctx, const kq_tree_desc* desc, kq_stream stream);
+/* The workspace a call with this descriptor needs (its addresses are not looked at; 0 when it is
+ * not a valid one). It does not grow with the contexts' lengths. */
+uint64_t kq_tree_workspace(kq_ctx* ctx, const kq_tree_desc* desc);
+
 /* ---- Row-sharded stacks: a matvec whose epilogue also pushes its outputs to other GPUs ----
  *
  * With the rows of a matrix split over N GPUs, every GPU needs the whole output vector for the

@@ -66,6 +66,8 @@ EXPORTS = (
     "kq_gguf_open", "kq_gguf_close", "kq_gguf_tensor_count", "kq_gguf_tensor_at", "kq_gguf_find",
     "kq_gguf_meta_int", "kq_gguf_meta_str", "kq_module_image", "kq_matvec_plan",
     "kq_rope_append", "kq_attention_decode", "kq_attention_workspace", "kq_tagged_unpack",
+    "kq_rope_init", "kq_rope_apply", "kq_cache_bytes", "kq_cache_write", "kq_cache_read", "kq_cache_move",
+    "kq_attention_tree", "kq_tree_workspace",
 )
 
 
@@ -134,6 +136,93 @@ class KqChainJob(ctypes.Structure):
 
 CHAIN_MAX_JOBS = 8
 
+# Activations' element types (the rotary, cache and tree attention calls).
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 30
+ROPE_PAIRS = 0
+ROPE_HALVES = 1
+CACHE_F16 = 0
+CACHE_Q8 = 1
+CACHE_Q4 = 2
+
+
+class KqRopeParams(ctypes.Structure):
+    _fields_ = [
+        ("rot_dim", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("base", ctypes.c_double),
+        ("freq_scale", ctypes.c_double), ("ext_factor", ctypes.c_double), ("attn_factor", ctypes.c_double),
+        ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double), ("orig_ctx", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32), ("freq_factors", ctypes.POINTER(ctypes.c_float)),
+    ]
+
+
+class KqRope(ctypes.Structure):
+    _fields_ = [
+        ("rot_dim", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("gain", ctypes.c_float),
+        ("reserved", ctypes.c_uint32), ("turns", ctypes.c_double * 128),
+    ]
+
+
+class KqRopeDesc(ctypes.Structure):
+    """``kq_rope_desc`` (include/kq.h), made by :func:`rope_desc`."""
+    _fields_ = [
+        ("rope", ctypes.POINTER(KqRope)), ("x", ctypes.c_uint64), ("y", ctypes.c_uint64),
+        ("positions", ctypes.c_uint64), ("type", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+        ("heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("x_token", ctypes.c_uint64),
+        ("x_head", ctypes.c_uint64), ("y_token", ctypes.c_uint64), ("y_head", ctypes.c_uint64),
+    ]
+
+
+class KqCache(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_uint32), ("n_kv", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+        ("page_size", ctypes.c_uint32), ("n_pages", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+        ("k", ctypes.c_uint64), ("v", ctypes.c_uint64),
+    ]
+
+
+class KqCacheWriteDesc(ctypes.Structure):
+    """``kq_cache_write_desc`` (include/kq.h), made by :func:`cache_write_desc`."""
+    _fields_ = [
+        ("cache", ctypes.POINTER(KqCache)), ("rope", ctypes.POINTER(KqRope)), ("q", ctypes.c_uint64),
+        ("k", ctypes.c_uint64), ("v", ctypes.c_uint64), ("q_out", ctypes.c_uint64),
+        ("positions", ctypes.c_uint64), ("slots", ctypes.c_uint64), ("q_token", ctypes.c_uint64),
+        ("k_token", ctypes.c_uint64), ("v_token", ctypes.c_uint64), ("q_out_token", ctypes.c_uint64),
+        ("type", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("n_heads", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+class KqCacheReadDesc(ctypes.Structure):
+    """``kq_cache_read_desc`` (include/kq.h), made by :func:`cache_read_desc`."""
+    _fields_ = [
+        ("cache", ctypes.POINTER(KqCache)), ("k_out", ctypes.c_uint64), ("v_out", ctypes.c_uint64),
+        ("slots", ctypes.c_uint64), ("token_stride", ctypes.c_uint64), ("type", ctypes.c_uint32),
+        ("count", ctypes.c_uint32),
+    ]
+
+
+class KqCacheMoveDesc(ctypes.Structure):
+    """``kq_cache_move_desc`` (include/kq.h), made by :func:`cache_move_desc`."""
+    _fields_ = [
+        ("cache", ctypes.POINTER(KqCache)), ("src", ctypes.c_uint64), ("dst", ctypes.c_uint64),
+        ("starts", ctypes.c_uint64), ("groups", ctypes.c_uint32), ("moves", ctypes.c_uint32),
+    ]
+
+
+class KqTreeDesc(ctypes.Structure):
+    """``kq_tree_desc`` (include/kq.h), made by :func:`tree_desc`."""
+    _fields_ = [
+        ("cache", ctypes.POINTER(KqCache)), ("q", ctypes.c_uint64), ("out", ctypes.c_uint64),
+        ("q_token", ctypes.c_uint64), ("out_token", ctypes.c_uint64), ("starts", ctypes.c_uint64),
+        ("prefix", ctypes.c_uint64), ("pages", ctypes.c_uint64), ("mask", ctypes.c_uint64),
+        ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64), ("type", ctypes.c_uint32),
+        ("n_heads", ctypes.c_uint32), ("n_seq", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+        ("max_drafts", ctypes.c_uint32), ("max_len", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 IPC_HANDLE_BYTES = 64
 
 _lib: ctypes.CDLL | None = None
@@ -190,9 +279,20 @@ def lib() -> ctypes.CDLL:
     L.kq_gguf_find.argtypes = [vp, ctypes.c_char_p, ctypes.POINTER(KqGgufTensor)]
     L.kq_gguf_meta_int.argtypes = [vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]
     L.kq_gguf_meta_str.argtypes = [vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p)]
+    L.kq_rope_init.argtypes = [ctypes.POINTER(KqRopeParams), ctypes.POINTER(KqRope)]
+    L.kq_rope_apply.argtypes = [vp, ctypes.POINTER(KqRopeDesc), vp]
+    L.kq_cache_bytes.argtypes = [ctypes.POINTER(KqCache)]
+    L.kq_cache_bytes.restype = u64
+    L.kq_cache_write.argtypes = [vp, ctypes.POINTER(KqCacheWriteDesc), vp]
+    L.kq_cache_read.argtypes = [vp, ctypes.POINTER(KqCacheReadDesc), vp]
+    L.kq_cache_move.argtypes = [vp, ctypes.POINTER(KqCacheMoveDesc), vp]
+    L.kq_attention_tree.argtypes = [vp, ctypes.POINTER(KqTreeDesc), vp]
+    L.kq_tree_workspace.argtypes = [vp, ctypes.POINTER(KqTreeDesc)]
+    L.kq_tree_workspace.restype = u64
     for name in EXPORTS:
         fn = getattr(L, name)
-        if name not in ("kq_last_error", "kq_stream_key", "kq_gguf_tensor_count", "kq_attention_workspace"):
+        if name not in ("kq_last_error", "kq_stream_key", "kq_gguf_tensor_count", "kq_attention_workspace",
+                        "kq_cache_bytes", "kq_tree_workspace"):
             fn.restype = i32
     _lib = L
     return L
@@ -417,6 +517,46 @@ class Kernels:
                                          n_heads, n_kv, head_dim, length, _addr(workspace),
                                          workspace_bytes, _stream(stream)), "kq_attention_decode")
 
+    # The calls on drafted tokens take a descriptor, made once beside the buffers it names
+    # (rope_desc and the others below) and launched every step, as a chain's jobs are.
+
+    def rope(self, desc: "KqRopeDesc", stream=None) -> None:
+        """``kq_rope_apply``: heads rotated by each token's position."""
+        rc = lib().kq_rope_apply(self._ctx, desc, _stream(stream))
+        if rc:
+            _check(rc, "kq_rope_apply")
+
+    def cache_write(self, desc: "KqCacheWriteDesc", stream=None) -> None:
+        """``kq_cache_write``: query heads rotated, key heads rotated and kept, value heads kept."""
+        rc = lib().kq_cache_write(self._ctx, desc, _stream(stream))
+        if rc:
+            _check(rc, "kq_cache_write")
+
+    def cache_read(self, desc: "KqCacheReadDesc", stream=None) -> None:
+        """``kq_cache_read``: slots of the cache back as values."""
+        rc = lib().kq_cache_read(self._ctx, desc, _stream(stream))
+        if rc:
+            _check(rc, "kq_cache_read")
+
+    def cache_move(self, desc: "KqCacheMoveDesc", stream=None) -> None:
+        """``kq_cache_move``: rows of the cache to other slots."""
+        rc = lib().kq_cache_move(self._ctx, desc, _stream(stream))
+        if rc:
+            _check(rc, "kq_cache_move")
+
+    def attention_tree(self, desc: "KqTreeDesc", stream=None) -> None:
+        """``kq_attention_tree``: drafted tokens' attention over their sequences' caches."""
+        rc = lib().kq_attention_tree(self._ctx, desc, _stream(stream))
+        if rc:
+            _check(rc, "kq_attention_tree")
+
+    def tree_workspace(self, desc: "KqTreeDesc") -> int:
+        """Bytes of workspace ``attention_tree(desc)`` needs."""
+        n = int(lib().kq_tree_workspace(self._ctx, desc))
+        if n == 0:
+            _check(KQ_E_INVALID, "kq_tree_workspace")
+        return n
+
     def matvec_chain(self, jobs, epoch: int, stream=None) -> None:
         """``kq_matvec_chain``: up to 8 batch-1 matvecs of one type and k in one launch, each
         waiting for its counter before it reads x (see include/kq.h). ``jobs`` is a sequence of
@@ -460,6 +600,116 @@ class Kernels:
     def device_error(self) -> None:
         """Synchronises the GPU and raises if a kernel's bounded wait gave up."""
         _check(lib().kq_device_error(self._ctx), "kq_device_error")
+
+
+class Rope:
+    """A rotary embedding's table (``kq_rope_init``): ``rot_dim`` elements of a head rotated, pair i
+    by position * base^(-2i/rot_dim) (/ ``freq_factors[i]``), slowed by ``freq_scale`` for contexts
+    longer than the model's, by parts with ``ext_factor`` (then ``orig_ctx`` says what it was trained
+    on). See kq_rope_params in include/kq.h."""
+
+    def __init__(self, rot_dim: int, layout: int = ROPE_PAIRS, base: float = 10000.0, *,
+                 freq_scale: float = 1.0, ext_factor: float = 0.0, attn_factor: float = 1.0,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, orig_ctx: int = 0, freq_factors=None):
+        factors = None
+        if freq_factors is not None:
+            if len(freq_factors) != rot_dim // 2:
+                raise Error("kq_rope_init", "freq_factors must have rot_dim / 2 values", KQ_E_INVALID)
+            factors = (ctypes.c_float * len(freq_factors))(*[float(f) for f in freq_factors])
+        p = KqRopeParams(rot_dim=rot_dim, layout=layout, base=base, freq_scale=freq_scale,
+                         ext_factor=ext_factor, attn_factor=attn_factor, beta_fast=beta_fast,
+                         beta_slow=beta_slow, orig_ctx=orig_ctx, reserved=0,
+                         freq_factors=ctypes.cast(factors, ctypes.POINTER(ctypes.c_float)) if factors else None)
+        self.c = KqRope()
+        _check(lib().kq_rope_init(ctypes.byref(p), ctypes.byref(self.c)), "kq_rope_init")
+
+
+class KvCache:
+    """A paged key/value cache over the caller's two device buffers (``kq_cache`` in include/kq.h):
+    ``cache_bytes`` gives the size of each."""
+
+    def __init__(self, type: int, n_kv: int, head_dim: int, page_size: int, n_pages: int, k, v):
+        self.c = KqCache(type=type, n_kv=n_kv, head_dim=head_dim, page_size=page_size, n_pages=n_pages,
+                         reserved=0, k=_addr(k), v=_addr(v))
+        self.k, self.v = k, v
+
+
+def cache_bytes(type: int, n_kv: int, head_dim: int, page_size: int, n_pages: int) -> int:
+    """Bytes of each of a cache's two buffers."""
+    n = int(lib().kq_cache_bytes(ctypes.byref(KqCache(type=type, n_kv=n_kv, head_dim=head_dim,
+                                                      page_size=page_size, n_pages=n_pages))))
+    if n == 0:
+        raise Error("kq_cache_bytes", "not a valid cache", KQ_E_INVALID)
+    return n
+
+
+def _desc(cls, keep, **fields):
+    """A descriptor that keeps alive what it points to on the host (and the tensors it names)."""
+    d = cls(**fields)
+    d._keep = keep
+    return d
+
+
+def rope_desc(rope: Rope, y, x, positions, tokens: int, heads: int, head_dim: int, *, type: int = TYPE_F32,
+              x_token: int = 0, x_head: int = 0, y_token: int = 0, y_head: int = 0) -> KqRopeDesc:
+    """What :meth:`Kernels.rope` rotates: ``tokens`` x ``heads`` x ``head_dim`` elements of x into y, by
+    i32 ``positions`` on the device (strides in elements, 0 = dense)."""
+    return _desc(KqRopeDesc, (rope, y, x, positions), rope=ctypes.pointer(rope.c), x=_addr(x), y=_addr(y),
+                 positions=_addr(positions), type=type, tokens=tokens, heads=heads, head_dim=head_dim,
+                 x_token=x_token, x_head=x_head, y_token=y_token, y_head=y_head)
+
+
+_SIZES = {TYPE_F32: 4, TYPE_F16: 2, TYPE_BF16: 2}
+
+
+def cache_write_desc(cache: KvCache, rope: Rope | None, qkv, q_out, positions, slots, tokens: int,
+                     n_heads: int, *, type: int = TYPE_F32, token_stride: int = 0,
+                     q_out_token: int = 0) -> KqCacheWriteDesc:
+    """What :meth:`Kernels.cache_write` writes: ``tokens`` rows of q | k | v (a batch of a q|k|v
+    projection's outputs; ``token_stride`` elements apart, 0 = dense), their queries rotated into
+    ``q_out``, keys and values into i64 ``slots`` of the cache. ``n_heads`` 0: rows of k | v."""
+    dim, size = cache.c.head_dim, _SIZES.get(type, 4)
+    base = _addr(qkv)
+    k = base + n_heads * dim * size
+    stride = token_stride or (n_heads + 2 * cache.c.n_kv) * dim
+    return _desc(KqCacheWriteDesc, (cache, rope, qkv, q_out, positions, slots),
+                 cache=ctypes.pointer(cache.c), rope=ctypes.pointer(rope.c) if rope is not None else None,
+                 q=base if n_heads else 0, k=k, v=k + cache.c.n_kv * dim * size,
+                 q_out=_addr(q_out) if n_heads else 0, positions=_addr(positions), slots=_addr(slots),
+                 q_token=stride, k_token=stride, v_token=stride, q_out_token=q_out_token, type=type,
+                 tokens=tokens, n_heads=n_heads, reserved=0)
+
+
+def cache_read_desc(cache: KvCache, k_out, v_out, slots, count: int, *, type: int = TYPE_F32,
+                    token_stride: int = 0) -> KqCacheReadDesc:
+    """What :meth:`Kernels.cache_read` reads: i64 ``slots``[count] of the cache into rows of ``k_out``
+    and ``v_out`` (either may be None)."""
+    return _desc(KqCacheReadDesc, (cache, k_out, v_out, slots), cache=ctypes.pointer(cache.c),
+                 k_out=_addr(k_out), v_out=_addr(v_out), slots=_addr(slots), token_stride=token_stride,
+                 type=type, count=count)
+
+
+def cache_move_desc(cache: KvCache, src, dst, starts, groups: int, moves: int) -> KqCacheMoveDesc:
+    """What :meth:`Kernels.cache_move` moves: i64 slots ``src`` to ``dst``, in ``groups`` (i32
+    ``starts``[groups + 1]) that each read before they write."""
+    return _desc(KqCacheMoveDesc, (cache, src, dst, starts), cache=ctypes.pointer(cache.c), src=_addr(src),
+                 dst=_addr(dst), starts=_addr(starts), groups=groups, moves=moves)
+
+
+def tree_desc(cache: KvCache, out, q, n_heads: int, starts, prefix, pages, max_pages: int, n_seq: int,
+              tokens: int, max_drafts: int, max_len: int, *, mask=None, scale: float = 0.0,
+              type: int = TYPE_F32, q_token: int = 0, out_token: int = 0, workspace=None,
+              workspace_bytes: int = 0) -> KqTreeDesc:
+    """What :meth:`Kernels.attention_tree` computes (``kq_tree_desc`` in include/kq.h): ``tokens``
+    drafted tokens of ``n_seq`` sequences over their pages of the cache. ``mask``: u64 words (an int64
+    tensor's bits), None for drafts in a chain. Give it the workspace that
+    :meth:`Kernels.tree_workspace` asks for."""
+    return _desc(KqTreeDesc, (cache, out, q, starts, prefix, pages, mask, workspace),
+                 cache=ctypes.pointer(cache.c), q=_addr(q), out=_addr(out), q_token=q_token,
+                 out_token=out_token, starts=_addr(starts), prefix=_addr(prefix), pages=_addr(pages),
+                 mask=_addr(mask), workspace=_addr(workspace), workspace_bytes=workspace_bytes, type=type,
+                 n_heads=n_heads, n_seq=n_seq, tokens=tokens, max_drafts=max_drafts, max_len=max_len,
+                 max_pages=max_pages, scale=scale)
 
 
 class DeviceArray:

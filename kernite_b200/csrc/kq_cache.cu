@@ -1,0 +1,619 @@
+// kq_cache.cu -- rotary positions, and the quantised paged cache: written (heads rotated on the way),
+// read back, and its rows moved. The format is kq_cache.cuh's.
+//
+// All four move bytes once and are bound by memory, or, for a few tokens, by one launch.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <string>
+
+#include "kq_cache.cuh"
+#include "kq_device.cuh"
+#include "kq_internal.h"
+
+namespace kq {
+namespace {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kWarps = kThreads / 32;
+constexpr uint32_t kMaxMoves = 64;
+
+// One kernel rotates heads into an array (queries, kq_rope_apply) and into the cache (keys), and
+// copies heads into the cache (values). A CTA takes one token and a share of its rows (heads); a warp
+// takes the rows of `together` heads at once, VE consecutive elements a lane.
+struct RopeArgs {
+  kq_rope rope;
+  const void* q;   // rows [0, nq): to q_out
+  const void* k;   // rows [nq, nq + n_kv): rotated, to the cache
+  const void* v;   // rows [nq + n_kv, nq + 2 n_kv): to the cache
+  void* q_out;
+  const int* positions;
+  const long long* slots;
+  uint64_t q_token, q_head, k_token, v_token, out_token, out_head;
+  uint32_t nq, dim;
+  uint32_t rot_half;  // rotated pairs a head (0: none)
+  uint32_t together;  // heads a warp takes at once
+  CacheView cache;
+  unsigned* err;
+};
+
+// (x_a, x_b) of a pair whose (gain cos, gain sin) is w.
+__device__ __forceinline__ float turned_a(float a, float b, float2 w) { return fmaf(a, w.x, -b * w.y); }
+__device__ __forceinline__ float turned_b(float a, float b, float2 w) { return fmaf(a, w.y, b * w.x); }
+
+// VE neighbouring elements e.. of a row, pairs (2i, 2i + 1), rotated; elements past the rotated part
+// (rot_half pairs) as they are. VE == 1 reads the pair's other element too.
+template <typename T, int VE>
+__device__ __forceinline__ void rotate_pairs(const T* row, uint32_t e, uint32_t rot_half, const float2* cs,
+                                             float (&y)[VE]) {
+  load_act<T, VE>(row + e, y);
+  if constexpr (VE == 1) {
+    if (e < 2 * rot_half) {
+      const float other = act_to_f32<T>(row[e ^ 1u]);
+      y[0] = (e & 1u) ? turned_b(other, y[0], cs[e >> 1]) : turned_a(y[0], other, cs[e >> 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; i += 2) {
+      if (e + i < 2 * rot_half) {
+        const float2 w = cs[(e + i) >> 1];
+        const float x0 = y[i], x1 = y[i + 1];
+        y[i] = turned_a(x0, x1, w);
+        y[i + 1] = turned_b(x0, x1, w);
+      }
+    }
+  }
+}
+
+// The same for pairs (i, i + rot_half); the partners come from memory too (the same row, so from L1).
+// rot_half is a multiple of VE.
+template <typename T, int VE>
+__device__ __forceinline__ void rotate_halves(const T* row, uint32_t e, uint32_t rot_half, const float2* cs,
+                                              float (&y)[VE]) {
+  load_act<T, VE>(row + e, y);
+  if (e >= 2 * rot_half) return;
+  const bool first = e < rot_half;
+  float o[VE];
+  load_act<T, VE>(row + (first ? e + rot_half : e - rot_half), o);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const float2 w = cs[(first ? e : e - rot_half) + i];
+    y[i] = first ? turned_a(y[i], o[i], w) : turned_b(o[i], y[i], w);
+  }
+}
+
+// VE values of elements e.. of position p into a head's record; the 32 / VE lanes of a block of 32
+// elements call this together (mask: the lanes that do).
+template <int VE>
+__device__ __forceinline__ void keep(const CacheView& c, uint8_t* record, uint32_t p, uint32_t e,
+                                     const float (&y)[VE], uint32_t mask) {
+  if (c.kind == KQ_CACHE_F16) {
+    __half h[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) h[i] = __float2half_rn(y[i]);
+    uint8_t* to = record + cache_offset(p, 2 * e, c.row);
+    if constexpr (VE == 8) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
+    else if constexpr (VE == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(h);
+    else *reinterpret_cast<__half*>(to) = h[0];
+    return;
+  }
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 16 / VE; o; o >>= 1) most = max(most, __shfl_xor_sync(mask, most, o));
+  const uint32_t byte = scale_byte(most, c.kind);
+  const float scale = scale_value(byte), top = cache_top(c.kind);
+  uint32_t u[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    // a correctly rounded quotient: which codes a value near a tie gets must not depend on how the
+    // division was made
+    const float code = byte == 0 || byte == kScaleNan ? 0.f : rintf(__fdiv_rn(y[i], scale));
+    u[i] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(code, -top), top)) +
+                                 (c.kind == KQ_CACHE_Q8 ? 128 : 8));
+  }
+  if (e % 32 == 0) record[c.page() * c.row + p * c.scales + e / 32] = static_cast<uint8_t>(byte);
+  if (c.kind == KQ_CACHE_Q8) {
+    uint8_t* to = record + cache_offset(p, e, c.row);
+    if constexpr (VE == 8) {
+      *reinterpret_cast<uint2*>(to) = make_uint2(u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24,
+                                                 u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24);
+    } else if constexpr (VE == 4) {
+      *reinterpret_cast<uint32_t*>(to) = u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24;
+    } else {
+      *to = static_cast<uint8_t>(u[0]);
+    }
+    return;
+  }
+  // eight elements a word, element 2i at nibble i and 2i + 1 at nibble i + 4
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const uint32_t j = (e + i) & 7u;
+    word |= u[i] << (4 * ((j >> 1) + 4 * (j & 1)));
+  }
+#pragma unroll
+  for (int o = 4 / VE; o; o >>= 1) word |= __shfl_xor_sync(mask, word, o);
+  if (e % 8 == 0) *reinterpret_cast<uint32_t*>(record + cache_offset(p, e / 2, c.row)) = word;
+}
+
+// Grid (tokens, shares of the rows). The angles of a token are taken once a CTA: position * turns in
+// f64 (position 100000 turns pair 0 by 16000 turns: f32 would leave 10 bits of the fraction), its
+// fraction exactly to f32, then sincospi of twice that.
+template <typename T, int VE>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+  __shared__ float2 cs[128];
+  const uint32_t t = blockIdx.x;
+  for (uint32_t i = threadIdx.x; i < a.rot_half; i += kThreads) {
+    const double turns = static_cast<double>(a.positions[t]) * a.rope.turns[i];
+    const float part = static_cast<float>(turns - rint(turns));
+    float s, c;
+    sincospif(2.f * part, &s, &c);
+    cs[i] = make_float2(a.rope.gain * c, a.rope.gain * s);
+  }
+  __syncthreads();
+  long long slot = -1;
+  if (a.slots) {
+    slot = a.slots[t];
+    if (slot >= 0 && static_cast<uint64_t>(slot) >> a.cache.page_log2 >= a.cache.n_pages) {
+      if (threadIdx.x == 0) report_error(a.err, kErrCacheRange);
+      slot = -1;
+    }
+  }
+  const uint32_t rows = a.nq + (slot >= 0 ? 2 * a.cache.n_kv : 0);
+  const uint32_t page = static_cast<uint32_t>(slot >= 0 ? slot >> a.cache.page_log2 : 0);
+  const uint32_t p = static_cast<uint32_t>(slot) & (a.cache.page() - 1);
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t step = gridDim.y * kWarps * a.together;
+  const bool halves = a.rope.layout == KQ_ROPE_HALVES;
+  for (uint32_t r0 = (blockIdx.y * kWarps + warp) * a.together; r0 < rows; r0 += step) {
+    if (r0 < a.nq) {
+      // queries: a lane takes VE elements, for halves with their partners, so that nothing it reads
+      // is written by another pass of the row (q_out may be q)
+      const uint32_t width = halves ? a.dim - a.rot_half : a.dim;
+      for (uint32_t at = lane * VE; at < a.together * width + lane * VE; at += 32 * VE) {
+        const uint32_t row = r0 + at / width;
+        uint32_t e = at % width;
+        const bool in = at < a.together * width;
+        const T* x = static_cast<const T*>(a.q) + t * a.q_token + row * a.q_head;
+        T* y = static_cast<T*>(a.q_out) + t * a.out_token + row * a.out_head;
+        if (halves) {
+          if (!in) continue;
+          if (e < a.rot_half) {
+            float u[VE], v[VE];
+            load_act<T, VE>(x + e, u);
+            load_act<T, VE>(x + e + a.rot_half, v);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+              const float2 w = cs[e + i];
+              const float u0 = u[i];
+              u[i] = turned_a(u0, v[i], w);
+              v[i] = turned_b(u0, v[i], w);
+            }
+            store_act<T, VE>(y + e, u);
+            store_act<T, VE>(y + e + a.rot_half, v);
+          } else {
+            float u[VE];
+            e += a.rot_half;
+            load_act<T, VE>(x + e, u);
+            store_act<T, VE>(y + e, u);
+          }
+        } else {
+          float u[VE];
+          if (in) rotate_pairs<T, VE>(x, e, a.rot_half, cs, u);
+          __syncwarp();  // both elements of a pair are read before either is written
+          if (in) store_act<T, VE>(y + e, u);
+        }
+      }
+      continue;
+    }
+    const uint32_t width = a.cache.pitch;
+    for (uint32_t c0 = 0; c0 < a.together * width; c0 += 32 * VE) {
+      const uint32_t at = c0 + lane * VE;
+      const uint32_t row = r0 + at / width - a.nq, e = at % width;
+      const bool in = at < a.together * width && row < 2 * a.cache.n_kv;
+      const uint32_t mask = __ballot_sync(0xffffffffu, in);
+      if (!in) continue;
+      const bool key = row < a.cache.n_kv;
+      const uint32_t h = key ? row : row - a.cache.n_kv;
+      const T* x = key ? static_cast<const T*>(a.k) + t * a.k_token + h * a.dim
+                       : static_cast<const T*>(a.v) + t * a.v_token + h * a.dim;
+      float y[VE];
+      if (e >= a.dim) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) y[i] = 0.f;
+      } else if (!key) {
+        load_act<T, VE>(x + e, y);
+      } else if (halves) {
+        rotate_halves<T, VE>(x, e, a.rot_half, cs, y);
+      } else {
+        rotate_pairs<T, VE>(x, e, a.rot_half, cs, y);
+      }
+      __syncwarp(mask);
+      keep<VE>(a.cache, (key ? a.cache.k : a.cache.v) + a.cache.at(page, h), p, e, y, mask);
+    }
+  }
+}
+
+template <typename T, int VE>
+int launch_rope(const RopeArgs& a, uint32_t tokens, uint32_t rows, int sm_count, cudaStream_t s,
+                const char* call) {
+  // One CTA a token leaves most SMs idle below some hundred tokens: the rows are then shared by more
+  // CTAs, each taking the token's angles again.
+  const uint32_t groups = (rows + kWarps * a.together - 1) / (kWarps * a.together);
+  const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(groups, 4u * sm_count / tokens));
+  rope_kernel<T, VE><<<dim3(tokens, shares), kThreads, 0, s>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", call);
+}
+
+// The wide form wants every row it reads or writes on 16 bytes and, for halves, partners a whole lane
+// apart; anything else is served one element a lane.
+template <typename T>
+int dispatch_rope(RopeArgs& a, bool aligned, uint32_t tokens, uint32_t rows, int sm_count, cudaStream_t s,
+                  const char* call) {
+  constexpr int VE = 16 / sizeof(T);
+  const bool wide = aligned && a.dim % VE == 0 &&
+                    (a.rope.layout == KQ_ROPE_PAIRS || a.rot_half % VE == 0);
+  if (wide) {
+    // narrow heads: a warp takes several at once, where the queries come out even
+    const uint32_t width = a.slots ? a.cache.pitch : a.dim;
+    const uint32_t n = std::max<uint32_t>(1, 32 * VE / width);
+    a.together = a.nq % n == 0 ? n : 1;
+    return launch_rope<T, VE>(a, tokens, rows, sm_count, s, call);
+  }
+  a.together = 1;
+  return launch_rope<T, 1>(a, tokens, rows, sm_count, s, call);
+}
+
+uint32_t type_size(uint32_t type) {
+  return type == KQ_TYPE_F32 ? 4 : type == KQ_TYPE_F16 || type == KQ_TYPE_BF16 ? 2 : 0;
+}
+
+int run_rope(RopeArgs& a, uint32_t type, bool aligned, uint32_t tokens, uint32_t rows, int sm_count,
+             cudaStream_t s, const char* call) {
+  if (type == KQ_TYPE_F32) return dispatch_rope<float>(a, aligned, tokens, rows, sm_count, s, call);
+  if (type == KQ_TYPE_F16) return dispatch_rope<__half>(a, aligned, tokens, rows, sm_count, s, call);
+  return dispatch_rope<__nv_bfloat16>(a, aligned, tokens, rows, sm_count, s, call);
+}
+
+bool rope_ok(const kq_rope* r) {
+  return r->rot_dim >= 2 && r->rot_dim <= 256 && r->rot_dim % 2 == 0 && r->layout <= KQ_ROPE_HALVES;
+}
+
+bool on16(uint64_t bytes) { return bytes % 16 == 0; }
+
+// ---------------------------------------------------------------- reading back
+
+// Eight elements a thread, a grid over (rows of the output, K then V).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheView c, T* k_out, T* v_out,
+                                                              const long long* slots, uint64_t token_stride,
+                                                              uint32_t count, bool wide, unsigned* err) {
+  const bool value = blockIdx.y;
+  T* out = value ? v_out : k_out;
+  const uint8_t* base = value ? c.v : c.k;
+  const uint32_t units = c.dim / 8;
+  const uint64_t total = uint64_t(count) * c.n_kv * units;
+  for (uint64_t i = blockIdx.x * uint64_t(kThreads) + threadIdx.x; i < total; i += uint64_t(gridDim.x) * kThreads) {
+    const uint32_t unit = i % units;
+    const uint32_t h = (i / units) % c.n_kv;
+    const uint64_t r = i / units / c.n_kv;
+    const long long slot = slots[r];
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = 0.f;
+    if (slot >= 0) {
+      if (static_cast<uint64_t>(slot) >> c.page_log2 >= c.n_pages) {
+        report_error(err, kErrCacheRange);
+        continue;
+      }
+      const uint8_t* rec = base + c.at(static_cast<uint32_t>(slot >> c.page_log2), h);
+      const uint32_t p = static_cast<uint32_t>(slot) & (c.page() - 1), e = 8 * unit;
+      if (c.kind == KQ_CACHE_F16) {
+        load_act<__half, 8>(reinterpret_cast<const __half*>(rec + cache_offset(p, 2 * e, c.row)), y);
+      } else {
+        const float s = scale_value(rec[c.page() * c.row + p * c.scales + e / 32]);
+        if (c.kind == KQ_CACHE_Q8) {
+          const uint2 w = *reinterpret_cast<const uint2*>(rec + cache_offset(p, e, c.row));
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            y[j] = (static_cast<float>(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u) - 128.f) * s;
+        } else {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + cache_offset(p, e / 2, c.row));
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            y[j] = (static_cast<float>((w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u) - 8.f) * s;
+        }
+      }
+    }
+    T* to = out + r * token_stride + h * c.dim + 8 * unit;
+    if (wide) {
+      if constexpr (sizeof(T) == 4) {
+        const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
+        store_act<T, 4>(to, lo);
+        store_act<T, 4>(to + 4, hi);
+      } else {
+        store_act<T, 8>(to, y);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) to[j] = act_from_f32<T>(y[j]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- moving rows
+
+// A CTA takes one head of one group, keys or values: every source row (codes and scales) into shared
+// memory, then out, so a group's rows may slide over one another. The permutation of units depends
+// on the position, so rows move as unpermuted 16-byte units.
+__global__ void __launch_bounds__(kThreads) cache_move_kernel(CacheView c, const long long* src,
+                                                              const long long* dst, const int* starts,
+                                                              uint32_t moves, unsigned* err) {
+  extern __shared__ uint4 rows[];
+  __shared__ uint8_t scales[kMaxMoves][8];
+  uint8_t* base = blockIdx.z ? c.v : c.k;
+  const uint32_t h = blockIdx.y;
+  const int a = starts[blockIdx.x], b = starts[blockIdx.x + 1];
+  if (a < 0 || b < a || static_cast<uint32_t>(b) > moves || b - a > static_cast<int>(kMaxMoves)) {
+    if (threadIdx.x == 0) report_error(err, kErrCacheRange);
+    return;
+  }
+  const uint32_t n = b - a, units = c.row / 16;
+  const uint64_t capacity = uint64_t(c.n_pages) << c.page_log2;
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+    if ((src[a + i] >= 0 && static_cast<uint64_t>(src[a + i]) >= capacity) ||
+        (dst[a + i] >= 0 && static_cast<uint64_t>(dst[a + i]) >= capacity))
+      report_error(err, kErrCacheRange);
+  for (int write = 0; write < 2; ++write) {
+    for (uint32_t i = threadIdx.x; i < n * (units + 1); i += kThreads) {
+      const uint32_t m = i / (units + 1), u = i % (units + 1);
+      const long long from = src[a + m], to = dst[a + m];
+      if (from < 0 || to < 0 || static_cast<uint64_t>(from) >= capacity || static_cast<uint64_t>(to) >= capacity)
+        continue;
+      const long long slot = write ? to : from;
+      const uint32_t p = static_cast<uint32_t>(slot) & (c.page() - 1);
+      uint8_t* rec = base + c.at(static_cast<uint32_t>(slot >> c.page_log2), h);
+      if (u < units) {
+        uint4* at = reinterpret_cast<uint4*>(rec + cache_offset(p, 16 * u, c.row));
+        if (write) *at = rows[m * units + u];
+        else rows[m * units + u] = *at;
+      } else {
+        uint8_t* at = rec + c.page() * c.row + p * c.scales;
+        for (uint32_t j = 0; j < c.scales; ++j) {
+          if (write) at[j] = scales[m][j];
+          else scales[m][j] = at[j];
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+int cache_view(const kq_cache* c, CacheView* out) {
+  if (c->type > KQ_CACHE_Q4 || c->n_kv == 0 || c->head_dim == 0 || c->head_dim % 32 || c->head_dim > 256 ||
+      c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)) || c->n_pages == 0 ||
+      c->n_pages > 0x7fffffffu || c->n_kv > 0xffffu)
+    return KQ_E_INVALID;
+  CacheView v = {};
+  v.k = reinterpret_cast<uint8_t*>(c->k);
+  v.v = reinterpret_cast<uint8_t*>(c->v);
+  v.kind = c->type;
+  v.n_kv = c->n_kv;
+  v.dim = c->head_dim;
+  v.pitch = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+  while ((1u << v.page_log2) < c->page_size) ++v.page_log2;
+  v.n_pages = c->n_pages;
+  v.row = c->type == KQ_CACHE_F16 ? 2 * v.pitch : c->type == KQ_CACHE_Q8 ? v.pitch : v.pitch / 2;
+  v.scales = c->type == KQ_CACHE_F16 ? 0 : v.pitch / 32;
+  v.record = uint64_t(c->page_size) * (v.row + v.scales);
+  *out = v;
+  return KQ_OK;
+}
+
+uint64_t cache_bytes(const kq_cache& c) {
+  CacheView v;
+  return cache_view(&c, &v) == KQ_OK ? v.at(v.n_pages, 0) : 0;
+}
+
+int check_cache(const kq_cache* c, const char* call, CacheView* out) {
+  if (!c) return fail(KQ_E_INVALID, call, "null cache");
+  if (cache_view(c, out) != KQ_OK)
+    return fail(KQ_E_INVALID, call, "the cache wants a type F16, Q8 or Q4, n_kv 1..65535, head_dim a multiple "
+                                    "of 32 up to 256, page_size 16, 32, 64, 128 or 256 and pages");
+  if (!c->k || !c->v || !on16(c->k) || !on16(c->v))
+    return fail(KQ_E_INVALID, call, "the cache's k and v must be 16-byte aligned and not null");
+  return KQ_OK;
+}
+
+int cache_prepare(kq_ctx* ctx) {
+  const cudaError_t e = cudaFuncSetAttribute(cache_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(kMaxMoves * 512));
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute", "cache move kernel");
+  return KQ_OK;
+}
+
+int rope_init(const kq_rope_params* p, kq_rope* out) {
+  const char* call = "kq_rope_init";
+  if (!p || !out) return fail(KQ_E_INVALID, call, "null argument");
+  if (p->rot_dim < 2 || p->rot_dim > 256 || p->rot_dim % 2 || p->layout > KQ_ROPE_HALVES)
+    return fail(KQ_E_INVALID, call, "rot_dim must be even, 2..256, and the layout a KQ_ROPE_* one");
+  if (!(p->base > 1.0) || !(p->freq_scale > 0.0) || !(p->ext_factor >= 0.0) || !(p->attn_factor > 0.0) ||
+      !std::isfinite(p->base) || !std::isfinite(p->freq_scale) || !std::isfinite(p->ext_factor) ||
+      !std::isfinite(p->attn_factor))
+    return fail(KQ_E_INVALID, call, "base must be above 1, freq_scale and attn_factor above 0, ext_factor >= 0");
+  if (p->ext_factor > 0.0 && (p->orig_ctx == 0 || !(p->beta_fast > 0.0) || !(p->beta_slow > 0.0) ||
+                              !std::isfinite(p->beta_fast) || !std::isfinite(p->beta_slow)))
+    return fail(KQ_E_INVALID, call, "ext_factor needs orig_ctx, beta_fast and beta_slow");
+  constexpr double kTwoPi = 6.283185307179586476925;
+  const double rot = p->rot_dim;
+  double low = 0, high = 0;
+  if (p->ext_factor > 0.0) {
+    // the pair that turns beta times in orig_ctx positions
+    const auto pair = [&](double beta) {
+      return rot * std::log(p->orig_ctx / (beta * kTwoPi)) / (2 * std::log(p->base));
+    };
+    low = std::max(0.0, std::floor(pair(p->beta_fast)));
+    high = std::min(rot - 1, std::ceil(pair(p->beta_slow)));
+  }
+  kq_rope r = {};
+  r.rot_dim = p->rot_dim;
+  r.layout = p->layout;
+  r.gain = static_cast<float>(p->attn_factor *
+                              (p->ext_factor > 0.0 ? 1.0 + 0.1 * std::log(1.0 / p->freq_scale) : 1.0));
+  for (uint32_t i = 0; i < p->rot_dim / 2; ++i) {
+    double f = std::pow(p->base, -2.0 * i / rot);
+    if (p->freq_factors) {
+      if (!(p->freq_factors[i] > 0.f) || !std::isfinite(p->freq_factors[i]))
+        return fail(KQ_E_INVALID, call, "freq_factors must be above 0");
+      f /= p->freq_factors[i];
+    }
+    double slow = p->freq_scale;
+    if (p->ext_factor > 0.0) {
+      const double ramp = std::min(1.0, std::max(0.0, (i - low) / std::max(0.001, high - low)));
+      const double mix = (1.0 - ramp) * p->ext_factor;
+      slow = p->freq_scale * (1.0 - mix) + mix;
+    }
+    r.turns[i] = f * slow / kTwoPi;
+  }
+  *out = r;
+  return KQ_OK;
+}
+
+int rope_apply(kq_ctx* ctx, const kq_rope_desc& d, cudaStream_t s) {
+  const char* call = "kq_rope_apply";
+  const uint32_t size = type_size(d.type);
+  if (!size) return fail(KQ_E_INVALID, call, "type must be F32, F16 or BF16");
+  if (!d.rope || !rope_ok(d.rope)) return fail(KQ_E_INVALID, call, "rope must come from kq_rope_init");
+  if (d.tokens == 0 || d.heads == 0) return KQ_OK;
+  if (!d.x || !d.y || !d.positions) return fail(KQ_E_INVALID, call, "null pointer");
+  if (d.head_dim == 0 || d.head_dim > 1024 || d.head_dim < d.rope->rot_dim)
+    return fail(KQ_E_INVALID, call, "head_dim must be rot_dim..1024");
+  if (d.tokens > 0x7fffffffu || d.heads > 0xffffffu)
+    return fail(KQ_E_INVALID, call, "too many tokens or heads");
+  if (d.x % size || d.y % size || d.positions % 4)
+    return fail(KQ_E_INVALID, call, "x and y must be aligned to their elements, positions to 4 bytes");
+  RopeArgs a = {};
+  a.rope = *d.rope;
+  a.q = reinterpret_cast<const void*>(d.x);
+  a.q_out = reinterpret_cast<void*>(d.y);
+  a.positions = reinterpret_cast<const int*>(d.positions);
+  a.q_head = d.x_head ? d.x_head : d.head_dim;
+  a.q_token = d.x_token ? d.x_token : uint64_t(d.heads) * d.head_dim;
+  a.out_head = d.y_head ? d.y_head : d.head_dim;
+  a.out_token = d.y_token ? d.y_token : uint64_t(d.heads) * d.head_dim;
+  a.nq = d.heads;
+  a.dim = d.head_dim;
+  a.rot_half = d.rope->rot_dim / 2;
+  a.err = ctx->err;
+  const bool aligned = on16(d.x) && on16(d.y) && on16(a.q_head * size) && on16(a.q_token * size) &&
+                       on16(a.out_head * size) && on16(a.out_token * size);
+  return run_rope(a, d.type, aligned, d.tokens, d.heads, ctx->sm_count, s, call);
+}
+
+int cache_write(kq_ctx* ctx, const kq_cache_write_desc& d, cudaStream_t s) {
+  const char* call = "kq_cache_write";
+  RopeArgs a = {};
+  int rc = check_cache(d.cache, call, &a.cache);
+  if (rc) return rc;
+  const uint32_t size = type_size(d.type);
+  if (!size) return fail(KQ_E_INVALID, call, "type must be F32, F16 or BF16");
+  if (d.rope && (!rope_ok(d.rope) || d.rope->rot_dim > d.cache->head_dim))
+    return fail(KQ_E_INVALID, call, "rope must come from kq_rope_init with rot_dim up to head_dim");
+  if (d.tokens == 0) return KQ_OK;
+  if (!d.k || !d.v || !d.slots || (d.rope && !d.positions) || (d.q && !d.q_out))
+    return fail(KQ_E_INVALID, call, "null pointer");
+  if (d.q && d.n_heads == 0) return fail(KQ_E_INVALID, call, "queries without heads");
+  if (d.tokens > 0x7fffffffu || d.n_heads > 0xffffffu)
+    return fail(KQ_E_INVALID, call, "too many tokens or heads");
+  if (d.q % size || d.k % size || d.v % size || d.q_out % size || d.positions % 4 || d.slots % 8)
+    return fail(KQ_E_INVALID, call, "q, k, v and q_out must be aligned to their elements, positions to 4 bytes, "
+                                    "slots to 8");
+  if (d.rope) a.rope = *d.rope;
+  a.q = reinterpret_cast<const void*>(d.q);
+  a.k = reinterpret_cast<const void*>(d.k);
+  a.v = reinterpret_cast<const void*>(d.v);
+  a.q_out = reinterpret_cast<void*>(d.q_out);
+  a.positions = reinterpret_cast<const int*>(d.positions);
+  a.slots = reinterpret_cast<const long long*>(d.slots);
+  const uint64_t dim = d.cache->head_dim;
+  const uint64_t packed = (uint64_t(d.n_heads) + 2ull * d.cache->n_kv) * dim;
+  a.q_head = a.out_head = dim;
+  a.q_token = d.q_token ? d.q_token : packed;
+  a.k_token = d.k_token ? d.k_token : packed;
+  a.v_token = d.v_token ? d.v_token : packed;
+  a.out_token = d.q_out_token ? d.q_out_token : uint64_t(d.n_heads) * dim;
+  a.nq = d.q ? d.n_heads : 0;
+  a.dim = d.cache->head_dim;
+  a.rot_half = d.rope ? d.rope->rot_dim / 2 : 0;
+  a.err = ctx->err;
+  const bool aligned = on16(d.q) && on16(d.k) && on16(d.v) && on16(d.q_out) && on16(a.q_token * size) &&
+                       on16(a.k_token * size) && on16(a.v_token * size) && on16(a.out_token * size);
+  return run_rope(a, d.type, aligned, d.tokens, a.nq + 2 * d.cache->n_kv, ctx->sm_count, s, call);
+}
+
+int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s) {
+  const char* call = "kq_cache_read";
+  CacheView c;
+  int rc = check_cache(d.cache, call, &c);
+  if (rc) return rc;
+  const uint32_t size = type_size(d.type);
+  if (!size) return fail(KQ_E_INVALID, call, "type must be F32, F16 or BF16");
+  if (d.count == 0 || (!d.k_out && !d.v_out)) return KQ_OK;
+  if (!d.slots) return fail(KQ_E_INVALID, call, "null slots");
+  const uint64_t dense = uint64_t(c.n_kv) * c.dim;
+  const uint64_t stride = d.token_stride ? d.token_stride : dense;
+  if (stride < dense) return fail(KQ_E_INVALID, call, "token_stride must be at least n_kv * head_dim");
+  if (d.k_out % size || d.v_out % size || d.slots % 8)
+    return fail(KQ_E_INVALID, call, "k_out and v_out must be aligned to their elements, slots to 8 bytes");
+  const bool wide = on16(d.k_out) && on16(d.v_out) && on16(stride * size);
+  const uint64_t total = uint64_t(d.count) * dense / 8;
+  const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>((total + kThreads - 1) / kThreads, 8u * ctx->sm_count));
+  const auto slots = reinterpret_cast<const long long*>(d.slots);
+  // a grid row for each output that is wanted
+  const auto go = [&](auto* zero) {
+    using T = std::remove_pointer_t<decltype(zero)>;
+    CacheView view = c;
+    T* k = reinterpret_cast<T*>(d.k_out);
+    T* v = reinterpret_cast<T*>(d.v_out);
+    uint32_t arrays = 2;
+    if (!k) {  // values alone, as the grid's first row
+      k = v;
+      view.k = view.v;
+      arrays = 1;
+    } else if (!v) {
+      arrays = 1;
+    }
+    cache_read_kernel<T><<<dim3(grid, arrays), kThreads, 0, s>>>(view, k, v, slots, stride, d.count, wide, ctx->err);
+  };
+  if (d.type == KQ_TYPE_F32) go(static_cast<float*>(nullptr));
+  else if (d.type == KQ_TYPE_F16) go(static_cast<__half*>(nullptr));
+  else go(static_cast<__nv_bfloat16*>(nullptr));
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", call);
+}
+
+int cache_move(kq_ctx* ctx, const kq_cache_move_desc& d, cudaStream_t s) {
+  const char* call = "kq_cache_move";
+  CacheView c;
+  int rc = check_cache(d.cache, call, &c);
+  if (rc) return rc;
+  if (d.groups == 0 || d.moves == 0) return KQ_OK;
+  if (!d.src || !d.dst || !d.starts) return fail(KQ_E_INVALID, call, "null pointer");
+  if (d.src % 8 || d.dst % 8 || d.starts % 4)
+    return fail(KQ_E_INVALID, call, "src and dst must be 8-byte aligned, starts 4-byte aligned");
+  if (d.groups > 0x7fffffffu || d.moves > 0x7fffffffu) return fail(KQ_E_INVALID, call, "too many moves");
+  cache_move_kernel<<<dim3(d.groups, c.n_kv, 2), kThreads, std::min(d.moves, kMaxMoves) * c.row, s>>>(
+      c, reinterpret_cast<const long long*>(d.src), reinterpret_cast<const long long*>(d.dst),
+      reinterpret_cast<const int*>(d.starts), d.moves, ctx->err);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", call);
+}
+
+}  // namespace kq

@@ -1,0 +1,123 @@
+// kq_cache.cuh -- the paged cache's format (include/kq.h, kq_cache) as the kernels see it: record
+// geometry, the unit permutation, the scale bytes, and activations in and out of f32.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kq.h"
+
+namespace kq {
+
+// Geometry of a cache, passed to kernels by value.
+struct CacheView {
+  uint8_t* k;
+  uint8_t* v;
+  uint64_t record;     // bytes of one head's part of a page
+  uint32_t kind;       // KQ_CACHE_*
+  uint32_t n_kv, dim, pitch;
+  uint32_t page_log2;  // log2(page_size)
+  uint32_t n_pages;
+  uint32_t row;        // bytes of one position's codes
+  uint32_t scales;     // scale bytes of one position (0: f16)
+
+  __host__ __device__ uint32_t page() const { return 1u << page_log2; }
+  // Byte offset of head h's record in page p of k or v.
+  __host__ __device__ uint64_t at(uint32_t p, uint32_t h) const { return (uint64_t(p) * n_kv + h) * record; }
+};
+
+// What the 16-byte unit index of position p is XORed with, in rows of `row` bytes.
+__host__ __device__ __forceinline__ uint32_t cache_swizzle(uint32_t p, uint32_t row) {
+  return row >= 128 ? (p & 7u) : row == 64 ? ((p >> 1) & 3u) << 1 : ((p >> 2) & 1u) << 2;
+}
+
+// Offset in a record's codes of byte `byte` of position p's row.
+__host__ __device__ __forceinline__ uint32_t cache_offset(uint32_t p, uint32_t byte, uint32_t row) {
+  return (p * row + byte) ^ (cache_swizzle(p, row) << 4);
+}
+
+// The largest code and the largest scale byte (the largest code times its scale stays below 65504).
+__host__ __device__ constexpr float cache_top(uint32_t kind) { return kind == KQ_CACHE_Q8 ? 127.f : 7.f; }
+__host__ __device__ constexpr uint32_t cache_last_scale(uint32_t kind) {
+  return kind == KQ_CACHE_Q8 ? 0xC0u : 0xE1u;  // 512 and 9216
+}
+constexpr uint32_t kScaleNan = 0xFFu;
+
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(byte << 7)));
+}
+
+// The scale byte of a block whose largest magnitude has the bits `most` (f32): the smallest value of
+// 4 significant bits not below most / top. Magnitudes compare as their bits do, NaN above infinity.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t most, uint32_t kind) {
+  if (most >= 0x7f800000u) return kScaleNan;
+  const float want = __fdiv_rn(__uint_as_float(most), cache_top(kind));
+  // normal f16 range: round the fraction up to 3 bits and rebias the exponent (127 - 15); below
+  // it the values are multiples of 2^-17
+  const uint32_t b = want >= 0x1p-14f ? ((__float_as_uint(want) + 0xFFFFFu) >> 20) - (112u << 3)
+                                      : static_cast<uint32_t>(ceilf(want * 0x1p17f));
+  return min(b, cache_last_scale(kind));
+}
+
+// ---------------------------------------------------------------- activations
+
+template <typename T>
+__device__ __forceinline__ float act_to_f32(T x);
+template <>
+__device__ __forceinline__ float act_to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float act_to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float act_to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T act_from_f32(float x);
+template <>
+__device__ __forceinline__ float act_from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half act_from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 act_from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// N consecutive elements at p, one wide access (p aligned to it) when N * sizeof(T) is 8 or 16, else
+// one by one.
+template <typename T, int N>
+__device__ __forceinline__ void load_act(const T* p, float (&v)[N]) {
+  if constexpr (N * sizeof(T) == 16) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = act_to_f32<T>(e[i]);
+  } else if constexpr (N * sizeof(T) == 8) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = act_to_f32<T>(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = act_to_f32<T>(p[i]);
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_act(T* p, const float (&v)[N]) {
+  if constexpr (N * sizeof(T) == 16) {
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = act_from_f32<T>(v[i]);
+    *reinterpret_cast<uint4*>(p) = raw;
+  } else if constexpr (N * sizeof(T) == 8) {
+    uint2 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = act_from_f32<T>(v[i]);
+    *reinterpret_cast<uint2*>(p) = raw;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = act_from_f32<T>(v[i]);
+  }
+}
+
+}  // namespace kq

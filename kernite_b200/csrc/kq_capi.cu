@@ -120,6 +120,8 @@ int kq_ctx_create(int device, kq_ctx** out) {
   if (rc == KQ_OK) rc = kq::warpmma_prepare(ctx);
   if (rc == KQ_OK) rc = kq::aux_prepare(ctx);
   if (rc == KQ_OK) rc = kq::types_prepare(ctx);
+  if (rc == KQ_OK) rc = kq::cache_prepare(ctx);
+  if (rc == KQ_OK) rc = kq::tree_prepare(ctx);
   if (rc != KQ_OK) {
     cudaFree(ctx->scratch);
     cudaFree(ctx->err);
@@ -177,6 +179,8 @@ int kq_device_error(kq_ctx* ctx) {
   const char* what = word == kq::kErrWaitFull    ? "a consumer gave up waiting for a bulk copy"
                      : word == kq::kErrWaitEmpty ? "the producer gave up waiting for a free slot"
                      : word == kq::kErrWaitPeer  ? "a wait on another GPU's flag gave up"
+                     : word == kq::kErrCacheRange
+                         ? "a slot, page, length or range of a cache call was out of its array"
                                                  : "unknown";
   return fail(KQ_E_DEVICE, "kq_device_error",
               "device error word " + std::to_string(word) + ": " + what);
@@ -364,6 +368,29 @@ uint64_t kq_attention_workspace(kq_ctx* ctx, uint32_t n_heads, uint32_t n_kv, ui
                                 uint32_t len) {
   if (!ctx || !n_kv) return 0;
   return kq::attention_workspace_bytes(ctx, n_heads, n_kv, head_dim, len ? len : 1);
+}
+
+int kq_rope_init(const kq_rope_params* params, kq_rope* out) { return kq::rope_init(params, out); }
+
+uint64_t kq_cache_bytes(const kq_cache* cache) { return cache ? kq::cache_bytes(*cache) : 0; }
+
+#define KQ_DESC_ENTRY(name, desc_type, impl)                                                \
+  int name(kq_ctx* ctx, const desc_type* desc, kq_stream stream) {                          \
+    if (!ctx || !desc) return fail(KQ_E_INVALID, #name, "null ctx or descriptor");         \
+    kq::DeviceScope scope;                                                                  \
+    int rc = scope.enter(ctx);                                                              \
+    if (rc) return rc;                                                                      \
+    return kq::impl(ctx, *desc, static_cast<cudaStream_t>(stream));                         \
+  }
+
+KQ_DESC_ENTRY(kq_rope_apply, kq_rope_desc, rope_apply)
+KQ_DESC_ENTRY(kq_cache_write, kq_cache_write_desc, cache_write)
+KQ_DESC_ENTRY(kq_cache_read, kq_cache_read_desc, cache_read)
+KQ_DESC_ENTRY(kq_cache_move, kq_cache_move_desc, cache_move)
+KQ_DESC_ENTRY(kq_attention_tree, kq_tree_desc, attention_tree)
+
+uint64_t kq_tree_workspace(kq_ctx* ctx, const kq_tree_desc* desc) {
+  return ctx && desc ? kq::tree_workspace_bytes(ctx, *desc) : 0;
 }
 
 // The warp-MMA kernels' cubin, embedded at build time (kernite_b200/build.py).

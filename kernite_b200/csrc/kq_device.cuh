@@ -21,6 +21,7 @@ enum : unsigned {
   kErrWaitFull = 1,   // a consumer gave up waiting for a stage's bulk copy
   kErrWaitEmpty = 2,  // the producer gave up waiting for consumers to free a stage
   kErrWaitPeer = 3,   // a wait on another GPU's flag gave up
+  kErrCacheRange = 4, // a slot, page, length or range read on the device is out of its array
 };
 
 // About two seconds: far above any legitimate wait of these kernels (microseconds).

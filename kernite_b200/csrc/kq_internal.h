@@ -97,4 +97,21 @@ int attention_decode(kq_ctx* ctx, uint64_t out, uint64_t q, uint64_t k_cache, ui
                      uint32_t nh, uint32_t nkv, uint32_t d, uint32_t len, uint64_t workspace,
                      uint64_t workspace_bytes, cudaStream_t s);
 
+struct CacheView;
+int cache_prepare(kq_ctx* ctx);
+// The geometry of a cache (KQ_E_INVALID when it is not a valid one); check_cache also wants its
+// addresses and says what is wrong.
+int cache_view(const kq_cache* c, CacheView* out);
+int check_cache(const kq_cache* c, const char* call, CacheView* out);
+uint64_t cache_bytes(const kq_cache& c);
+int rope_init(const kq_rope_params* p, kq_rope* out);
+int rope_apply(kq_ctx* ctx, const kq_rope_desc& d, cudaStream_t s);
+int cache_write(kq_ctx* ctx, const kq_cache_write_desc& d, cudaStream_t s);
+int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s);
+int cache_move(kq_ctx* ctx, const kq_cache_move_desc& d, cudaStream_t s);
+
+int tree_prepare(kq_ctx* ctx);
+uint64_t tree_workspace_bytes(kq_ctx* ctx, const kq_tree_desc& d);
+int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s);
+
 }  // namespace kq

@@ -1,0 +1,8 @@
+// kq_tree_f16.cu -- the attention of drafted tokens over caches of kind F16 (kq_tree.cuh).
+#include "kq_tree.cuh"
+
+namespace kq {
+namespace tree {
+KQ_TREE_KIND(KQ_CACHE_F16)
+}  // namespace tree
+}  // namespace kq
