@@ -17,11 +17,11 @@ cudaError_t prepare_kind<KQ_CACHE_Q8>();
 template <>
 cudaError_t prepare_kind<KQ_CACHE_Q4>();
 template <>
-cudaError_t launch_kind<KQ_CACHE_F16>(const TreeArgs&, bool, uint32_t, cudaStream_t);
+cudaError_t launch_kind<KQ_CACHE_F16>(const TreeArgs&, bool, bool, uint32_t, cudaStream_t);
 template <>
-cudaError_t launch_kind<KQ_CACHE_Q8>(const TreeArgs&, bool, uint32_t, cudaStream_t);
+cudaError_t launch_kind<KQ_CACHE_Q8>(const TreeArgs&, bool, bool, uint32_t, cudaStream_t);
 template <>
-cudaError_t launch_kind<KQ_CACHE_Q4>(const TreeArgs&, bool, uint32_t, cudaStream_t);
+cudaError_t launch_kind<KQ_CACHE_Q4>(const TreeArgs&, bool, bool, uint32_t, cudaStream_t);
 }  // namespace tree
 
 namespace {
@@ -30,7 +30,9 @@ constexpr uint32_t kMaxTreeGroup = 64;
 
 struct Plan {
   bool split;      // f32 activations: operands as sums of two f16
+  bool wide;       // the tcgen05 kernel, else the warp-MMA one
   uint32_t rows;   // rows an item
+  uint32_t tile;   // positions a tile
   uint32_t ctas;
   uint64_t bytes;  // workspace
 };
@@ -50,10 +52,12 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   if (!std::isfinite(d.scale) || d.scale < 0.f) return fail(KQ_E_INVALID, call, "scale must be finite and not negative");
   Plan p = {};
   p.split = d.type == KQ_TYPE_F32;
-  p.rows = p.split ? 8 : 16;
   const uint32_t group = d.n_heads / c.n_kv;
+  p.wide = d.max_drafts * group > (p.split ? 8u : 16u);
+  p.rows = p.wide ? (p.split ? 64 : 128) : p.split ? 8 : 16;
+  p.tile = p.wide && c.pitch == 256 ? 64 : 128;
   const uint64_t row_tiles = (uint64_t(d.max_drafts) * group + p.rows - 1) / p.rows;
-  const uint64_t tiles = (uint64_t(d.max_len) + tree::kTile - 1) / tree::kTile;
+  const uint64_t tiles = (uint64_t(d.max_len) + p.tile - 1) / p.tile;
   const uint64_t items = uint64_t(d.n_seq) * c.n_kv * row_tiles;
   if (items > 0x7fffffffu) return fail(KQ_E_INVALID, call, "too many sequences, heads and drafts");
   p.ctas = static_cast<uint32_t>(std::min<uint64_t>(ctx->sm_count, std::max<uint64_t>(1, items * tiles)));
@@ -62,11 +66,12 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   return KQ_OK;
 }
 
-template <uint32_t ROWS>
-void launch_join(const tree::TreeArgs& a, uint32_t blocks, uint32_t ctas, cudaStream_t s) {
-  if (a.c.pitch == 64) tree::join_kernel<ROWS, 64><<<blocks, 128, 0, s>>>(a, ctas);
-  else if (a.c.pitch == 128) tree::join_kernel<ROWS, 128><<<blocks, 128, 0, s>>>(a, ctas);
-  else tree::join_kernel<ROWS, 256><<<blocks, 128, 0, s>>>(a, ctas);
+template <uint32_t ROWS, uint32_t TW256>
+void launch_join(const tree::TreeArgs& a, uint32_t items, uint32_t ctas, cudaStream_t s) {
+  const dim3 grid(items, ROWS / 8);
+  if (a.c.pitch == 64) tree::join_kernel<ROWS, 64, 128><<<grid, 256, 0, s>>>(a, ctas);
+  else if (a.c.pitch == 128) tree::join_kernel<ROWS, 128, 128><<<grid, 256, 0, s>>>(a, ctas);
+  else tree::join_kernel<ROWS, 256, TW256><<<grid, 256, 0, s>>>(a, ctas);
 }
 
 bool on16(uint64_t bytes) { return bytes % 16 == 0; }
@@ -133,13 +138,16 @@ int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {
   a.max_pages = d.max_pages;
   a.type = d.type;
   a.err = ctx->err;
-  cudaError_t e = a.c.kind == KQ_CACHE_F16  ? tree::launch_kind<KQ_CACHE_F16>(a, p.split, p.ctas, s)
-                  : a.c.kind == KQ_CACHE_Q8 ? tree::launch_kind<KQ_CACHE_Q8>(a, p.split, p.ctas, s)
-                                            : tree::launch_kind<KQ_CACHE_Q4>(a, p.split, p.ctas, s);
+  const auto launch = a.c.kind == KQ_CACHE_F16  ? tree::launch_kind<KQ_CACHE_F16>
+                      : a.c.kind == KQ_CACHE_Q8 ? tree::launch_kind<KQ_CACHE_Q8>
+                                                : tree::launch_kind<KQ_CACHE_Q4>;
+  cudaError_t e = launch(a, p.split, p.wide, p.ctas, s);
   if (e != cudaSuccess) return cuda_fail(e, "cudaLaunchKernel", call);
-  const uint32_t blocks = d.n_seq * a.c.n_kv * ((d.max_drafts * a.group + p.rows - 1) / p.rows);
-  if (p.rows == 8) launch_join<8>(a, blocks, p.ctas, s);
-  else launch_join<16>(a, blocks, p.ctas, s);
+  const uint32_t items = d.n_seq * a.c.n_kv * ((d.max_drafts * a.group + p.rows - 1) / p.rows);
+  if (p.rows == 8) launch_join<8, 128>(a, items, p.ctas, s);
+  else if (p.rows == 16) launch_join<16, 128>(a, items, p.ctas, s);
+  else if (p.rows == 64) launch_join<64, 64>(a, items, p.ctas, s);
+  else launch_join<128, 64>(a, items, p.ctas, s);
   e = cudaGetLastError();
   return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", "tree attention join");
 }

@@ -4,7 +4,7 @@
 //
 // The work. An item is (sequence, key/value head, tile of rows): a row is a drafted token with one of
 // the head's group of query heads, r = token * group + head, so that a position's key and value serve
-// all of them. An item's positions come in tiles of kTile. The tiles of all items, in order, are cut
+// all of them. An item's positions come in tiles of TW (64 or 128). The tiles of all items, in order, are cut
 // into equal ranges, one a CTA, whatever the sequences' lengths: a CTA does the end of one item, some
 // whole ones and the start of another. Whole ones are written out; parts leave (max, sum, unnormalised
 // output) in the workspace, two slots a CTA at most, and the join kernel finds by the same arithmetic
@@ -22,7 +22,7 @@
 namespace kq {
 namespace tree {
 
-constexpr uint32_t kTile = 128;      // positions a tile
+constexpr uint32_t kTile = 128;      // positions a tile of the warp-MMA kernel
 constexpr uint32_t kMaxDrafts = 64;  // bits of a mask word
 
 struct TreeArgs {
@@ -65,11 +65,14 @@ __device__ __forceinline__ uint32_t row_tiles(const TreeArgs& a, const Seq& s) {
   return (s.drafts * a.group + ROWS - 1) / ROWS;
 }
 
-__device__ __forceinline__ uint32_t position_tiles(const Seq& s) { return (s.length() + kTile - 1) / kTile; }
+template <uint32_t TW>
+__device__ __forceinline__ uint32_t position_tiles(const Seq& s) {
+  return (s.length() + TW - 1) / TW;
+}
 
-template <uint32_t ROWS>
+template <uint32_t ROWS, uint32_t TW>
 __device__ __forceinline__ uint64_t seq_work(const TreeArgs& a, const Seq& s) {
-  return s.drafts ? uint64_t(position_tiles(s)) * a.c.n_kv * row_tiles<ROWS>(a, s) : 0;
+  return s.drafts ? uint64_t(position_tiles<TW>(s)) * a.c.n_kv * row_tiles<ROWS>(a, s) : 0;
 }
 
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
@@ -79,10 +82,10 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 }
 
 // The tiles of sequences [0, n). Called by whole warps.
-template <uint32_t ROWS>
+template <uint32_t ROWS, uint32_t TW>
 __device__ __forceinline__ uint64_t work_before(const TreeArgs& a, uint32_t n) {
   uint64_t w = 0;
-  for (uint32_t s = threadIdx.x % 32; s < n; s += 32) w += seq_work<ROWS>(a, load_seq(a, s));
+  for (uint32_t s = threadIdx.x % 32; s < n; s += 32) w += seq_work<ROWS, TW>(a, load_seq(a, s));
   return warp_sum(w);
 }
 
@@ -94,12 +97,12 @@ struct Place {
 };
 
 // The place of tile `at` of the whole work. Called by whole warps, at < total.
-template <uint32_t ROWS>
+template <uint32_t ROWS, uint32_t TW>
 __device__ __forceinline__ Place locate(const TreeArgs& a, uint64_t at) {
   const uint32_t lane = threadIdx.x % 32;
   Place p = {};
   for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
-    const uint64_t w = s0 + lane < a.n_seq ? seq_work<ROWS>(a, load_seq(a, s0 + lane)) : 0;
+    const uint64_t w = s0 + lane < a.n_seq ? seq_work<ROWS, TW>(a, load_seq(a, s0 + lane)) : 0;
     uint64_t upto = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -112,7 +115,7 @@ __device__ __forceinline__ Place locate(const TreeArgs& a, uint64_t at) {
       p.s = s0 + who;
       const uint64_t rest = at - __shfl_sync(0xffffffffu, upto - w, who);
       p.seq = load_seq(a, p.s);
-      const uint32_t pt = position_tiles(p.seq), rt = row_tiles<ROWS>(a, p.seq);
+      const uint32_t pt = position_tiles<TW>(p.seq), rt = row_tiles<ROWS>(a, p.seq);
       p.tile = static_cast<uint32_t>(rest % pt);
       const uint64_t item = rest / pt;
       p.rows = static_cast<uint32_t>(item % rt);
@@ -298,13 +301,13 @@ struct PageWindow {
   uint32_t id;
 };
 
-template <class S>
+template <class S, uint32_t TW>
 __device__ __forceinline__ void produce_tile(const TreeArgs& a, const Place& p, const uint8_t* src, uint32_t dst,
                                              uint32_t bar, PageWindow& w) {
   const uint32_t lane = threadIdx.x % 32;
-  const uint32_t seg_log2 = min(a.c.page_log2, 7u), seg = 1u << seg_log2;
-  const uint32_t base = p.tile * kTile;
-  const uint32_t n = (min(kTile, p.seq.length() - base) + seg - 1) >> seg_log2;
+  const uint32_t seg_log2 = min(a.c.page_log2, TW == 128 ? 7u : 6u), seg = 1u << seg_log2;
+  const uint32_t base = p.tile * TW;
+  const uint32_t n = (min(TW, p.seq.length() - base) + seg - 1) >> seg_log2;
   const uint32_t first = base >> a.c.page_log2;
   const uint32_t pages = ((n << seg_log2) + (1u << a.c.page_log2) - 1) >> a.c.page_log2;
   if (w.s != p.s || first < w.base || first + pages > w.base + 32) {
@@ -326,7 +329,7 @@ __device__ __forceinline__ void produce_tile(const TreeArgs& a, const Place& p, 
   const uint32_t mine = __shfl_sync(0xffffffffu, w.id, ((base + lane * seg) >> a.c.page_log2) - w.base);
   if (lane < n) {
     const uint8_t* rec = src + a.c.at(mine, p.head);
-    if (a.c.page_log2 <= 7) {
+    if (a.c.page_log2 == seg_log2) {
       bulk_g2s(dst + lane * seg * row, rec, seg * row, bar);
     } else {
       const uint32_t at = base & (a.c.page() - 1);
@@ -524,19 +527,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     fence_mbar_init();
   }
   __syncthreads();
-  const uint64_t total = work_before<ROWS>(a, a.n_seq);
+  const uint64_t total = work_before<ROWS, kTile>(a, a.n_seq);
   const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(gridDim.x), total));
   if (blockIdx.x >= ctas) return;
   uint64_t at = range_start(total, blockIdx.x, ctas);
   const uint64_t end = range_start(total, blockIdx.x + 1, ctas);
-  Place p = locate<ROWS>(a, at);
+  Place p = locate<ROWS, kTile>(a, at);
   uint32_t it = 0;    // slots used so far: tiles of keys and of values in turn
   bool live = true;   // no wait has given up
 
   if (warp == kWarps) {
     PageWindow window = {0xffffffffu, 0, 0};
     while (at < end) {
-      const uint32_t tiles = position_tiles(p.seq);
+      const uint32_t tiles = position_tiles<kTile>(p.seq);
       for (; p.tile < tiles && at < end; ++p.tile, ++at) {
 #pragma unroll 1
         for (uint32_t kv = 0; kv < 2; ++kv, ++it) {
@@ -546,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
             live = false;
           }
           live = __all_sync(0xffffffffu, live);
-          if (live) produce_tile<S>(a, p, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bars + 16 * slot, window);
+          if (live) produce_tile<S, kTile>(a, p, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bars + 16 * slot, window);
         }
       }
       if (at < end) next_item<ROWS>(a, p);
@@ -634,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
       for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    const uint32_t tiles = position_tiles(p.seq), first_tile = p.tile;
+    const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
     for (; p.tile < tiles && at < end; ++p.tile, ++at, it += 2) {
       const uint32_t base = p.tile * kTile, left = p.seq.length() - base;  // positions left in the cache
       const uint32_t p0 = warp * 16;
@@ -798,60 +801,60 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
 
 // ---------------------------------------------------------------- the join of split items
 
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over an item's parts, in their order. A CTA an
-// item (sequence, head, row tile of the largest tree); items that one CTA did whole are done.
-template <uint32_t ROWS, uint32_t D>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TreeArgs a, uint32_t grid) {
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over an item's parts, in their order. Grid: (items
+// of a largest tree a sequence and head, eight rows each); items that one CTA did whole are done.
+template <uint32_t ROWS, uint32_t D, uint32_t TW>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeArgs a, uint32_t grid) {
   const uint32_t max_rt = (a.max_drafts * a.group + ROWS - 1) / ROWS;
   const uint32_t rt = blockIdx.x % max_rt, head = blockIdx.x / max_rt % a.c.n_kv;
   const uint32_t s = blockIdx.x / max_rt / a.c.n_kv;
   const Seq seq = load_seq(a, s);
-  const uint32_t rts = row_tiles<ROWS>(a, seq), tiles = position_tiles(seq);
-  if (seq.drafts == 0 || rt >= rts) return;
-  const uint64_t before = work_before<ROWS>(a, s);
-  const uint64_t total = before + seq_work<ROWS>(a, seq) + [&] {
-    uint64_t w = 0;
-    for (uint32_t i = s + 1 + threadIdx.x % 32; i < a.n_seq; i += 32) w += seq_work<ROWS>(a, load_seq(a, i));
-    return warp_sum(w);
-  }();
+  const uint32_t rts = row_tiles<ROWS>(a, seq), tiles = position_tiles<TW>(seq);
+  const uint32_t row = blockIdx.y * 8 + threadIdx.x / 32, rr = rt * ROWS + row;
+  if (rr >= seq.drafts * a.group) return;
+  uint64_t before = 0, total = 0;
+  for (uint32_t i = threadIdx.x % 32; i < a.n_seq; i += 32) {
+    const uint64_t w = seq_work<ROWS, TW>(a, load_seq(a, i));
+    total += w;
+    before += i < s ? w : 0;
+  }
+  before = warp_sum(before);
+  total = warp_sum(total);
   const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(grid), total));
   const uint64_t first = before + (uint64_t(head) * rts + rt) * tiles;
   const uint32_t c0 = range_owner(total, first, ctas), c1 = range_owner(total, first + tiles - 1, ctas);
   if (c0 == c1) return;
-  // the first part lies in its CTA's slot 1 (the item starts there); unless the CTA starts with it,
-  // where it is slot 1 as well: slot 0 is for items that an earlier CTA began
+  // slot 1 of the CTA the item starts in; slot 0 of the others, which an earlier one began
   const uint64_t stride = part_floats(ROWS, D);
   const auto slot = [&](uint32_t c) { return a.part + (uint64_t(c) * 2 + (c == c0 ? 1 : 0)) * stride; };
-  const uint32_t rows = min(ROWS, seq.drafts * a.group - rt * ROWS);
-  for (uint32_t row = threadIdx.x / 32; row < rows; row += 4) {
-    float mx = -INFINITY;
-    for (uint32_t c = c0; c <= c1; ++c) mx = fmaxf(mx, slot(c)[ROWS * D + row]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float den = 0.f, v[D / 32] = {};
-    for (uint32_t c = c0; c <= c1; ++c) {
-      const float* part = slot(c);
-      const float f = exp2f(part[ROWS * D + row] - ref);
-      den = fmaf(f, part[ROWS * (D + 1) + row], den);
+  const uint32_t lane = threadIdx.x % 32;
+  float mx = -INFINITY;
+  for (uint32_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, slot(c)[ROWS * D + row]);
 #pragma unroll
-      for (uint32_t i = 0; i < D / 32; ++i) v[i] = fmaf(f, part[row * D + threadIdx.x % 32 + 32 * i], v[i]);
-    }
-    const float inv = den == 0.f ? 0.f : 1.f / den;
-    const uint32_t rr = rt * ROWS + row;
-    const uint64_t to = (seq.first + rr / a.group) * a.out_token +
-                        uint64_t(head * a.group + rr % a.group) * a.c.dim;
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float den = 0.f, v[D / 32] = {};
+#pragma unroll 4
+  for (uint32_t c = c0; c <= c1; ++c) {
+    const float* part = slot(c);
+    const float f = exp2f(part[ROWS * D + row] - ref);
+    den = fmaf(f, part[ROWS * (D + 1) + row], den);
 #pragma unroll
-    for (uint32_t i = 0; i < D / 32; ++i) {
-      const uint32_t e = threadIdx.x % 32 + 32 * i;
-      if (e < a.c.dim) store_one(a.out, to + e, v[i] * inv, a.type);
-    }
+    for (uint32_t i = 0; i < D / 32; ++i) v[i] = fmaf(f, part[row * D + lane + 32 * i], v[i]);
   }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const uint64_t to = (seq.first + rr / a.group) * a.out_token +
+                      uint64_t(head * a.group + rr % a.group) * a.c.dim;
+#pragma unroll
+  for (uint32_t i = 0; i < D / 32; ++i)
+    if (lane + 32 * i < a.c.dim) store_one(a.out, to + lane + 32 * i, v[i] * inv, a.type);
 }
 
-// Prepares, and launches, the warp-MMA kernel of one kind of cache (pitch 64, 128 or 256).
+// Prepares, and launches, the kernels of one kind of cache.
 template <uint32_t KIND>
 cudaError_t prepare_kind();
 template <uint32_t KIND>
-cudaError_t launch_kind(const TreeArgs& a, bool split, uint32_t ctas, cudaStream_t s);
+cudaError_t launch_kind(const TreeArgs& a, bool split, bool wide, uint32_t ctas, cudaStream_t s);
 
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 cudaError_t prepare_one() {
@@ -864,26 +867,6 @@ cudaError_t launch_one(const TreeArgs& a, uint32_t ctas, cudaStream_t s) {
   tree_kernel<KIND, D, SPLIT><<<ctas, kThreads, Smem<KIND, D>::kBytes, s>>>(a);
   return cudaGetLastError();
 }
-
-#define KQ_TREE_KIND(KIND)                                                                       \
-  template <>                                                                                    \
-  cudaError_t prepare_kind<KIND>() {                                                             \
-    cudaError_t e = prepare_one<KIND, 64, false>();                                              \
-    if (e == cudaSuccess) e = prepare_one<KIND, 64, true>();                                     \
-    if (e == cudaSuccess) e = prepare_one<KIND, 128, false>();                                   \
-    if (e == cudaSuccess) e = prepare_one<KIND, 128, true>();                                    \
-    if (e == cudaSuccess) e = prepare_one<KIND, 256, false>();                                   \
-    if (e == cudaSuccess) e = prepare_one<KIND, 256, true>();                                    \
-    return e;                                                                                    \
-  }                                                                                              \
-  template <>                                                                                    \
-  cudaError_t launch_kind<KIND>(const TreeArgs& a, bool split, uint32_t ctas, cudaStream_t s) {  \
-    if (a.c.pitch == 64)                                                                         \
-      return split ? launch_one<KIND, 64, true>(a, ctas, s) : launch_one<KIND, 64, false>(a, ctas, s);    \
-    if (a.c.pitch == 128)                                                                        \
-      return split ? launch_one<KIND, 128, true>(a, ctas, s) : launch_one<KIND, 128, false>(a, ctas, s);  \
-    return split ? launch_one<KIND, 256, true>(a, ctas, s) : launch_one<KIND, 256, false>(a, ctas, s);    \
-  }
 
 }  // namespace tree
 }  // namespace kq

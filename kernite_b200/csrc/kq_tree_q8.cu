@@ -1,5 +1,6 @@
-// kq_tree_q8.cu -- the attention of drafted tokens over caches of kind Q8 (kq_tree.cuh).
-#include "kq_tree.cuh"
+// kq_tree_q8.cu -- the attention of drafted tokens over caches of kind Q8 (kq_tree.cuh,
+// kq_treewide.cuh).
+#include "kq_treewide.cuh"
 
 namespace kq {
 namespace tree {
