@@ -322,7 +322,7 @@ int kq_rope_apply(kq_ctx* ctx, const kq_rope_desc* desc, kq_stream stream);
  * as codes c (-127..127 or -7..7) and one scale byte b: the scale is the f16 with bits b << 7 (5
  * exponent, 3 fraction bits), the smallest one with scale * 127 (or 7) >= the block's largest
  * magnitude, c = the nearest integer to x / scale (ties to even), the value c * scale, which f16
- * holds exactly. Magnitudes above 65024 (Q8) or 64512 (Q4) saturate; a block with an infinity or a
+ * holds exactly. Magnitudes above 7112 (Q8) or 6272 (Q4) saturate; a block with an infinity or a
  * NaN reads back as NaN.
  * Layout: [page][kv head][record]; a record is page_size rows of row_bytes codes, then (Q8, Q4)
  * page_size x pitch / 32 scale bytes. pitch = head_dim rounded up to 64, 128 or 256 (elements past

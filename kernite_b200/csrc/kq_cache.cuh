@@ -37,10 +37,12 @@ __host__ __device__ __forceinline__ uint32_t cache_offset(uint32_t p, uint32_t b
   return (p * row + byte) ^ (cache_swizzle(p, row) << 4);
 }
 
-// The largest code and the largest scale byte (the largest code times its scale stays below 65504).
+// The largest code and the largest scale byte. A kernel turns a code u (stored with its offset) into
+// its value by one fused multiply-add, (1024 + u) * scale - (1024 + offset) * scale, exact as long as
+// the subtrahend is an f16: 1152 * 56 and 72 * 896 are the largest such.
 __host__ __device__ constexpr float cache_top(uint32_t kind) { return kind == KQ_CACHE_Q8 ? 127.f : 7.f; }
 __host__ __device__ constexpr uint32_t cache_last_scale(uint32_t kind) {
-  return kind == KQ_CACHE_Q8 ? 0xC0u : 0xE1u;  // 512 and 9216
+  return kind == KQ_CACHE_Q8 ? 0xA6u : 0xC6u;  // 56 and 896
 }
 constexpr uint32_t kScaleNan = 0xFFu;
 

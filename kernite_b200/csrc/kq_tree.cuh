@@ -162,7 +162,15 @@ __device__ __forceinline__ bool sees(unsigned long long bits, uint32_t pos, cons
 }
 
 __device__ __forceinline__ unsigned long long mask_bits(const TreeArgs& a, const Seq& s, uint32_t t) {
-  return a.mask ? a.mask[s.first + t] : (2ull << t) - 1ull;
+  // without a mask the drafts up to t; bits of drafts that are not there do not count
+  return (a.mask ? a.mask[s.first + t] : (2ull << t) - 1ull) & ~0ull >> (kMaxDrafts - s.drafts);
+}
+
+// Bit i: whether position base + c + i is seen, base + c = the prefix's end + from (i < 32).
+__device__ __forceinline__ uint32_t seen_word(unsigned long long bits, int from) {
+  if (from <= -32) return ~0u;
+  if (from >= static_cast<int>(kMaxDrafts)) return 0u;
+  return from < 0 ? static_cast<uint32_t>(bits << -from) | ((1u << -from) - 1u) : static_cast<uint32_t>(bits >> from);
 }
 
 __device__ __forceinline__ float load_one(const void* p, uint64_t i, uint32_t type) {
@@ -208,14 +216,42 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 __device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
-// (1024 + u0, 1024 + u1) as f16 bits -> (u - offset) * scale, exact.
-__device__ __forceinline__ uint32_t decode2(uint32_t magic, uint32_t offset2, uint32_t scale2) {
-  return h2(__hmul2(__hsub2(as_h2(magic), as_h2(offset2)), as_h2(scale2)));
+// 2^x, to 2^-22 of it; results below f32's normal range are zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
+// Codes as f16 pairs: a code under the exponent of 1024 is 1024 + u (8 bits) or 1024 + 16 u (a nibble
+// at bits 4..7), and one fused multiply-add gives (u - offset) * scale, exactly (kq_cache.cuh).
 constexpr uint32_t kMagic = 0x64646464u;
-constexpr uint32_t kOffset8 = 0x64806480u;  // 1024 + 128
-constexpr uint32_t kOffset4 = 0x64086408u;  // 1024 + 8
+
+// A block's scale for decode2: the factor and the subtrahend, twice each.
+struct Scale2 {
+  __half2 by, minus;
+};
+
+template <uint32_t KIND>
+__device__ __forceinline__ Scale2 scale2(uint32_t low_byte, uint32_t high_byte) {
+  const __half2 s = as_h2(low_byte << 7 | high_byte << 23);
+  if constexpr (KIND == KQ_CACHE_Q4)
+    return {__hmul2(s, __float2half2_rn(0.0625f)), __hmul2(s, __float2half2_rn(-72.f))};
+  else
+    return {s, __hmul2(s, __float2half2_rn(-1152.f))};
+}
+
+__device__ __forceinline__ uint32_t decode2(uint32_t magic, const Scale2& s) {
+  return h2(__hfma2(as_h2(magic), s.by, s.minus));
+}
+
+// Nibble e (0..3) of both halves of v moved to bits 4..7.
+__device__ __forceinline__ constexpr uint32_t nibble_up(uint32_t v, uint32_t e) {
+  return e == 0 ? v << 4 : v >> (4 * e - 4);
+}
+
+// The nibbles at bits 4..7 of both halves of v.
+__device__ __forceinline__ uint32_t nibbles(uint32_t v) { return (v & 0x00f000f0u) | (kMagic & 0xff00ff00u); }
 
 // hi + lo of a pair of f32: f16(x), f16(x - f16(x)).
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -373,17 +409,17 @@ __device__ __forceinline__ void key_fragments(const TileView<Shape<KIND, D>>& ti
         b[2 * j + k][1] = w[2 * k + 1];
       }
     } else {
-      const uint32_t s2 = lds_u8(tile.scale(p) + S::EK * (t + 4 * j) / 32) * 0x00800080u;
+      const uint32_t byte = lds_u8(tile.scale(p) + S::EK * (t + 4 * j) / 32);
+      const Scale2 s2 = scale2<KIND>(byte, byte);
 #pragma unroll
       for (uint32_t k = 0; k < S::EK / 4; ++k) {
         uint32_t lo, hi;
         if constexpr (KIND == KQ_CACHE_Q8) {
-          lo = decode2(prmt(w[k], kMagic, 0x4140), kOffset8, s2);
-          hi = decode2(prmt(w[k], kMagic, 0x4342), kOffset8, s2);
+          lo = decode2(prmt(w[k], kMagic, 0x4140), s2);
+          hi = decode2(prmt(w[k], kMagic, 0x4342), s2);
         } else {
-          const uint32_t v = w[k / 2] >> (8 * (k % 2));
-          lo = decode2((v & 0x000f000fu) | (kMagic & 0xff00ff00u), kOffset4, s2);
-          hi = decode2(((v >> 4) & 0x000f000fu) | (kMagic & 0xff00ff00u), kOffset4, s2);
+          lo = decode2(nibbles(nibble_up(w[k / 2], 2 * (k % 2))), s2);
+          hi = decode2(nibbles(nibble_up(w[k / 2], 2 * (k % 2) + 1)), s2);
         }
         b[j * (S::EK / 4) + k][0] = lo;
         b[j * (S::EK / 4) + k][1] = hi;
@@ -413,7 +449,7 @@ __device__ __forceinline__ void value_product(const TileView<Shape<KIND, D>>& ti
 #pragma unroll
   for (uint32_t jj = 0; jj < D / 8 / S::EV; ++jj) {
     uint32_t w[4][B / 4];
-    uint32_t s2[2] = {0, 0};
+    uint32_t byte[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       lds_words<B>(tile.code(p[i], B * (pg + 8 * jj)), w[i]);
@@ -423,11 +459,11 @@ __device__ __forceinline__ void value_product(const TileView<Shape<KIND, D>>& ti
           for (uint32_t k = 0; k < B / 4; ++k) w[i][k] = p[i] < left ? finite_or_zero(w[i][k]) : 0u;
         }
       } else {
-        uint32_t s = lds_u8(tile.scale(p[i]) + S::EV * (pg + 8 * jj) / 32);
-        if constexpr (EDGE) s = p[i] < left && s < 0xf8u ? s : 0u;
-        s2[i / 2] |= s << (7 + 16 * (i % 2));
+        byte[i] = lds_u8(tile.scale(p[i]) + S::EV * (pg + 8 * jj) / 32);
+        if constexpr (EDGE) byte[i] = p[i] < left && byte[i] < 0xf8u ? byte[i] : 0u;
       }
     }
+    const Scale2 s2[2] = {scale2<KIND>(byte[0], byte[1]), scale2<KIND>(byte[2], byte[3])};
 #pragma unroll
     for (uint32_t k = 0; k < B / 4; ++k) {
       // operand pairs (position p[0], p[1]) and (p[2], p[3]) of each element of word k
@@ -439,10 +475,10 @@ __device__ __forceinline__ void value_product(const TileView<Shape<KIND, D>>& ti
         for (uint32_t half = 0; half < 2; ++half) {
           const uint32_t x = prmt(w[0][k], w[1][k], half ? 0x7362 : 0x5140);
           const uint32_t y = prmt(w[2][k], w[3][k], half ? 0x7362 : 0x5140);
-          mma16816(o[jj * S::EV + 4 * k + 2 * half], a, decode2(prmt(x, kMagic, 0x4140), kOffset8, s2[0]),
-                   decode2(prmt(y, kMagic, 0x4140), kOffset8, s2[1]));
-          mma16816(o[jj * S::EV + 4 * k + 2 * half + 1], a, decode2(prmt(x, kMagic, 0x4342), kOffset8, s2[0]),
-                   decode2(prmt(y, kMagic, 0x4342), kOffset8, s2[1]));
+          mma16816(o[jj * S::EV + 4 * k + 2 * half], a, decode2(prmt(x, kMagic, 0x4140), s2[0]),
+                   decode2(prmt(y, kMagic, 0x4140), s2[1]));
+          mma16816(o[jj * S::EV + 4 * k + 2 * half + 1], a, decode2(prmt(x, kMagic, 0x4342), s2[0]),
+                   decode2(prmt(y, kMagic, 0x4342), s2[1]));
         }
       } else {
 #pragma unroll
@@ -451,9 +487,8 @@ __device__ __forceinline__ void value_product(const TileView<Shape<KIND, D>>& ti
           const uint32_t y = prmt(w[2][k], w[3][k], odd ? 0x7632 : 0x5410);
 #pragma unroll
           for (uint32_t e = 0; e < 4; ++e)
-            mma16816(o[jj * S::EV + 8 * k + 2 * e + odd], a,
-                     decode2((x >> (4 * e) & 0x000f000fu) | (kMagic & 0xff00ff00u), kOffset4, s2[0]),
-                     decode2((y >> (4 * e) & 0x000f000fu) | (kMagic & 0xff00ff00u), kOffset4, s2[1]));
+            mma16816(o[jj * S::EV + 8 * k + 2 * e + odd], a, decode2(nibbles(nibble_up(x, e)), s2[0]),
+                     decode2(nibbles(nibble_up(y, e)), s2[1]));
         }
       }
     }
@@ -711,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
           const float ref = m[half] == -INFINITY ? 0.f : m[half] - kLift;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float w0 = exp2f(c[j][2 * half] - ref), w1 = exp2f(c[j][2 * half + 1] - ref);
+            const float w0 = exp2_fast(c[j][2 * half] - ref), w1 = exp2_fast(c[j][2 * half + 1] - ref);
             if constexpr (SPLIT) {
               split2(w0, w1, pa[2 * j], pa[2 * j + 1]);
               l[0] += w0 + w1;

@@ -58,25 +58,77 @@ struct WideBars {
   __device__ uint32_t drained() const { return base + 240; }
 };
 
+// True in one lane of a converged warp. The compiler knows that one thread runs what this guards, which a
+// comparison of lane numbers does not tell it: a tcgen05.mma then costs its own time to issue instead
+// of about 200 cycles (measured, M = 128, N = 16..128).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b32 r;\n\telect.sync r|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(one));
+  return one != 0;
+}
+
 // One bounded wait of a warp: false (for good) once any wait of it has given up.
 __device__ __forceinline__ void wait_or_die(bool& live, uint32_t bar, uint32_t parity, unsigned* err, unsigned code) {
-  if (live && !mbar_wait(bar, parity)) {
+  if (live && !mbar_wait_sleep(bar, parity)) {
     report_error(err, code);
     live = false;
   }
   live = __all_sync(0xffffffffu, live);
 }
 
-// Eight consecutive elements (one core-matrix row) of a position from its codes.
-__device__ __forceinline__ uint4 decode_q8(uint32_t w0, uint32_t w1, uint32_t s2) {
-  return make_uint4(decode2(prmt(w0, kMagic, 0x4140), kOffset8, s2), decode2(prmt(w0, kMagic, 0x4342), kOffset8, s2),
-                    decode2(prmt(w1, kMagic, 0x4140), kOffset8, s2), decode2(prmt(w1, kMagic, 0x4342), kOffset8, s2));
+// Warp-collective: N consecutive 32-bit columns of each thread's own lane, waited for in the same
+// statement, so that nothing that uses them can come before the wait.
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16]; tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+      "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+      "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
 }
 
-__device__ __forceinline__ uint4 decode_q4(uint32_t w, uint32_t s2) {
-  constexpr uint32_t m = kMagic & 0xff00ff00u, k = 0x000f000fu;
-  return make_uint4(decode2((w & k) | m, kOffset4, s2), decode2((w >> 4 & k) | m, kOffset4, s2),
-                    decode2((w >> 8 & k) | m, kOffset4, s2), decode2((w >> 12 & k) | m, kOffset4, s2));
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32]; tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+      "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+      "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+      "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+      "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Two runs of 16.
+__device__ __forceinline__ void tmem_read(uint32_t ta, uint32_t (&u)[16], uint32_t tb, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%32]; tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, "
+      "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33]; "
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+      "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
+      "=r"(u[14]), "=r"(u[15]), "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]),
+      "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+      "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(ta), "r"(tb)
+      : "memory");
+}
+
+// Eight consecutive elements (one core-matrix row) of a position from its codes.
+template <uint32_t KIND>
+__device__ __forceinline__ uint4 decode8(uint32_t w0, uint32_t w1, const Scale2& s) {
+  if constexpr (KIND == KQ_CACHE_Q8)
+    return make_uint4(decode2(prmt(w0, kMagic, 0x4140), s), decode2(prmt(w0, kMagic, 0x4342), s),
+                      decode2(prmt(w1, kMagic, 0x4140), s), decode2(prmt(w1, kMagic, 0x4342), s));
+  else  // w0 alone
+    return make_uint4(decode2(nibbles(nibble_up(w0, 0)), s), decode2(nibbles(nibble_up(w0, 1)), s),
+                      decode2(nibbles(nibble_up(w0, 2)), s), decode2(nibbles(nibble_up(w0, 3)), s));
 }
 
 __device__ __forceinline__ void sts_v4(uint32_t addr, uint4 v) {
@@ -88,57 +140,88 @@ __device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// One tile of keys or values from its copy into the operand's layout. left: positions the sequence has
-// from the tile's first on. Values past the end, and not finite ones of drafts (from `drafts_at` on),
-// become zero (see value_product); returns the drafts that had such values, as bits.
+// A decoding thread's share of every tile: position p, units [part * UNITS / PARTS, ...) of its row.
+// row = multiple of 32 bytes, a power of two, and 16 u < row, so (p row + 16 u) ^ swizzle is
+// (p row ^ swizzle) ^ 16 u.
 template <uint32_t KIND, uint32_t D>
-__device__ __forceinline__ unsigned long long decode_tile(uint32_t raw, uint32_t seg_log2, uint32_t to, bool value,
-                                                          uint32_t left, int drafts_at) {
+struct Decoder {
   using W = Wide<KIND, D>;
   using S = Shape<KIND, D>;
-  constexpr uint32_t PARTS = kDecodeWarps * 32 / W::TW;
-  constexpr uint32_t UNITS = S::kRow / 16;  // 16-byte units of a row
-  constexpr uint32_t E8 = S::kMost / 8;     // core-matrix rows a unit (f16: 1, Q8: 2, Q4: 4)
-  const uint32_t id = threadIdx.x - 128, p = id % W::TW, part = id / W::TW;
-  const TileView<S> tile = {raw, seg_log2};
-  const bool gone = value && p >= left;
-  const bool draft = value && static_cast<int>(p) >= drafts_at;
-  bool special = false;
+  static constexpr uint32_t PARTS = kDecodeWarps * 32 / W::TW;
+  static constexpr uint32_t N = S::kRow / 16 / PARTS;  // 16-byte units of a thread
+  static constexpr uint32_t E8 = S::kMost / 8;         // core-matrix rows a unit (f16: 1, Q8: 2, Q4: 4)
+  static constexpr uint32_t kStep = W::TW / 8 * 128;   // from one eight elements to the next
+  uint32_t p, part, seg, row, scale, to;
+
+  __device__ explicit Decoder(uint32_t seg_log2) {
+    const uint32_t id = threadIdx.x - 128;
+    p = id % W::TW;
+    part = id / W::TW;
+    const uint32_t in = p & ((1u << seg_log2) - 1);
+    seg = ((p >> seg_log2) << seg_log2) * (S::kRow + S::kScales);
+    row = in * S::kRow ^ cache_swizzle(in, S::kRow) << 4;
+    scale = seg + (S::kRow << seg_log2) + in * S::kScales + part * N * S::kMost / 32;
+    to = (part * N * E8 * (W::TW / 8) + p / 8) * 128 + (p % 8) * 16;
+  }
+
+  // A tile from its copy into the operand's layout. EDGE (values of a tile that reaches past the prefix;
+  // left: positions the sequence has from its first on): values past the end, and not finite ones of
+  // drafts (positions from drafts_at on), become zero (see value_product); returns the drafts that had
+  // such values, as bits.
+  template <bool EDGE>
+  __device__ __forceinline__ unsigned long long run(uint32_t raw, uint32_t out, uint32_t left, int drafts_at) const {
+    const bool gone = EDGE && p >= left;
+    const bool draft = EDGE && static_cast<int>(p) >= drafts_at;
+    bool special = false;
+    uint32_t bytes = 0;
+    if constexpr (S::kScales != 0)
+      bytes = N * S::kMost > 32 ? lds_u16(raw + scale) : lds_u8(raw + scale);
+    uint4 w[N];
 #pragma unroll
-  for (uint32_t i = 0; i < UNITS / PARTS; ++i) {
-    const uint32_t u = part * (UNITS / PARTS) + i;
-    const uint4 w = lds_v4(tile.code(p, 16 * u));
-    const uint32_t at = to + (u * E8 * (W::TW / 8) + p / 8) * 128 + (p % 8) * 16;
-    constexpr uint32_t step = W::TW / 8 * 128;
-    if constexpr (KIND == KQ_CACHE_F16) {
-      uint4 v = w;
-      if (draft) {
-        v = make_uint4(finite_or_zero(w.x), finite_or_zero(w.y), finite_or_zero(w.z), finite_or_zero(w.w));
-        special |= v.x != w.x || v.y != w.y || v.z != w.z || v.w != w.w;
-      }
-      if (gone) v = make_uint4(0, 0, 0, 0);
-      sts_v4(at, v);
-    } else {
-      uint32_t s = lds_u8(tile.scale(p) + u * S::kMost / 32);
-      if (draft && s >= 0xf8u) {
-        special = true;
-        s = 0;
-      }
-      if (gone) s = 0;
-      const uint32_t s2 = s * 0x00800080u;
-      if constexpr (KIND == KQ_CACHE_Q8) {
-        sts_v4(at, decode_q8(w.x, w.y, s2));
-        sts_v4(at + step, decode_q8(w.z, w.w, s2));
-      } else {
-        sts_v4(at, decode_q4(w.x, s2));
-        sts_v4(at + step, decode_q4(w.y, s2));
-        sts_v4(at + 2 * step, decode_q4(w.z, s2));
-        sts_v4(at + 3 * step, decode_q4(w.w, s2));
+    for (uint32_t i = 0; i < N; ++i) w[i] = lds_v4(raw + seg + (row ^ 16 * (part * N + i)));
+    Scale2 s[2];
+    if constexpr (S::kScales != 0) {
+#pragma unroll
+      for (uint32_t i = 0; i < (N * S::kMost + 31) / 32; ++i) {
+        uint32_t b = bytes >> (8 * i) & 0xffu;
+        if constexpr (EDGE) {
+          if (draft && b >= 0xf8u) {
+            special = true;
+            b = 0;
+          }
+          if (gone) b = 0;
+        }
+        s[i] = scale2<KIND>(b, b);
       }
     }
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const uint32_t at = out + to + i * E8 * kStep;
+      if constexpr (KIND == KQ_CACHE_F16) {
+        uint4 v = w[i];
+        if constexpr (EDGE) {
+          if (draft) {
+            v = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
+            special |= v.x != w[i].x || v.y != w[i].y || v.z != w[i].z || v.w != w[i].w;
+          }
+          if (gone) v = make_uint4(0, 0, 0, 0);
+        }
+        sts_v4(at, v);
+      } else if constexpr (KIND == KQ_CACHE_Q8) {
+        const Scale2& z = s[i * S::kMost / 32];
+        sts_v4(at, decode8<KIND>(w[i].x, w[i].y, z));
+        sts_v4(at + kStep, decode8<KIND>(w[i].z, w[i].w, z));
+      } else {
+        const Scale2& z = s[i * S::kMost / 32];
+        sts_v4(at, decode8<KIND>(w[i].x, 0, z));
+        sts_v4(at + kStep, decode8<KIND>(w[i].y, 0, z));
+        sts_v4(at + 2 * kStep, decode8<KIND>(w[i].z, 0, z));
+        sts_v4(at + 3 * kStep, decode8<KIND>(w[i].w, 0, z));
+      }
+    }
+    return special && !gone ? 1ull << (static_cast<int>(p) - drafts_at) : 0ull;
   }
-  return special && !gone ? 1ull << (static_cast<int>(p) - drafts_at) : 0ull;
-}
+};
 
 // Element e of the value at position pos, from the cache itself.
 template <uint32_t KIND, uint32_t D>
@@ -241,18 +324,24 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       if (at < end) next_item<ROWS>(a, p);
     }
   } else if (warp == 5 + kDecodeWarps) {
-    // ---- MMAs. Tile i's S goes to buffer i % 2, its P over it; QK of tile i + 1 is issued before PV
-    // of tile i, and after PV of tile i - 1, which read the buffer.
-    constexpr uint32_t idesc_qk = idesc_f16_f32(128, TW);
-    constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // B is N-major
-    constexpr uint32_t q_lbo = 16 * 128, op_lbo = TW / 8 * 128;
-    uint32_t n = 0, items = 0;  // tiles, items so far
-    const auto qk = [&](uint32_t i) {
-      // operand use 2i: keys of tile i
-      const uint32_t use = 2 * i, slot = use % W::kOperands;
-      wait_or_die(live, bar.op_full(slot), (use / W::kOperands) & 1, a.err, kErrWaitFull);
-      tc_fence_after();
-      if (live && lane == 0) {
+    // ---- MMAs, all from one thread. Tile i's S goes to buffer i % 2, its P over it; QK of tile i + 1 is
+    // issued before PV of tile i, and after PV of tile i - 1, which read the buffer.
+    if (elect_one()) {
+      constexpr uint32_t idesc_qk = idesc_f16_f32(128, TW);
+      constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // B is N-major
+      constexpr uint32_t q_lbo = 16 * 128, op_lbo = TW / 8 * 128;
+      uint32_t n = 0, items = 0;  // tiles, items so far
+      const auto wait = [&](uint32_t b, uint32_t parity) {
+        if (live && !mbar_wait(b, parity)) {
+          report_error(a.err, kErrWaitFull);
+          live = false;
+        }
+      };
+      const auto qk = [&](uint32_t i) {
+        const uint32_t use = 2 * i, slot = use % W::kOperands;  // operand use 2i: keys of tile i
+        wait(bar.op_full(slot), (use / W::kOperands) & 1);
+        if (!live) return;
+        tc_fence_after();
         const uint32_t d = tmem + (i & 1) * W::kS;
 #pragma unroll
         for (uint32_t ks = 0; ks < D / 16; ++ks)
@@ -260,23 +349,20 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
                      smem_desc(ops + slot * W::kOperand + ks * 2 * op_lbo, op_lbo, 128), idesc_qk, ks > 0);
         mma_commit(bar.op_empty(slot));
         mma_commit(bar.s_full(i & 1));
-      }
-      __syncwarp();
-    };
-    while (at < end) {
-      const uint32_t tiles = position_tiles<TW>(p.seq);
-      const uint32_t count = static_cast<uint32_t>(min(uint64_t(tiles - p.tile), end - at));
-      wait_or_die(live, bar.q_full(), items & 1, a.err, kErrWaitFull);
-      tc_fence_after();
-      qk(n);
-      for (uint32_t j = 0; j < count; ++j) {
-        const uint32_t i = n + j;
-        if (j + 1 < count) qk(i + 1);
-        wait_or_die(live, bar.p_full(i & 1), (i >> 1) & 1, a.err, kErrWaitFull);
-        const uint32_t use = 2 * i + 1, slot = use % W::kOperands;
-        wait_or_die(live, bar.op_full(slot), (use / W::kOperands) & 1, a.err, kErrWaitFull);
-        tc_fence_after();
-        if (live && lane == 0) {
+      };
+      while (at < end) {
+        const uint32_t tiles = position_tiles<TW>(p.seq);
+        const uint32_t count = static_cast<uint32_t>(min(uint64_t(tiles - p.tile), end - at));
+        wait(bar.q_full(), items & 1);
+        qk(n);
+        for (uint32_t j = 0; j < count; ++j) {
+          const uint32_t i = n + j;
+          if (j + 1 < count) qk(i + 1);
+          wait(bar.p_full(i & 1), (i >> 1) & 1);
+          const uint32_t use = 2 * i + 1, slot = use % W::kOperands;
+          wait(bar.op_full(slot), (use / W::kOperands) & 1);
+          if (!live) continue;
+          tc_fence_after();
           const uint32_t pa = tmem + (i & 1) * W::kS;
 #pragma unroll
           for (uint32_t kp = 0; kp < TW / 16; ++kp)
@@ -285,21 +371,20 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           mma_commit(bar.op_empty(slot));
           mma_commit(bar.pv_done());
         }
-        __syncwarp();
+        n += count;
+        at += count;
+        p.tile += count;
+        ++items;
+        if (at < end) next_item<ROWS>(a, p);
       }
-      n += count;
-      at += count;
-      p.tile += count;
-      ++items;
-      if (at < end) next_item<ROWS>(a, p);
-    }
-    // nothing of this thread's is in flight after this, whatever happened before
-    if (lane == 0) {
+      // nothing of this thread's is in flight after this, whatever happened before
       mma_commit(bar.drained());
       if (!mbar_wait(bar.drained(), 0)) report_error(a.err, kErrWaitFull);
     }
+    __syncwarp();
   } else if (warp >= 4) {
     // ---- decode: copied tiles to operands
+    const Decoder<KIND, D> decoder(seg_log2);
     uint32_t it = 0;
     uint32_t items = 0;
     while (at < end) {
@@ -313,9 +398,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           wait_or_die(live, bar.raw_full(raw), (it / W::kRaws) & 1, a.err, kErrWaitFull);
           if (it >= W::kOperands)
             wait_or_die(live, bar.op_empty(slot), (it / W::kOperands - 1) & 1, a.err, kErrWaitEmpty);
-          const unsigned long long odd = decode_tile<KIND, D>(raws + raw * W::kRaw, seg_log2, ops + slot * W::kOperand,
-                                                        kv, left, drafts_at);
-          if (odd) atomicOr(special + (items & 1), odd);
+          const uint32_t from = raws + raw * W::kRaw, to = ops + slot * W::kOperand;
+          if (kv && drafts_at < static_cast<int>(TW)) {
+            const unsigned long long odd = decoder.template run<true>(from, to, left, drafts_at);
+            if (odd) atomicOr(special + (items & 1), odd);
+          } else {
+            decoder.template run<false>(from, to, left, drafts_at);
+          }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -391,43 +480,53 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         const uint32_t sbuf = lanes + (n & 1) * W::kS;
         wait_or_die(live, bar.s_full(n & 1), (n >> 1) & 1, a.err, kErrWaitFull);
         tc_fence_after();
-        // the lane's logits (times unit: log2 units), masked
+        const int from = static_cast<int>(base + col0) - static_cast<int>(p.seq.prefix);
+        // the lane's logits (times unit: log2 units), masked in tiles that reach past the prefix
         float s[SPLIT ? COLS : 1];
         float mx = -INFINITY;
         if constexpr (SPLIT) {
 #pragma unroll
           for (uint32_t c = 0; c < COLS; c += 16) {
             uint32_t u[16], v[16];
-            tmem_ld16(sbuf + c, u);
-            tmem_ld16(sbuf + c + TW / 2, v);
-            tmem_wait_ld();
+            tmem_read(sbuf + c, u, sbuf + c + TW / 2, v);
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
               // each half of the pair of lanes keeps half of the columns
               const uint32_t keep = lane < 16 ? u[i] : v[i], send = lane < 16 ? v[i] : u[i];
-              float x = __uint_as_float(keep) + __uint_as_float(__shfl_xor_sync(0xffffffffu, send, 16));
-              if (edge && !sees(bits, base + col0 + c + i, p.seq)) x = -INFINITY;
-              s[c + i] = x;
-              mx = fmaxf(mx, x);
+              s[c + i] = __uint_as_float(keep) + __uint_as_float(__shfl_xor_sync(0xffffffffu, send, 16));
             }
           }
+          if (edge) {
+#pragma unroll
+            for (uint32_t c = 0; c < COLS; c += 32) {
+              const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
+#pragma unroll
+              for (uint32_t i = 0; i < 32; ++i)
+                if (!(seen >> i & 1u)) s[c + i] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (uint32_t c = 0; c < COLS; ++c) mx = fmaxf(mx, s[c]);
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        } else if (!edge) {
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (uint32_t c = 0; c < COLS; c += 32) {
+            uint32_t u[32];
+            tmem_read(sbuf + c, u);
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(u[i]));
+          }
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         } else {
 #pragma unroll 1
           for (uint32_t c = 0; c < COLS; c += 32) {
-            uint32_t u[16], v[16];
-            tmem_ld16(sbuf + c, u);
-            tmem_ld16(sbuf + c + 16, v);
-            tmem_wait_ld();
+            const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
+            uint32_t u[32];
+            tmem_read(sbuf + c, u);
 #pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-              float x = __uint_as_float(u[i]), y = __uint_as_float(v[i]);
-              if (edge) {
-                if (!sees(bits, base + c + i, p.seq)) x = -INFINITY;
-                if (!sees(bits, base + c + 16 + i, p.seq)) y = -INFINITY;
-              }
-              mx = fmaxf(mx, fmaxf(x, y));
-            }
+            for (uint32_t i = 0; i < 32; ++i)
+              if (seen >> i & 1u) mx = fmaxf(mx, __uint_as_float(u[i]));
           }
         }
         mx *= unit;
@@ -444,8 +543,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
 #pragma unroll 1
             for (uint32_t c = 0; c < D; c += 16) {
               uint32_t u[16];
-              tmem_ld16(lanes + W::kO + c, u);
-              tmem_wait_ld();
+              tmem_read(lanes + W::kO + c, u);
 #pragma unroll
               for (uint32_t i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
               tmem_st16(lanes + W::kO + c, u);
@@ -462,7 +560,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             uint32_t first[16], second[16];  // words of columns [c, c + 32) and TW / 2 + the same
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              const float w0 = exp2f(fmaf(s[c + 2 * i], unit, -ref)), w1 = exp2f(fmaf(s[c + 2 * i + 1], unit, -ref));
+              const float w0 = exp2_fast(fmaf(s[c + 2 * i], unit, -ref));
+              const float w1 = exp2_fast(fmaf(s[c + 2 * i + 1], unit, -ref));
               l += w0 + w1;
               uint32_t hi, lo;
               split2(w0, w1, hi, lo);
@@ -474,27 +573,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             tmem_st16(sbuf + c / 2 + TW / 4, second);
           }
         } else {
-#pragma unroll 1
-          for (uint32_t c = 0; c < COLS; c += 32) {
-            uint32_t u[16], v[16], w[16];
-            tmem_ld16(sbuf + c, u);
-            tmem_ld16(sbuf + c + 16, v);
-            tmem_wait_ld();
+          // columns [c, c + 32) become words [c / 2, c / 2 + 16): over columns already read
+          const auto weights = [&](uint32_t c, uint32_t seen) {
+            uint32_t u[32], w[16];
+            tmem_read(sbuf + c, u);
+            float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              float x = __uint_as_float(i < 8 ? u[2 * i] : v[2 * i - 16]);
-              float y = __uint_as_float(i < 8 ? u[2 * i + 1] : v[2 * i - 15]);
-              if (edge) {
-                if (!sees(bits, base + c + 2 * i, p.seq)) x = -INFINITY;
-                if (!sees(bits, base + c + 2 * i + 1, p.seq)) y = -INFINITY;
-              }
-              const __half2 h = __floats2half2_rn(exp2f(fmaf(x, unit, -ref)), exp2f(fmaf(y, unit, -ref)));
-              w[i] = h2(h);
-              const float2 f = __half22float2(h);
-              l += f.x + f.y;
+              float x = exp2_fast(fmaf(__uint_as_float(u[2 * i]), unit, -ref));
+              float y = exp2_fast(fmaf(__uint_as_float(u[2 * i + 1]), unit, -ref));
+              if (!(seen >> (2 * i) & 1u)) x = 0.f;
+              if (!(seen >> (2 * i + 1) & 1u)) y = 0.f;
+              w[i] = h2(__floats2half2_rn(x, y));
+              sum[0] += x;
+              sum[1] += y;
             }
-            // columns [c, c + 32) become words [c / 2, c / 2 + 16): over columns already read
+            l += sum[0] + sum[1];
             tmem_st16(sbuf + c / 2, w);
+          };
+          if (!edge) {
+#pragma unroll
+            for (uint32_t c = 0; c < COLS; c += 32) weights(c, ~0u);
+          } else {
+#pragma unroll 1
+            for (uint32_t c = 0; c < COLS; c += 32) weights(c, seen_word(bits, from + static_cast<int>(c)));
           }
         }
         tmem_wait_st();
@@ -521,9 +623,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
 #pragma unroll 1
       for (uint32_t c = 0; c < HALF; c += 16) {
         uint32_t u[16], v[16];
-        tmem_ld16(lanes + W::kO + c, u);
-        if constexpr (SPLIT) tmem_ld16(lanes + W::kO + c + HALF, v);
-        tmem_wait_ld();
+        if constexpr (SPLIT) tmem_read(lanes + W::kO + c, u, lanes + W::kO + c + HALF, v);
+        else tmem_read(lanes + W::kO + c, u);
         float y[16];
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i) {

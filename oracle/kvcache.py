@@ -9,7 +9,7 @@ import numpy as np
 
 F16, Q8, Q4 = 0, 1, 2
 TOP = {Q8: 127, Q4: 7}
-LAST = {Q8: 0xC0, Q4: 0xE1}  # the largest scale byte
+LAST = {Q8: 0xA6, Q4: 0xC6}  # the largest scale byte
 NAN_SCALE = 0xFF
 
 
