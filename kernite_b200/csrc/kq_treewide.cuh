@@ -4,17 +4,18 @@
 // The 128 lanes of the tensor core's M are rows (drafted token x query head of the group): 128 of them
 // for 16-bit activations; for f32 64 rows twice, as the f16 rounding of the operand and the f16
 // rounding of what that left, 16 and 16 in the 32 lanes of a warp, so that the two halves of a row meet
-// by a shuffle. S = Q K^T (Q and K in shared memory) and O += P V (P in tensor memory, where the
-// softmax warps put it over the S they read) accumulate in tensor memory in f32.
+// by a shuffle. S = Q K^T and O += P V accumulate in tensor memory in f32; Q and P are operands there
+// too (P over the S it comes from), so that shared memory, which the decoding loads already, gives the
+// tensor core K and V alone.
 //
 // What the tensor core reads has to be f16 in its own layout, so the codes take one more step than in
 // the warp-MMA kernel: eight warps turn a copied tile into the operand (each value exactly), once for
 // all rows of the item. K and V use the same layout, 8 positions x 8 elements to a 128-byte core matrix:
 // K-major for K (positions are N), N-major for V (elements are N).
 //
-// Roles: warps 0-3 softmax (warp w reads lanes 32 w ..), 4-11 decode, 12 copies, 13 issues the MMAs. In
-// the steady state QK of the next tile and PV of this one run while the softmax of the next waits only
-// for its own S (two S buffers).
+// Roles: warps 0-7 softmax (warp w has lanes 32 (w mod 4) .., half of a tile's columns), 8-15 decode, 16
+// copies, 17 issues the MMAs. In the steady state QK of the next tile and PV of this one run while the
+// softmax of the next waits only for its own S (two S buffers).
 #pragma once
 
 #include "kq_tc.cuh"
@@ -23,25 +24,26 @@
 namespace kq {
 namespace tree {
 
-constexpr uint32_t kDecodeWarps = 8;
-constexpr uint32_t kWideThreads = (4 + kDecodeWarps + 2) * 32;
+constexpr uint32_t kSoftWarps = 8, kDecodeWarps = 8;
+constexpr uint32_t kCopyWarp = kSoftWarps + kDecodeWarps, kMmaWarp = kCopyWarp + 1;
+constexpr uint32_t kWideThreads = (kSoftWarps + kDecodeWarps + 2) * 32;
 
 template <uint32_t KIND, uint32_t D>
 struct Wide {
   using S = Shape<KIND, D>;
   static constexpr uint32_t TW = D == 256 ? 64 : 128;      // positions a tile
   static constexpr uint32_t kOperand = TW * D * 2;         // bytes of a K or V operand
-  static constexpr uint32_t kOperands = 3;
-  static constexpr uint32_t kQ = 128 * D * 2;
+  static constexpr uint32_t kOperands = 4;
   static constexpr uint32_t kRaw = TW * (S::kRow + S::kScales);
-  static constexpr uint32_t kFixed = kQ + kOperands * kOperand + 1024;
+  static constexpr uint32_t kFixed = kOperands * kOperand + 4096;
   static constexpr uint32_t kFit = (227 * 1024 - kFixed) / kRaw;
   static constexpr uint32_t kRaws = kFit > 6 ? 6 : kFit;
   static constexpr uint32_t kBytes = kFixed + kRaws * kRaw;
   static_assert(kRaws >= 2 && kBytes <= 227 * 1024, "ring");
-  // tensor memory columns: two S (or one after the other's P), O
+  // tensor memory columns: two S (and P), O, Q
   static constexpr uint32_t kS = TW;
-  static constexpr uint32_t kO = 256;
+  static constexpr uint32_t kO = 2 * TW;
+  static constexpr uint32_t kQ = 384;
 };
 
 // Barriers of the wide kernel, 8 bytes each, from `bars`.
@@ -154,7 +156,7 @@ struct Decoder {
   uint32_t p, part, seg, row, scale, to;
 
   __device__ explicit Decoder(uint32_t seg_log2) {
-    const uint32_t id = threadIdx.x - 128;
+    const uint32_t id = threadIdx.x - kSoftWarps * 32;
     p = id % W::TW;
     part = id / W::TW;
     const uint32_t in = p & ((1u << seg_log2) - 1);
@@ -176,9 +178,6 @@ struct Decoder {
     uint32_t bytes = 0;
     if constexpr (S::kScales != 0)
       bytes = N * S::kMost > 32 ? lds_u16(raw + scale) : lds_u8(raw + scale);
-    uint4 w[N];
-#pragma unroll
-    for (uint32_t i = 0; i < N; ++i) w[i] = lds_v4(raw + seg + (row ^ 16 * (part * N + i)));
     Scale2 s[2];
     if constexpr (S::kScales != 0) {
 #pragma unroll
@@ -194,29 +193,36 @@ struct Decoder {
         s[i] = scale2<KIND>(b, b);
       }
     }
+    constexpr uint32_t AT_ONCE = N < 4 ? N : 4;
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) {
-      const uint32_t at = out + to + i * E8 * kStep;
-      if constexpr (KIND == KQ_CACHE_F16) {
-        uint4 v = w[i];
-        if constexpr (EDGE) {
-          if (draft) {
-            v = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
-            special |= v.x != w[i].x || v.y != w[i].y || v.z != w[i].z || v.w != w[i].w;
+    for (uint32_t i0 = 0; i0 < N; i0 += AT_ONCE) {
+      uint4 w[AT_ONCE];
+#pragma unroll
+      for (uint32_t k = 0; k < AT_ONCE; ++k) w[k] = lds_v4(raw + seg + (row ^ 16 * (part * N + i0 + k)));
+#pragma unroll
+      for (uint32_t k = 0; k < AT_ONCE; ++k) {
+        const uint32_t i = i0 + k, at = out + to + i * E8 * kStep;
+        if constexpr (KIND == KQ_CACHE_F16) {
+          uint4 v = w[k];
+          if constexpr (EDGE) {
+            if (draft) {
+              v = make_uint4(finite_or_zero(v.x), finite_or_zero(v.y), finite_or_zero(v.z), finite_or_zero(v.w));
+              special |= v.x != w[k].x || v.y != w[k].y || v.z != w[k].z || v.w != w[k].w;
+            }
+            if (gone) v = make_uint4(0, 0, 0, 0);
           }
-          if (gone) v = make_uint4(0, 0, 0, 0);
+          sts_v4(at, v);
+        } else if constexpr (KIND == KQ_CACHE_Q8) {
+          const Scale2& z = s[i * S::kMost / 32];
+          sts_v4(at, decode8<KIND>(w[k].x, w[k].y, z));
+          sts_v4(at + kStep, decode8<KIND>(w[k].z, w[k].w, z));
+        } else {
+          const Scale2& z = s[i * S::kMost / 32];
+          sts_v4(at, decode8<KIND>(w[k].x, 0, z));
+          sts_v4(at + kStep, decode8<KIND>(w[k].y, 0, z));
+          sts_v4(at + 2 * kStep, decode8<KIND>(w[k].z, 0, z));
+          sts_v4(at + 3 * kStep, decode8<KIND>(w[k].w, 0, z));
         }
-        sts_v4(at, v);
-      } else if constexpr (KIND == KQ_CACHE_Q8) {
-        const Scale2& z = s[i * S::kMost / 32];
-        sts_v4(at, decode8<KIND>(w[i].x, w[i].y, z));
-        sts_v4(at + kStep, decode8<KIND>(w[i].z, w[i].w, z));
-      } else {
-        const Scale2& z = s[i * S::kMost / 32];
-        sts_v4(at, decode8<KIND>(w[i].x, 0, z));
-        sts_v4(at + kStep, decode8<KIND>(w[i].y, 0, z));
-        sts_v4(at + 2 * kStep, decode8<KIND>(w[i].z, 0, z));
-        sts_v4(at + 3 * kStep, decode8<KIND>(w[i].w, 0, z));
       }
     }
     return special && !gone ? 1ull << (static_cast<int>(p) - drafts_at) : 0ull;
@@ -236,24 +242,20 @@ __device__ __forceinline__ float value_at(const TreeArgs& a, const Place& p, uin
   return rec[a.c.page() * S::kRow + in * S::kScales + e / 32] >= 0xf8u ? __int_as_float(0x7fc00000) : 0.f;
 }
 
-// E consecutive activations from element i on.
-template <uint32_t E>
-__device__ __forceinline__ void load_acts(const void* p, uint64_t i, uint32_t type, float (&x)[E]) {
+// Eight activations from element i on.
+__device__ __forceinline__ void load_acts(const void* p, uint64_t i, uint32_t type, float (&x)[8]) {
   if (type == KQ_TYPE_F32) {
-    if constexpr (E == 2) load_act<float, 2>(static_cast<const float*>(p) + i, x);
-    else {
+    float y[4];
+    load_act<float, 4>(static_cast<const float*>(p) + i, y);
 #pragma unroll
-      for (uint32_t j = 0; j < E; j += 4) {
-        float y[4];
-        load_act<float, 4>(static_cast<const float*>(p) + i + j, y);
+    for (uint32_t k = 0; k < 4; ++k) x[k] = y[k];
+    load_act<float, 4>(static_cast<const float*>(p) + i + 4, y);
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) x[j + k] = y[k];
-      }
-    }
+    for (uint32_t k = 0; k < 4; ++k) x[4 + k] = y[k];
   } else if (type == KQ_TYPE_F16) {
-    load_act<__half, E>(static_cast<const __half*>(p) + i, x);
+    load_act<__half, 8>(static_cast<const __half*>(p) + i, x);
   } else {
-    load_act<__nv_bfloat16, E>(static_cast<const __nv_bfloat16*>(p) + i, x);
+    load_act<__nv_bfloat16, 8>(static_cast<const __nv_bfloat16*>(p) + i, x);
   }
 }
 
@@ -264,11 +266,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   constexpr uint32_t ROWS = SPLIT ? 64 : 128;
   constexpr uint32_t TW = W::TW;
   extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t q_op = smem_u32(smem), ops = q_op + W::kQ, raws = ops + W::kOperands * W::kOperand;
-  const uint32_t tail = W::kQ + W::kOperands * W::kOperand + W::kRaws * W::kRaw;
-  const WideBars bar = {q_op + tail};
+  const uint32_t ops = smem_u32(smem), raws = ops + W::kOperands * W::kOperand;
+  const uint32_t tail = W::kOperands * W::kOperand + W::kRaws * W::kRaw;
+  const WideBars bar = {ops + tail};
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + tail + 256);
   unsigned long long* special = reinterpret_cast<unsigned long long*>(smem + tail + 264);  // of the item's drafts
+  // what the two halves of a row's columns tell each other: [tile parity][half][lane of 128]
+  float* exchange = reinterpret_cast<float*>(smem + tail + 512);
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -282,9 +286,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(bar.s_full(i), 1);
-      mbar_init(bar.p_full(i), 4);
+      mbar_init(bar.p_full(i), kSoftWarps);
     }
-    mbar_init(bar.q_full(), 4);
+    mbar_init(bar.q_full(), kSoftWarps);
     mbar_init(bar.pv_done(), 1);
     mbar_init(bar.drained(), 1);
     fence_mbar_init();
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   bool live = true;
   const uint32_t seg_log2 = min(a.c.page_log2, TW == 128 ? 7u : 6u);
 
-  if (warp == 4 + kDecodeWarps) {
+  if (warp == kCopyWarp) {
     // ---- copies: raw tiles, keys and values in turn
     PageWindow window = {0xffffffffu, 0, 0};
     uint32_t it = 0;
@@ -323,13 +327,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       }
       if (at < end) next_item<ROWS>(a, p);
     }
-  } else if (warp == 5 + kDecodeWarps) {
+  } else if (warp == kMmaWarp) {
     // ---- MMAs, all from one thread. Tile i's S goes to buffer i % 2, its P over it; QK of tile i + 1 is
     // issued before PV of tile i, and after PV of tile i - 1, which read the buffer.
     if (elect_one()) {
       constexpr uint32_t idesc_qk = idesc_f16_f32(128, TW);
       constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // B is N-major
-      constexpr uint32_t q_lbo = 16 * 128, op_lbo = TW / 8 * 128;
+      constexpr uint32_t op_lbo = TW / 8 * 128;
       uint32_t n = 0, items = 0;  // tiles, items so far
       const auto wait = [&](uint32_t b, uint32_t parity) {
         if (live && !mbar_wait(b, parity)) {
@@ -345,8 +349,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         const uint32_t d = tmem + (i & 1) * W::kS;
 #pragma unroll
         for (uint32_t ks = 0; ks < D / 16; ++ks)
-          mma_f16_ss(d, smem_desc(q_op + ks * 2 * q_lbo, q_lbo, 128),
-                     smem_desc(ops + slot * W::kOperand + ks * 2 * op_lbo, op_lbo, 128), idesc_qk, ks > 0);
+          mma_f16_ts(d, tmem + W::kQ + ks * 8, smem_desc(ops + slot * W::kOperand + ks * 2 * op_lbo, op_lbo, 128),
+                     idesc_qk, ks > 0);
         mma_commit(bar.op_empty(slot));
         mma_commit(bar.s_full(i & 1));
       };
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           const uint32_t pa = tmem + (i & 1) * W::kS;
 #pragma unroll
           for (uint32_t kp = 0; kp < TW / 16; ++kp)
-            mma_f16_ts(tmem + W::kO, pa + kp * 8, smem_desc(ops + slot * W::kOperand + kp * 256, 128, op_lbo),
+            mma_f16_ts(tmem + W::kO, pa + kp / (TW / 32) * (TW / 2) + kp % (TW / 32) * 8, smem_desc(ops + slot * W::kOperand + kp * 256, 128, op_lbo),
                        idesc_pv, j > 0 || kp > 0);
           mma_commit(bar.op_empty(slot));
           mma_commit(bar.pv_done());
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       if (!mbar_wait(bar.drained(), 0)) report_error(a.err, kErrWaitFull);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp >= kSoftWarps) {
     // ---- decode: copied tiles to operands
     const Decoder<KIND, D> decoder(seg_log2);
     uint32_t it = 0;
@@ -418,81 +422,87 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     }
   } else {
     // ---- softmax
-    const uint32_t lanes = tmem + ((warp * 32) << 16);
-    uint32_t n = 0, items = 0;
+    const uint32_t quad = warp % 4, half = warp / 4;
+    const uint32_t lanes = tmem + ((quad * 32) << 16);
+    const uint32_t slot = quad * 32 + lane;
+    // a value of this row's half for the other half's thread, and the other's (the two warps of a quad)
+    const auto swap = [&](uint32_t parity, float mine) {
+      exchange[(parity * 2 + half) * 128 + slot] = mine;
+      named_barrier(2 + quad, 64);
+      return exchange[(parity * 2 + 1 - half) * 128 + slot];
+    };
+    uint32_t n = 0, items = 0, swaps = 0;
     while (at < end) {
       // Q as operand A: lane m's row is 16 (m / 32) + m % 16, parts (m % 32) / 16, or row m; each row
-      // scaled by a power of two to a largest element in [2^7, 2^8)
+      // scaled by a power of two to a largest element in [2^7, 2^8). This thread: half of its row.
       const uint32_t rows = p.seq.drafts * a.group;
-      const uint32_t my_row = p.rows * ROWS + (SPLIT ? warp * 16 + lane % 16 : warp * 32 + lane);
-      float unit = a.scale_log2;
-      constexpr uint32_t E = D / 32, AHEAD = 4;
-#pragma unroll 1
-      for (uint32_t r0 = 0; r0 < ROWS / 4; r0 += AHEAD) {
-        float x[AHEAD][E];
+      const uint32_t in_tile = SPLIT ? quad * 16 + lane % 16 : slot;
+      const uint32_t my_row = p.rows * ROWS + in_tile;
+      const bool have = my_row < rows;
+      const bool second = SPLIT && lane >= 16;
+      const uint64_t q_row = have ? (p.seq.first + my_row / a.group) * a.q_token +
+                                        uint64_t(p.head * a.group + my_row % a.group) * a.c.dim
+                                  : 0;
+      float most = 0.f;
+#pragma unroll 4
+      for (uint32_t e = half * (D / 2); e < (half + 1) * (D / 2); e += 8) {
+        if (have && e < a.c.dim) {
+          float x[8];
+          load_acts(a.q, q_row + e, a.type, x);
 #pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-          const uint32_t r = p.rows * ROWS + warp * (ROWS / 4) + r0 + k;
-#pragma unroll
-          for (uint32_t j = 0; j < E; ++j) x[k][j] = 0.f;
-          if (r < rows && lane * E < a.c.dim)
-            load_acts<E>(a.q, (p.seq.first + r / a.group) * a.q_token +
-                                  uint64_t(p.head * a.group + r % a.group) * a.c.dim + lane * E, a.type, x[k]);
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < AHEAD; ++k) {
-          float most = 0.f;
-#pragma unroll
-          for (uint32_t j = 0; j < E; ++j) most = fmaxf(most, fabsf(x[k][j]));
-#pragma unroll
-          for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
-          const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
-          const float up = __int_as_float((127 + sh) << 23);
-          const uint32_t r = r0 + k;  // of the warp's
-          if ((SPLIT ? lane % 16 : lane) == r) unit = __int_as_float((127 - sh) << 23) * a.scale_log2;
-          const uint32_t m = warp * 32 + r;
-#pragma unroll
-          for (uint32_t j = 0; j < E; j += 2) {
-            const uint32_t e = lane * E + j;
-            uint32_t hi, lo;
-            split2(x[k][j] * up, x[k][j + 1] * up, hi, lo);
-            const uint32_t to = q_op + (e / 8 * 16 + m / 8) * 128 + (m % 8) * 16 + (e % 8) * 2;
-            sts_u32(to, hi);
-            if constexpr (SPLIT) sts_u32(to + 256, lo);  // lane m + 16
-          }
+          for (uint32_t k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[k]));
         }
       }
-      fence_proxy_async_smem();
+      most = fmaxf(most, swap(swaps++ & 1, most));
+      const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+      const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
+      const float up = __int_as_float((127 + sh) << 23);
+      const float unit = __int_as_float((127 - sh) << 23) * a.scale_log2;
+#pragma unroll 1
+      for (uint32_t e = half * (D / 2); e < (half + 1) * (D / 2); e += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          if (have && e + 8 * j < a.c.dim) load_acts(a.q, q_row + e + 8 * j, a.type, x);
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) {
+            uint32_t hi, lo;
+            split2(x[2 * k] * up, x[2 * k + 1] * up, hi, lo);
+            w[4 * j + k] = second ? lo : hi;
+          }
+        }
+        tmem_st16(lanes + W::kQ + e / 2, w);
+      }
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar.q_full());
-      const bool have = my_row < rows;
       const unsigned long long bits = have ? mask_bits(a, p.seq, my_row / a.group) : 0ull;
 
       float m = -INFINITY, l = 0.f;
       const uint32_t tiles = position_tiles<TW>(p.seq), first_tile = p.tile;
-      constexpr uint32_t COLS = SPLIT ? TW / 2 : TW;  // columns a lane has of its row
-      const uint32_t col0 = SPLIT && lane >= 16 ? TW / 2 : 0;
+      constexpr uint32_t COLS = SPLIT ? TW / 4 : TW / 2;  // columns a lane has of its row
+      const uint32_t col0 = half * (TW / 2) + (second ? COLS : 0);
       for (; p.tile < tiles && at < end; ++p.tile, ++at, ++n) {
         const uint32_t base = p.tile * TW;
         const bool edge = base + TW > p.seq.prefix;
-        const uint32_t sbuf = lanes + (n & 1) * W::kS;
+        const uint32_t sbuf = lanes + (n & 1) * W::kS + half * (TW / 2);  // this half's columns, then words
         wait_or_die(live, bar.s_full(n & 1), (n >> 1) & 1, a.err, kErrWaitFull);
         tc_fence_after();
-        const int from = static_cast<int>(base + col0) - static_cast<int>(p.seq.prefix);
         // the lane's logits (times unit: log2 units), masked in tiles that reach past the prefix
         float s[SPLIT ? COLS : 1];
-        float mx = -INFINITY;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const int from = static_cast<int>(base + col0) - static_cast<int>(p.seq.prefix);
         if constexpr (SPLIT) {
 #pragma unroll
           for (uint32_t c = 0; c < COLS; c += 16) {
             uint32_t u[16], v[16];
-            tmem_read(sbuf + c, u, sbuf + c + TW / 2, v);
+            tmem_read(sbuf + c, u, sbuf + c + COLS, v);
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              // each half of the pair of lanes keeps half of the columns
-              const uint32_t keep = lane < 16 ? u[i] : v[i], send = lane < 16 ? v[i] : u[i];
+              // each of the pair of lanes keeps half of the columns
+              const uint32_t keep = second ? v[i] : u[i], send = second ? u[i] : v[i];
               s[c + i] = __uint_as_float(keep) + __uint_as_float(__shfl_xor_sync(0xffffffffu, send, 16));
             }
           }
@@ -501,35 +511,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             for (uint32_t c = 0; c < COLS; c += 32) {
               const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
 #pragma unroll
-              for (uint32_t i = 0; i < 32; ++i)
+              for (uint32_t i = 0; i < 32 && c + i < COLS; ++i)
                 if (!(seen >> i & 1u)) s[c + i] = -INFINITY;
             }
           }
 #pragma unroll
-          for (uint32_t c = 0; c < COLS; ++c) mx = fmaxf(mx, s[c]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        } else if (!edge) {
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (uint32_t c = 0; c < COLS; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+        } else {
 #pragma unroll
           for (uint32_t c = 0; c < COLS; c += 32) {
             uint32_t u[32];
             tmem_read(sbuf + c, u);
+            if (edge) {
+              const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
+#pragma unroll
+              for (uint32_t i = 0; i < 32; ++i)
+                if (!(seen >> i & 1u)) u[i] = 0xff800000u;
+            }
 #pragma unroll
             for (uint32_t i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(u[i]));
           }
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        } else {
-#pragma unroll 1
-          for (uint32_t c = 0; c < COLS; c += 32) {
-            const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
-            uint32_t u[32];
-            tmem_read(sbuf + c, u);
-#pragma unroll
-            for (uint32_t i = 0; i < 32; ++i)
-              if (seen >> i & 1u) mx = fmaxf(mx, __uint_as_float(u[i]));
-          }
         }
-        mx *= unit;
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        if constexpr (SPLIT) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = fmaxf(mx, swap(swaps++ & 1, mx)) * unit;
         const bool grow = mx > m + kSlack || (m == -INFINITY && mx > m);
         if (__any_sync(0xffffffffu, grow)) {
           const float to = grow ? mx : m;
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             wait_or_die(live, bar.pv_done(), (n - 1) & 1, a.err, kErrWaitFull);
             tc_fence_after();
 #pragma unroll 1
-            for (uint32_t c = 0; c < D; c += 16) {
+            for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 16) {
               uint32_t u[16];
               tmem_read(lanes + W::kO + c, u);
 #pragma unroll
@@ -552,84 +557,89 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           }
         }
         const float ref = m == -INFINITY ? 0.f : m - kLift;
+        float sum[2] = {0.f, 0.f};
         if constexpr (SPLIT) {
           // weights as two f16; the pair of lanes exchanges so that one has the first parts of all
           // columns, the other the second ones
+          uint32_t first[COLS / 2], last[COLS / 2];  // words of the pair's first columns, and the others
 #pragma unroll
-          for (uint32_t c = 0; c < COLS; c += 32) {
-            uint32_t first[16], second[16];  // words of columns [c, c + 32) and TW / 2 + the same
+          for (uint32_t i = 0; i < COLS / 2; ++i) {
+            const float w0 = exp2_fast(fmaf(s[2 * i], unit, -ref)), w1 = exp2_fast(fmaf(s[2 * i + 1], unit, -ref));
+            sum[0] += w0;
+            sum[1] += w1;
+            uint32_t hi, lo;
+            split2(w0, w1, hi, lo);
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, second ? hi : lo, 16);
+            first[i] = second ? got : hi;
+            last[i] = second ? lo : got;
+          }
+          if constexpr (COLS == 32) {
+            tmem_st16(sbuf, first);
+            tmem_st16(sbuf + 16, last);
+          } else {
+            uint32_t w[16];
 #pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-              const float w0 = exp2_fast(fmaf(s[c + 2 * i], unit, -ref));
-              const float w1 = exp2_fast(fmaf(s[c + 2 * i + 1], unit, -ref));
-              l += w0 + w1;
-              uint32_t hi, lo;
-              split2(w0, w1, hi, lo);
-              const uint32_t got = __shfl_xor_sync(0xffffffffu, lane < 16 ? lo : hi, 16);
-              first[i] = lane < 16 ? hi : got;
-              second[i] = lane < 16 ? got : lo;
+            for (uint32_t i = 0; i < 8; ++i) {
+              w[i] = first[i];
+              w[8 + i] = last[i];
             }
-            tmem_st16(sbuf + c / 2, first);
-            tmem_st16(sbuf + c / 2 + TW / 4, second);
+            tmem_st16(sbuf, w);
           }
         } else {
-          // columns [c, c + 32) become words [c / 2, c / 2 + 16): over columns already read
-          const auto weights = [&](uint32_t c, uint32_t seen) {
+#pragma unroll
+          for (uint32_t c = 0; c < COLS; c += 32) {
+            // the columns again (words go over ones already read)
             uint32_t u[32], w[16];
             tmem_read(sbuf + c, u);
-            float sum[2] = {0.f, 0.f};
+            if (edge) {
+              const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
+#pragma unroll
+              for (uint32_t i = 0; i < 32; ++i)
+                if (!(seen >> i & 1u)) u[i] = 0xff800000u;
+            }
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              float x = exp2_fast(fmaf(__uint_as_float(u[2 * i]), unit, -ref));
-              float y = exp2_fast(fmaf(__uint_as_float(u[2 * i + 1]), unit, -ref));
-              if (!(seen >> (2 * i) & 1u)) x = 0.f;
-              if (!(seen >> (2 * i + 1) & 1u)) y = 0.f;
-              w[i] = h2(__floats2half2_rn(x, y));
+              const float x = exp2_fast(fmaf(__uint_as_float(u[2 * i]), unit, -ref));
+              const float y = exp2_fast(fmaf(__uint_as_float(u[2 * i + 1]), unit, -ref));
               sum[0] += x;
               sum[1] += y;
+              w[i] = h2(__floats2half2_rn(x, y));
             }
-            l += sum[0] + sum[1];
             tmem_st16(sbuf + c / 2, w);
-          };
-          if (!edge) {
-#pragma unroll
-            for (uint32_t c = 0; c < COLS; c += 32) weights(c, ~0u);
-          } else {
-#pragma unroll 1
-            for (uint32_t c = 0; c < COLS; c += 32) weights(c, seen_word(bits, from + static_cast<int>(c)));
           }
         }
+        l += sum[0] + sum[1];
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar.p_full(n & 1));
       }
 
-      // ---- the item's output
+      // ---- the item's output, half of the columns (and for pairs of lanes a quarter) a thread
       const bool whole = first_tile == 0 && p.tile == tiles;
       float* part = a.part + (uint64_t(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * part_floats(ROWS, D);
+      if constexpr (SPLIT) l += __shfl_xor_sync(0xffffffffu, l, 16);
+      l += swap(swaps++ & 1, l);
       wait_or_die(live, bar.pv_done(), (n - 1) & 1, a.err, kErrWaitFull);
       tc_fence_after();
-      if constexpr (SPLIT) l += __shfl_xor_sync(0xffffffffu, l, 16);
       const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
       // every tile's values were decoded before their product: the flags are complete, and the next
       // item's go to the other word
       const unsigned long long odd = *reinterpret_cast<volatile unsigned long long*>(special + (items & 1)) & bits;
-      const uint32_t in_tile = my_row - p.rows * ROWS;
       const uint64_t to = (p.seq.first + (have ? my_row / a.group : 0)) * a.out_token +
                           uint64_t(p.head * a.group + my_row % a.group) * a.c.dim;
-      constexpr uint32_t HALF = SPLIT ? D / 2 : D;
-      const uint32_t e0 = SPLIT && lane >= 16 ? HALF : 0;
+      constexpr uint32_t WIDE = SPLIT ? D / 4 : D / 2;
+      const uint32_t o0 = half * (D / 2), e0 = o0 + (second ? WIDE : 0);
 #pragma unroll 1
-      for (uint32_t c = 0; c < HALF; c += 16) {
+      for (uint32_t c = 0; c < WIDE; c += 16) {
         uint32_t u[16], v[16];
-        if constexpr (SPLIT) tmem_read(lanes + W::kO + c, u, lanes + W::kO + c + HALF, v);
-        else tmem_read(lanes + W::kO + c, u);
+        if constexpr (SPLIT) tmem_read(lanes + W::kO + o0 + c, u, lanes + W::kO + o0 + c + WIDE, v);
+        else tmem_read(lanes + W::kO + o0 + c, u);
         float y[16];
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i) {
           if constexpr (SPLIT) {
-            const uint32_t keep = lane < 16 ? u[i] : v[i], send = lane < 16 ? v[i] : u[i];
+            const uint32_t keep = second ? v[i] : u[i], send = second ? u[i] : v[i];
             y[i] = __uint_as_float(keep) + __uint_as_float(__shfl_xor_sync(0xffffffffu, send, 16));
           } else {
             y[i] = __uint_as_float(u[i]);
@@ -671,12 +681,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           }
         }
       }
-      if (have && !whole && (!SPLIT || lane < 16)) {
+      if (have && !whole && half == 0 && !second) {
         part[ROWS * D + in_tile] = m;
         part[ROWS * (D + 1) + in_tile] = l;
       }
       tc_fence_before();  // O is read before the next item's first product writes it
-      named_barrier(1, 128);
+      named_barrier(1, kSoftWarps * 32);
       if (threadIdx.x == 0) special[items & 1] = 0;
       ++items;
       if (at < end) next_item<ROWS>(a, p);
