@@ -55,7 +55,7 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   const uint32_t group = d.n_heads / c.n_kv;
   p.wide = d.max_drafts * group > (p.split ? 8u : 16u);
   p.rows = p.wide ? (p.split ? 64 : 128) : p.split ? 8 : 16;
-  p.tile = p.wide && c.pitch == 256 ? 64 : 128;
+  p.tile = p.wide ? 64 : 128;
   const uint64_t row_tiles = (uint64_t(d.max_drafts) * group + p.rows - 1) / p.rows;
   const uint64_t tiles = (uint64_t(d.max_len) + p.tile - 1) / p.tile;
   const uint64_t items = uint64_t(d.n_seq) * c.n_kv * row_tiles;
@@ -66,12 +66,12 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   return KQ_OK;
 }
 
-template <uint32_t ROWS, uint32_t TW256>
+template <uint32_t ROWS, uint32_t TW>
 void launch_join(const tree::TreeArgs& a, uint32_t items, uint32_t ctas, cudaStream_t s) {
   const dim3 grid(items, ROWS / 8);
-  if (a.c.pitch == 64) tree::join_kernel<ROWS, 64, 128><<<grid, 256, 0, s>>>(a, ctas);
-  else if (a.c.pitch == 128) tree::join_kernel<ROWS, 128, 128><<<grid, 256, 0, s>>>(a, ctas);
-  else tree::join_kernel<ROWS, 256, TW256><<<grid, 256, 0, s>>>(a, ctas);
+  if (a.c.pitch == 64) tree::join_kernel<ROWS, 64, TW><<<grid, 256, 0, s>>>(a, ctas);
+  else if (a.c.pitch == 128) tree::join_kernel<ROWS, 128, TW><<<grid, 256, 0, s>>>(a, ctas);
+  else tree::join_kernel<ROWS, 256, TW><<<grid, 256, 0, s>>>(a, ctas);
 }
 
 bool on16(uint64_t bytes) { return bytes % 16 == 0; }

@@ -537,8 +537,12 @@ __device__ __forceinline__ void add_special(const TileView<Shape<KIND, D>>& tile
   }
 }
 
-constexpr float kLift = 6.f;  // weights are kept times 2^6: their f16 parts reach 2^-30 of the largest
-constexpr float kSlack = 8.f; // outputs are rescaled when the maximum grows by more than 2^8
+// Weights are kept times 2^kLift of the reference they were taken to, and outputs are rescaled to a new
+// reference only when the maximum is more than 2^kSlack above it, which after an item's first tile hardly
+// happens: the largest weight is below 2^15, in f16's range, and what f16 loses of a small one (2^-25) is
+// 2^-27 of the reference's own weight at most.
+constexpr float kLift = 2.f;
+constexpr float kSlack = 13.f;
 
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ TreeArgs a) {

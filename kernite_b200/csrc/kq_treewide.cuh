@@ -13,9 +13,11 @@
 // all rows of the item. K and V use the same layout, 8 positions x 8 elements to a 128-byte core matrix:
 // K-major for K (positions are N), N-major for V (elements are N).
 //
-// Roles: warps 0-7 softmax (warp w has lanes 32 (w mod 4) .., half of a tile's columns), 8-15 decode, 16
-// copies, 17 issues the MMAs. In the steady state QK of the next tile and PV of this one run while the
-// softmax of the next waits only for its own S (two S buffers).
+// Roles: warps 0-3 and 4-7 softmax, of even and of odd tiles (warp w has lanes 32 (w mod 4) ..); 8-11
+// decode keys, 12-15 values; 16 issues the MMAs; 17 and 18 copy keys and values. A buffer's way round (QK, softmax, PV, the
+// next QK) is long against any one of its steps, so tiles are short (64 positions) and four S buffers are
+// under way at once. The softmax groups share a row's maximum: a tile's is passed on, as soon as it is
+// known, to the group that has the next tile.
 #pragma once
 
 #include "kq_tc.cuh"
@@ -25,25 +27,26 @@ namespace kq {
 namespace tree {
 
 constexpr uint32_t kSoftWarps = 8, kDecodeWarps = 8;
-constexpr uint32_t kCopyWarp = kSoftWarps + kDecodeWarps, kMmaWarp = kCopyWarp + 1;
-constexpr uint32_t kWideThreads = (kSoftWarps + kDecodeWarps + 2) * 32;
+constexpr uint32_t kMmaWarp = kSoftWarps + kDecodeWarps, kCopyWarp = kMmaWarp + 1;  // and + 2
+constexpr uint32_t kWideThreads = (kSoftWarps + kDecodeWarps + 3) * 32;
 
 template <uint32_t KIND, uint32_t D>
 struct Wide {
   using S = Shape<KIND, D>;
-  static constexpr uint32_t TW = D == 256 ? 64 : 128;      // positions a tile
+  static constexpr uint32_t TW = 64;                       // positions a tile
   static constexpr uint32_t kOperand = TW * D * 2;         // bytes of a K or V operand
-  static constexpr uint32_t kOperands = 4;
+  static constexpr uint32_t kOperands = D == 256 ? 4 : 8;  // keys and values in turn
   static constexpr uint32_t kRaw = TW * (S::kRow + S::kScales);
   static constexpr uint32_t kFixed = kOperands * kOperand + 4096;
   static constexpr uint32_t kFit = (227 * 1024 - kFixed) / kRaw;
-  static constexpr uint32_t kRaws = kFit > 6 ? 6 : kFit;
+  static constexpr uint32_t kRaws = kFit > 8 ? 8 : kFit;
   static constexpr uint32_t kBytes = kFixed + kRaws * kRaw;
   static_assert(kRaws >= 2 && kBytes <= 227 * 1024, "ring");
-  // tensor memory columns: two S (and P), O, Q
+  // tensor memory columns: S (then P) buffers, O, Q
+  static constexpr uint32_t kBufs = D == 256 ? 2 : 4;
   static constexpr uint32_t kS = TW;
-  static constexpr uint32_t kO = 2 * TW;
-  static constexpr uint32_t kQ = 384;
+  static constexpr uint32_t kO = kBufs * TW;
+  static constexpr uint32_t kQ = kO + D;
 };
 
 // Barriers of the wide kernel, 8 bytes each, from `bars`.
@@ -52,12 +55,12 @@ struct WideBars {
   __device__ uint32_t raw_full(uint32_t i) const { return base + 8 * i; }
   __device__ uint32_t raw_empty(uint32_t i) const { return base + 64 + 8 * i; }
   __device__ uint32_t op_full(uint32_t i) const { return base + 128 + 8 * i; }
-  __device__ uint32_t op_empty(uint32_t i) const { return base + 160 + 8 * i; }
-  __device__ uint32_t s_full(uint32_t i) const { return base + 192 + 8 * i; }
-  __device__ uint32_t p_full(uint32_t i) const { return base + 208 + 8 * i; }
-  __device__ uint32_t q_full() const { return base + 224; }
-  __device__ uint32_t pv_done() const { return base + 232; }
-  __device__ uint32_t drained() const { return base + 240; }
+  __device__ uint32_t op_empty(uint32_t i) const { return base + 192 + 8 * i; }
+  __device__ uint32_t s_full(uint32_t i) const { return base + 256 + 8 * i; }
+  __device__ uint32_t p_full(uint32_t i) const { return base + 288 + 8 * i; }
+  __device__ uint32_t pv_done(uint32_t i) const { return base + 320 + 8 * i; }
+  __device__ uint32_t q_full() const { return base + 352; }
+  __device__ uint32_t drained() const { return base + 360; }
 };
 
 // True in one lane of a converged warp. The compiler knows that one thread runs what this guards, which a
@@ -70,9 +73,54 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
+// The numbers of a tile's pages, as the table has them.
+template <uint32_t TW>
+struct PageIds {
+  uint32_t id[TW / 16];
+
+  __device__ __forceinline__ void load(const TreeArgs& a, const Place& p) {
+    const uint32_t base = p.tile * TW, length = p.seq.length();
+    const int* row = a.pages + uint64_t(p.s) * a.max_pages + (base >> a.c.page_log2);
+    const uint32_t n = (min(TW, length - base) + a.c.page() - 1) >> a.c.page_log2;
+    id[0] = static_cast<uint32_t>(row[0]);
+#pragma unroll
+    for (uint32_t i = 1; i < TW / 16; ++i) id[i] = i < n ? static_cast<uint32_t>(row[i]) : 0u;
+  }
+};
+
+// One thread's copies of a tile: whole records where a page is at most a tile, else its rows and its
+// scales. A page that is not there is recorded, and page 0 copied.
+template <class S, uint32_t TW>
+__device__ __forceinline__ void copy_tile(const TreeArgs& a, const Place& p, const PageIds<TW>& ids,
+                                          const uint8_t* src, uint32_t dst, uint32_t bar) {
+  constexpr uint32_t row = S::kRow + S::kScales;
+  const uint32_t base = p.tile * TW, left = p.seq.length() - base;
+  const auto record = [&](uint32_t id) {
+    if (id >= a.c.n_pages) {
+      report_error(a.err, kErrCacheRange);
+      id = 0;
+    }
+    return src + a.c.at(id, p.head);
+  };
+  if (a.c.page() > TW) {
+    const uint8_t* rec = record(ids.id[0]);
+    const uint32_t at = base & (a.c.page() - 1);
+    mbar_arrive_expect_tx(bar, TW * row);
+    bulk_g2s(dst, rec + at * S::kRow, TW * S::kRow, bar);
+    if constexpr (S::kScales != 0)
+      bulk_g2s(dst + TW * S::kRow, rec + a.c.page() * S::kRow + at * S::kScales, TW * S::kScales, bar);
+    return;
+  }
+  const uint32_t n = (min(TW, left) + a.c.page() - 1) >> a.c.page_log2, bytes = row << a.c.page_log2;
+  mbar_arrive_expect_tx(bar, n * bytes);
+#pragma unroll
+  for (uint32_t i = 0; i < TW / 16; ++i)
+    if (i < n) bulk_g2s(dst + i * bytes, record(ids.id[i]), bytes, bar);
+}
+
 // One bounded wait of a warp: false (for good) once any wait of it has given up.
 __device__ __forceinline__ void wait_or_die(bool& live, uint32_t bar, uint32_t parity, unsigned* err, unsigned code) {
-  if (live && !mbar_wait_sleep(bar, parity)) {
+  if (live && !mbar_wait(bar, parity)) {
     report_error(err, code);
     live = false;
   }
@@ -142,27 +190,29 @@ __device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// A decoding thread's share of every tile: position p, units [part * UNITS / PARTS, ...) of its row.
-// row = multiple of 32 bytes, a power of two, and 16 u < row, so (p row + 16 u) ^ swizzle is
+// A decoding thread's share of its group's tiles (keys or values): position p, N units of its row from
+// part * N on. row = a power of two above 16, and 16 u < row, so (p row + 16 u) ^ swizzle is
 // (p row ^ swizzle) ^ 16 u.
 template <uint32_t KIND, uint32_t D>
 struct Decoder {
   using W = Wide<KIND, D>;
   using S = Shape<KIND, D>;
-  static constexpr uint32_t PARTS = kDecodeWarps * 32 / W::TW;
+  static constexpr uint32_t PARTS = kDecodeWarps / 2 * 32 / W::TW;
   static constexpr uint32_t N = S::kRow / 16 / PARTS;  // 16-byte units of a thread
   static constexpr uint32_t E8 = S::kMost / 8;         // core-matrix rows a unit (f16: 1, Q8: 2, Q4: 4)
   static constexpr uint32_t kStep = W::TW / 8 * 128;   // from one eight elements to the next
+  static_assert(PARTS >= 1 && N >= 1, "a thread's share is whole units");
+  static constexpr uint32_t kBytes = N * S::kMost / 32;  // scale bytes: 1, 2 or 4
   uint32_t p, part, seg, row, scale, to;
 
   __device__ explicit Decoder(uint32_t seg_log2) {
-    const uint32_t id = threadIdx.x - kSoftWarps * 32;
+    const uint32_t id = (threadIdx.x - kSoftWarps * 32) % (kDecodeWarps / 2 * 32);
     p = id % W::TW;
     part = id / W::TW;
     const uint32_t in = p & ((1u << seg_log2) - 1);
     seg = ((p >> seg_log2) << seg_log2) * (S::kRow + S::kScales);
     row = in * S::kRow ^ cache_swizzle(in, S::kRow) << 4;
-    scale = seg + (S::kRow << seg_log2) + in * S::kScales + part * N * S::kMost / 32;
+    scale = seg + (S::kRow << seg_log2) + in * S::kScales + part * kBytes;
     to = (part * N * E8 * (W::TW / 8) + p / 8) * 128 + (p % 8) * 16;
   }
 
@@ -177,11 +227,11 @@ struct Decoder {
     bool special = false;
     uint32_t bytes = 0;
     if constexpr (S::kScales != 0)
-      bytes = N * S::kMost > 32 ? lds_u16(raw + scale) : lds_u8(raw + scale);
-    Scale2 s[2];
+      bytes = kBytes == 4 ? lds_u32(raw + scale) : kBytes == 2 ? lds_u16(raw + scale) : lds_u8(raw + scale);
+    Scale2 s[kBytes];
     if constexpr (S::kScales != 0) {
 #pragma unroll
-      for (uint32_t i = 0; i < (N * S::kMost + 31) / 32; ++i) {
+      for (uint32_t i = 0; i < kBytes; ++i) {
         uint32_t b = bytes >> (8 * i) & 0xffu;
         if constexpr (EDGE) {
           if (draft && b >= 0xf8u) {
@@ -269,27 +319,27 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   const uint32_t ops = smem_u32(smem), raws = ops + W::kOperands * W::kOperand;
   const uint32_t tail = W::kOperands * W::kOperand + W::kRaws * W::kRaw;
   const WideBars bar = {ops + tail};
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + tail + 256);
-  unsigned long long* special = reinterpret_cast<unsigned long long*>(smem + tail + 264);  // of the item's drafts
-  // what the two halves of a row's columns tell each other: [tile parity][half][lane of 128]
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + tail + 384);
+  unsigned long long* special = reinterpret_cast<unsigned long long*>(smem + tail + 392);  // of the item's drafts
+  // what the two softmax groups tell each other
   float* exchange = reinterpret_cast<float*>(smem + tail + 512);
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < W::kRaws; ++i) {
       mbar_init(bar.raw_full(i), 1);
-      mbar_init(bar.raw_empty(i), kDecodeWarps);
+      mbar_init(bar.raw_empty(i), kDecodeWarps / 2);
     }
     for (uint32_t i = 0; i < W::kOperands; ++i) {
-      mbar_init(bar.op_full(i), kDecodeWarps);
+      mbar_init(bar.op_full(i), kDecodeWarps / 2);
       mbar_init(bar.op_empty(i), 1);
     }
-    for (uint32_t i = 0; i < 2; ++i) {
+    for (uint32_t i = 0; i < W::kBufs; ++i) {
       mbar_init(bar.s_full(i), 1);
-      mbar_init(bar.p_full(i), kSoftWarps);
+      mbar_init(bar.p_full(i), kSoftWarps / 2);
+      mbar_init(bar.pv_done(i), 1);
     }
     mbar_init(bar.q_full(), kSoftWarps);
-    mbar_init(bar.pv_done(), 1);
     mbar_init(bar.drained(), 1);
     fence_mbar_init();
     special[0] = special[1] = 0;
@@ -311,25 +361,41 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   bool live = true;
   const uint32_t seg_log2 = min(a.c.page_log2, TW == 128 ? 7u : 6u);
 
-  if (warp == kCopyWarp) {
-    // ---- copies: raw tiles, keys and values in turn
-    PageWindow window = {0xffffffffu, 0, 0};
-    uint32_t it = 0;
-    while (at < end) {
-      const uint32_t tiles = position_tiles<TW>(p.seq);
-      for (; p.tile < tiles && at < end; ++p.tile, ++at) {
-#pragma unroll 1
-        for (uint32_t kv = 0; kv < 2; ++kv, ++it) {
+  if (warp >= kCopyWarp) {
+    // ---- copies, from one thread: raw tiles of keys (use 2 i of the ring) or of values (2 i + 1)
+    if (elect_one()) {
+      const uint32_t kv = warp - kCopyWarp;
+      const uint8_t* src = kv ? a.c.v : a.c.k;
+      PageIds<TW> ids;
+      ids.load(a, p);
+      uint32_t it = kv;
+      while (at < end) {
+        const uint32_t tiles = position_tiles<TW>(p.seq);
+        while (p.tile < tiles && at < end) {
           const uint32_t slot = it % W::kRaws;
-          if (it >= W::kRaws) wait_or_die(live, bar.raw_empty(slot), (it / W::kRaws - 1) & 1, a.err, kErrWaitEmpty);
-          if (live) produce_tile<S, TW>(a, p, kv ? a.c.v : a.c.k, raws + slot * W::kRaw, bar.raw_full(slot), window);
+          const Place now = p;
+          const PageIds<TW> these = ids;
+          // the next tile's pages come in while this one waits for its slot
+          ++p.tile;
+          ++at;
+          if (at < end && p.tile < tiles) ids.load(a, p);
+          if (it >= W::kRaws && live && !mbar_wait(bar.raw_empty(slot), (it / W::kRaws - 1) & 1)) {
+            report_error(a.err, kErrWaitEmpty);
+            live = false;
+          }
+          if (live) copy_tile<S, TW>(a, now, these, src, raws + slot * W::kRaw, bar.raw_full(slot));
+          it += 2;
+        }
+        if (at < end) {
+          next_item<ROWS>(a, p);
+          ids.load(a, p);
         }
       }
-      if (at < end) next_item<ROWS>(a, p);
     }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
-    // ---- MMAs, all from one thread. Tile i's S goes to buffer i % 2, its P over it; QK of tile i + 1 is
-    // issued before PV of tile i, and after PV of tile i - 1, which read the buffer.
+    // ---- MMAs, all from one thread. Tile i's S goes to buffer i % kBufs, its P over it; QK of tile
+    // i + kBufs - 1 is issued before PV of tile i, and after PV of tile i - 1, which read the buffer.
     if (elect_one()) {
       constexpr uint32_t idesc_qk = idesc_f16_f32(128, TW);
       constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // B is N-major
@@ -346,34 +412,34 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         wait(bar.op_full(slot), (use / W::kOperands) & 1);
         if (!live) return;
         tc_fence_after();
-        const uint32_t d = tmem + (i & 1) * W::kS;
+        const uint32_t d = tmem + i % W::kBufs * W::kS;
 #pragma unroll
         for (uint32_t ks = 0; ks < D / 16; ++ks)
           mma_f16_ts(d, tmem + W::kQ + ks * 8, smem_desc(ops + slot * W::kOperand + ks * 2 * op_lbo, op_lbo, 128),
                      idesc_qk, ks > 0);
         mma_commit(bar.op_empty(slot));
-        mma_commit(bar.s_full(i & 1));
+        mma_commit(bar.s_full(i % W::kBufs));
       };
       while (at < end) {
         const uint32_t tiles = position_tiles<TW>(p.seq);
         const uint32_t count = static_cast<uint32_t>(min(uint64_t(tiles - p.tile), end - at));
         wait(bar.q_full(), items & 1);
-        qk(n);
+        for (uint32_t j = 0; j < min(count, W::kBufs - 1); ++j) qk(n + j);
         for (uint32_t j = 0; j < count; ++j) {
-          const uint32_t i = n + j;
-          if (j + 1 < count) qk(i + 1);
-          wait(bar.p_full(i & 1), (i >> 1) & 1);
+          const uint32_t i = n + j, buf = i % W::kBufs;
+          if (j + W::kBufs - 1 < count) qk(i + W::kBufs - 1);
+          wait(bar.p_full(buf), (i / W::kBufs) & 1);
           const uint32_t use = 2 * i + 1, slot = use % W::kOperands;
           wait(bar.op_full(slot), (use / W::kOperands) & 1);
           if (!live) continue;
           tc_fence_after();
-          const uint32_t pa = tmem + (i & 1) * W::kS;
+          const uint32_t pa = tmem + buf * W::kS;
 #pragma unroll
           for (uint32_t kp = 0; kp < TW / 16; ++kp)
-            mma_f16_ts(tmem + W::kO, pa + kp / (TW / 32) * (TW / 2) + kp % (TW / 32) * 8, smem_desc(ops + slot * W::kOperand + kp * 256, 128, op_lbo),
+            mma_f16_ts(tmem + W::kO, pa + kp * 8, smem_desc(ops + slot * W::kOperand + kp * 256, 128, op_lbo),
                        idesc_pv, j > 0 || kp > 0);
           mma_commit(bar.op_empty(slot));
-          mma_commit(bar.pv_done());
+          mma_commit(bar.pv_done(buf));
         }
         n += count;
         at += count;
@@ -387,34 +453,32 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     }
     __syncwarp();
   } else if (warp >= kSoftWarps) {
-    // ---- decode: copied tiles to operands
+    // ---- decode: copied tiles to operands, use 2 i + kv of both rings for tile i
+    const uint32_t kv = (warp - kSoftWarps) / (kDecodeWarps / 2);
     const Decoder<KIND, D> decoder(seg_log2);
-    uint32_t it = 0;
+    uint32_t it = kv;
     uint32_t items = 0;
     while (at < end) {
       const uint32_t tiles = position_tiles<TW>(p.seq);
-      for (; p.tile < tiles && at < end; ++p.tile, ++at) {
+      for (; p.tile < tiles && at < end; ++p.tile, ++at, it += 2) {
         const uint32_t base = p.tile * TW, left = p.seq.length() - base;
         const int drafts_at = static_cast<int>(p.seq.prefix) - static_cast<int>(base);
-#pragma unroll 1
-        for (uint32_t kv = 0; kv < 2; ++kv, ++it) {
-          const uint32_t raw = it % W::kRaws, slot = it % W::kOperands;
-          wait_or_die(live, bar.raw_full(raw), (it / W::kRaws) & 1, a.err, kErrWaitFull);
-          if (it >= W::kOperands)
-            wait_or_die(live, bar.op_empty(slot), (it / W::kOperands - 1) & 1, a.err, kErrWaitEmpty);
-          const uint32_t from = raws + raw * W::kRaw, to = ops + slot * W::kOperand;
-          if (kv && drafts_at < static_cast<int>(TW)) {
-            const unsigned long long odd = decoder.template run<true>(from, to, left, drafts_at);
-            if (odd) atomicOr(special + (items & 1), odd);
-          } else {
-            decoder.template run<false>(from, to, left, drafts_at);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(bar.raw_empty(raw));
-            mbar_arrive(bar.op_full(slot));
-          }
+        const uint32_t raw = it % W::kRaws, slot = it % W::kOperands;
+        wait_or_die(live, bar.raw_full(raw), (it / W::kRaws) & 1, a.err, kErrWaitFull);
+        if (it >= W::kOperands)
+          wait_or_die(live, bar.op_empty(slot), (it / W::kOperands - 1) & 1, a.err, kErrWaitEmpty);
+        const uint32_t from = raws + raw * W::kRaw, to = ops + slot * W::kOperand;
+        if (kv && drafts_at < static_cast<int>(TW)) {
+          const unsigned long long odd = decoder.template run<true>(from, to, left, drafts_at);
+          if (odd) atomicOr(special + (items & 1), odd);
+        } else {
+          decoder.template run<false>(from, to, left, drafts_at);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar.raw_empty(raw));
+          mbar_arrive(bar.op_full(slot));
         }
       }
       ++items;
@@ -422,15 +486,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     }
   } else {
     // ---- softmax
-    const uint32_t quad = warp % 4, half = warp / 4;
+    const uint32_t quad = warp % 4, half = warp / 4;  // the group: even or odd tiles, half of Q's and O's columns
     const uint32_t lanes = tmem + ((quad * 32) << 16);
     const uint32_t slot = quad * 32 + lane;
-    // a value of this row's half for the other half's thread, and the other's (the two warps of a quad)
+    // a value of this row's for the other group's thread, and the other's
     const auto swap = [&](uint32_t parity, float mine) {
       exchange[(parity * 2 + half) * 128 + slot] = mine;
       named_barrier(2 + quad, 64);
       return exchange[(parity * 2 + 1 - half) * 128 + slot];
     };
+    float* chain = exchange + 512;  // [group][lane]: a row's maximum after the group's last tile
     uint32_t n = 0, items = 0, swaps = 0;
     while (at < end) {
       // Q as operand A: lane m's row is 16 (m / 32) + m % 16, parts (m % 32) / 16, or row m; each row
@@ -482,13 +547,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
 
       float m = -INFINITY, l = 0.f;
       const uint32_t tiles = position_tiles<TW>(p.seq), first_tile = p.tile;
-      constexpr uint32_t COLS = SPLIT ? TW / 4 : TW / 2;  // columns a lane has of its row
-      const uint32_t col0 = half * (TW / 2) + (second ? COLS : 0);
+      constexpr uint32_t COLS = SPLIT ? TW / 2 : TW;  // columns a lane has of its row
+      const uint32_t col0 = second ? COLS : 0;
       for (; p.tile < tiles && at < end; ++p.tile, ++at, ++n) {
+        if ((n & 1) != half) continue;
         const uint32_t base = p.tile * TW;
         const bool edge = base + TW > p.seq.prefix;
-        const uint32_t sbuf = lanes + (n & 1) * W::kS + half * (TW / 2);  // this half's columns, then words
-        wait_or_die(live, bar.s_full(n & 1), (n >> 1) & 1, a.err, kErrWaitFull);
+        const uint32_t buf = n % W::kBufs, sbuf = lanes + buf * W::kS;
+        wait_or_die(live, bar.s_full(buf), (n / W::kBufs) & 1, a.err, kErrWaitFull);
         tc_fence_after();
         // the lane's logits (times unit: log2 units), masked in tiles that reach past the prefix
         float s[SPLIT ? COLS : 1];
@@ -511,116 +577,129 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             for (uint32_t c = 0; c < COLS; c += 32) {
               const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
 #pragma unroll
-              for (uint32_t i = 0; i < 32 && c + i < COLS; ++i)
+              for (uint32_t i = 0; i < 32; ++i)
                 if (!(seen >> i & 1u)) s[c + i] = -INFINITY;
             }
           }
 #pragma unroll
           for (uint32_t c = 0; c < COLS; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
         } else {
-#pragma unroll
-          for (uint32_t c = 0; c < COLS; c += 32) {
+          const auto largest = [&](uint32_t c, uint32_t seen) {
             uint32_t u[32];
             tmem_read(sbuf + c, u);
-            if (edge) {
-              const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
 #pragma unroll
-              for (uint32_t i = 0; i < 32; ++i)
-                if (!(seen >> i & 1u)) u[i] = 0xff800000u;
-            }
+            for (uint32_t i = 0; i < 32; ++i)
+              m4[i & 3] = fmaxf(m4[i & 3], seen >> i & 1u ? __uint_as_float(u[i]) : -INFINITY);
+          };
+          if (!edge) {
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(u[i]));
+            for (uint32_t c = 0; c < COLS; c += 32) largest(c, ~0u);
+          } else {
+#pragma unroll 1
+            for (uint32_t c = 0; c < COLS; c += 32) largest(c, seen_word(bits, from + static_cast<int>(c)));
           }
         }
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if constexpr (SPLIT) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        mx = fmaxf(mx, swap(swaps++ & 1, mx)) * unit;
-        const bool grow = mx > m + kSlack || (m == -INFINITY && mx > m);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float to = grow ? mx : m;
-          const float f = grow ? exp2f(m - to) : 1.f;
-          m = to;
-          l *= f;
-          if (p.tile > first_tile) {
-            // the output so far is rescaled once the product that adds to it is done
-            wait_or_die(live, bar.pv_done(), (n - 1) & 1, a.err, kErrWaitFull);
-            tc_fence_after();
+        mx *= unit;
+        // the maximum so far, from the group that has the tile before; this one's for the next
+        float before = m;
+        if (p.tile > first_tile) {
+          named_barrier(6 + 2 * quad + (1 - half), 64);
+          before = chain[(1 - half) * 128 + slot];
+        }
+        const bool grow = mx > before + kSlack || (before == -INFINITY && mx > before);
+        const float now = grow ? mx : before;
+        if (p.tile + 1 < tiles && at + 1 < end) {
+          chain[half * 128 + slot] = now;
+          __syncwarp();
+          asm volatile("bar.arrive %0, %1;" ::"r"(6 + 2 * quad + half), "r"(64) : "memory");
+        }
+        if (now != m) {  // (the first time both are -inf or the sum is 0)
+          l *= exp2f(m - now);
+          m = now;
+        }
+        if (__any_sync(0xffffffffu, grow) && p.tile > first_tile) {
+          // the output so far is rescaled once the product that adds to it is done (its buffer's product
+          // before that one was done when this tile's S was)
+          const float f = grow ? exp2f(before - now) : 1.f;
+          wait_or_die(live, bar.pv_done((n - 1) % W::kBufs), ((n - 1) / W::kBufs) & 1, a.err, kErrWaitFull);
+          tc_fence_after();
 #pragma unroll 1
-            for (uint32_t c = half * (D / 2); c < (half + 1) * (D / 2); c += 16) {
-              uint32_t u[16];
-              tmem_read(lanes + W::kO + c, u);
+          for (uint32_t c = 0; c < D; c += 16) {
+            uint32_t u[16];
+            tmem_read(lanes + W::kO + c, u);
 #pragma unroll
-              for (uint32_t i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
-              tmem_st16(lanes + W::kO + c, u);
-            }
-            tmem_wait_st();
+            for (uint32_t i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
+            tmem_st16(lanes + W::kO + c, u);
           }
+          tmem_wait_st();
         }
         const float ref = m == -INFINITY ? 0.f : m - kLift;
         float sum[2] = {0.f, 0.f};
         if constexpr (SPLIT) {
           // weights as two f16; the pair of lanes exchanges so that one has the first parts of all
           // columns, the other the second ones
-          uint32_t first[COLS / 2], last[COLS / 2];  // words of the pair's first columns, and the others
-#pragma unroll
-          for (uint32_t i = 0; i < COLS / 2; ++i) {
-            const float w0 = exp2_fast(fmaf(s[2 * i], unit, -ref)), w1 = exp2_fast(fmaf(s[2 * i + 1], unit, -ref));
-            sum[0] += w0;
-            sum[1] += w1;
-            uint32_t hi, lo;
-            split2(w0, w1, hi, lo);
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, second ? hi : lo, 16);
-            first[i] = second ? got : hi;
-            last[i] = second ? lo : got;
-          }
-          if constexpr (COLS == 32) {
-            tmem_st16(sbuf, first);
-            tmem_st16(sbuf + 16, last);
-          } else {
-            uint32_t w[16];
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-              w[i] = first[i];
-              w[8 + i] = last[i];
-            }
-            tmem_st16(sbuf, w);
-          }
-        } else {
 #pragma unroll
           for (uint32_t c = 0; c < COLS; c += 32) {
-            // the columns again (words go over ones already read)
-            uint32_t u[32], w[16];
-            tmem_read(sbuf + c, u);
-            if (edge) {
-              const uint32_t seen = seen_word(bits, from + static_cast<int>(c));
-#pragma unroll
-              for (uint32_t i = 0; i < 32; ++i)
-                if (!(seen >> i & 1u)) u[i] = 0xff800000u;
-            }
+            uint32_t first[16], last[16];  // words of columns [c, c + 32) and COLS + the same
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              const float x = exp2_fast(fmaf(__uint_as_float(u[2 * i]), unit, -ref));
-              const float y = exp2_fast(fmaf(__uint_as_float(u[2 * i + 1]), unit, -ref));
+              const float w0 = exp2_fast(fmaf(s[c + 2 * i], unit, -ref));
+              const float w1 = exp2_fast(fmaf(s[c + 2 * i + 1], unit, -ref));
+              sum[0] += w0;
+              sum[1] += w1;
+              uint32_t hi, lo;
+              split2(w0, w1, hi, lo);
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, second ? hi : lo, 16);
+              first[i] = second ? got : hi;
+              last[i] = second ? lo : got;
+            }
+            tmem_st16(sbuf + c / 2, first);
+            tmem_st16(sbuf + (COLS + c) / 2, last);
+          }
+        } else {
+          // the columns again; columns [c, c + 32) become words [c / 2, c / 2 + 16), over ones already read
+          const auto weights = [&](uint32_t c, uint32_t seen) {
+            uint32_t u[32], w[16];
+            tmem_read(sbuf + c, u);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+              float x = exp2_fast(fmaf(__uint_as_float(u[2 * i]), unit, -ref));
+              float y = exp2_fast(fmaf(__uint_as_float(u[2 * i + 1]), unit, -ref));
+              x = seen >> (2 * i) & 1u ? x : 0.f;
+              y = seen >> (2 * i + 1) & 1u ? y : 0.f;
               sum[0] += x;
               sum[1] += y;
               w[i] = h2(__floats2half2_rn(x, y));
             }
             tmem_st16(sbuf + c / 2, w);
+          };
+          if (!edge) {
+#pragma unroll
+            for (uint32_t c = 0; c < COLS; c += 32) weights(c, ~0u);
+          } else {
+#pragma unroll 1
+            for (uint32_t c = 0; c < COLS; c += 32) weights(c, seen_word(bits, from + static_cast<int>(c)));
           }
         }
         l += sum[0] + sum[1];
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar.p_full(n & 1));
+        if (lane == 0) mbar_arrive(bar.p_full(buf));
       }
 
       // ---- the item's output, half of the columns (and for pairs of lanes a quarter) a thread
       const bool whole = first_tile == 0 && p.tile == tiles;
       float* part = a.part + (uint64_t(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * part_floats(ROWS, D);
+      // the groups' sums, over the later maximum
       if constexpr (SPLIT) l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const float last_m = fmaxf(m, swap(swaps++ & 1, m));
+      if (m != last_m) l *= exp2f(m - last_m);
+      m = last_m;
       l += swap(swaps++ & 1, l);
-      wait_or_die(live, bar.pv_done(), (n - 1) & 1, a.err, kErrWaitFull);
+      wait_or_die(live, bar.pv_done((n - 1) % W::kBufs), ((n - 1) / W::kBufs) & 1, a.err, kErrWaitFull);
       tc_fence_after();
       const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
       // every tile's values were decoded before their product: the flags are complete, and the next
