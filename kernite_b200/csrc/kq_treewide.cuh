@@ -14,10 +14,11 @@
 // K-major for K (positions are N), N-major for V (elements are N).
 //
 // Roles: warps 0-3 and 4-7 softmax, of even and of odd tiles (warp w has lanes 32 (w mod 4) ..); 8-11
-// decode keys, 12-15 values; 16 issues the MMAs; 17 and 18 copy keys and values. A buffer's way round (QK, softmax, PV, the
-// next QK) is long against any one of its steps, so tiles are short (64 positions) and four S buffers are
-// under way at once. The softmax groups share a row's maximum: a tile's is passed on, as soon as it is
-// known, to the group that has the next tile.
+// decode keys, 12-15 values; 16 issues the MMAs; 17 and 18 copy keys and values. A buffer's way round
+// (QK, softmax, PV, the next QK) is long against any one of its steps, so tiles are short (64 positions)
+// and three or four S buffers are under way at once. Each softmax group has its own maxima, sums and,
+// up to a pitch of 128, its own O, joined at an item's end; at 256 there is room for one O, and a tile's
+// maximum is passed on to the group that has the next tile.
 #pragma once
 
 #include "kq_tc.cuh"
@@ -42,11 +43,13 @@ struct Wide {
   static constexpr uint32_t kRaws = kFit > 8 ? 8 : kFit;
   static constexpr uint32_t kBytes = kFixed + kRaws * kRaw;
   static_assert(kRaws >= 2 && kBytes <= 227 * 1024, "ring");
-  // tensor memory columns: S (then P) buffers, O, Q
-  static constexpr uint32_t kBufs = D == 256 ? 2 : 4;
+  // tensor memory columns: S (then P) buffers, O (one a softmax group where there is room), Q
+  static constexpr bool kOwnO = D <= 128;
+  static constexpr uint32_t kBufs = D == 256 ? 2 : D == 128 ? 3 : 4;
   static constexpr uint32_t kS = TW;
   static constexpr uint32_t kO = kBufs * TW;
-  static constexpr uint32_t kQ = kO + D;
+  static constexpr uint32_t kQ = kO + (kOwnO ? 2 : 1) * D;
+  static_assert(kQ + D / 2 <= 512, "tensor memory");
 };
 
 // Barriers of the wide kernel, 8 bytes each, from `bars`.
@@ -71,6 +74,29 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\t.reg .b32 r;\n\telect.sync r|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(one));
   return one != 0;
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // The numbers of a tile's pages, as the table has them.
@@ -400,6 +426,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       constexpr uint32_t idesc_qk = idesc_f16_f32(128, TW);
       constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // B is N-major
       constexpr uint32_t op_lbo = TW / 8 * 128;
+      // an operand's descriptors; another slot or step is an addition to the address field (16 bytes a unit)
+      const uint64_t k_desc = smem_desc(ops, op_lbo, 128), v_desc = smem_desc(ops, 128, op_lbo);
       uint32_t n = 0, items = 0;  // tiles, items so far
       const auto wait = [&](uint32_t b, uint32_t parity) {
         if (live && !mbar_wait(b, parity)) {
@@ -413,10 +441,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         if (!live) return;
         tc_fence_after();
         const uint32_t d = tmem + i % W::kBufs * W::kS;
+        const uint64_t b = k_desc + slot * (W::kOperand >> 4);
 #pragma unroll
         for (uint32_t ks = 0; ks < D / 16; ++ks)
-          mma_f16_ts(d, tmem + W::kQ + ks * 8, smem_desc(ops + slot * W::kOperand + ks * 2 * op_lbo, op_lbo, 128),
-                     idesc_qk, ks > 0);
+          mma_f16_ts(d, tmem + W::kQ + ks * 8, b + ks * (2 * op_lbo >> 4), idesc_qk, ks > 0);
         mma_commit(bar.op_empty(slot));
         mma_commit(bar.s_full(i % W::kBufs));
       };
@@ -434,10 +462,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           if (!live) continue;
           tc_fence_after();
           const uint32_t pa = tmem + buf * W::kS;
+          const uint64_t b = v_desc + slot * (W::kOperand >> 4);
 #pragma unroll
           for (uint32_t kp = 0; kp < TW / 16; ++kp)
-            mma_f16_ts(tmem + W::kO, pa + kp * 8, smem_desc(ops + slot * W::kOperand + kp * 256, 128, op_lbo),
-                       idesc_pv, j > 0 || kp > 0);
+            mma_f16_ts(tmem + W::kO + (W::kOwnO ? (i & 1) * D : 0), pa + kp * 8, b + kp * (256 >> 4), idesc_pv,
+                       kp > 0 || j > (W::kOwnO ? 1 : 0));
           mma_commit(bar.op_empty(slot));
           mma_commit(bar.pv_done(buf));
         }
@@ -495,6 +524,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       named_barrier(2 + quad, 64);
       return exchange[(parity * 2 + 1 - half) * 128 + slot];
     };
+    const uint32_t my_o = lanes + W::kO + (W::kOwnO ? half * D : 0);
     float* chain = exchange + 512;  // [group][lane]: a row's maximum after the group's last tile
     uint32_t n = 0, items = 0, swaps = 0;
     while (at < end) {
@@ -508,36 +538,39 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       const uint64_t q_row = have ? (p.seq.first + my_row / a.group) * a.q_token +
                                         uint64_t(p.head * a.group + my_row % a.group) * a.c.dim
                                   : 0;
-      float most = 0.f;
-#pragma unroll 4
-      for (uint32_t e = half * (D / 2); e < (half + 1) * (D / 2); e += 8) {
-        if (have && e < a.c.dim) {
-          float x[8];
-          load_acts(a.q, q_row + e, a.type, x);
+      float unit;
+      {
+        float x[D / 16][8];  // all of this thread's part, so that its loads are one latency
 #pragma unroll
-          for (uint32_t k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[k]));
+        for (uint32_t j = 0; j < D / 16; ++j) {
+          const uint32_t e = half * (D / 2) + 8 * j;
+#pragma unroll
+          for (uint32_t k = 0; k < 8; ++k) x[j][k] = 0.f;
+          if (have && e < a.c.dim) load_acts(a.q, q_row + e, a.type, x[j]);
         }
-      }
-      most = fmaxf(most, swap(swaps++ & 1, most));
-      const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
-      const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
-      const float up = __int_as_float((127 + sh) << 23);
-      const float unit = __int_as_float((127 - sh) << 23) * a.scale_log2;
-#pragma unroll 1
-      for (uint32_t e = half * (D / 2); e < (half + 1) * (D / 2); e += 32) {
-        uint32_t w[16];
+        float most = 0.f;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-          float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (have && e + 8 * j < a.c.dim) load_acts(a.q, q_row + e + 8 * j, a.type, x);
+        for (uint32_t j = 0; j < D / 16; ++j)
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) {
-            uint32_t hi, lo;
-            split2(x[2 * k] * up, x[2 * k + 1] * up, hi, lo);
-            w[4 * j + k] = second ? lo : hi;
-          }
+          for (uint32_t k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[j][k]));
+        most = fmaxf(most, swap(swaps++ & 1, most));
+        const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+        const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
+        const float up = __int_as_float((127 + sh) << 23);
+        unit = __int_as_float((127 - sh) << 23) * a.scale_log2;
+#pragma unroll
+        for (uint32_t j0 = 0; j0 < D / 16; j0 += 4) {
+          uint32_t w[16];
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j)
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+              uint32_t hi, lo;
+              split2(x[j0 + j][2 * k] * up, x[j0 + j][2 * k + 1] * up, hi, lo);
+              w[4 * j + k] = second ? lo : hi;
+            }
+          tmem_st16(lanes + W::kQ + half * (D / 4) + 4 * j0, w);
         }
-        tmem_st16(lanes + W::kQ + e / 2, w);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -582,14 +615,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             }
           }
 #pragma unroll
-          for (uint32_t c = 0; c < COLS; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+          for (uint32_t c = 0; c < COLS; c += 2) m4[c / 2 & 3] = max3(m4[c / 2 & 3], s[c], s[c + 1]);
         } else {
           const auto largest = [&](uint32_t c, uint32_t seen) {
             uint32_t u[32];
             tmem_read(sbuf + c, u);
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i)
-              m4[i & 3] = fmaxf(m4[i & 3], seen >> i & 1u ? __uint_as_float(u[i]) : -INFINITY);
+            for (uint32_t i = 0; i < 32; i += 2)
+              m4[i / 2 & 3] = max3(m4[i / 2 & 3], seen >> i & 1u ? __uint_as_float(u[i]) : -INFINITY,
+                                   seen >> (i + 1) & 1u ? __uint_as_float(u[i + 1]) : -INFINITY);
           };
           if (!edge) {
 #pragma unroll
@@ -602,41 +636,49 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if constexpr (SPLIT) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         mx *= unit;
-        // the maximum so far, from the group that has the tile before; this one's for the next
+        // the maximum so far: the group's own, or from the group that has the tile before (and this
+        // one's for the next)
         float before = m;
-        if (p.tile > first_tile) {
-          named_barrier(6 + 2 * quad + (1 - half), 64);
-          before = chain[(1 - half) * 128 + slot];
+        if constexpr (!W::kOwnO) {
+          if (p.tile > first_tile) {
+            named_barrier(6 + 2 * quad + (1 - half), 64);
+            before = chain[(1 - half) * 128 + slot];
+          }
         }
         const bool grow = mx > before + kSlack || (before == -INFINITY && mx > before);
         const float now = grow ? mx : before;
-        if (p.tile + 1 < tiles && at + 1 < end) {
-          chain[half * 128 + slot] = now;
-          __syncwarp();
-          asm volatile("bar.arrive %0, %1;" ::"r"(6 + 2 * quad + half), "r"(64) : "memory");
-        }
-        if (now != m) {  // (the first time both are -inf or the sum is 0)
-          l *= exp2f(m - now);
-          m = now;
-        }
-        if (__any_sync(0xffffffffu, grow) && p.tile > first_tile) {
-          // the output so far is rescaled once the product that adds to it is done (its buffer's product
-          // before that one was done when this tile's S was)
-          const float f = grow ? exp2f(before - now) : 1.f;
-          wait_or_die(live, bar.pv_done((n - 1) % W::kBufs), ((n - 1) / W::kBufs) & 1, a.err, kErrWaitFull);
-          tc_fence_after();
-#pragma unroll 1
-          for (uint32_t c = 0; c < D; c += 16) {
-            uint32_t u[16];
-            tmem_read(lanes + W::kO + c, u);
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
-            tmem_st16(lanes + W::kO + c, u);
+        if constexpr (!W::kOwnO) {
+          if (p.tile + 1 < tiles && at + 1 < end) {
+            chain[half * 128 + slot] = now;
+            __syncwarp();
+            asm volatile("bar.arrive %0, %1;" ::"r"(6 + 2 * quad + half), "r"(64) : "memory");
           }
-          tmem_wait_st();
+        }
+        constexpr uint32_t BACK = W::kOwnO ? 2 : 1;  // the tile whose product this one's adds to
+        if (__any_sync(0xffffffffu, now != m)) {
+          if (now != m) l *= exp2f(m - now);  // (the first time the sum is 0)
+          m = now;
+          if (__any_sync(0xffffffffu, grow) && p.tile >= first_tile + BACK) {
+            // the output so far is rescaled once the product that adds to it is done (its buffer's
+            // product before that one was done when this tile's S was)
+            const float f = grow ? exp2f(before - now) : 1.f;
+            const uint32_t prev = n - BACK;
+            wait_or_die(live, bar.pv_done(prev % W::kBufs), (prev / W::kBufs) & 1, a.err, kErrWaitFull);
+            tc_fence_after();
+#pragma unroll 1
+            for (uint32_t c = 0; c < D; c += 16) {
+              uint32_t u[16];
+              tmem_read(my_o + c, u);
+#pragma unroll
+              for (uint32_t i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
+              tmem_st16(my_o + c, u);
+            }
+            tmem_wait_st();
+          }
         }
         const float ref = m == -INFINITY ? 0.f : m - kLift;
-        float sum[2] = {0.f, 0.f};
+        const float2 unit2 = make_float2(unit, unit), ref2 = make_float2(-ref, -ref);
+        float2 sum = make_float2(0.f, 0.f);
         if constexpr (SPLIT) {
           // weights as two f16; the pair of lanes exchanges so that one has the first parts of all
           // columns, the other the second ones
@@ -645,10 +687,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             uint32_t first[16], last[16];  // words of columns [c, c + 32) and COLS + the same
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              const float w0 = exp2_fast(fmaf(s[c + 2 * i], unit, -ref));
-              const float w1 = exp2_fast(fmaf(s[c + 2 * i + 1], unit, -ref));
-              sum[0] += w0;
-              sum[1] += w1;
+              const float2 z = fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), unit2, ref2);
+              const float w0 = exp2_fast(z.x), w1 = exp2_fast(z.y);
+              sum = add2(sum, make_float2(w0, w1));
               uint32_t hi, lo;
               split2(w0, w1, hi, lo);
               const uint32_t got = __shfl_xor_sync(0xffffffffu, second ? hi : lo, 16);
@@ -665,12 +706,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             tmem_read(sbuf + c, u);
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              float x = exp2_fast(fmaf(__uint_as_float(u[2 * i]), unit, -ref));
-              float y = exp2_fast(fmaf(__uint_as_float(u[2 * i + 1]), unit, -ref));
-              x = seen >> (2 * i) & 1u ? x : 0.f;
-              y = seen >> (2 * i + 1) & 1u ? y : 0.f;
-              sum[0] += x;
-              sum[1] += y;
+              const float2 z = fma2(make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), unit2, ref2);
+              const float x = seen >> (2 * i) & 1u ? exp2_fast(z.x) : 0.f;
+              const float y = seen >> (2 * i + 1) & 1u ? exp2_fast(z.y) : 0.f;
+              sum = add2(sum, make_float2(x, y));
               w[i] = h2(__floats2half2_rn(x, y));
             }
             tmem_st16(sbuf + c / 2, w);
@@ -683,7 +722,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             for (uint32_t c = 0; c < COLS; c += 32) weights(c, seen_word(bits, from + static_cast<int>(c)));
           }
         }
-        l += sum[0] + sum[1];
+        l += sum.x + sum.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -693,15 +732,27 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       // ---- the item's output, half of the columns (and for pairs of lanes a quarter) a thread
       const bool whole = first_tile == 0 && p.tile == tiles;
       float* part = a.part + (uint64_t(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * part_floats(ROWS, D);
-      // the groups' sums, over the later maximum
+      // the groups' sums (and outputs) over the larger maximum
       if constexpr (SPLIT) l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const float last_m = fmaxf(m, swap(swaps++ & 1, m));
-      if (m != last_m) l *= exp2f(m - last_m);
-      m = last_m;
+      const float other_m = swap(swaps++ & 1, m);
+      const float last_m = fmaxf(m, other_m);
+      const float mine = m == last_m ? 1.f : exp2f(m - last_m);
+      const float theirs = other_m == last_m ? 1.f : exp2f(other_m - last_m);
+      l *= mine;
       l += swap(swaps++ & 1, l);
+      m = last_m;
+      // the item's last products (after the swaps both groups are past their last tile's S)
+      const bool two = W::kOwnO && p.tile - first_tile > 1;
       wait_or_die(live, bar.pv_done((n - 1) % W::kBufs), ((n - 1) / W::kBufs) & 1, a.err, kErrWaitFull);
+      if (two) wait_or_die(live, bar.pv_done((n - 2) % W::kBufs), ((n - 2) / W::kBufs) & 1, a.err, kErrWaitFull);
       tc_fence_after();
       const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+      // the last tile's group's O, and the other's: factors of this thread's row
+      const uint32_t last_half = (n - 1) & 1;
+      const uint32_t o_last = lanes + W::kO + (W::kOwnO ? last_half * D : 0);
+      const uint32_t o_other = lanes + W::kO + (1 - last_half) * D;
+      const float f_last = W::kOwnO ? (last_half == half ? mine : theirs) : 1.f;
+      const float f_other = last_half == half ? theirs : mine;
       // every tile's values were decoded before their product: the flags are complete, and the next
       // item's go to the other word
       const unsigned long long odd = *reinterpret_cast<volatile unsigned long long*>(special + (items & 1)) & bits;
@@ -712,16 +763,22 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
 #pragma unroll 1
       for (uint32_t c = 0; c < WIDE; c += 16) {
         uint32_t u[16], v[16];
-        if constexpr (SPLIT) tmem_read(lanes + W::kO + o0 + c, u, lanes + W::kO + o0 + c + WIDE, v);
-        else tmem_read(lanes + W::kO + o0 + c, u);
         float y[16];
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-          if constexpr (SPLIT) {
-            const uint32_t keep = second ? v[i] : u[i], send = second ? u[i] : v[i];
-            y[i] = __uint_as_float(keep) + __uint_as_float(__shfl_xor_sync(0xffffffffu, send, 16));
-          } else {
-            y[i] = __uint_as_float(u[i]);
+        for (uint32_t g = 0; g < (W::kOwnO ? 2u : 1u); ++g) {
+          if (g == 1 && !two) break;
+          const uint32_t o = (g ? o_other : o_last) + o0 + c;
+          const float f = g ? f_other : f_last;
+          if constexpr (SPLIT) tmem_read(o, u, o + WIDE, v);
+          else tmem_read(o, u);
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) {
+            float z = __uint_as_float(u[i]);
+            if constexpr (SPLIT) {
+              const float w = __uint_as_float(v[i]);
+              z = (second ? w : z) + __shfl_xor_sync(0xffffffffu, second ? z : w, 16);
+            }
+            y[i] = g ? fmaf(f, z, y[i]) : f * z;
           }
         }
         for (unsigned long long left = odd; left; left &= left - 1) {
