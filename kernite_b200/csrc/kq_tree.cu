@@ -53,14 +53,15 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   Plan p = {};
   p.split = d.type == KQ_TYPE_F32;
   const uint32_t group = d.n_heads / c.n_kv;
-  p.wide = d.max_drafts * group > (p.split ? 8u : 16u);
-  p.rows = p.wide ? (p.split ? 64 : 128) : p.split ? 8 : 16;
+  p.wide = d.max_drafts * group > 8u;
+  p.rows = p.wide ? (p.split ? 64 : 128) : 8;
   p.tile = p.wide ? 64 : 128;
   const uint64_t row_tiles = (uint64_t(d.max_drafts) * group + p.rows - 1) / p.rows;
   const uint64_t tiles = (uint64_t(d.max_len) + p.tile - 1) / p.tile;
   const uint64_t items = uint64_t(d.n_seq) * c.n_kv * row_tiles;
   if (items > 0x7fffffffu) return fail(KQ_E_INVALID, call, "too many sequences, heads and drafts");
-  p.ctas = static_cast<uint32_t>(std::min<uint64_t>(ctx->sm_count, std::max<uint64_t>(1, items * tiles)));
+  p.ctas = static_cast<uint32_t>(std::min<uint64_t>(
+      uint64_t(ctx->sm_count) * (p.wide ? 1 : tree::narrow_ctas(c.kind, c.pitch)), std::max<uint64_t>(1, items * tiles)));
   p.bytes = uint64_t(p.ctas) * 2 * tree::part_floats(p.rows, c.pitch) * 4;
   *out = p;
   return KQ_OK;
@@ -145,7 +146,6 @@ int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaLaunchKernel", call);
   const uint32_t items = d.n_seq * a.c.n_kv * ((d.max_drafts * a.group + p.rows - 1) / p.rows);
   if (p.rows == 8) launch_join<8, 128>(a, items, p.ctas, s);
-  else if (p.rows == 16) launch_join<16, 128>(a, items, p.ctas, s);
   else if (p.rows == 64) launch_join<64, 64>(a, items, p.ctas, s);
   else launch_join<128, 64>(a, items, p.ctas, s);
   e = cudaGetLastError();

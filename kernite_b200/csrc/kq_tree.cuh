@@ -16,6 +16,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "kq_cache.cuh"
 #include "kq_device.cuh"
 
@@ -173,12 +175,6 @@ __device__ __forceinline__ uint32_t seen_word(unsigned long long bits, int from)
   return from < 0 ? static_cast<uint32_t>(bits << -from) | ((1u << -from) - 1u) : static_cast<uint32_t>(bits >> from);
 }
 
-__device__ __forceinline__ float load_one(const void* p, uint64_t i, uint32_t type) {
-  return type == KQ_TYPE_F32 ? static_cast<const float*>(p)[i]
-         : type == KQ_TYPE_F16 ? __half2float(static_cast<const __half*>(p)[i])
-                               : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-
 __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t type) {
   if (type == KQ_TYPE_F32) static_cast<float*>(p)[i] = v;
   else if (type == KQ_TYPE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
@@ -187,28 +183,37 @@ __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t
 
 // ---------------------------------------------------------------- the warp-MMA kernel
 //
-// mma.sync.m16n8k16 (f16 in, f32 accumulated), all from registers: S = Q K^T with the rows as M, then
-// O += P V with the accumulators of S as the next A operand. A warp takes 16 of a tile's positions and
-// all of an item's rows; the eight warps keep separate maxima, sums and outputs and join them at an
-// item's end. For f32 activations the 16 rows of the MMA are 8 rows twice: the f16 rounding of the
-// operand and the f16 rounding of what that left, so one MMA gives about 22 bits, and sums of the two
-// halves lie in one thread.
+// For few rows (8 an item). mma.sync.m16n8k16 (f16 in, f32 accumulated), operands from registers: the
+// positions are M of S^T = K Q^T, the head's elements M of O^T += V^T P^T, and the rows N = 8 of both, so
+// no part of an MMA is spent on rows that are not there; P^T comes from S^T by movmatrix. A warp takes 16
+// of a tile's 128 positions; the eight warps keep separate maxima, sums and outputs and join them at an
+// item's end. For f32 activations Q and P are sums of two f16 (about 22 bits): two MMAs into one sum.
 //
-// Codes become f16 in registers (exactly: c * scale has at most 11 bits). The order of a contraction
-// is free, so a thread's B fragment of K is four consecutive elements of a row it reads 16 bytes at a
-// time, and the columns of V's fragments are consecutive elements too; position n of an n-tile is
-// pi(n) = 4 (n mod 2) + n / 2, so that with the cache's unit permutation the reads of a warp meet no
-// bank twice.
+// Codes become f16 in registers, exactly. The order of a contraction is free, so a thread's piece of a
+// key row is 16 consecutive bytes, and the element M index of V^T is chosen the same way. Index n of 8
+// positions is position pi(n) = 4 (n mod 2) + n / 2: with the cache's unit permutation the reads of a warp
+// then meet no bank twice.
+//
+// What bounds it: the instructions (about 290 a warp for 16 positions of 128 elements in 8 bits) against
+// the bytes' time. Warps 0 and 1 also start the copies (keys, values) of a tile some tiles ahead.
 
-constexpr uint32_t kWarps = 8;                    // consumers
-constexpr uint32_t kThreads = kWarps * 32 + 32;   // and the producer's warp
+constexpr uint32_t kWarps = 8;
+constexpr uint32_t kThreads = kWarps * 32;
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The transpose of an 8 x 8 matrix of 16-bit elements, two of a row a thread.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
@@ -221,6 +226,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // Codes as f16 pairs: a code under the exponent of 1024 is 1024 + u (8 bits) or 1024 + 16 u (a nibble
@@ -261,8 +289,8 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = h2(__floats2half2_rn(x - f.x, y - f.y));
 }
 
-// How a head of pitch D lies in rows of codes, per kind: BYTES of a row, EK elements of a thread's
-// piece of a key row, EV of its piece of a value row.
+// How a head of pitch D lies in rows of codes, per kind: bytes of a row, EK elements of a thread's piece of
+// a key row, EV of its piece of a value row.
 template <uint32_t KIND, uint32_t D>
 struct Shape {
   static constexpr uint32_t kBits = KIND == KQ_CACHE_F16 ? 16 : KIND == KQ_CACHE_Q8 ? 8 : 4;
@@ -272,23 +300,22 @@ struct Shape {
   static constexpr uint32_t EK = kMost < D / 4 ? kMost : D / 4;
   static constexpr uint32_t EV = kMost < D / 8 ? kMost : D / 8;
   static constexpr uint32_t kSteps = D / 16;      // MMAs along a head
-  static constexpr uint32_t kCols = D / 8;        // n-tiles of the output
   static constexpr bool kPermuted = EV * kBits == 128;  // value pieces of 16 bytes go in the order pi
   static constexpr uint32_t kSlot = kTile * (kRow + kScales);
 };
 
 __device__ __forceinline__ uint32_t pi8(uint32_t n) { return ((n & 1u) << 2) | (n >> 1); }
 
-// First element of step ks of thread t's key pieces.
+// First of the four elements of step ks in thread t's key pieces.
 template <class S>
 __device__ __forceinline__ constexpr uint32_t key_element(uint32_t ks, uint32_t t) {
   return S::EK * (t + 4 * (ks / (S::EK / 4))) + 4 * (ks % (S::EK / 4));
 }
 
-// Element of column n (0..7) of output n-tile j.
+// The element that M index g (h = 0) or g + 8 (h = 1) of O^T's tile j stands for.
 template <class S>
-__device__ __forceinline__ constexpr uint32_t value_element(uint32_t j, uint32_t n) {
-  return S::EV * (8 * (j / S::EV) + (S::kPermuted ? ((n & 1u) << 2 | n >> 1) : n)) + j % S::EV;
+__device__ __forceinline__ uint32_t value_element(uint32_t j, uint32_t g, uint32_t h) {
+  return S::EV * (8 * (j / (S::EV / 2)) + (S::kPermuted ? pi8(g) : g)) + 2 * (j % (S::EV / 2)) + h;
 }
 
 // `B` bytes of shared memory as words.
@@ -315,65 +342,49 @@ __device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
   return v;
 }
 
-// Shared memory of the warp-MMA kernel: the ring of key and value tiles, the join of the warps.
-template <uint32_t KIND, uint32_t D>
-struct Smem {
-  using S = Shape<KIND, D>;
-  static constexpr uint32_t kJoinRow = D + 4;
-  static constexpr uint32_t kJoin = kWarps * 8 * kJoinRow * 4 + 2 * kWarps * 16 * 4;
-  static constexpr uint32_t kQ = D == 256 ? S::kSteps * 32 * 16 : 0;  // operand A where registers are short
-  static constexpr uint32_t kBars = 16 * 16;
-  static constexpr uint32_t kFixed = kJoin + kQ + kBars;
-  static constexpr uint32_t kFit = (224 * 1024 - kFixed) / S::kSlot;
-  static constexpr uint32_t kSlots = kFit > 12 ? 12 : kFit / 2 * 2;  // keys and values in turn
-  static constexpr uint32_t kBytes = kFixed + kSlots * S::kSlot + 128;
-  static_assert(kSlots >= 2, "a key tile and a value tile must fit");
+// The numbers of a tile's pages, as the table has them.
+template <uint32_t TW>
+struct PageIds {
+  uint32_t id[TW / 16];
+
+  __device__ __forceinline__ void load(const TreeArgs& a, const Place& p) {
+    const uint32_t base = p.tile * TW, length = p.seq.length();
+    const int* row = a.pages + uint64_t(p.s) * a.max_pages + (base >> a.c.page_log2);
+    const uint32_t n = (min(TW, length - base) + a.c.page() - 1) >> a.c.page_log2;
+    id[0] = static_cast<uint32_t>(row[0]);
+#pragma unroll
+    for (uint32_t i = 1; i < TW / 16; ++i) id[i] = i < n ? static_cast<uint32_t>(row[i]) : 0u;
+  }
 };
 
-// The producer's copies of one tile of keys (or values): whole records where a page is at most a tile,
-// else its rows and its scales. Pages' numbers sit in the warp's lanes, 32 consecutive ones at a time.
-struct PageWindow {
-  uint32_t s, base;
-  uint32_t id;
-};
-
+// One thread's copies of a tile: whole records where a page is at most a tile, else its rows and its
+// scales. A page that is not there is recorded, and page 0 copied.
 template <class S, uint32_t TW>
-__device__ __forceinline__ void produce_tile(const TreeArgs& a, const Place& p, const uint8_t* src, uint32_t dst,
-                                             uint32_t bar, PageWindow& w) {
-  const uint32_t lane = threadIdx.x % 32;
-  const uint32_t seg_log2 = min(a.c.page_log2, TW == 128 ? 7u : 6u), seg = 1u << seg_log2;
-  const uint32_t base = p.tile * TW;
-  const uint32_t n = (min(TW, p.seq.length() - base) + seg - 1) >> seg_log2;
-  const uint32_t first = base >> a.c.page_log2;
-  const uint32_t pages = ((n << seg_log2) + (1u << a.c.page_log2) - 1) >> a.c.page_log2;
-  if (w.s != p.s || first < w.base || first + pages > w.base + 32) {
-    w.s = p.s;
-    w.base = first;
-    const uint32_t used = (p.seq.length() + a.c.page() - 1) >> a.c.page_log2;
-    w.id = 0;
-    if (first + lane < used) {
-      w.id = static_cast<uint32_t>(a.pages[uint64_t(p.s) * a.max_pages + first + lane]);
-      if (w.id >= a.c.n_pages) {
-        report_error(a.err, kErrCacheRange);
-        w.id = 0;
-      }
-    }
-  }
+__device__ __forceinline__ void copy_tile(const TreeArgs& a, const Place& p, const PageIds<TW>& ids,
+                                          const uint8_t* src, uint32_t dst, uint32_t bar) {
   constexpr uint32_t row = S::kRow + S::kScales;
-  if (lane == 0) mbar_arrive_expect_tx(bar, n * seg * row);
-  __syncwarp();
-  const uint32_t mine = __shfl_sync(0xffffffffu, w.id, ((base + lane * seg) >> a.c.page_log2) - w.base);
-  if (lane < n) {
-    const uint8_t* rec = src + a.c.at(mine, p.head);
-    if (a.c.page_log2 == seg_log2) {
-      bulk_g2s(dst + lane * seg * row, rec, seg * row, bar);
-    } else {
-      const uint32_t at = base & (a.c.page() - 1);
-      bulk_g2s(dst, rec + at * S::kRow, seg * S::kRow, bar);
-      if constexpr (S::kScales != 0)
-        bulk_g2s(dst + seg * S::kRow, rec + a.c.page() * S::kRow + at * S::kScales, seg * S::kScales, bar);
+  const uint32_t base = p.tile * TW, left = p.seq.length() - base;
+  const auto record = [&](uint32_t id) {
+    if (id >= a.c.n_pages) {
+      report_error(a.err, kErrCacheRange);
+      id = 0;
     }
+    return src + a.c.at(id, p.head);
+  };
+  if (a.c.page() > TW) {
+    const uint8_t* rec = record(ids.id[0]);
+    const uint32_t at = base & (a.c.page() - 1);
+    mbar_arrive_expect_tx(bar, TW * row);
+    bulk_g2s(dst, rec + at * S::kRow, TW * S::kRow, bar);
+    if constexpr (S::kScales != 0)
+      bulk_g2s(dst + TW * S::kRow, rec + a.c.page() * S::kRow + at * S::kScales, TW * S::kScales, bar);
+    return;
   }
+  const uint32_t n = (min(TW, left) + a.c.page() - 1) >> a.c.page_log2, bytes = row << a.c.page_log2;
+  mbar_arrive_expect_tx(bar, n * bytes);
+#pragma unroll
+  for (uint32_t i = 0; i < TW / 16; ++i)
+    if (i < n) bulk_g2s(dst + i * bytes, record(ids.id[i]), bytes, bar);
 }
 
 // Positions of a tile in shared memory: where a position's row starts (its swizzle apart) and its
@@ -392,42 +403,6 @@ struct TileView {
   }
 };
 
-// The K operand of n-tile j (positions 16 warp + 8 j + pi(n)): b0, b1 of every step.
-template <uint32_t KIND, uint32_t D>
-__device__ __forceinline__ void key_fragments(const TileView<Shape<KIND, D>>& tile, uint32_t p, uint32_t t,
-                                              uint32_t (&b)[D / 16][2]) {
-  using S = Shape<KIND, D>;
-  constexpr uint32_t B = S::EK * S::kBits / 8;
-#pragma unroll
-  for (uint32_t j = 0; j < D / 4 / S::EK; ++j) {
-    uint32_t w[B / 4];
-    lds_words<B>(tile.code(p, B * (t + 4 * j)), w);
-    if constexpr (KIND == KQ_CACHE_F16) {
-#pragma unroll
-      for (uint32_t k = 0; k < 2; ++k) {
-        b[2 * j + k][0] = w[2 * k];
-        b[2 * j + k][1] = w[2 * k + 1];
-      }
-    } else {
-      const uint32_t byte = lds_u8(tile.scale(p) + S::EK * (t + 4 * j) / 32);
-      const Scale2 s2 = scale2<KIND>(byte, byte);
-#pragma unroll
-      for (uint32_t k = 0; k < S::EK / 4; ++k) {
-        uint32_t lo, hi;
-        if constexpr (KIND == KQ_CACHE_Q8) {
-          lo = decode2(prmt(w[k], kMagic, 0x4140), s2);
-          hi = decode2(prmt(w[k], kMagic, 0x4342), s2);
-        } else {
-          lo = decode2(nibbles(nibble_up(w[k / 2], 2 * (k % 2))), s2);
-          hi = decode2(nibbles(nibble_up(w[k / 2], 2 * (k % 2) + 1)), s2);
-        }
-        b[j * (S::EK / 4) + k][0] = lo;
-        b[j * (S::EK / 4) + k][1] = hi;
-      }
-    }
-  }
-}
-
 // f16 pairs whose exponent is all ones (infinity, NaN) become zero.
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t v) {
   if ((v & 0x7c00u) == 0x7c00u) v &= 0xffff0000u;
@@ -435,75 +410,168 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t v) {
   return v;
 }
 
-// O += P V for the warp's 16 positions. a: P as operand A. EDGE: the tile reaches past the prefix, so
-// rows past the end and values that are not finite count as zero here (P is zero where a position is
-// masked, and zero times those would not be); add_special adds the latter where they are seen.
-template <uint32_t KIND, uint32_t D, bool EDGE>
-__device__ __forceinline__ void value_product(const TileView<Shape<KIND, D>>& tile, uint32_t p0, uint32_t g,
-                                              uint32_t t, uint32_t left, const uint32_t (&a)[4],
-                                              float (&o)[D / 8][4]) {
+// Shared memory of the warp-MMA kernel: the ring of key and value tiles, the join of the warps (four at a
+// time), Q where registers are short. Two CTAs a SM where five slots fit twice, so that one's waits and
+// joins are the other's time.
+template <uint32_t KIND, uint32_t D>
+struct Narrow {
+  using S = Shape<KIND, D>;
+  static constexpr uint32_t kJoinRow = D + 16;
+  static constexpr uint32_t kJoin = 4 * 8 * kJoinRow * 4 + kWarps * 8 * 2 * 4;
+  static constexpr uint32_t kQ = D == 256 ? S::kSteps * 32 * 16 : 0;
+  static constexpr uint32_t kFixed = kJoin + kQ + 256;
+  static constexpr uint32_t kCtas = kFixed + 5 * S::kSlot <= 113 * 1024 ? 2 : 1;
+  static constexpr uint32_t kFit = ((kCtas == 2 ? 113 : 226) * 1024 - kFixed) / S::kSlot;
+  static constexpr uint32_t kSlots = kFit > 12 ? 12 : kFit;  // keys and values in turn
+  static constexpr uint32_t kBytes = kFixed + kSlots * S::kSlot;
+  static_assert(kSlots >= 2, "a tile");
+};
+
+// Where a lane's pieces lie in a tile. Of its two key positions pi(g), pi(g) + 8 and four value positions
+// t, t + 4, t + 8, t + 12 the ones 8 apart differ by 8 rows (their units are permuted alike); a key row's
+// pieces are 4 units apart, the second in the other half of a line of 128 bytes.
+template <class S>
+struct Lane {
+  uint32_t key[2], value[2], key_scale, value_scale;
+
+  __device__ Lane(uint32_t p0, uint32_t g, uint32_t t, uint32_t seg_log2) {
+    const uint32_t in = p0 & ((1u << seg_log2) - 1), pg = S::kPermuted ? pi8(g) : g;
+    const uint32_t seg = ((p0 >> seg_log2) << seg_log2) * (S::kRow + S::kScales);
+    constexpr uint32_t BK = S::EK * S::kBits / 8, BV = S::EV * S::kBits / 8;
+    key[0] = seg + cache_offset(in + pi8(g), BK * t, S::kRow);
+    key[1] = seg + (cache_offset(in + pi8(g), BK * t, S::kRow) ^ 64u);
+    value[0] = seg + cache_offset(in + t, BV * pg, S::kRow);
+    value[1] = seg + cache_offset(in + t + 4, BV * pg, S::kRow);
+    key_scale = seg + (S::kRow << seg_log2) + (in + pi8(g)) * S::kScales + S::EK * t / 32;
+    value_scale = seg + (S::kRow << seg_log2) + (in + t) * S::kScales + S::EV * pg / 32;
+  }
+};
+
+// S^T of the warp's 16 positions: c = sum of K Q^T over the head, q the rows' operand B (hi, and lo).
+template <uint32_t KIND, uint32_t D, bool SPLIT, class Q>
+__device__ __forceinline__ void key_product(uint32_t slot, const Lane<Shape<KIND, D>>& at, const Q& q,
+                                            float (&c)[4]) {
+  using S = Shape<KIND, D>;
+  constexpr uint32_t B = S::EK * S::kBits / 8;
+  float acc[SPLIT ? 4 : 2][4];  // independent sums: an MMA's result is some 20 cycles away
+#pragma unroll
+  for (uint32_t i = 0; i < (SPLIT ? 4 : 2); ++i)
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) acc[i][k] = 0.f;
+#pragma unroll
+  for (uint32_t j = 0; j < D / 4 / S::EK; ++j) {
+    uint32_t w[2][B / 4];
+    Scale2 s[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      lds_words<B>(slot + at.key[j & 1] + h * 8 * S::kRow + (j >> 1) * 128, w[h]);
+      if constexpr (S::kScales != 0) {
+        const uint32_t b = lds_u8(slot + at.key_scale + h * 8 * S::kScales + j * (S::EK * 4 / 32));
+        s[h] = scale2<KIND>(b, b);
+      }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < S::EK / 4; ++k) {
+      uint32_t f[2][2];  // positions pi(g) and pi(g) + 8, the step's first and last two elements
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        if constexpr (KIND == KQ_CACHE_F16) {
+          f[h][0] = w[h][2 * k];
+          f[h][1] = w[h][2 * k + 1];
+        } else if constexpr (KIND == KQ_CACHE_Q8) {
+          f[h][0] = decode2(prmt(w[h][k], kMagic, 0x4140), s[h]);
+          f[h][1] = decode2(prmt(w[h][k], kMagic, 0x4342), s[h]);
+        } else {
+          f[h][0] = decode2(nibbles(nibble_up(w[h][k / 2], 2 * (k % 2))), s[h]);
+          f[h][1] = decode2(nibbles(nibble_up(w[h][k / 2], 2 * (k % 2) + 1)), s[h]);
+        }
+      }
+      const uint32_t ks = j * (S::EK / 4) + k;
+      uint32_t b[4];
+      q(ks, b);
+      mma16816(acc[ks & 1], f[0][0], f[1][0], f[0][1], f[1][1], b[0], b[1]);
+      if constexpr (SPLIT) mma16816(acc[2 + (ks & 1)], f[0][0], f[1][0], f[0][1], f[1][1], b[2], b[3]);
+    }
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    c[k] = acc[0][k] + acc[1][k];
+    if constexpr (SPLIT) c[k] += acc[2][k] + acc[3][k];
+  }
+}
+
+// O^T += V^T P^T of the warp's 16 positions, b the weights as operand B (hi, and lo). EDGE: the tile
+// reaches past the prefix, so rows past the end (left: positions the tile has) and values that are not
+// finite count as zero here (P is zero where a position is masked, and zero times those would not be);
+// add_special adds the latter where they are seen.
+template <uint32_t KIND, uint32_t D, bool SPLIT, bool EDGE>
+__device__ __forceinline__ void value_product(uint32_t slot, const Lane<Shape<KIND, D>>& at, uint32_t first,
+                                              uint32_t left, const uint32_t (&b)[4], float (&o)[D / 16][4]) {
   using S = Shape<KIND, D>;
   constexpr uint32_t B = S::EV * S::kBits / 8;
-  const uint32_t pg = S::kPermuted ? pi8(g) : g;
-  const uint32_t p[4] = {p0 + t, p0 + 4 + t, p0 + 8 + t, p0 + 12 + t};
 #pragma unroll
   for (uint32_t jj = 0; jj < D / 8 / S::EV; ++jj) {
     uint32_t w[4][B / 4];
     uint32_t byte[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lds_words<B>(tile.code(p[i], B * (pg + 8 * jj)), w[i]);
+    for (uint32_t i = 0; i < 4; ++i) {  // position first + 4 i
+      lds_words<B>(slot + at.value[i & 1] + (i >> 1) * 8 * S::kRow + jj * 128, w[i]);
+      const bool there = !EDGE || first + 4 * i < left;
       if constexpr (KIND == KQ_CACHE_F16) {
         if constexpr (EDGE) {
 #pragma unroll
-          for (uint32_t k = 0; k < B / 4; ++k) w[i][k] = p[i] < left ? finite_or_zero(w[i][k]) : 0u;
+          for (uint32_t k = 0; k < B / 4; ++k) w[i][k] = there ? finite_or_zero(w[i][k]) : 0u;
         }
       } else {
-        byte[i] = lds_u8(tile.scale(p[i]) + S::EV * (pg + 8 * jj) / 32);
-        if constexpr (EDGE) byte[i] = p[i] < left && byte[i] < 0xf8u ? byte[i] : 0u;
+        byte[i] = lds_u8(slot + at.value_scale + i * 4 * S::kScales + jj * (S::EV * 8 / 32));
+        if constexpr (EDGE) byte[i] = there && byte[i] < 0xf8u ? byte[i] : 0u;
       }
     }
-    const Scale2 s2[2] = {scale2<KIND>(byte[0], byte[1]), scale2<KIND>(byte[2], byte[3])};
+    Scale2 s[2];
+    if constexpr (S::kScales != 0) {
+      s[0] = scale2<KIND>(byte[0], byte[1]);
+      s[1] = scale2<KIND>(byte[2], byte[3]);
+    }
+    const auto product = [&](uint32_t j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+      mma16816(o[j], a0, a1, a2, a3, b[0], b[1]);
+      if constexpr (SPLIT) mma16816(o[j], a0, a1, a2, a3, b[2], b[3]);
+    };
 #pragma unroll
     for (uint32_t k = 0; k < B / 4; ++k) {
-      // operand pairs (position p[0], p[1]) and (p[2], p[3]) of each element of word k
+      // pairs (position first, + 4) and (+ 8, + 12) of each element of word k
+      const uint32_t j0 = jj * (S::EV / 2);
       if constexpr (KIND == KQ_CACHE_F16) {
-        mma16816(o[jj * S::EV + 2 * k], a, prmt(w[0][k], w[1][k], 0x5410), prmt(w[2][k], w[3][k], 0x5410));
-        mma16816(o[jj * S::EV + 2 * k + 1], a, prmt(w[0][k], w[1][k], 0x7632), prmt(w[2][k], w[3][k], 0x7632));
+        product(j0 + k, prmt(w[0][k], w[1][k], 0x5410), prmt(w[0][k], w[1][k], 0x7632),
+                prmt(w[2][k], w[3][k], 0x5410), prmt(w[2][k], w[3][k], 0x7632));
       } else if constexpr (KIND == KQ_CACHE_Q8) {
 #pragma unroll
         for (uint32_t half = 0; half < 2; ++half) {
           const uint32_t x = prmt(w[0][k], w[1][k], half ? 0x7362 : 0x5140);
           const uint32_t y = prmt(w[2][k], w[3][k], half ? 0x7362 : 0x5140);
-          mma16816(o[jj * S::EV + 4 * k + 2 * half], a, decode2(prmt(x, kMagic, 0x4140), s2[0]),
-                   decode2(prmt(y, kMagic, 0x4140), s2[1]));
-          mma16816(o[jj * S::EV + 4 * k + 2 * half + 1], a, decode2(prmt(x, kMagic, 0x4342), s2[0]),
-                   decode2(prmt(y, kMagic, 0x4342), s2[1]));
+          product(j0 + 2 * k + half, decode2(prmt(x, kMagic, 0x4140), s[0]), decode2(prmt(x, kMagic, 0x4342), s[0]),
+                  decode2(prmt(y, kMagic, 0x4140), s[1]), decode2(prmt(y, kMagic, 0x4342), s[1]));
         }
       } else {
+        // elements 2 e at nibbles e of the low halves, 2 e + 1 of the high ones
+        const uint32_t x0 = prmt(w[0][k], w[1][k], 0x5410), x1 = prmt(w[0][k], w[1][k], 0x7632);
+        const uint32_t y0 = prmt(w[2][k], w[3][k], 0x5410), y1 = prmt(w[2][k], w[3][k], 0x7632);
 #pragma unroll
-        for (uint32_t odd = 0; odd < 2; ++odd) {
-          const uint32_t x = prmt(w[0][k], w[1][k], odd ? 0x7632 : 0x5410);
-          const uint32_t y = prmt(w[2][k], w[3][k], odd ? 0x7632 : 0x5410);
-#pragma unroll
-          for (uint32_t e = 0; e < 4; ++e)
-            mma16816(o[jj * S::EV + 8 * k + 2 * e + odd], a, decode2(nibbles(nibble_up(x, e)), s2[0]),
-                     decode2(nibbles(nibble_up(y, e)), s2[1]));
-        }
+        for (uint32_t e = 0; e < 4; ++e)
+          product(j0 + 4 * k + e, decode2(nibbles(nibble_up(x0, e)), s[0]), decode2(nibbles(nibble_up(x1, e)), s[0]),
+                  decode2(nibbles(nibble_up(y0, e)), s[1]), decode2(nibbles(nibble_up(y1, e)), s[1]));
       }
     }
   }
 }
 
-// The values value_product<EDGE> left out, of the warp's positions below `left`: infinities and NaN
-// reach the rows that see their position (bits: the mask words of rows g and g + 8; in split form
-// both are row g's and the sums of the two halves are what counts).
-template <uint32_t KIND, uint32_t D, bool SPLIT>
-__device__ __forceinline__ void add_special(const TileView<Shape<KIND, D>>& tile, uint32_t p0, uint32_t base,
-                                            uint32_t left, const Seq& seq, const unsigned long long (&bits)[2],
-                                            float (&o)[D / 8][4]) {
+// The values value_product<EDGE> left out, of the warp's positions p0 .. p0 + 15 below `left`: infinities
+// and NaN reach the rows that see their position. bits: the mask words of rows 2 t and 2 t + 1.
+template <uint32_t KIND, uint32_t D>
+__device__ __noinline__ void add_special(const TileView<Shape<KIND, D>>& tile, uint32_t p0, uint32_t base,
+                                         uint32_t left, const Seq& seq, const unsigned long long (&bits)[2],
+                                         float (&o)[D / 16][4]) {
   using S = Shape<KIND, D>;
-  const uint32_t lane = threadIdx.x % 32, t = lane & 3u;
+  const uint32_t lane = threadIdx.x % 32, g = lane >> 2;
   for (uint32_t p = p0; p < p0 + 16 && p < left; ++p) {
     bool odd = false;
     if constexpr (KIND == KQ_CACHE_F16) {
@@ -518,10 +586,10 @@ __device__ __forceinline__ void add_special(const TileView<Shape<KIND, D>>& tile
     }
     if (!__any_sync(0xffffffffu, odd)) continue;
 #pragma unroll
-    for (uint32_t j = 0; j < D / 8; ++j)
+    for (uint32_t j = 0; j < D / 16; ++j)
 #pragma unroll
-      for (uint32_t c = 0; c < 2; ++c) {
-        const uint32_t e = value_element<S>(j, 2 * t + c);
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t e = value_element<S>(j, g, h);
         float add = 0.f;
         if constexpr (KIND == KQ_CACHE_F16) {
           const uint32_t v = lds_u16(tile.code(p, 2 * e));
@@ -529,34 +597,30 @@ __device__ __forceinline__ void add_special(const TileView<Shape<KIND, D>>& tile
         } else {
           if (lds_u8(tile.scale(p) + e / 32) >= 0xf8u) add = __int_as_float(0x7fc00000);
         }
-        if (sees(bits[0], base + p, seq)) o[j][c] += add;
-        if constexpr (!SPLIT) {
-          if (sees(bits[1], base + p, seq)) o[j][2 + c] += add;
-        }
+        if (sees(bits[0], base + p, seq)) o[j][2 * h] += add;
+        if (sees(bits[1], base + p, seq)) o[j][2 * h + 1] += add;
       }
   }
 }
 
 // Weights are kept times 2^kLift of the reference they were taken to, and outputs are rescaled to a new
-// reference only when the maximum is more than 2^kSlack above it, which after an item's first tile hardly
+// reference only when a logit is more than 2^kSlack above it, which after an item's first tile hardly
 // happens: the largest weight is below 2^15, in f16's range, and what f16 loses of a small one (2^-25) is
 // 2^-27 of the reference's own weight at most.
 constexpr float kLift = 2.f;
 constexpr float kSlack = 13.f;
 
 template <uint32_t KIND, uint32_t D, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(const __grid_constant__ TreeArgs a) {
   using S = Shape<KIND, D>;
-  using M = Smem<KIND, D>;
-  constexpr uint32_t ROWS = SPLIT ? 8 : 16;
-  constexpr uint32_t NS = M::kSlots;
+  using M = Narrow<KIND, D>;
+  constexpr uint32_t ROWS = 8, NS = M::kSlots;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* join = reinterpret_cast<float*>(smem + NS * S::kSlot);
-  float* join_m = join + kWarps * 8 * M::kJoinRow;  // [warp][16]
-  float* join_l = join_m + kWarps * 16;
-  uint4* q_smem = reinterpret_cast<uint4*>(join_l + kWarps * 16);
-  const uint32_t bars = smem_u32(smem) + NS * S::kSlot + M::kJoin + M::kQ;  // full, empty of each slot
-  const uint32_t ring = smem_u32(smem);
+  float* join = reinterpret_cast<float*>(smem + NS * S::kSlot);  // 4 warps x 8 rows
+  float* join_m = join + 4 * 8 * M::kJoinRow;                    // [warp][row], then sums
+  float* join_l = join_m + kWarps * 8;
+  uint4* q_smem = reinterpret_cast<uint4*>(join_l + kWarps * 8);
+  const uint32_t ring = smem_u32(smem), bars = ring + NS * S::kSlot + M::kJoin + M::kQ;  // full, empty of each slot
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < NS; ++i) {
@@ -572,213 +636,204 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
   uint64_t at = range_start(total, blockIdx.x, ctas);
   const uint64_t end = range_start(total, blockIdx.x + 1, ctas);
   Place p = locate<ROWS, kTile>(a, at);
-  uint32_t it = 0;    // slots used so far: tiles of keys and of values in turn
-  bool live = true;   // no wait has given up
+  bool live = true;  // no wait has given up
 
-  if (warp == kWarps) {
-    PageWindow window = {0xffffffffu, 0, 0};
-    while (at < end) {
-      const uint32_t tiles = position_tiles<kTile>(p.seq);
-      for (; p.tile < tiles && at < end; ++p.tile, ++at) {
-#pragma unroll 1
-        for (uint32_t kv = 0; kv < 2; ++kv, ++it) {
-          const uint32_t slot = it % NS;
-          if (it >= NS && live && !mbar_wait(bars + 16 * slot + 8, (it / NS - 1) & 1)) {
-            report_error(a.err, kErrWaitEmpty);
-            live = false;
-          }
-          live = __all_sync(0xffffffffu, live);
-          if (live) produce_tile<S, kTile>(a, p, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bars + 16 * slot, window);
-        }
+  // ---- copies: thread 0 of warp 0 keys (uses 2 i of the ring), of warp 1 values (2 i + 1)
+  const bool copies = warp < 2 && lane == 0;
+  Place cp = p;
+  uint64_t c_at = at;
+  uint32_t c_use = warp;
+  // starts the copies of uses below `upto`; all but the NS last uses before it have been read
+  const auto copy = [&](uint32_t upto) {
+    while (c_use < upto && c_at < end) {
+      const uint32_t slot = c_use % NS;
+      if (c_use >= NS && live && !mbar_wait(bars + 16 * slot + 8, (c_use / NS - 1) & 1)) {
+        report_error(a.err, kErrWaitEmpty);
+        live = false;
       }
-      if (at < end) next_item<ROWS>(a, p);
+      if (!live) return;
+      PageIds<kTile> ids;
+      ids.load(a, cp);
+      copy_tile<S, kTile>(a, cp, ids, warp ? a.c.v : a.c.k, ring + slot * S::kSlot, bars + 16 * slot);
+      c_use += 2;
+      ++c_at;
+      if (++cp.tile == position_tiles<kTile>(cp.seq) && c_at < end) next_item<ROWS>(a, cp);
     }
-    return;
-  }
+  };
+  if (copies) copy(NS);
+  __syncwarp();
 
   const uint32_t g = lane >> 2, t = lane & 3u;
-  const uint32_t seg_log2 = min(a.c.page_log2, 7u);
+  const uint32_t seg_log2 = min(a.c.page_log2, 7u), p0 = warp * 16;
+  const Lane<S> place(p0, g, t, seg_log2);
+  uint32_t it = 0;  // uses of the ring read
   while (at < end) {
-    // ---- the item's rows as operand A, each row scaled by a power of two to a largest element in
-    // [2^7, 2^8), so that f16's range fits any q
+    // ---- the item's rows as operand B (row n = g), each scaled by a power of two to a largest element in
+    // [2^7, 2^8), so that f16's range fits any q; and what rows 2 t, 2 t + 1 need
     const uint32_t rows = p.seq.drafts * a.group;
-    uint32_t r[2], tok[2];
-    unsigned long long bits[2];
-    float unit[2];  // logits in log2 units a unit of the scaled product
-    uint32_t qa[D == 256 ? 1 : S::kSteps][4];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      r[half] = p.rows * ROWS + g + (SPLIT ? 0 : 8 * half);
-      const bool have = r[half] < rows;
-      tok[half] = have ? r[half] / a.group : 0;
-      bits[half] = have ? mask_bits(a, p.seq, tok[half]) : 0ull;
-      if (SPLIT && half == 1) {
-        unit[1] = unit[0];
-        continue;
-      }
-      const uint64_t row = (p.seq.first + tok[half]) * a.q_token +
-                           uint64_t(p.head * a.group + r[half] % a.group) * a.c.dim;
+    uint32_t qb[D == 256 ? 1 : S::kSteps][4];
+    float2 unit2;  // logits in log2 units a unit of the scaled product, of rows 2 t and 2 t + 1
+    {
+      const uint32_t r = p.rows * ROWS + g;
+      const bool have = r < rows;
+      const uint64_t row = have ? (p.seq.first + r / a.group) * a.q_token +
+                                      uint64_t(p.head * a.group + r % a.group) * a.c.dim
+                                : 0;
       float most = 0.f;
+      const auto load4 = [&](uint32_t ks, float (&x)[4]) {
+        const uint32_t e = key_element<S>(ks, t);
+        x[0] = x[1] = x[2] = x[3] = 0.f;
+        if (!have || e >= a.c.dim) return;
+        if (a.type == KQ_TYPE_F32) load_act<float, 4>(static_cast<const float*>(a.q) + row + e, x);
+        else if (a.type == KQ_TYPE_F16) load_act<__half, 4>(static_cast<const __half*>(a.q) + row + e, x);
+        else load_act<__nv_bfloat16, 4>(static_cast<const __nv_bfloat16*>(a.q) + row + e, x);
+      };
 #pragma unroll
-      for (uint32_t ks = 0; ks < S::kSteps; ++ks)
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const uint32_t e = key_element<S>(ks, t) + i;
-          if (have && e < a.c.dim) most = fmaxf(most, fabsf(load_one(a.q, row + e, a.type)));
-        }
+      for (uint32_t ks = 0; ks < S::kSteps; ++ks) {
+        float x[4];
+        load4(ks, x);
+        most = fmaxf(most, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+      }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       // 2^(7 - floor(log2(most))), kept inside f32's normal range; 1 for a row of zeros (or infinities)
       const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
       const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
       const float up = __int_as_float((127 + sh) << 23);
-      unit[half] = __int_as_float((127 - sh) << 23) * a.scale_log2;
+      const float unit = __int_as_float((127 - sh) << 23) * a.scale_log2;
+      unit2.x = __shfl_sync(0xffffffffu, unit, 8 * t);
+      unit2.y = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
 #pragma unroll
       for (uint32_t ks = 0; ks < S::kSteps; ++ks) {
         float x[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const uint32_t e = key_element<S>(ks, t) + i;
-          x[i] = have && e < a.c.dim ? load_one(a.q, row + e, a.type) * up : 0.f;
-        }
+        load4(ks, x);
         uint32_t hi0, lo0, hi1, lo1;
-        split2(x[0], x[1], hi0, lo0);
-        split2(x[2], x[3], hi1, lo1);
+        split2(x[0] * up, x[1] * up, hi0, lo0);
+        split2(x[2] * up, x[3] * up, hi1, lo1);
         if constexpr (D == 256) {
-          // every warp writes the same words; the barrier below orders them before the reads
-          uint32_t* to = reinterpret_cast<uint32_t*>(q_smem + ks * 32 + lane);
-          if constexpr (SPLIT) {
-            to[0] = hi0;
-            to[1] = lo0;
-            to[2] = hi1;
-            to[3] = lo1;
-          } else {
-            to[half] = hi0;
-            to[2 + half] = hi1;
-          }
-        } else if constexpr (SPLIT) {
-          qa[ks][0] = hi0;
-          qa[ks][1] = lo0;
-          qa[ks][2] = hi1;
-          qa[ks][3] = lo1;
+          // every warp writes the same words, and reads its own
+          q_smem[ks * 32 + lane] = make_uint4(hi0, hi1, lo0, lo1);
         } else {
-          qa[ks][half] = hi0;
-          qa[ks][2 + half] = hi1;
+          qb[ks][0] = hi0;
+          qb[ks][1] = hi1;
+          qb[ks][2] = lo0;
+          qb[ks][3] = lo1;
         }
       }
+      if constexpr (D == 256) __syncwarp();
     }
-    if constexpr (D == 256) __syncwarp();
-
-    float o[D / 8][4];
+    const auto q_at = [&](uint32_t ks, uint32_t (&b)[4]) {
+      if constexpr (D == 256) {
+        const uint4 w = q_smem[ks * 32 + lane];
+        b[0] = w.x;
+        b[1] = w.y;
+        b[2] = w.z;
+        b[3] = w.w;
+      } else {
 #pragma unroll
-    for (uint32_t j = 0; j < D / 8; ++j)
+        for (uint32_t i = 0; i < 4; ++i) b[i] = qb[ks][i];
+      }
+    };
+
+    float o[D / 16][4];
+#pragma unroll
+    for (uint32_t j = 0; j < D / 16; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float m[2] = {-INFINITY, -INFINITY};  // rows 2 t, 2 t + 1, the same in all g
+    float2 l = make_float2(0.f, 0.f), minus = make_float2(0.f, 0.f);  // sums (this thread's), -(m - kLift)
+    float limit = -INFINITY;  // weights' exponents above this want a new reference
 
     const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
     for (; p.tile < tiles && at < end; ++p.tile, ++at, it += 2) {
+      if (copies) copy(it + NS);
+      __syncwarp();
       const uint32_t base = p.tile * kTile, left = p.seq.length() - base;  // positions left in the cache
-      const uint32_t p0 = warp * 16;
       const bool edge = base + kTile > p.seq.prefix;
-      const uint32_t ks_slot = it % NS, v_slot = (it + 1) % NS;
-      if (live && !mbar_wait(bars + 16 * ks_slot, (it / NS) & 1)) {
+      const uint32_t k_slot = it % NS, v_slot = (it + 1) % NS;
+      if (live && !mbar_wait(bars + 16 * k_slot, (it / NS) & 1)) {
         report_error(a.err, kErrWaitFull);
         live = false;
       }
-      live = __all_sync(0xffffffffu, live);
-      uint32_t pa[4];
+      __syncwarp();
+      uint32_t pb[4];
+      unsigned long long bits[2];
       if (p0 < left) {
-        const TileView<S> keys = {ring + ks_slot * S::kSlot, seg_log2};
-        float c[2][4];
+        float c[4];
+        key_product<KIND, D, SPLIT>(ring + k_slot * S::kSlot, place, q_at, c);
+        // rows 2 t, 2 t + 1 at position pi(g), then at pi(g) + 8: logits in log2 units, to the reference
+        float2 z0 = fma2(make_float2(c[0], c[1]), unit2, minus), z1 = fma2(make_float2(c[2], c[3]), unit2, minus);
+        if (edge) {
 #pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) {
-          uint32_t b[S::kSteps][2];
-          key_fragments<KIND, D>(keys, p0 + 8 * j + pi8(g), t, b);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
-#pragma unroll
-          for (uint32_t ks = 0; ks < S::kSteps; ++ks) {
-            if constexpr (D == 256) {
-              const uint4 w = q_smem[ks * 32 + lane];
-              const uint32_t qw[4] = {w.x, w.y, w.z, w.w};
-              mma16816(c[j], qw, b[ks][0], b[ks][1]);
-            } else {
-              mma16816(c[j], qa[ks], b[ks][0], b[ks][1]);
-            }
+          for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t r = p.rows * ROWS + 2 * t + i;
+            bits[i] = r < rows ? mask_bits(a, p.seq, r / a.group) : 0ull;
           }
+          const uint32_t pos = base + p0 + pi8(g);
+          if (!sees(bits[0], pos, p.seq)) z0.x = -INFINITY;
+          if (!sees(bits[1], pos, p.seq)) z0.y = -INFINITY;
+          if (!sees(bits[0], pos + 8, p.seq)) z1.x = -INFINITY;
+          if (!sees(bits[1], pos + 8, p.seq)) z1.y = -INFINITY;
         }
+        if (__any_sync(0xffffffffu, max3(fmaxf(z0.x, z0.y), z1.x, z1.y) > limit)) {
+          // a new reference for the rows that want one (all rows have one after this, but those that see
+          // nothing yet, whose weights are zero whatever it is)
+          float top[2] = {fmaxf(z0.x, z1.x), fmaxf(z0.y, z1.y)}, f[2], down[2];
+#pragma unroll
+          for (uint32_t i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], s));
+            const float old = i ? minus.y : minus.x;
+            const bool fresh = m[i] == -INFINITY;
+            const float now = fresh || top[i] > kSlack + kLift ? top[i] - old : m[i];  // a logit itself
+            const float next = now == -INFINITY ? 0.f : kLift - now;
+            f[i] = fresh ? 0.f : exp2f(m[i] - now);
+            down[i] = next - old;
+            m[i] = now;
+            (i ? minus.y : minus.x) = next;
+          }
+          z0 = add2(z0, make_float2(down[0], down[1]));
+          z1 = add2(z1, make_float2(down[0], down[1]));
+          l.x *= f[0];
+          l.y *= f[1];
+#pragma unroll
+          for (uint32_t j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) o[j][i] *= f[i & 1];
+          limit = __any_sync(0xffffffffu, m[0] == -INFINITY || m[1] == -INFINITY) ? -INFINITY : kSlack + kLift;
+        }
+        const float2 w0 = make_float2(exp2_fast(z0.x), exp2_fast(z0.y));
+        const float2 w1 = make_float2(exp2_fast(z1.x), exp2_fast(z1.y));
+        l = add2(l, add2(w0, w1));
         if constexpr (SPLIT) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            c[j][0] += c[j][2];
-            c[j][1] += c[j][3];
-          }
-        }
-        // ---- logits in log2 units, masked; the running maximum; the weights
-        constexpr int HALVES = SPLIT ? 1 : 2;
-#pragma unroll
-        for (int half = 0; half < HALVES; ++half) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& v = c[j][2 * half + i];
-              v *= unit[half];
-              if (edge && !sees(bits[half], base + p0 + 8 * j + 4 * i + t, p.seq)) v = -INFINITY;
-              mx = fmaxf(mx, v);
-            }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const bool grow = mx > m[half] + kSlack || (m[half] == -INFINITY && mx > m[half]);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float to = grow ? mx : m[half];
-            const float f = grow ? exp2f(m[half] - to) : 1.f;
-            m[half] = to;
-            l[half] *= f;
-#pragma unroll
-            for (uint32_t j = 0; j < D / 8; ++j) {
-              o[j][2 * half] *= f;
-              o[j][2 * half + 1] *= f;
-              if constexpr (SPLIT) {
-                o[j][2] *= f;
-                o[j][3] *= f;
-              }
-            }
-          }
-          const float ref = m[half] == -INFINITY ? 0.f : m[half] - kLift;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float w0 = exp2_fast(c[j][2 * half] - ref), w1 = exp2_fast(c[j][2 * half + 1] - ref);
-            if constexpr (SPLIT) {
-              split2(w0, w1, pa[2 * j], pa[2 * j + 1]);
-              l[0] += w0 + w1;
-            } else {
-              const __half2 h = __floats2half2_rn(w0, w1);
-              pa[2 * j + half] = h2(h);
-              // the sum of what multiplies the values: rounding the weights then leaves their mean
-              // weight exact
-              const float2 f = __half22float2(h);
-              l[half] += f.x + f.y;
-            }
-          }
+          uint32_t hi0, lo0, hi1, lo1;
+          split2(w0.x, w0.y, hi0, lo0);
+          split2(w1.x, w1.y, hi1, lo1);
+          pb[0] = transpose8(hi0);
+          pb[1] = transpose8(hi1);
+          pb[2] = transpose8(lo0);
+          pb[3] = transpose8(lo1);
+        } else {
+          pb[0] = transpose8(h2(__floats2half2_rn(w0.x, w0.y)));
+          pb[1] = transpose8(h2(__floats2half2_rn(w1.x, w1.y)));
+          pb[2] = pb[3] = 0;
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars + 16 * ks_slot + 8);
+      if (lane == 0) mbar_arrive(bars + 16 * k_slot + 8);
       if (live && !mbar_wait(bars + 16 * v_slot, ((it + 1) / NS) & 1)) {
         report_error(a.err, kErrWaitFull);
         live = false;
       }
-      live = __all_sync(0xffffffffu, live);
+      __syncwarp();
       if (p0 < left) {
-        const TileView<S> values = {ring + v_slot * S::kSlot, seg_log2};
+        const uint32_t slot = ring + v_slot * S::kSlot;
         if (edge) {
-          value_product<KIND, D, true>(values, p0, g, t, left, pa, o);
-          add_special<KIND, D, SPLIT>(values, p0, base, left, p.seq, bits, o);
+          value_product<KIND, D, SPLIT, true>(slot, place, p0 + t, left, pb, o);
+          const TileView<S> values = {slot, seg_log2};
+          add_special<KIND, D>(values, p0, base, left, p.seq, bits, o);
         } else {
-          value_product<KIND, D, false>(values, p0, g, t, left, pa, o);
+          value_product<KIND, D, SPLIT, false>(slot, place, p0 + t, left, pb, o);
         }
       }
       __syncwarp();
@@ -787,54 +842,90 @@ __global__ void __launch_bounds__(kThreads, 1) tree_kernel(const __grid_constant
     const bool whole = first_tile == 0 && p.tile == tiles;
     float* part = a.part + (uint64_t(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * part_floats(ROWS, D);
 
-    // ---- the warps' maxima, sums and outputs joined, eight rows at a time
+    // ---- the warps' maxima, sums and outputs joined: warps 4-7 give theirs to 0-3, register for
+    // register; those lay rows out, and a warp sums a row
+    constexpr uint32_t RAW = D / 16 * 4 + 4;  // floats a lane gives
+    static_assert(RAW * 32 <= 8 * M::kJoinRow, "a warp's registers fit its rows");
+    float* mine = join + (warp & 3) * 8 * M::kJoinRow;
+    if (warp >= 4) {
 #pragma unroll
-    for (int half = 0; half < (SPLIT ? 1 : 2); ++half) {
-      float sum = l[half];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == 0) {
-        join_m[warp * 16 + g] = m[half];
-        join_l[warp * 16 + g] = sum;
+      for (uint32_t j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) mine[(j * 4 + i) * 32 + lane] = o[j][i];
+      mine[(RAW - 4) * 32 + lane] = m[0];
+      mine[(RAW - 3) * 32 + lane] = m[1];
+      mine[(RAW - 2) * 32 + lane] = l.x;
+      mine[(RAW - 1) * 32 + lane] = l.y;
+    }
+    __syncthreads();
+    if (warp < 4) {
+      float f[2], h[2];
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        const float other = mine[(RAW - 4 + i) * 32 + lane], now = fmaxf(m[i], other);
+        f[i] = m[i] == now ? 1.f : exp2f(m[i] - now);
+        h[i] = other == now ? 1.f : exp2f(other - now);
+        m[i] = now;
       }
+      l.x = fmaf(h[0], mine[(RAW - 2) * 32 + lane], f[0] * l.x);
+      l.y = fmaf(h[1], mine[(RAW - 1) * 32 + lane], f[1] * l.y);
 #pragma unroll
-      for (uint32_t j = 0; j < D / 8; ++j)
+      for (uint32_t j = 0; j < D / 16; ++j)
 #pragma unroll
-        for (uint32_t c = 0; c < 2; ++c)
-          join[(warp * 8 + g) * M::kJoinRow + value_element<S>(j, 2 * t + c)] =
-              SPLIT ? o[j][c] + o[j][2 + c] : o[j][2 * half + c];
-      named_barrier(1, kWarps * 32);
-      const uint32_t row = warp;  // a warp a row now
+        for (uint32_t i = 0; i < 4; ++i) o[j][i] = fmaf(h[i & 1], mine[(j * 4 + i) * 32 + lane], f[i & 1] * o[j][i]);
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1) {
+        l.x += __shfl_xor_sync(0xffffffffu, l.x, s);
+        l.y += __shfl_xor_sync(0xffffffffu, l.y, s);
+      }
+      __syncwarp();
+#pragma unroll
+      for (uint32_t j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          mine[(2 * t + (i & 1)) * M::kJoinRow + value_element<S>(j, g, i >> 1)] = o[j][i];
+      if (g == 0) {
+        join_m[warp * 8 + 2 * t] = m[0];
+        join_m[warp * 8 + 2 * t + 1] = m[1];
+        join_l[warp * 8 + 2 * t] = l.x;
+        join_l[warp * 8 + 2 * t + 1] = l.y;
+      }
+    }
+    __syncthreads();
+    {
+      const uint32_t row = warp, rr = p.rows * ROWS + row;
       float mx = -INFINITY;
 #pragma unroll
-      for (uint32_t w = 0; w < kWarps; ++w) mx = fmaxf(mx, join_m[w * 16 + row]);
+      for (uint32_t w = 0; w < 4; ++w) mx = fmaxf(mx, join_m[w * 8 + row]);
       const float ref = mx == -INFINITY ? 0.f : mx;
-      float f[kWarps], den = 0.f;
+      float f[4], den = 0.f;
 #pragma unroll
-      for (uint32_t w = 0; w < kWarps; ++w) {
-        f[w] = exp2f(join_m[w * 16 + row] - ref);
-        den = fmaf(f[w], join_l[w * 16 + row], den);
+      for (uint32_t w = 0; w < 4; ++w) {
+        f[w] = exp2f(join_m[w * 8 + row] - ref);
+        den = fmaf(f[w], join_l[w * 8 + row], den);
       }
-      const uint32_t rr = p.rows * ROWS + 8 * half + row;
       if (rr < rows) {
         const float inv = whole ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
         const uint64_t to = (p.seq.first + rr / a.group) * a.out_token +
                             uint64_t(p.head * a.group + rr % a.group) * a.c.dim;
+#pragma unroll
         for (uint32_t e = lane; e < D; e += 32) {
           float v = 0.f;
 #pragma unroll
-          for (uint32_t w = 0; w < kWarps; ++w) v = fmaf(f[w], join[(w * 8 + row) * M::kJoinRow + e], v);
-          if (!whole) part[(8 * half + row) * D + e] = v;
+          for (uint32_t w = 0; w < 4; ++w) v = fmaf(f[w], join[(w * 8 + row) * M::kJoinRow + e], v);
+          if (!whole) part[row * D + e] = v;
           else if (e < a.c.dim) store_one(a.out, to + e, v * inv, a.type);
         }
         if (!whole && lane == 0) {
-          part[ROWS * D + 8 * half + row] = mx;
-          part[ROWS * (D + 1) + 8 * half + row] = den;
+          part[ROWS * D + row] = mx;
+          part[ROWS * (D + 1) + row] = den;
         }
       }
-      named_barrier(1, kWarps * 32);  // read, before the next item's (or half's) are written
     }
-    if (at < end) next_item<ROWS>(a, p);
+    if (at < end) {
+      next_item<ROWS>(a, p);
+      __syncthreads();  // read, before the next item's are written
+    }
   }
 }
 
@@ -889,6 +980,17 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeA
     if (lane + 32 * i < a.c.dim) store_one(a.out, to + lane + 32 * i, v[i] * inv, a.type);
 }
 
+// CTAs of the warp-MMA kernel a SM holds.
+inline uint32_t narrow_ctas(uint32_t kind, uint32_t pitch) {
+  const auto of = [&](auto kind_tag) {
+    constexpr uint32_t K = decltype(kind_tag)::value;
+    return pitch == 64 ? Narrow<K, 64>::kCtas : pitch == 128 ? Narrow<K, 128>::kCtas : Narrow<K, 256>::kCtas;
+  };
+  return kind == KQ_CACHE_F16  ? of(std::integral_constant<uint32_t, KQ_CACHE_F16>())
+         : kind == KQ_CACHE_Q8 ? of(std::integral_constant<uint32_t, KQ_CACHE_Q8>())
+                               : of(std::integral_constant<uint32_t, KQ_CACHE_Q4>());
+}
+
 // Prepares, and launches, the kernels of one kind of cache.
 template <uint32_t KIND>
 cudaError_t prepare_kind();
@@ -898,12 +1000,12 @@ cudaError_t launch_kind(const TreeArgs& a, bool split, bool wide, uint32_t ctas,
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 cudaError_t prepare_one() {
   return cudaFuncSetAttribute(tree_kernel<KIND, D, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              Smem<KIND, D>::kBytes);
+                              Narrow<KIND, D>::kBytes);
 }
 
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 cudaError_t launch_one(const TreeArgs& a, uint32_t ctas, cudaStream_t s) {
-  tree_kernel<KIND, D, SPLIT><<<ctas, kThreads, Smem<KIND, D>::kBytes, s>>>(a);
+  tree_kernel<KIND, D, SPLIT><<<ctas, kThreads, Narrow<KIND, D>::kBytes, s>>>(a);
   return cudaGetLastError();
 }
 

@@ -76,74 +76,6 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
-// Two f32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\t"
-      "mov.b64 {%0, %1}, a;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-// The numbers of a tile's pages, as the table has them.
-template <uint32_t TW>
-struct PageIds {
-  uint32_t id[TW / 16];
-
-  __device__ __forceinline__ void load(const TreeArgs& a, const Place& p) {
-    const uint32_t base = p.tile * TW, length = p.seq.length();
-    const int* row = a.pages + uint64_t(p.s) * a.max_pages + (base >> a.c.page_log2);
-    const uint32_t n = (min(TW, length - base) + a.c.page() - 1) >> a.c.page_log2;
-    id[0] = static_cast<uint32_t>(row[0]);
-#pragma unroll
-    for (uint32_t i = 1; i < TW / 16; ++i) id[i] = i < n ? static_cast<uint32_t>(row[i]) : 0u;
-  }
-};
-
-// One thread's copies of a tile: whole records where a page is at most a tile, else its rows and its
-// scales. A page that is not there is recorded, and page 0 copied.
-template <class S, uint32_t TW>
-__device__ __forceinline__ void copy_tile(const TreeArgs& a, const Place& p, const PageIds<TW>& ids,
-                                          const uint8_t* src, uint32_t dst, uint32_t bar) {
-  constexpr uint32_t row = S::kRow + S::kScales;
-  const uint32_t base = p.tile * TW, left = p.seq.length() - base;
-  const auto record = [&](uint32_t id) {
-    if (id >= a.c.n_pages) {
-      report_error(a.err, kErrCacheRange);
-      id = 0;
-    }
-    return src + a.c.at(id, p.head);
-  };
-  if (a.c.page() > TW) {
-    const uint8_t* rec = record(ids.id[0]);
-    const uint32_t at = base & (a.c.page() - 1);
-    mbar_arrive_expect_tx(bar, TW * row);
-    bulk_g2s(dst, rec + at * S::kRow, TW * S::kRow, bar);
-    if constexpr (S::kScales != 0)
-      bulk_g2s(dst + TW * S::kRow, rec + a.c.page() * S::kRow + at * S::kScales, TW * S::kScales, bar);
-    return;
-  }
-  const uint32_t n = (min(TW, left) + a.c.page() - 1) >> a.c.page_log2, bytes = row << a.c.page_log2;
-  mbar_arrive_expect_tx(bar, n * bytes);
-#pragma unroll
-  for (uint32_t i = 0; i < TW / 16; ++i)
-    if (i < n) bulk_g2s(dst + i * bytes, record(ids.id[i]), bytes, bar);
-}
-
 // One bounded wait of a warp: false (for good) once any wait of it has given up.
 __device__ __forceinline__ void wait_or_die(bool& live, uint32_t bar, uint32_t parity, unsigned* err, unsigned code) {
   if (live && !mbar_wait(bar, parity)) {
