@@ -69,10 +69,11 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
 
 template <uint32_t ROWS, uint32_t TW>
 void launch_join(const tree::TreeArgs& a, uint32_t items, uint32_t ctas, cudaStream_t s) {
-  const dim3 grid(items, ROWS / 8);
-  if (a.c.pitch == 64) tree::join_kernel<ROWS, 64, TW><<<grid, 256, 0, s>>>(a, ctas);
-  else if (a.c.pitch == 128) tree::join_kernel<ROWS, 128, TW><<<grid, 256, 0, s>>>(a, ctas);
-  else tree::join_kernel<ROWS, 256, TW><<<grid, 256, 0, s>>>(a, ctas);
+  const dim3 grid(items, ROWS);
+  constexpr uint32_t threads = tree::kJoinWarps * 32;
+  if (a.c.pitch == 64) tree::join_kernel<ROWS, 64, TW><<<grid, threads, 0, s>>>(a, ctas);
+  else if (a.c.pitch == 128) tree::join_kernel<ROWS, 128, TW><<<grid, threads, 0, s>>>(a, ctas);
+  else tree::join_kernel<ROWS, 256, TW><<<grid, threads, 0, s>>>(a, ctas);
 }
 
 bool on16(uint64_t bytes) { return bytes % 16 == 0; }
@@ -134,6 +135,7 @@ int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {
   a.n_seq = d.n_seq;
   a.n_heads = d.n_heads;
   a.group = d.n_heads / a.c.n_kv;
+  a.per_group = a.group == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + a.group - 1) / a.group);
   a.tokens = d.tokens;
   a.max_drafts = d.max_drafts;
   a.max_pages = d.max_pages;

@@ -39,9 +39,16 @@ struct TreeArgs {
   float* part;
   float scale_log2;
   uint32_t n_seq, n_heads, group, tokens, max_drafts, max_pages;
+  uint32_t per_group;  // ceil(2^32 / group); 0 for a group of one
   uint32_t type;
   unsigned* err;
 };
+
+// Row r's drafted token and query head in the group (r < 2^16, so the product is exact).
+__device__ __forceinline__ uint32_t token_of(const TreeArgs& a, uint32_t r) {
+  return a.per_group ? __umulhi(r, a.per_group) : r;
+}
+__device__ __forceinline__ uint32_t head_of(const TreeArgs& a, uint32_t r, uint32_t token) { return r - token * a.group; }
 
 // A sequence as the kernels take it: no drafts when there are none, or when its numbers do not fit
 // (recorded in the error word).
@@ -202,8 +209,7 @@ constexpr uint32_t kThreads = kWarps * 32;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -402,6 +408,35 @@ struct TileView {
     return seg_base(p) + (S::kRow << seg_log2) + (p & ((1u << seg_log2) - 1)) * S::kScales;
   }
 };
+
+// A warp's copies of a tile of kTile positions, lane i's of segment i (a page, or a tile's part of one):
+// its record, or where a page is longer than a tile its rows and its scales. id: the segment's page. A
+// page that is not there is recorded, and page 0 copied.
+template <class S>
+__device__ __forceinline__ void copy_segments(const TreeArgs& a, const Place& p, uint32_t id, const uint8_t* src,
+                                              uint32_t dst, uint32_t bar) {
+  constexpr uint32_t row = S::kRow + S::kScales;
+  const uint32_t lane = threadIdx.x % 32, base = p.tile * kTile;
+  const uint32_t seg_log2 = min(a.c.page_log2, 7u), bytes = row << seg_log2;
+  const uint32_t n = (min(kTile, p.seq.length() - base) + (1u << seg_log2) - 1) >> seg_log2;
+  if (id >= a.c.n_pages) {
+    report_error(a.err, kErrCacheRange);
+    id = 0;
+  }
+  const uint8_t* rec = src + a.c.at(id, p.head);
+  if (lane == 0) mbar_arrive_expect_tx(bar, n * bytes);
+  __syncwarp();
+  if (lane < n) {
+    if (a.c.page_log2 <= 7) {
+      bulk_g2s(dst + lane * bytes, rec, bytes, bar);
+    } else {  // a page of two tiles
+      const uint32_t at = base & (a.c.page() - 1);
+      bulk_g2s(dst, rec + at * S::kRow, kTile * S::kRow, bar);
+      if constexpr (S::kScales != 0)
+        bulk_g2s(dst + kTile * S::kRow, rec + a.c.page() * S::kRow + at * S::kScales, kTile * S::kScales, bar);
+    }
+  }
+}
 
 // f16 pairs whose exponent is all ones (infinity, NaN) become zero.
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t v) {
@@ -638,33 +673,42 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   Place p = locate<ROWS, kTile>(a, at);
   bool live = true;  // no wait has given up
 
-  // ---- copies: thread 0 of warp 0 keys (uses 2 i of the ring), of warp 1 values (2 i + 1)
-  const bool copies = warp < 2 && lane == 0;
+  // ---- copies: warp 0 keys (uses 2 i of the ring), warp 1 values (2 i + 1); lane i segment i of a tile
   Place cp = p;
   uint64_t c_at = at;
   uint32_t c_use = warp;
+  uint32_t c_page = 0;  // the lane's page of cp's tile, loaded a tile ahead
+  const uint32_t seg_log2 = min(a.c.page_log2, 7u);
+  const auto page_of = [&]() {
+    const uint32_t pos = cp.tile * kTile + (lane << seg_log2);
+    return c_at < end && lane < kTile >> seg_log2 && pos < cp.seq.length()
+               ? static_cast<uint32_t>(a.pages[uint64_t(cp.s) * a.max_pages + (pos >> a.c.page_log2)])
+               : 0u;
+  };
   // starts the copies of uses below `upto`; all but the NS last uses before it have been read
   const auto copy = [&](uint32_t upto) {
     while (c_use < upto && c_at < end) {
-      const uint32_t slot = c_use % NS;
-      if (c_use >= NS && live && !mbar_wait(bars + 16 * slot + 8, (c_use / NS - 1) & 1)) {
+      const uint32_t slot = c_use % NS, bar = bars + 16 * slot;
+      if (c_use >= NS && live && !mbar_wait(bar + 8, (c_use / NS - 1) & 1)) {
         report_error(a.err, kErrWaitEmpty);
         live = false;
       }
+      live = __all_sync(0xffffffffu, live);
       if (!live) return;
-      PageIds<kTile> ids;
-      ids.load(a, cp);
-      copy_tile<S, kTile>(a, cp, ids, warp ? a.c.v : a.c.k, ring + slot * S::kSlot, bars + 16 * slot);
+      copy_segments<S>(a, cp, c_page, warp ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
       c_use += 2;
       ++c_at;
       if (++cp.tile == position_tiles<kTile>(cp.seq) && c_at < end) next_item<ROWS>(a, cp);
+      c_page = page_of();
     }
   };
-  if (copies) copy(NS);
-  __syncwarp();
+  if (warp < 2) {
+    c_page = page_of();
+    copy(NS);
+  }
 
   const uint32_t g = lane >> 2, t = lane & 3u;
-  const uint32_t seg_log2 = min(a.c.page_log2, 7u), p0 = warp * 16;
+  const uint32_t p0 = warp * 16;
   const Lane<S> place(p0, g, t, seg_log2);
   uint32_t it = 0;  // uses of the ring read
   while (at < end) {
@@ -676,10 +720,13 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
     {
       const uint32_t r = p.rows * ROWS + g;
       const bool have = r < rows;
-      const uint64_t row = have ? (p.seq.first + r / a.group) * a.q_token +
-                                      uint64_t(p.head * a.group + r % a.group) * a.c.dim
+      const uint32_t tok = token_of(a, r);
+      const uint64_t row = have ? (p.seq.first + tok) * a.q_token +
+                                      uint64_t(p.head * a.group + head_of(a, r, tok)) * a.c.dim
                                 : 0;
       float most = 0.f;
+      constexpr uint32_t HOLD = D == 256 ? 1 : S::kSteps;  // steps held: all, where registers allow
+      float x[HOLD][4];
       const auto load4 = [&](uint32_t ks, float (&x)[4]) {
         const uint32_t e = key_element<S>(ks, t);
         x[0] = x[1] = x[2] = x[3] = 0.f;
@@ -690,9 +737,9 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       };
 #pragma unroll
       for (uint32_t ks = 0; ks < S::kSteps; ++ks) {
-        float x[4];
-        load4(ks, x);
-        most = fmaxf(most, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+        float(&y)[4] = x[ks % HOLD];
+        load4(ks, y);
+        most = fmaxf(most, fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
       }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -705,11 +752,11 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       unit2.y = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
 #pragma unroll
       for (uint32_t ks = 0; ks < S::kSteps; ++ks) {
-        float x[4];
-        load4(ks, x);
+        float(&y)[4] = x[ks % HOLD];
+        if constexpr (HOLD == 1) load4(ks, y);
         uint32_t hi0, lo0, hi1, lo1;
-        split2(x[0] * up, x[1] * up, hi0, lo0);
-        split2(x[2] * up, x[3] * up, hi1, lo1);
+        split2(y[0] * up, y[1] * up, hi0, lo0);
+        split2(y[2] * up, y[3] * up, hi1, lo1);
         if constexpr (D == 256) {
           // every warp writes the same words, and reads its own
           q_smem[ks * 32 + lane] = make_uint4(hi0, hi1, lo0, lo1);
@@ -746,8 +793,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
 
     const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
     for (; p.tile < tiles && at < end; ++p.tile, ++at, it += 2) {
-      if (copies) copy(it + NS);
-      __syncwarp();
+      if (warp < 2) copy(it + NS);
       const uint32_t base = p.tile * kTile, left = p.seq.length() - base;  // positions left in the cache
       const bool edge = base + kTile > p.seq.prefix;
       const uint32_t k_slot = it % NS, v_slot = (it + 1) % NS;
@@ -767,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
 #pragma unroll
           for (uint32_t i = 0; i < 2; ++i) {
             const uint32_t r = p.rows * ROWS + 2 * t + i;
-            bits[i] = r < rows ? mask_bits(a, p.seq, r / a.group) : 0ull;
+            bits[i] = r < rows ? mask_bits(a, p.seq, token_of(a, r)) : 0ull;
           }
           const uint32_t pos = base + p0 + pi8(g);
           if (!sees(bits[0], pos, p.seq)) z0.x = -INFINITY;
@@ -906,8 +952,9 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       }
       if (rr < rows) {
         const float inv = whole ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
-        const uint64_t to = (p.seq.first + rr / a.group) * a.out_token +
-                            uint64_t(p.head * a.group + rr % a.group) * a.c.dim;
+        const uint32_t tok = token_of(a, rr);
+        const uint64_t to = (p.seq.first + tok) * a.out_token +
+                            uint64_t(p.head * a.group + head_of(a, rr, tok)) * a.c.dim;
 #pragma unroll
         for (uint32_t e = lane; e < D; e += 32) {
           float v = 0.f;
@@ -931,16 +978,20 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
 
 // ---------------------------------------------------------------- the join of split items
 
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over an item's parts, in their order. Grid: (items
-// of a largest tree a sequence and head, eight rows each); items that one CTA did whole are done.
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over an item's parts, in a fixed order. Grid: (items
+// of a largest tree a sequence and head, rows); items that one CTA did whole are done. Four warps share a
+// row's parts (a long context's are dozens) and join what they have.
+constexpr uint32_t kJoinWarps = 4;
+
 template <uint32_t ROWS, uint32_t D, uint32_t TW>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeArgs a, uint32_t grid) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ TreeArgs a, uint32_t grid) {
+  __shared__ float sums[kJoinWarps][D + 1];
   const uint32_t max_rt = (a.max_drafts * a.group + ROWS - 1) / ROWS;
   const uint32_t rt = blockIdx.x % max_rt, head = blockIdx.x / max_rt % a.c.n_kv;
   const uint32_t s = blockIdx.x / max_rt / a.c.n_kv;
   const Seq seq = load_seq(a, s);
   const uint32_t rts = row_tiles<ROWS>(a, seq), tiles = position_tiles<TW>(seq);
-  const uint32_t row = blockIdx.y * 8 + threadIdx.x / 32, rr = rt * ROWS + row;
+  const uint32_t row = blockIdx.y, rr = rt * ROWS + row;
   if (rr >= seq.drafts * a.group) return;
   uint64_t before = 0, total = 0;
   for (uint32_t i = threadIdx.x % 32; i < a.n_seq; i += 32) {
@@ -955,9 +1006,9 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeA
   const uint32_t c0 = range_owner(total, first, ctas), c1 = range_owner(total, first + tiles - 1, ctas);
   if (c0 == c1) return;
   // slot 1 of the CTA the item starts in; slot 0 of the others, which an earlier one began
-  const uint64_t stride = part_floats(ROWS, D);
+  constexpr uint64_t stride = part_floats(ROWS, D);
   const auto slot = [&](uint32_t c) { return a.part + (uint64_t(c) * 2 + (c == c0 ? 1 : 0)) * stride; };
-  const uint32_t lane = threadIdx.x % 32;
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   float mx = -INFINITY;
   for (uint32_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, slot(c)[ROWS * D + row]);
 #pragma unroll
@@ -965,19 +1016,29 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeA
   const float ref = mx == -INFINITY ? 0.f : mx;
   float den = 0.f, v[D / 32] = {};
 #pragma unroll 4
-  for (uint32_t c = c0; c <= c1; ++c) {
+  for (uint32_t c = c0 + warp; c <= c1; c += kJoinWarps) {
     const float* part = slot(c);
     const float f = exp2f(part[ROWS * D + row] - ref);
     den = fmaf(f, part[ROWS * (D + 1) + row], den);
 #pragma unroll
     for (uint32_t i = 0; i < D / 32; ++i) v[i] = fmaf(f, part[row * D + lane + 32 * i], v[i]);
   }
-  const float inv = den == 0.f ? 0.f : 1.f / den;
-  const uint64_t to = (seq.first + rr / a.group) * a.out_token +
-                      uint64_t(head * a.group + rr % a.group) * a.c.dim;
 #pragma unroll
-  for (uint32_t i = 0; i < D / 32; ++i)
-    if (lane + 32 * i < a.c.dim) store_one(a.out, to + lane + 32 * i, v[i] * inv, a.type);
+  for (uint32_t i = 0; i < D / 32; ++i) sums[warp][lane + 32 * i] = v[i];
+  if (lane == 0) sums[warp][D] = den;
+  __syncthreads();
+  den = 0.f;
+#pragma unroll
+  for (uint32_t w = 0; w < kJoinWarps; ++w) den += sums[w][D];
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const uint32_t tok = token_of(a, rr);
+  const uint64_t to = (seq.first + tok) * a.out_token + uint64_t(head * a.group + head_of(a, rr, tok)) * a.c.dim;
+  for (uint32_t e = threadIdx.x; e < a.c.dim; e += kJoinWarps * 32) {
+    float x = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < kJoinWarps; ++w) x += sums[w][e];
+    store_one(a.out, to + e, x * inv, a.type);
+  }
 }
 
 // CTAs of the warp-MMA kernel a SM holds.

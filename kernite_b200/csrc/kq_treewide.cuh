@@ -467,9 +467,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       const uint32_t my_row = p.rows * ROWS + in_tile;
       const bool have = my_row < rows;
       const bool second = SPLIT && lane >= 16;
-      const uint64_t q_row = have ? (p.seq.first + my_row / a.group) * a.q_token +
-                                        uint64_t(p.head * a.group + my_row % a.group) * a.c.dim
-                                  : 0;
+      const uint32_t token = have ? token_of(a, my_row) : 0;
+      const uint32_t q_head = p.head * a.group + (have ? head_of(a, my_row, token) : 0);
+      const uint64_t q_row = (p.seq.first + token) * a.q_token + uint64_t(q_head) * a.c.dim;
       float unit;
       {
         float x[D / 16][8];  // all of this thread's part, so that its loads are one latency
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar.q_full());
-      const unsigned long long bits = have ? mask_bits(a, p.seq, my_row / a.group) : 0ull;
+      const unsigned long long bits = have ? mask_bits(a, p.seq, token) : 0ull;
 
       float m = -INFINITY, l = 0.f;
       const uint32_t tiles = position_tiles<TW>(p.seq), first_tile = p.tile;
@@ -688,8 +688,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       // every tile's values were decoded before their product: the flags are complete, and the next
       // item's go to the other word
       const unsigned long long odd = *reinterpret_cast<volatile unsigned long long*>(special + (items & 1)) & bits;
-      const uint64_t to = (p.seq.first + (have ? my_row / a.group : 0)) * a.out_token +
-                          uint64_t(p.head * a.group + my_row % a.group) * a.c.dim;
+      const uint64_t to = (p.seq.first + token) * a.out_token + uint64_t(q_head) * a.c.dim;
       constexpr uint32_t WIDE = SPLIT ? D / 4 : D / 2;
       const uint32_t o0 = half * (D / 2), e0 = o0 + (second ? WIDE : 0);
 #pragma unroll 1
