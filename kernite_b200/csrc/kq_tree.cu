@@ -68,12 +68,11 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
 }
 
 template <uint32_t ROWS, uint32_t TW>
-void launch_join(const tree::TreeArgs& a, uint32_t items, uint32_t ctas, cudaStream_t s) {
-  const dim3 grid(items, ROWS);
-  constexpr uint32_t threads = tree::kJoinWarps * 32;
-  if (a.c.pitch == 64) tree::join_kernel<ROWS, 64, TW><<<grid, threads, 0, s>>>(a, ctas);
-  else if (a.c.pitch == 128) tree::join_kernel<ROWS, 128, TW><<<grid, threads, 0, s>>>(a, ctas);
-  else tree::join_kernel<ROWS, 256, TW><<<grid, threads, 0, s>>>(a, ctas);
+cudaError_t launch_join(const tree::TreeArgs& a, uint32_t ctas, cudaStream_t s) {
+  return launch_pdl(a.c.pitch == 64    ? tree::join_kernel<ROWS, 64, TW>
+                    : a.c.pitch == 128 ? tree::join_kernel<ROWS, 128, TW>
+                                       : tree::join_kernel<ROWS, 256, TW>,
+                    dim3(ctas, ROWS / 8), 256, 0, s, a, ctas);
 }
 
 bool on16(uint64_t bytes) { return bytes % 16 == 0; }
@@ -145,13 +144,12 @@ int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {
                       : a.c.kind == KQ_CACHE_Q8 ? tree::launch_kind<KQ_CACHE_Q8>
                                                 : tree::launch_kind<KQ_CACHE_Q4>;
   cudaError_t e = launch(a, p.split, p.wide, p.ctas, s);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaLaunchKernel", call);
-  const uint32_t items = d.n_seq * a.c.n_kv * ((d.max_drafts * a.group + p.rows - 1) / p.rows);
-  if (p.rows == 8) launch_join<8, 128>(a, items, p.ctas, s);
-  else if (p.rows == 64) launch_join<64, 64>(a, items, p.ctas, s);
-  else launch_join<128, 64>(a, items, p.ctas, s);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", "tree attention join");
+  if (e != cudaSuccess) return cuda_fail(e, "cudaLaunchKernelExC", call);
+  if (p.ctas == 1) return KQ_OK;  // nothing is split
+  e = p.rows == 8 ? launch_join<8, 128>(a, p.ctas, s)
+      : p.rows == 64 ? launch_join<64, 64>(a, p.ctas, s)
+                     : launch_join<128, 64>(a, p.ctas, s);
+  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernelExC", "tree attention join");
 }
 
 }  // namespace kq

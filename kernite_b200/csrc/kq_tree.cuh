@@ -8,8 +8,8 @@
 // into equal ranges, one a CTA, whatever the sequences' lengths: a CTA does the end of one item, some
 // whole ones and the start of another. Whole ones are written out; parts leave (max, sum, unnormalised
 // output) in the workspace, two slots a CTA at most, and the join kernel finds by the same arithmetic
-// which CTAs hold an item's parts. So a long context is split over the whole GPU, and a ragged batch
-// leaves no CTA idle.
+// which CTAs hold an item's parts. So a long context is split over the whole GPU, and a ragged batch leaves
+// no CTA idle.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -20,6 +20,7 @@
 
 #include "kq_cache.cuh"
 #include "kq_device.cuh"
+#include "kq_launch.h"
 
 namespace kq {
 namespace tree {
@@ -57,8 +58,10 @@ struct Seq {
   __device__ uint32_t length() const { return prefix + drafts; }
 };
 
+// Read through L2: the join kernel looks before its pdl_wait(), when its SM's L1 may hold what an earlier
+// step had there.
 __device__ __forceinline__ Seq load_seq(const TreeArgs& a, uint32_t s) {
-  const int b = a.starts[s], e = a.starts[s + 1], p = a.prefix[s];
+  const int b = __ldcg(a.starts + s), e = __ldcg(a.starts + s + 1), p = __ldcg(a.prefix + s);
   Seq q = {static_cast<uint32_t>(b), static_cast<uint32_t>(e - b), static_cast<uint32_t>(p)};
   const bool ok = b >= 0 && e >= b && static_cast<uint32_t>(e) <= a.tokens && q.drafts <= a.max_drafts &&
                   p >= 0 && uint64_t(q.prefix) + q.drafts <= uint64_t(a.max_pages) << a.c.page_log2;
@@ -90,13 +93,23 @@ __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
   return v;
 }
 
-// The tiles of sequences [0, n). Called by whole warps.
+// All sequences' tiles; the first 32 sequences stay in the warp's lanes. Made by whole warps.
 template <uint32_t ROWS, uint32_t TW>
-__device__ __forceinline__ uint64_t work_before(const TreeArgs& a, uint32_t n) {
-  uint64_t w = 0;
-  for (uint32_t s = threadIdx.x % 32; s < n; s += 32) w += seq_work<ROWS, TW>(a, load_seq(a, s));
-  return warp_sum(w);
-}
+struct Work {
+  Seq seq;         // of sequence `lane`
+  uint64_t tiles;  // its tiles
+  uint64_t total;
+
+  __device__ explicit Work(const TreeArgs& a) {
+    const uint32_t lane = threadIdx.x % 32;
+    seq = Seq{0, 0, 0};
+    if (lane < a.n_seq) seq = load_seq(a, lane);
+    tiles = seq_work<ROWS, TW>(a, seq);
+    uint64_t w = tiles;
+    for (uint32_t s = 32 + lane; s < a.n_seq; s += 32) w += seq_work<ROWS, TW>(a, load_seq(a, s));
+    total = warp_sum(w);
+  }
+};
 
 // Where a CTA is: an item and the next of its tiles.
 struct Place {
@@ -107,11 +120,17 @@ struct Place {
 
 // The place of tile `at` of the whole work. Called by whole warps, at < total.
 template <uint32_t ROWS, uint32_t TW>
-__device__ __forceinline__ Place locate(const TreeArgs& a, uint64_t at) {
+__device__ __forceinline__ Place locate(const TreeArgs& a, const Work<ROWS, TW>& work, uint64_t at) {
   const uint32_t lane = threadIdx.x % 32;
   Place p = {};
+  Seq seq = work.seq;
+  uint64_t w = work.tiles;
   for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
-    const uint64_t w = s0 + lane < a.n_seq ? seq_work<ROWS, TW>(a, load_seq(a, s0 + lane)) : 0;
+    if (s0) {
+      seq = Seq{0, 0, 0};
+      if (s0 + lane < a.n_seq) seq = load_seq(a, s0 + lane);
+      w = seq_work<ROWS, TW>(a, seq);
+    }
     uint64_t upto = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -122,13 +141,15 @@ __device__ __forceinline__ Place locate(const TreeArgs& a, uint64_t at) {
     if (past) {
       const int who = __ffs(past) - 1;
       p.s = s0 + who;
-      const uint64_t rest = at - __shfl_sync(0xffffffffu, upto - w, who);
-      p.seq = load_seq(a, p.s);
+      const uint32_t rest = static_cast<uint32_t>(at - __shfl_sync(0xffffffffu, upto - w, who));
+      p.seq.first = __shfl_sync(0xffffffffu, seq.first, who);
+      p.seq.drafts = __shfl_sync(0xffffffffu, seq.drafts, who);
+      p.seq.prefix = __shfl_sync(0xffffffffu, seq.prefix, who);
       const uint32_t pt = position_tiles<TW>(p.seq), rt = row_tiles<ROWS>(a, p.seq);
-      p.tile = static_cast<uint32_t>(rest % pt);
-      const uint64_t item = rest / pt;
-      p.rows = static_cast<uint32_t>(item % rt);
-      p.head = static_cast<uint32_t>(item / rt);
+      const uint32_t item = rest / pt;
+      p.tile = rest - item * pt;
+      p.head = item / rt;
+      p.rows = item - p.head * rt;
       return p;
     }
     at -= __shfl_sync(0xffffffffu, upto, 31);
@@ -665,12 +686,15 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
     fence_mbar_init();
   }
   __syncthreads();
-  const uint64_t total = work_before<ROWS, kTile>(a, a.n_seq);
+  pdl_wait();
+  pdl_launch_dependents();
+  const Work<ROWS, kTile> work(a);
+  const uint64_t total = work.total;
   const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(gridDim.x), total));
   if (blockIdx.x >= ctas) return;
   uint64_t at = range_start(total, blockIdx.x, ctas);
   const uint64_t end = range_start(total, blockIdx.x + 1, ctas);
-  Place p = locate<ROWS, kTile>(a, at);
+  Place p = locate(a, work, at);
   bool live = true;  // no wait has given up
 
   // ---- copies: warp 0 keys (uses 2 i of the ring), warp 1 values (2 i + 1); lane i segment i of a tile
@@ -969,76 +993,82 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         }
       }
     }
-    if (at < end) {
-      next_item<ROWS>(a, p);
-      __syncthreads();  // read, before the next item's are written
-    }
+    __syncthreads();  // read (and the part written), before the next item's are written
+    if (at < end) next_item<ROWS>(a, p);
   }
 }
 
 // ---------------------------------------------------------------- the join of split items
 
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over an item's parts, in a fixed order. Grid: (items
-// of a largest tree a sequence and head, rows); items that one CTA did whole are done. Four warps share a
-// row's parts (a long context's are dozens) and join what they have.
-constexpr uint32_t kJoinWarps = 4;
-
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over the parts of each item that more than one CTA
+// did, in the parts' order, with a running maximum M. Grid: (the CTAs that left parts, rows / 8): an item
+// is joined by the blocks of the CTA that began it (each began at most one that another went on with),
+// a warp a row, CB parts at a time so that their loads share L2's latency.
+//
+// Joining in the main kernel, by the CTA that leaves an item's last part, was slower (one token over
+// 131001 positions 94 us against 92, 25 drafts 56 against 49): that CTA joins alone, after the fences.
 template <uint32_t ROWS, uint32_t D, uint32_t TW>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ TreeArgs a, uint32_t grid) {
-  __shared__ float sums[kJoinWarps][D + 1];
-  const uint32_t max_rt = (a.max_drafts * a.group + ROWS - 1) / ROWS;
-  const uint32_t rt = blockIdx.x % max_rt, head = blockIdx.x / max_rt % a.c.n_kv;
-  const uint32_t s = blockIdx.x / max_rt / a.c.n_kv;
-  const Seq seq = load_seq(a, s);
-  const uint32_t rts = row_tiles<ROWS>(a, seq), tiles = position_tiles<TW>(seq);
-  const uint32_t row = blockIdx.y, rr = rt * ROWS + row;
-  if (rr >= seq.drafts * a.group) return;
-  uint64_t before = 0, total = 0;
-  for (uint32_t i = threadIdx.x % 32; i < a.n_seq; i += 32) {
-    const uint64_t w = seq_work<ROWS, TW>(a, load_seq(a, i));
-    total += w;
-    before += i < s ? w : 0;
-  }
-  before = warp_sum(before);
-  total = warp_sum(total);
-  const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(grid), total));
-  const uint64_t first = before + (uint64_t(head) * rts + rt) * tiles;
-  const uint32_t c0 = range_owner(total, first, ctas), c1 = range_owner(total, first + tiles - 1, ctas);
-  if (c0 == c1) return;
-  // slot 1 of the CTA the item starts in; slot 0 of the others, which an earlier one began
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeArgs a, uint32_t grid) {
+  // Where the parts are, while the main kernel is at work: the lengths were there before it (it lets this
+  // kernel start after its own pdl_wait).
+  const Work<ROWS, TW> work(a);
+  const uint64_t total = work.total;
+  const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(grid), total)), c0 = blockIdx.x;
+  const bool splits = c0 + 1 < ctas;
+  const uint64_t last = splits ? range_start(total, c0 + 1, ctas) - 1 : 0;  // the CTA's last tile
+  const Place p = locate(a, work, last);
+  const uint64_t item = last - p.tile;
+  const uint32_t tiles = position_tiles<TW>(p.seq);
+  const uint32_t row = blockIdx.y * 8 + threadIdx.x / 32, rr = p.rows * ROWS + row;
+  const bool mine = splits && item + tiles != last + 1 && item >= range_start(total, c0, ctas) &&
+                    rr < p.seq.drafts * a.group;
+  pdl_wait();  // in every block: a kernel after this one waits for this one alone
+  pdl_launch_dependents();
+  if (!mine) return;
+  const uint32_t c1 = range_owner(total, item + tiles - 1, ctas);
   constexpr uint64_t stride = part_floats(ROWS, D);
-  const auto slot = [&](uint32_t c) { return a.part + (uint64_t(c) * 2 + (c == c0 ? 1 : 0)) * stride; };
-  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  float mx = -INFINITY;
-  for (uint32_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, slot(c)[ROWS * D + row]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  float den = 0.f, v[D / 32] = {};
-#pragma unroll 4
-  for (uint32_t c = c0 + warp; c <= c1; c += kJoinWarps) {
-    const float* part = slot(c);
-    const float f = exp2f(part[ROWS * D + row] - ref);
-    den = fmaf(f, part[ROWS * (D + 1) + row], den);
-#pragma unroll
-    for (uint32_t i = 0; i < D / 32; ++i) v[i] = fmaf(f, part[row * D + lane + 32 * i], v[i]);
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < D / 32; ++i) sums[warp][lane + 32 * i] = v[i];
-  if (lane == 0) sums[warp][D] = den;
-  __syncthreads();
-  den = 0.f;
-#pragma unroll
-  for (uint32_t w = 0; w < kJoinWarps; ++w) den += sums[w][D];
-  const float inv = den == 0.f ? 0.f : 1.f / den;
+  constexpr uint32_t V = D / 32, CB = 8;
+  const uint32_t lane = threadIdx.x % 32;
   const uint32_t tok = token_of(a, rr);
-  const uint64_t to = (seq.first + tok) * a.out_token + uint64_t(head * a.group + head_of(a, rr, tok)) * a.c.dim;
-  for (uint32_t e = threadIdx.x; e < a.c.dim; e += kJoinWarps * 32) {
-    float x = 0.f;
+  const uint64_t to = (p.seq.first + tok) * a.out_token + uint64_t(p.head * a.group + head_of(a, rr, tok)) * a.c.dim;
+  float top = -INFINITY, den = 0.f, v[V] = {};
+#pragma unroll 1
+  for (uint32_t c = c0; c <= c1; c += CB) {
+    float m[CB], l[CB], x[CB][V];
 #pragma unroll
-    for (uint32_t w = 0; w < kJoinWarps; ++w) x += sums[w][e];
-    store_one(a.out, to + e, x * inv, a.type);
+    for (uint32_t j = 0; j < CB; ++j) {
+      const bool there = c + j <= c1;
+      // slot 1 of the CTA that began the item, slot 0 of those that went on
+      const float* part = a.part + (uint64_t(c + j) * 2 + (c + j == c0 ? 1 : 0)) * stride;
+      m[j] = there ? part[ROWS * D + row] : -INFINITY;
+      l[j] = there ? part[ROWS * (D + 1) + row] : 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < V; i += 2) {
+        const float2 y = there ? *reinterpret_cast<const float2*>(part + row * D + lane * V + i) : make_float2(0.f, 0.f);
+        x[j][i] = y.x;
+        x[j][i + 1] = y.y;
+      }
+    }
+    float mx = top;
+#pragma unroll
+    for (uint32_t j = 0; j < CB; ++j) mx = fmaxf(mx, m[j]);
+    const float ref = mx == -INFINITY ? 0.f : mx, keep = exp2f(top - ref);
+    top = mx;
+    den *= keep;
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i) v[i] *= keep;
+#pragma unroll
+    for (uint32_t j = 0; j < CB; ++j) {
+      const float f = exp2f(m[j] - ref);
+      den = fmaf(f, l[j], den);
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) v[i] = fmaf(f, x[j][i], v[i]);
+    }
   }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+  for (uint32_t i = 0; i < V; ++i)
+    if (lane * V + i < a.c.dim) store_one(a.out, to + lane * V + i, v[i] * inv, a.type);
 }
 
 // CTAs of the warp-MMA kernel a SM holds.
@@ -1066,8 +1096,7 @@ cudaError_t prepare_one() {
 
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 cudaError_t launch_one(const TreeArgs& a, uint32_t ctas, cudaStream_t s) {
-  tree_kernel<KIND, D, SPLIT><<<ctas, kThreads, Narrow<KIND, D>::kBytes, s>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(tree_kernel<KIND, D, SPLIT>, dim3(ctas), kThreads, Narrow<KIND, D>::kBytes, s, a);
 }
 
 }  // namespace tree

@@ -302,7 +302,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     fence_mbar_init();
     special[0] = special[1] = 0;
   }
-  const uint64_t total = work_before<ROWS, TW>(a, a.n_seq);
+  pdl_wait();
+  pdl_launch_dependents();
+  const Work<ROWS, TW> work(a);
+  const uint64_t total = work.total;
   const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(gridDim.x), total));
   if (blockIdx.x >= ctas) return;
   if (warp == 0) {
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   const uint32_t tmem = *tmem_slot;
   uint64_t at = range_start(total, blockIdx.x, ctas);
   const uint64_t end = range_start(total, blockIdx.x + 1, ctas);
-  Place p = locate<ROWS, TW>(a, at);
+  Place p = locate(a, work, at);
   bool live = true;
   const uint32_t seg_log2 = min(a.c.page_log2, TW == 128 ? 7u : 6u);
 
@@ -775,8 +778,7 @@ cudaError_t prepare_wide() {
 
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 cudaError_t launch_wide(const TreeArgs& a, uint32_t ctas, cudaStream_t s) {
-  wide_kernel<KIND, D, SPLIT><<<ctas, kWideThreads, Wide<KIND, D>::kBytes, s>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(wide_kernel<KIND, D, SPLIT>, dim3(ctas), kWideThreads, Wide<KIND, D>::kBytes, s, a);
 }
 
 // Prepares, and launches, the kernels of one kind of cache (pitch 64, 128 or 256).
