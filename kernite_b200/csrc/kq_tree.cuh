@@ -474,7 +474,8 @@ struct Narrow {
   using S = Shape<KIND, D>;
   static constexpr uint32_t kJoinRow = D + 16;
   static constexpr uint32_t kJoin = 4 * 8 * kJoinRow * 4 + kWarps * 8 * 2 * 4;
-  static constexpr uint32_t kQ = D == 256 ? S::kSteps * 32 * 16 : 0;
+  static constexpr bool kQShared = D >= 128;
+  static constexpr uint32_t kQ = kQShared ? S::kSteps * 32 * 16 : 0;
   static constexpr uint32_t kFixed = kJoin + kQ + 256;
   static constexpr uint32_t kCtas = kFixed + 5 * S::kSlot <= 113 * 1024 ? 2 : 1;
   static constexpr uint32_t kFit = ((kCtas == 2 ? 113 : 226) * 1024 - kFixed) / S::kSlot;
@@ -509,9 +510,9 @@ __device__ __forceinline__ void key_product(uint32_t slot, const Lane<Shape<KIND
                                             float (&c)[4]) {
   using S = Shape<KIND, D>;
   constexpr uint32_t B = S::EK * S::kBits / 8;
-  float acc[SPLIT ? 4 : 2][4];  // independent sums: an MMA's result is some 20 cycles away
+  float acc[2][4];  // two sums: an MMA's result is some 20 cycles away
 #pragma unroll
-  for (uint32_t i = 0; i < (SPLIT ? 4 : 2); ++i)
+  for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) acc[i][k] = 0.f;
 #pragma unroll
@@ -545,14 +546,13 @@ __device__ __forceinline__ void key_product(uint32_t slot, const Lane<Shape<KIND
       const uint32_t ks = j * (S::EK / 4) + k;
       uint32_t b[4];
       q(ks, b);
-      mma16816(acc[ks & 1], f[0][0], f[1][0], f[0][1], f[1][1], b[0], b[1]);
-      if constexpr (SPLIT) mma16816(acc[2 + (ks & 1)], f[0][0], f[1][0], f[0][1], f[1][1], b[2], b[3]);
+      mma16816(acc[SPLIT ? 0 : ks & 1], f[0][0], f[1][0], f[0][1], f[1][1], b[0], b[1]);
+      if constexpr (SPLIT) mma16816(acc[1], f[0][0], f[1][0], f[0][1], f[1][1], b[2], b[3]);
     }
   }
 #pragma unroll
   for (uint32_t k = 0; k < 4; ++k) {
     c[k] = acc[0][k] + acc[1][k];
-    if constexpr (SPLIT) c[k] += acc[2][k] + acc[3][k];
   }
 }
 
@@ -666,6 +666,12 @@ __device__ __noinline__ void add_special(const TileView<Shape<KIND, D>>& tile, u
 constexpr float kLift = 2.f;
 constexpr float kSlack = 13.f;
 
+// What a copying warp has next: the tile, its first use of the ring, the tiles left.
+struct CopyState {
+  Place place;
+  uint32_t use, left;
+};
+
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(const __grid_constant__ TreeArgs a) {
   using S = Shape<KIND, D>;
@@ -676,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   float* join_m = join + 4 * 8 * M::kJoinRow;                    // [warp][row], then sums
   float* join_l = join_m + kWarps * 8;
   uint4* q_smem = reinterpret_cast<uint4*>(join_l + kWarps * 8);
+  __shared__ CopyState copies[2];
   const uint32_t ring = smem_u32(smem), bars = ring + NS * S::kSlot + M::kJoin + M::kQ;  // full, empty of each slot
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
@@ -697,37 +704,46 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   Place p = locate(a, work, at);
   bool live = true;  // no wait has given up
 
-  // ---- copies: warp 0 keys (uses 2 i of the ring), warp 1 values (2 i + 1); lane i segment i of a tile
-  Place cp = p;
-  uint64_t c_at = at;
-  uint32_t c_use = warp;
-  uint32_t c_page = 0;  // the lane's page of cp's tile, loaded a tile ahead
+  // ---- copies: warp 0 keys (uses 2 i of the ring), warp 1 values (2 i + 1); lane i segment i of a tile.
+  // Their place is in shared memory: registers are what the loop below is short of.
+  uint32_t todo = static_cast<uint32_t>(end - at);  // tiles of this CTA not yet read
   const uint32_t seg_log2 = min(a.c.page_log2, 7u);
-  const auto page_of = [&]() {
+  uint32_t c_page = 0;  // the lane's page of the copies' tile, loaded a tile ahead
+  const auto page_of = [&](const Place& cp) {
     const uint32_t pos = cp.tile * kTile + (lane << seg_log2);
-    return c_at < end && lane < kTile >> seg_log2 && pos < cp.seq.length()
+    return lane < kTile >> seg_log2 && pos < cp.seq.length()
                ? static_cast<uint32_t>(a.pages[uint64_t(cp.s) * a.max_pages + (pos >> a.c.page_log2)])
                : 0u;
   };
   // starts the copies of uses below `upto`; all but the NS last uses before it have been read
   const auto copy = [&](uint32_t upto) {
-    while (c_use < upto && c_at < end) {
-      const uint32_t slot = c_use % NS, bar = bars + 16 * slot;
-      if (c_use >= NS && live && !mbar_wait(bar + 8, (c_use / NS - 1) & 1)) {
+    CopyState& state = copies[warp];
+    while (state.use < upto && state.left) {
+      const uint32_t use = state.use, slot = use % NS, bar = bars + 16 * slot;
+      if (use >= NS && live && !mbar_wait(bar + 8, (use / NS - 1) & 1)) {
         report_error(a.err, kErrWaitEmpty);
         live = false;
       }
       live = __all_sync(0xffffffffu, live);
       if (!live) return;
+      Place cp = state.place;
+      const uint32_t left = state.left - 1;
       copy_segments<S>(a, cp, c_page, warp ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
-      c_use += 2;
-      ++c_at;
-      if (++cp.tile == position_tiles<kTile>(cp.seq) && c_at < end) next_item<ROWS>(a, cp);
-      c_page = page_of();
+      if (++cp.tile == position_tiles<kTile>(cp.seq) && left) next_item<ROWS>(a, cp);
+      if (left) c_page = page_of(cp);
+      __syncwarp();
+      if (lane == 0) {
+        state.place = cp;
+        state.use = use + 2;
+        state.left = left;
+      }
+      __syncwarp();
     }
   };
   if (warp < 2) {
-    c_page = page_of();
+    if (lane == 0) copies[warp] = {p, warp, todo};
+    c_page = page_of(p);
+    __syncwarp();
     copy(NS);
   }
 
@@ -735,11 +751,11 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   const uint32_t p0 = warp * 16;
   const Lane<S> place(p0, g, t, seg_log2);
   uint32_t it = 0;  // uses of the ring read
-  while (at < end) {
+  while (todo) {
     // ---- the item's rows as operand B (row n = g), each scaled by a power of two to a largest element in
     // [2^7, 2^8), so that f16's range fits any q; and what rows 2 t, 2 t + 1 need
     const uint32_t rows = p.seq.drafts * a.group;
-    uint32_t qb[D == 256 ? 1 : S::kSteps][4];
+    uint32_t qb[M::kQShared ? 1 : S::kSteps][4];
     float2 unit2;  // logits in log2 units a unit of the scaled product, of rows 2 t and 2 t + 1
     {
       const uint32_t r = p.rows * ROWS + g;
@@ -781,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         uint32_t hi0, lo0, hi1, lo1;
         split2(y[0] * up, y[1] * up, hi0, lo0);
         split2(y[2] * up, y[3] * up, hi1, lo1);
-        if constexpr (D == 256) {
+        if constexpr (M::kQShared) {
           // every warp writes the same words, and reads its own
           q_smem[ks * 32 + lane] = make_uint4(hi0, hi1, lo0, lo1);
         } else {
@@ -791,10 +807,10 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
           qb[ks][3] = lo1;
         }
       }
-      if constexpr (D == 256) __syncwarp();
+      if constexpr (M::kQShared) __syncwarp();
     }
     const auto q_at = [&](uint32_t ks, uint32_t (&b)[4]) {
-      if constexpr (D == 256) {
+      if constexpr (M::kQShared) {
         const uint4 w = q_smem[ks * 32 + lane];
         b[0] = w.x;
         b[1] = w.y;
@@ -816,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
     float limit = -INFINITY;  // weights' exponents above this want a new reference
 
     const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
-    for (; p.tile < tiles && at < end; ++p.tile, ++at, it += 2) {
+    for (; p.tile < tiles && todo; ++p.tile, --todo, it += 2) {
       if (warp < 2) copy(it + NS);
       const uint32_t base = p.tile * kTile, left = p.seq.length() - base;  // positions left in the cache
       const bool edge = base + kTile > p.seq.prefix;
@@ -827,18 +843,21 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       }
       __syncwarp();
       uint32_t pb[4];
-      unsigned long long bits[2];
+      const auto row_bits = [&](unsigned long long (&bits)[2]) {  // of rows 2 t, 2 t + 1
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+          const uint32_t r = p.rows * ROWS + 2 * t + i;
+          bits[i] = r < rows ? mask_bits(a, p.seq, token_of(a, r)) : 0ull;
+        }
+      };
       if (p0 < left) {
         float c[4];
         key_product<KIND, D, SPLIT>(ring + k_slot * S::kSlot, place, q_at, c);
         // rows 2 t, 2 t + 1 at position pi(g), then at pi(g) + 8: logits in log2 units, to the reference
         float2 z0 = fma2(make_float2(c[0], c[1]), unit2, minus), z1 = fma2(make_float2(c[2], c[3]), unit2, minus);
         if (edge) {
-#pragma unroll
-          for (uint32_t i = 0; i < 2; ++i) {
-            const uint32_t r = p.rows * ROWS + 2 * t + i;
-            bits[i] = r < rows ? mask_bits(a, p.seq, token_of(a, r)) : 0ull;
-          }
+          unsigned long long bits[2];
+          row_bits(bits);
           const uint32_t pos = base + p0 + pi8(g);
           if (!sees(bits[0], pos, p.seq)) z0.x = -INFINITY;
           if (!sees(bits[1], pos, p.seq)) z0.y = -INFINITY;
@@ -901,6 +920,8 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         if (edge) {
           value_product<KIND, D, SPLIT, true>(slot, place, p0 + t, left, pb, o);
           const TileView<S> values = {slot, seg_log2};
+          unsigned long long bits[2];
+          row_bits(bits);
           add_special<KIND, D>(values, p0, base, left, p.seq, bits, o);
         } else {
           value_product<KIND, D, SPLIT, false>(slot, place, p0 + t, left, pb, o);
@@ -994,7 +1015,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       }
     }
     __syncthreads();  // read (and the part written), before the next item's are written
-    if (at < end) next_item<ROWS>(a, p);
+    if (todo) next_item<ROWS>(a, p);
   }
 }
 
