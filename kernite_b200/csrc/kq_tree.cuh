@@ -559,7 +559,8 @@ __device__ __forceinline__ void key_product(uint32_t slot, const Lane<Shape<KIND
 // O^T += V^T P^T of the warp's 16 positions, b the weights as operand B (hi, and lo). EDGE: the tile
 // reaches past the prefix, so rows past the end (left: positions the tile has) and values that are not
 // finite count as zero here (P is zero where a position is masked, and zero times those would not be);
-// add_special adds the latter where they are seen.
+// the caller adds the latter where they are
+// seen.
 template <uint32_t KIND, uint32_t D, bool SPLIT, bool EDGE>
 __device__ __forceinline__ void value_product(uint32_t slot, const Lane<Shape<KIND, D>>& at, uint32_t first,
                                               uint32_t left, const uint32_t (&b)[4], float (&o)[D / 16][4]) {
@@ -620,42 +621,36 @@ __device__ __forceinline__ void value_product(uint32_t slot, const Lane<Shape<KI
   }
 }
 
-// The values value_product<EDGE> left out, of the warp's positions p0 .. p0 + 15 below `left`: infinities
-// and NaN reach the rows that see their position. bits: the mask words of rows 2 t and 2 t + 1.
+// Of the warp's positions p0 .. p0 + 15 below `left`, those with a value that is not finite, as bits.
 template <uint32_t KIND, uint32_t D>
-__device__ __noinline__ void add_special(const TileView<Shape<KIND, D>>& tile, uint32_t p0, uint32_t base,
-                                         uint32_t left, const Seq& seq, const unsigned long long (&bits)[2],
-                                         float (&o)[D / 16][4]) {
+__device__ __noinline__ uint32_t special_positions(TileView<Shape<KIND, D>> tile, uint32_t p0, uint32_t left) {
   using S = Shape<KIND, D>;
-  const uint32_t lane = threadIdx.x % 32, g = lane >> 2;
+  const uint32_t lane = threadIdx.x % 32;
+  uint32_t found = 0;
   for (uint32_t p = p0; p < p0 + 16 && p < left; ++p) {
     bool odd = false;
     if constexpr (KIND == KQ_CACHE_F16) {
       for (uint32_t u = lane; u < S::kRow / 16; u += 32) {
         const uint4 v = lds_v4(tile.code(p, 16 * u));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) odd |= finite_or_zero(w[i]) != w[i];
+        odd |= finite_or_zero(v.x) != v.x || finite_or_zero(v.y) != v.y || finite_or_zero(v.z) != v.z ||
+               finite_or_zero(v.w) != v.w;
       }
     } else {
       if (lane < S::kScales) odd = lds_u8(tile.scale(p) + lane) >= 0xf8u;
     }
-    if (!__any_sync(0xffffffffu, odd)) continue;
-#pragma unroll
-    for (uint32_t j = 0; j < D / 16; ++j)
-#pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t e = value_element<S>(j, g, h);
-        float add = 0.f;
-        if constexpr (KIND == KQ_CACHE_F16) {
-          const uint32_t v = lds_u16(tile.code(p, 2 * e));
-          if ((v & 0x7c00u) == 0x7c00u) add = h2f(v);
-        } else {
-          if (lds_u8(tile.scale(p) + e / 32) >= 0xf8u) add = __int_as_float(0x7fc00000);
-        }
-        if (sees(bits[0], base + p, seq)) o[j][2 * h] += add;
-        if (sees(bits[1], base + p, seq)) o[j][2 * h + 1] += add;
-      }
+    if (__any_sync(0xffffffffu, odd)) found |= 1u << (p - p0);
+  }
+  return found;
+}
+
+// What value_product<EDGE> left out of element e of position p: its value where that is not finite.
+template <uint32_t KIND, uint32_t D>
+__device__ __forceinline__ float special_value(const TileView<Shape<KIND, D>>& tile, uint32_t p, uint32_t e) {
+  if constexpr (KIND == KQ_CACHE_F16) {
+    const uint32_t v = lds_u16(tile.code(p, 2 * e));
+    return (v & 0x7c00u) == 0x7c00u ? h2f(v) : 0.f;
+  } else {
+    return lds_u8(tile.scale(p) + e / 32) >= 0xf8u ? __int_as_float(0x7fc00000) : 0.f;
   }
 }
 
@@ -920,9 +915,21 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         if (edge) {
           value_product<KIND, D, SPLIT, true>(slot, place, p0 + t, left, pb, o);
           const TileView<S> values = {slot, seg_log2};
-          unsigned long long bits[2];
-          row_bits(bits);
-          add_special<KIND, D>(values, p0, base, left, p.seq, bits, o);
+          // infinities and NaN reach the rows that see their position
+          for (uint32_t odd = special_positions<KIND, D>(values, p0, left); odd; odd &= odd - 1) {
+            const uint32_t pos = p0 + __ffs(odd) - 1;
+            unsigned long long bits[2];
+            row_bits(bits);
+            const bool see0 = sees(bits[0], base + pos, p.seq), see1 = sees(bits[1], base + pos, p.seq);
+#pragma unroll
+            for (uint32_t j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (uint32_t h = 0; h < 2; ++h) {
+                const float v = special_value<KIND, D>(values, pos, value_element<S>(j, g, h));
+                if (see0) o[j][2 * h] += v;
+                if (see1) o[j][2 * h + 1] += v;
+              }
+          }
         } else {
           value_product<KIND, D, SPLIT, false>(slot, place, p0 + t, left, pb, o);
         }
