@@ -223,7 +223,7 @@ __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t
 // then meet no bank twice.
 //
 // What bounds it: the instructions (about 290 a warp for 16 positions of 128 elements in 8 bits) against
-// the bytes' time. Warps 0 and 1 also start the copies (keys, values) of a tile some tiles ahead.
+// the bytes' time.
 
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kThreads = kWarps * 32;
@@ -661,12 +661,6 @@ __device__ __forceinline__ float special_value(const TileView<Shape<KIND, D>>& t
 constexpr float kLift = 2.f;
 constexpr float kSlack = 13.f;
 
-// What a copying warp has next: the tile, its first use of the ring, the tiles left.
-struct CopyState {
-  Place place;
-  uint32_t use, left;
-};
-
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(const __grid_constant__ TreeArgs a) {
   using S = Shape<KIND, D>;
@@ -677,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   float* join_m = join + 4 * 8 * M::kJoinRow;                    // [warp][row], then sums
   float* join_l = join_m + kWarps * 8;
   uint4* q_smem = reinterpret_cast<uint4*>(join_l + kWarps * 8);
-  __shared__ CopyState copies[2];
+  __shared__ Place places[kWarps];  // of each warp's next copies
   const uint32_t ring = smem_u32(smem), bars = ring + NS * S::kSlot + M::kJoin + M::kQ;  // full, empty of each slot
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
@@ -699,54 +693,62 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   Place p = locate(a, work, at);
   bool live = true;  // no wait has given up
 
-  // ---- copies: warp 0 keys (uses 2 i of the ring), warp 1 values (2 i + 1); lane i segment i of a tile.
-  // Their place is in shared memory: registers are what the loop below is short of.
-  uint32_t todo = static_cast<uint32_t>(end - at);  // tiles of this CTA not yet read
+  // ---- copies: warp w those of tiles w, w + 8, ... of this CTA (uses 2 i and 2 i + 1 of the ring for tile
+  // i's keys and values), lane k segment k. Taking turns keeps any one warp from being the slow one. Their
+  // place is in shared memory: registers are what the loop below is short of.
+  const uint32_t count = static_cast<uint32_t>(end - at);  // tiles of this CTA
   const uint32_t seg_log2 = min(a.c.page_log2, 7u);
-  uint32_t c_page = 0;  // the lane's page of the copies' tile, loaded a tile ahead
+  uint32_t c_tile = warp;  // the warp's next tile to copy
+  uint32_t c_page = 0;     // the lane's page of it
   const auto page_of = [&](const Place& cp) {
     const uint32_t pos = cp.tile * kTile + (lane << seg_log2);
     return lane < kTile >> seg_log2 && pos < cp.seq.length()
                ? static_cast<uint32_t>(a.pages[uint64_t(cp.s) * a.max_pages + (pos >> a.c.page_log2)])
                : 0u;
   };
-  // starts the copies of uses below `upto`; all but the NS last uses before it have been read
-  const auto copy = [&](uint32_t upto) {
-    CopyState& state = copies[warp];
-    while (state.use < upto && state.left) {
-      const uint32_t use = state.use, slot = use % NS, bar = bars + 16 * slot;
-      if (use >= NS && live && !mbar_wait(bar + 8, (use / NS - 1) & 1)) {
-        report_error(a.err, kErrWaitEmpty);
-        live = false;
-      }
-      live = __all_sync(0xffffffffu, live);
-      if (!live) return;
-      Place cp = state.place;
-      const uint32_t left = state.left - 1;
-      copy_segments<S>(a, cp, c_page, warp ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
-      if (++cp.tile == position_tiles<kTile>(cp.seq) && left) next_item<ROWS>(a, cp);
-      if (left) c_page = page_of(cp);
+  // the place n tiles on, c_tile being in this CTA's range
+  const auto advance = [&](Place cp, uint32_t n) {
+    uint32_t left = position_tiles<kTile>(cp.seq) - cp.tile;
+    while (n >= left) {
+      n -= left;
+      next_item<ROWS>(a, cp);
+      left = position_tiles<kTile>(cp.seq);
+    }
+    cp.tile += n;
+    if (lane == 0) places[warp] = cp;
+    c_page = page_of(cp);
+  };
+  const auto copy = [&](uint32_t kv) {
+    const uint32_t use = 2 * c_tile + kv, slot = use % NS, bar = bars + 16 * slot;
+    if (use >= NS && live && !mbar_wait(bar + 8, (use / NS - 1) & 1)) {
+      report_error(a.err, kErrWaitEmpty);
+      live = false;
+    }
+    live = __all_sync(0xffffffffu, live);
+    __syncwarp();
+    const Place cp = places[warp];
+    if (live) copy_segments<S>(a, cp, c_page, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
+    if (kv) {
+      c_tile += kWarps;
       __syncwarp();
-      if (lane == 0) {
-        state.place = cp;
-        state.use = use + 2;
-        state.left = left;
-      }
-      __syncwarp();
+      if (c_tile < count) advance(cp, kWarps);
     }
   };
-  if (warp < 2) {
-    if (lane == 0) copies[warp] = {p, warp, todo};
-    c_page = page_of(p);
-    __syncwarp();
-    copy(NS);
+  // tiles are copied AHEAD ones before they are read: keys when a tile starts, values after its keys have
+  // been read (the slot they get, where the ring is odd)
+  constexpr uint32_t AHEAD = NS % 2 ? (NS - 1) / 2 : (NS - 2) / 2;
+  if (c_tile < count) advance(p, warp);
+  __syncwarp();
+  if (c_tile < min(count, AHEAD)) {
+    copy(0);
+    copy(1);
   }
 
   const uint32_t g = lane >> 2, t = lane & 3u;
   const uint32_t p0 = warp * 16;
   const Lane<S> place(p0, g, t, seg_log2);
-  uint32_t it = 0;  // uses of the ring read
-  while (todo) {
+  uint32_t done = 0;  // tiles of this CTA read
+  while (done < count) {
     // ---- the item's rows as operand B (row n = g), each scaled by a power of two to a largest element in
     // [2^7, 2^8), so that f16's range fits any q; and what rows 2 t, 2 t + 1 need
     const uint32_t rows = p.seq.drafts * a.group;
@@ -827,8 +829,13 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
     float limit = -INFINITY;  // weights' exponents above this want a new reference
 
     const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
-    for (; p.tile < tiles && todo; ++p.tile, --todo, it += 2) {
-      if (warp < 2) copy(it + NS);
+    for (; p.tile < tiles && done < count; ++p.tile, ++done) {
+      const uint32_t it = 2 * done;
+      const bool copies = c_tile == done + AHEAD && c_tile < count;  // this warp's turn
+      if (copies) {
+        copy(0);
+        if constexpr (NS % 2 == 0) copy(1);
+      }
       const uint32_t base = p.tile * kTile, left = p.seq.length() - base;  // positions left in the cache
       const bool edge = base + kTile > p.seq.prefix;
       const uint32_t k_slot = it % NS, v_slot = (it + 1) % NS;
@@ -905,6 +912,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + 16 * k_slot + 8);
+      if (NS % 2 && copies) copy(1);
       if (live && !mbar_wait(bars + 16 * v_slot, ((it + 1) / NS) & 1)) {
         report_error(a.err, kErrWaitFull);
         live = false;
@@ -1022,7 +1030,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       }
     }
     __syncthreads();  // read (and the part written), before the next item's are written
-    if (todo) next_item<ROWS>(a, p);
+    if (done < count) next_item<ROWS>(a, p);
   }
 }
 
