@@ -213,20 +213,20 @@ __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t
 //
 // For few rows (8 an item). mma.sync.m16n8k16 (f16 in, f32 accumulated), operands from registers: the
 // positions are M of S^T = K Q^T, the head's elements M of O^T += V^T P^T, and the rows N = 8 of both, so
-// no part of an MMA is spent on rows that are not there; P^T comes from S^T by movmatrix. A warp takes 16
-// of a tile's 128 positions; the eight warps keep separate maxima, sums and outputs and join them at an
-// item's end. For f32 activations Q and P are sums of two f16 (about 22 bits): two MMAs into one sum.
+// no part of an MMA is spent on rows that are not there; P^T comes from S^T by movmatrix. Seven warps take
+// 16 positions each in turn and keep separate maxima, sums and outputs, joined at an item's end; the
+// eighth copies tiles of 128 positions into a ring, ahead over items' ends. For f32 activations Q and P are
+// sums of two f16 (about 22 bits): two MMAs into one sum.
 //
 // Codes become f16 in registers, exactly. The order of a contraction is free, so a thread's piece of a
 // key row is 16 consecutive bytes, and the element M index of V^T is chosen the same way. Index n of 8
 // positions is position pi(n) = 4 (n mod 2) + n / 2: with the cache's unit permutation the reads of a warp
 // then meet no bank twice.
-//
-// What bounds it: the instructions (about 290 a warp for 16 positions of 128 elements in 8 bits) against
-// the bytes' time.
 
-constexpr uint32_t kWarps = 8;
-constexpr uint32_t kThreads = kWarps * 32;
+constexpr uint32_t kReaders = 7;
+constexpr uint32_t kThreads = (kReaders + 1) * 32;
+constexpr uint32_t kPart = 16;                    // positions a warp takes at once
+constexpr uint32_t kParts = kTile / kPart;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -314,6 +314,30 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   const float2 f = __half22float2(h);
   hi = h2(h);
   lo = h2(__floats2half2_rn(x - f.x, y - f.y));
+}
+
+// How a row of q becomes an f16 operand: times `up`; and the logits (in log2 units) of the product: times
+// `unit`. The power of two in `up` brings the row's largest magnitude (most) to [2^7, 2^8) (or, split,
+// near it), so that f16's range fits any q; it is 1 for a row of zeros or with infinities. 16-bit rows stay
+// exact; split ones take the softmax's scale along, so that `unit` is a power of two and a product's
+// largest logit is the maximum exactly, however large.
+struct RowScale {
+  float up, unit;
+};
+
+template <bool SPLIT>
+__device__ __forceinline__ RowScale row_scale(float most, float scale_log2) {
+  const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
+  const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
+  const float up = __int_as_float((127 + sh) << 23), down = __int_as_float((127 - sh) << 23);
+  if constexpr (SPLIT) {
+    // scale_log2 = fraction x power of two, the fraction in [1, 2)
+    const uint32_t bits = __float_as_uint(scale_log2);
+    const float part = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+    const float power = __uint_as_float(bits & 0x7f800000u);
+    return {up * part, down * power};
+  }
+  return {up, down * scale_log2};
 }
 
 // How a head of pitch D lies in rows of codes, per kind: bytes of a row, EK elements of a thread's piece of
@@ -473,7 +497,7 @@ template <uint32_t KIND, uint32_t D>
 struct Narrow {
   using S = Shape<KIND, D>;
   static constexpr uint32_t kJoinRow = D + 16;
-  static constexpr uint32_t kJoin = 4 * 8 * kJoinRow * 4 + kWarps * 8 * 2 * 4;
+  static constexpr uint32_t kJoin = 4 * 8 * kJoinRow * 4 + 4 * 8 * 2 * 4;
   static constexpr bool kQShared = D >= 128;
   static constexpr uint32_t kQ = kQShared ? S::kSteps * 32 * 16 : 0;
   static constexpr uint32_t kFixed = kJoin + kQ + 256;
@@ -484,29 +508,44 @@ struct Narrow {
   static_assert(kSlots >= 2, "a tile");
 };
 
-// Where a lane's pieces lie in a tile. Of its two key positions pi(g), pi(g) + 8 and four value positions
-// t, t + 4, t + 8, t + 12 the ones 8 apart differ by 8 rows (their units are permuted alike); a key row's
-// pieces are 4 units apart, the second in the other half of a line of 128 bytes.
+// Where a lane's pieces lie in 16 positions. Of its two key positions pi(g), pi(g) + 8 and four value
+// positions t, t + 4, t + 8, t + 12 the ones 8 apart differ by 8 rows (their units are permuted alike); a
+// key row's pieces are 4 units apart, the second in the other half of a line of 128 bytes.
 template <class S>
 struct Lane {
   uint32_t key[2], value[2], key_scale, value_scale;
 
-  __device__ Lane(uint32_t p0, uint32_t g, uint32_t t, uint32_t seg_log2) {
-    const uint32_t in = p0 & ((1u << seg_log2) - 1), pg = S::kPermuted ? pi8(g) : g;
-    const uint32_t seg = ((p0 >> seg_log2) << seg_log2) * (S::kRow + S::kScales);
+  __device__ Lane(uint32_t g, uint32_t t) {
+    const uint32_t pg = S::kPermuted ? pi8(g) : g;
     constexpr uint32_t BK = S::EK * S::kBits / 8, BV = S::EV * S::kBits / 8;
-    key[0] = seg + cache_offset(in + pi8(g), BK * t, S::kRow);
-    key[1] = seg + (cache_offset(in + pi8(g), BK * t, S::kRow) ^ 64u);
-    value[0] = seg + cache_offset(in + t, BV * pg, S::kRow);
-    value[1] = seg + cache_offset(in + t + 4, BV * pg, S::kRow);
-    key_scale = seg + (S::kRow << seg_log2) + (in + pi8(g)) * S::kScales + S::EK * t / 32;
-    value_scale = seg + (S::kRow << seg_log2) + (in + t) * S::kScales + S::EV * pg / 32;
+    key[0] = cache_offset(pi8(g), BK * t, S::kRow);
+    key[1] = key[0] ^ 64u;
+    value[0] = cache_offset(t, BV * pg, S::kRow);
+    value[1] = cache_offset(t + 4, BV * pg, S::kRow);
+    key_scale = pi8(g) * S::kScales + S::EK * t / 32;
+    value_scale = t * S::kScales + S::EV * pg / 32;
+  }
+};
+
+// Where 16 positions (number `part` of a tile) lie: the first one's row and scales. A segment (a page, or a
+// tile's part of one) is its rows and then its scales; 16 rows are whole lines of 128 bytes, so the
+// permutation is that of the positions in them.
+template <class S>
+struct PartView {
+  uint32_t code, scale;
+
+  __device__ PartView(uint32_t slot, uint32_t part, uint32_t seg_log2) {
+    const uint32_t p0 = part * kPart, in = p0 & ((1u << seg_log2) - 1);
+    const uint32_t seg = slot + (p0 - in) * (S::kRow + S::kScales);
+    code = seg + in * S::kRow;
+    scale = seg + (S::kRow << seg_log2) + in * S::kScales;
   }
 };
 
 // S^T of the warp's 16 positions: c = sum of K Q^T over the head, q the rows' operand B (hi, and lo).
 template <uint32_t KIND, uint32_t D, bool SPLIT, class Q>
-__device__ __forceinline__ void key_product(uint32_t slot, const Lane<Shape<KIND, D>>& at, const Q& q,
+__device__ __forceinline__ void key_product(const PartView<Shape<KIND, D>>& part,
+                                            const Lane<Shape<KIND, D>>& at, const Q& q,
                                             float (&c)[4]) {
   using S = Shape<KIND, D>;
   constexpr uint32_t B = S::EK * S::kBits / 8;
@@ -521,9 +560,9 @@ __device__ __forceinline__ void key_product(uint32_t slot, const Lane<Shape<KIND
     Scale2 s[2];
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
-      lds_words<B>(slot + at.key[j & 1] + h * 8 * S::kRow + (j >> 1) * 128, w[h]);
+      lds_words<B>(part.code + at.key[j & 1] + h * 8 * S::kRow + (j >> 1) * 128, w[h]);
       if constexpr (S::kScales != 0) {
-        const uint32_t b = lds_u8(slot + at.key_scale + h * 8 * S::kScales + j * (S::EK * 4 / 32));
+        const uint32_t b = lds_u8(part.scale + at.key_scale + h * 8 * S::kScales + j * (S::EK * 4 / 32));
         s[h] = scale2<KIND>(b, b);
       }
     }
@@ -562,7 +601,8 @@ __device__ __forceinline__ void key_product(uint32_t slot, const Lane<Shape<KIND
 // the caller adds the latter where they are
 // seen.
 template <uint32_t KIND, uint32_t D, bool SPLIT, bool EDGE>
-__device__ __forceinline__ void value_product(uint32_t slot, const Lane<Shape<KIND, D>>& at, uint32_t first,
+__device__ __forceinline__ void value_product(const PartView<Shape<KIND, D>>& part,
+                                              const Lane<Shape<KIND, D>>& at, uint32_t first,
                                               uint32_t left, const uint32_t (&b)[4], float (&o)[D / 16][4]) {
   using S = Shape<KIND, D>;
   constexpr uint32_t B = S::EV * S::kBits / 8;
@@ -572,7 +612,7 @@ __device__ __forceinline__ void value_product(uint32_t slot, const Lane<Shape<KI
     uint32_t byte[4] = {0, 0, 0, 0};
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {  // position first + 4 i
-      lds_words<B>(slot + at.value[i & 1] + (i >> 1) * 8 * S::kRow + jj * 128, w[i]);
+      lds_words<B>(part.code + at.value[i & 1] + (i >> 1) * 8 * S::kRow + jj * 128, w[i]);
       const bool there = !EDGE || first + 4 * i < left;
       if constexpr (KIND == KQ_CACHE_F16) {
         if constexpr (EDGE) {
@@ -580,7 +620,7 @@ __device__ __forceinline__ void value_product(uint32_t slot, const Lane<Shape<KI
           for (uint32_t k = 0; k < B / 4; ++k) w[i][k] = there ? finite_or_zero(w[i][k]) : 0u;
         }
       } else {
-        byte[i] = lds_u8(slot + at.value_scale + i * 4 * S::kScales + jj * (S::EV * 8 / 32));
+        byte[i] = lds_u8(part.scale + at.value_scale + i * 4 * S::kScales + jj * (S::EV * 8 / 32));
         if constexpr (EDGE) byte[i] = there && byte[i] < 0xf8u ? byte[i] : 0u;
       }
     }
@@ -668,16 +708,15 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   constexpr uint32_t ROWS = 8, NS = M::kSlots;
   extern __shared__ __align__(128) uint8_t smem[];
   float* join = reinterpret_cast<float*>(smem + NS * S::kSlot);  // 4 warps x 8 rows
-  float* join_m = join + 4 * 8 * M::kJoinRow;                    // [warp][row], then sums
-  float* join_l = join_m + kWarps * 8;
-  uint4* q_smem = reinterpret_cast<uint4*>(join_l + kWarps * 8);
-  __shared__ Place places[kWarps];  // of each warp's next copies
+  float* join_m = join + 4 * 8 * M::kJoinRow;                    // [warp of 4][row], then sums
+  float* join_l = join_m + 4 * 8;
+  uint4* q_smem = reinterpret_cast<uint4*>(join_l + 4 * 8);
   const uint32_t ring = smem_u32(smem), bars = ring + NS * S::kSlot + M::kJoin + M::kQ;  // full, empty of each slot
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < NS; ++i) {
       mbar_init(bars + 16 * i, 1);
-      mbar_init(bars + 16 * i + 8, kWarps);
+      mbar_init(bars + 16 * i + 8, kParts);
     }
     fence_mbar_init();
   }
@@ -688,69 +727,47 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   const uint64_t total = work.total;
   const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(gridDim.x), total));
   if (blockIdx.x >= ctas) return;
-  uint64_t at = range_start(total, blockIdx.x, ctas);
-  const uint64_t end = range_start(total, blockIdx.x + 1, ctas);
+  const uint64_t at = range_start(total, blockIdx.x, ctas);
+  const uint32_t count = static_cast<uint32_t>(range_start(total, blockIdx.x + 1, ctas) - at);  // this CTA's tiles
   Place p = locate(a, work, at);
+  const uint32_t seg_log2 = min(a.c.page_log2, 7u);
   bool live = true;  // no wait has given up
 
-  // ---- copies: warp w those of tiles w, w + 8, ... of this CTA (uses 2 i and 2 i + 1 of the ring for tile
-  // i's keys and values), lane k segment k. Taking turns keeps any one warp from being the slow one. Their
-  // place is in shared memory: registers are what the loop below is short of.
-  const uint32_t count = static_cast<uint32_t>(end - at);  // tiles of this CTA
-  const uint32_t seg_log2 = min(a.c.page_log2, 7u);
-  uint32_t c_tile = warp;  // the warp's next tile to copy
-  uint32_t c_page = 0;     // the lane's page of it
-  const auto page_of = [&](const Place& cp) {
-    const uint32_t pos = cp.tile * kTile + (lane << seg_log2);
-    return lane < kTile >> seg_log2 && pos < cp.seq.length()
-               ? static_cast<uint32_t>(a.pages[uint64_t(cp.s) * a.max_pages + (pos >> a.c.page_log2)])
-               : 0u;
-  };
-  // the place n tiles on, c_tile being in this CTA's range
-  const auto advance = [&](Place cp, uint32_t n) {
-    uint32_t left = position_tiles<kTile>(cp.seq) - cp.tile;
-    while (n >= left) {
-      n -= left;
-      next_item<ROWS>(a, cp);
-      left = position_tiles<kTile>(cp.seq);
+  if (warp == kReaders) {
+    // ---- copies: uses 2 i and 2 i + 1 of the ring for tile i's keys and values, lane k segment k
+    const auto page_of = [&]() {
+      const uint32_t pos = p.tile * kTile + (lane << seg_log2);
+      return lane < kTile >> seg_log2 && pos < p.seq.length()
+                 ? static_cast<uint32_t>(a.pages[uint64_t(p.s) * a.max_pages + (pos >> a.c.page_log2)])
+                 : 0u;
+    };
+    uint32_t page = page_of();
+    for (uint32_t i = 0; i < count; ++i) {
+      const Place now = p;
+      const uint32_t now_page = page;
+      if (i + 1 < count) {  // the next tile's pages come in while this one waits for its slots
+        if (++p.tile == position_tiles<kTile>(p.seq)) next_item<ROWS>(a, p);
+        page = page_of();
+      }
+#pragma unroll
+      for (uint32_t kv = 0; kv < 2; ++kv) {
+        const uint32_t use = 2 * i + kv, slot = use % NS, bar = bars + 16 * slot;
+        if (use >= NS && live && !mbar_wait(bar + 8, (use / NS - 1) & 1)) {
+          report_error(a.err, kErrWaitEmpty);
+          live = false;
+        }
+        live = __all_sync(0xffffffffu, live);
+        if (live) copy_segments<S>(a, now, now_page, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
+      }
     }
-    cp.tile += n;
-    if (lane == 0) places[warp] = cp;
-    c_page = page_of(cp);
-  };
-  const auto copy = [&](uint32_t kv) {
-    const uint32_t use = 2 * c_tile + kv, slot = use % NS, bar = bars + 16 * slot;
-    if (use >= NS && live && !mbar_wait(bar + 8, (use / NS - 1) & 1)) {
-      report_error(a.err, kErrWaitEmpty);
-      live = false;
-    }
-    live = __all_sync(0xffffffffu, live);
-    __syncwarp();
-    const Place cp = places[warp];
-    if (live) copy_segments<S>(a, cp, c_page, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
-    if (kv) {
-      c_tile += kWarps;
-      __syncwarp();
-      if (c_tile < count) advance(cp, kWarps);
-    }
-  };
-  // tiles are copied AHEAD ones before they are read: keys when a tile starts, values after its keys have
-  // been read (the slot they get, where the ring is odd)
-  constexpr uint32_t AHEAD = NS % 2 ? (NS - 1) / 2 : (NS - 2) / 2;
-  if (c_tile < count) advance(p, warp);
-  __syncwarp();
-  if (c_tile < min(count, AHEAD)) {
-    copy(0);
-    copy(1);
+    return;
   }
 
   const uint32_t g = lane >> 2, t = lane & 3u;
-  const uint32_t p0 = warp * 16;
-  const Lane<S> place(p0, g, t, seg_log2);
+  const Lane<S> place(g, t);
   uint32_t done = 0;  // tiles of this CTA read
   while (done < count) {
-    // ---- the item's rows as operand B (row n = g), each scaled by a power of two to a largest element in
-    // [2^7, 2^8), so that f16's range fits any q; and what rows 2 t, 2 t + 1 need
+    // ---- the item's rows as operand B (row n = g), scaled (row_scale), and what rows 2 t, 2 t + 1 need
     const uint32_t rows = p.seq.drafts * a.group;
     uint32_t qb[M::kQShared ? 1 : S::kSteps][4];
     float2 unit2;  // logits in log2 units a unit of the scaled product, of rows 2 t and 2 t + 1
@@ -780,11 +797,8 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // 2^(7 - floor(log2(most))), kept inside f32's normal range; 1 for a row of zeros (or infinities)
-      const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
-      const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
-      const float up = __int_as_float((127 + sh) << 23);
-      const float unit = __int_as_float((127 - sh) << 23) * a.scale_log2;
+      const RowScale scale = row_scale<SPLIT>(most, a.scale_log2);
+      const float up = scale.up, unit = scale.unit;
       unit2.x = __shfl_sync(0xffffffffu, unit, 8 * t);
       unit2.y = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
 #pragma unroll
@@ -829,14 +843,10 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
     float limit = -INFINITY;  // weights' exponents above this want a new reference
 
     const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
-    for (; p.tile < tiles && done < count; ++p.tile, ++done) {
-      const uint32_t it = 2 * done;
-      const bool copies = c_tile == done + AHEAD && c_tile < count;  // this warp's turn
-      if (copies) {
-        copy(0);
-        if constexpr (NS % 2 == 0) copy(1);
-      }
-      const uint32_t base = p.tile * kTile, left = p.seq.length() - base;  // positions left in the cache
+    const uint32_t here = min(tiles - first_tile, count - done);  // of the item's tiles, this CTA's
+    for (uint32_t n = warp; n < here * kParts; n += kReaders) {
+      const uint32_t it = 2 * (done + n / kParts), part_no = n % kParts, p0 = part_no * kPart;
+      const uint32_t base = (first_tile + n / kParts) * kTile, left = p.seq.length() - base;  // positions left
       const bool edge = base + kTile > p.seq.prefix;
       const uint32_t k_slot = it % NS, v_slot = (it + 1) % NS;
       if (live && !mbar_wait(bars + 16 * k_slot, (it / NS) & 1)) {
@@ -854,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       };
       if (p0 < left) {
         float c[4];
-        key_product<KIND, D, SPLIT>(ring + k_slot * S::kSlot, place, q_at, c);
+        key_product<KIND, D, SPLIT>(PartView<S>(ring + k_slot * S::kSlot, part_no, seg_log2), place, q_at, c);
         // rows 2 t, 2 t + 1 at position pi(g), then at pi(g) + 8: logits in log2 units, to the reference
         float2 z0 = fma2(make_float2(c[0], c[1]), unit2, minus), z1 = fma2(make_float2(c[2], c[3]), unit2, minus);
         if (edge) {
@@ -869,22 +879,30 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         if (__any_sync(0xffffffffu, max3(fmaxf(z0.x, z0.y), z1.x, z1.y) > limit)) {
           // a new reference for the rows that want one (all rows have one after this, but those that see
           // nothing yet, whose weights are zero whatever it is)
-          float top[2] = {fmaxf(z0.x, z1.x), fmaxf(z0.y, z1.y)}, f[2], down[2];
+          // The logits themselves, each one rounded: the largest is then exactly the reference, however
+          // large it is.
+          const float x[4] = {__fmul_rn(c[0], unit2.x), __fmul_rn(c[1], unit2.y), __fmul_rn(c[2], unit2.x),
+                              __fmul_rn(c[3], unit2.y)};
+          float* z[4] = {&z0.x, &z0.y, &z1.x, &z1.y};
+          float f[2];
 #pragma unroll
           for (uint32_t i = 0; i < 2; ++i) {
+            float top = fmaxf(*z[i], *z[2 + i]);  // to the old reference
+            float now = fmaxf(*z[i] == -INFINITY ? -INFINITY : x[i], *z[2 + i] == -INFINITY ? -INFINITY : x[2 + i]);
 #pragma unroll
-            for (int s = 4; s < 32; s <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], s));
-            const float old = i ? minus.y : minus.x;
+            for (int s = 4; s < 32; s <<= 1) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+              now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+            }
             const bool fresh = m[i] == -INFINITY;
-            const float now = fresh || top[i] > kSlack + kLift ? top[i] - old : m[i];  // a logit itself
+            if (!fresh && !(top > kSlack + kLift)) now = m[i];
             const float next = now == -INFINITY ? 0.f : kLift - now;
             f[i] = fresh ? 0.f : exp2f(m[i] - now);
-            down[i] = next - old;
             m[i] = now;
             (i ? minus.y : minus.x) = next;
+            if (*z[i] != -INFINITY) *z[i] = x[i] + next;
+            if (*z[2 + i] != -INFINITY) *z[2 + i] = x[2 + i] + next;
           }
-          z0 = add2(z0, make_float2(down[0], down[1]));
-          z1 = add2(z1, make_float2(down[0], down[1]));
           l.x *= f[0];
           l.y *= f[1];
 #pragma unroll
@@ -912,7 +930,6 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + 16 * k_slot + 8);
-      if (NS % 2 && copies) copy(1);
       if (live && !mbar_wait(bars + 16 * v_slot, ((it + 1) / NS) & 1)) {
         report_error(a.err, kErrWaitFull);
         live = false;
@@ -921,7 +938,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       if (p0 < left) {
         const uint32_t slot = ring + v_slot * S::kSlot;
         if (edge) {
-          value_product<KIND, D, SPLIT, true>(slot, place, p0 + t, left, pb, o);
+          value_product<KIND, D, SPLIT, true>(PartView<S>(slot, part_no, seg_log2), place, p0 + t, left, pb, o);
           const TileView<S> values = {slot, seg_log2};
           // infinities and NaN reach the rows that see their position
           for (uint32_t odd = special_positions<KIND, D>(values, p0, left); odd; odd &= odd - 1) {
@@ -939,17 +956,18 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
               }
           }
         } else {
-          value_product<KIND, D, SPLIT, false>(slot, place, p0 + t, left, pb, o);
+          value_product<KIND, D, SPLIT, false>(PartView<S>(slot, part_no, seg_log2), place, p0 + t, left, pb, o);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + 16 * v_slot + 8);
     }
-    const bool whole = first_tile == 0 && p.tile == tiles;
+    done += here;
+    const bool whole = here == tiles;
     float* part = a.part + (uint64_t(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * part_floats(ROWS, D);
 
-    // ---- the warps' maxima, sums and outputs joined: warps 4-7 give theirs to 0-3, register for
-    // register; those lay rows out, and a warp sums a row
+    // ---- the warps' maxima, sums and outputs joined: warps 4-6 give theirs to 0-2, register for
+    // register; 0-3 lay rows out, and warps sum rows
     constexpr uint32_t RAW = D / 16 * 4 + 4;  // floats a lane gives
     static_assert(RAW * 32 <= 8 * M::kJoinRow, "a warp's registers fit its rows");
     float* mine = join + (warp & 3) * 8 * M::kJoinRow;
@@ -963,22 +981,25 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       mine[(RAW - 2) * 32 + lane] = l.x;
       mine[(RAW - 1) * 32 + lane] = l.y;
     }
-    __syncthreads();
+    named_barrier(1, kReaders * 32);
     if (warp < 4) {
-      float f[2], h[2];
+      if (warp < kReaders - 4) {
+        float f[2], h[2];
 #pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {
-        const float other = mine[(RAW - 4 + i) * 32 + lane], now = fmaxf(m[i], other);
-        f[i] = m[i] == now ? 1.f : exp2f(m[i] - now);
-        h[i] = other == now ? 1.f : exp2f(other - now);
-        m[i] = now;
+        for (uint32_t i = 0; i < 2; ++i) {
+          const float other = mine[(RAW - 4 + i) * 32 + lane], now = fmaxf(m[i], other);
+          f[i] = m[i] == now ? 1.f : exp2f(m[i] - now);
+          h[i] = other == now ? 1.f : exp2f(other - now);
+          m[i] = now;
+        }
+        l.x = fmaf(h[0], mine[(RAW - 2) * 32 + lane], f[0] * l.x);
+        l.y = fmaf(h[1], mine[(RAW - 1) * 32 + lane], f[1] * l.y);
+#pragma unroll
+        for (uint32_t j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i)
+            o[j][i] = fmaf(h[i & 1], mine[(j * 4 + i) * 32 + lane], f[i & 1] * o[j][i]);
       }
-      l.x = fmaf(h[0], mine[(RAW - 2) * 32 + lane], f[0] * l.x);
-      l.y = fmaf(h[1], mine[(RAW - 1) * 32 + lane], f[1] * l.y);
-#pragma unroll
-      for (uint32_t j = 0; j < D / 16; ++j)
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) o[j][i] = fmaf(h[i & 1], mine[(j * 4 + i) * 32 + lane], f[i & 1] * o[j][i]);
 #pragma unroll
       for (int s = 4; s < 32; s <<= 1) {
         l.x += __shfl_xor_sync(0xffffffffu, l.x, s);
@@ -997,9 +1018,10 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         join_l[warp * 8 + 2 * t + 1] = l.y;
       }
     }
-    __syncthreads();
-    {
-      const uint32_t row = warp, rr = p.rows * ROWS + row;
+    named_barrier(1, kReaders * 32);
+    for (uint32_t row = warp; row < 8; row += kReaders) {
+      const uint32_t rr = p.rows * ROWS + row;
+      if (rr >= rows) break;
       float mx = -INFINITY;
 #pragma unroll
       for (uint32_t w = 0; w < 4; ++w) mx = fmaxf(mx, join_m[w * 8 + row]);
@@ -1010,27 +1032,27 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         f[w] = exp2f(join_m[w * 8 + row] - ref);
         den = fmaf(f[w], join_l[w * 8 + row], den);
       }
-      if (rr < rows) {
-        const float inv = whole ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
-        const uint32_t tok = token_of(a, rr);
-        const uint64_t to = (p.seq.first + tok) * a.out_token +
-                            uint64_t(p.head * a.group + head_of(a, rr, tok)) * a.c.dim;
+      const float inv = whole ? (den == 0.f ? 0.f : 1.f / den) : 1.f;
+      const uint32_t tok = token_of(a, rr);
+      const uint64_t to = (p.seq.first + tok) * a.out_token +
+                          uint64_t(p.head * a.group + head_of(a, rr, tok)) * a.c.dim;
 #pragma unroll
-        for (uint32_t e = lane; e < D; e += 32) {
-          float v = 0.f;
+      for (uint32_t e = lane; e < D; e += 32) {
+        float v = 0.f;
 #pragma unroll
-          for (uint32_t w = 0; w < 4; ++w) v = fmaf(f[w], join[(w * 8 + row) * M::kJoinRow + e], v);
-          if (!whole) part[row * D + e] = v;
-          else if (e < a.c.dim) store_one(a.out, to + e, v * inv, a.type);
-        }
-        if (!whole && lane == 0) {
-          part[ROWS * D + row] = mx;
-          part[ROWS * (D + 1) + row] = den;
-        }
+        for (uint32_t w = 0; w < 4; ++w) v = fmaf(f[w], join[(w * 8 + row) * M::kJoinRow + e], v);
+        if (!whole) part[row * D + e] = v;
+        else if (e < a.c.dim) store_one(a.out, to + e, v * inv, a.type);
+      }
+      if (!whole && lane == 0) {
+        part[ROWS * D + row] = mx;
+        part[ROWS * (D + 1) + row] = den;
       }
     }
-    __syncthreads();  // read (and the part written), before the next item's are written
-    if (done < count) next_item<ROWS>(a, p);
+    if (done < count) {
+      next_item<ROWS>(a, p);
+      named_barrier(1, kReaders * 32);  // read, before the next item's are written
+    }
   }
 }
 

@@ -463,8 +463,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     float* chain = exchange + 512;  // [group][lane]: a row's maximum after the group's last tile
     uint32_t n = 0, items = 0, swaps = 0;
     while (at < end) {
-      // Q as operand A: lane m's row is 16 (m / 32) + m % 16, parts (m % 32) / 16, or row m; each row
-      // scaled by a power of two to a largest element in [2^7, 2^8). This thread: half of its row.
+      // Q as operand A: lane m's row is 16 (m / 32) + m % 16, parts (m % 32) / 16, or row m; scaled
+      // (row_scale). This thread: half of its row.
       const uint32_t rows = p.seq.drafts * a.group;
       const uint32_t in_tile = SPLIT ? quad * 16 + lane % 16 : slot;
       const uint32_t my_row = p.rows * ROWS + in_tile;
@@ -489,10 +489,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
 #pragma unroll
           for (uint32_t k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[j][k]));
         most = fmaxf(most, swap(swaps++ & 1, most));
-        const int ex = static_cast<int>(__float_as_uint(most) >> 23) - 127;
-        const int sh = most > 0.f && ex < 128 ? min(max(7 - ex, -120), 120) : 0;
-        const float up = __int_as_float((127 + sh) << 23);
-        unit = __int_as_float((127 - sh) << 23) * a.scale_log2;
+        const RowScale scale = row_scale<SPLIT>(most, a.scale_log2);
+        const float up = scale.up;
+        unit = scale.unit;
 #pragma unroll
         for (uint32_t j0 = 0; j0 < D / 16; j0 += 4) {
           uint32_t w[16];
@@ -636,12 +635,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           }
         } else {
           // the columns again; columns [c, c + 32) become words [c / 2, c / 2 + 16), over ones already read
-          const auto weights = [&](uint32_t c, uint32_t seen) {
+          // For logits in the millions one rounding of product and difference would leave more than a
+          // weight's size: the product is rounded first, so that the largest gives the reference's weight.
+          const auto weights = [&](uint32_t c, uint32_t seen, bool huge) {
             uint32_t u[32], w[16];
             tmem_read(sbuf + c, u);
 #pragma unroll
             for (uint32_t i = 0; i < 16; ++i) {
-              const float2 z = fma2(make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1])), unit2, ref2);
+              const float2 s2 = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+              const float2 z = huge ? make_float2(__fmul_rn(s2.x, unit) - ref, __fmul_rn(s2.y, unit) - ref)
+                                    : fma2(s2, unit2, ref2);
               const float x = seen >> (2 * i) & 1u ? exp2_fast(z.x) : 0.f;
               const float y = seen >> (2 * i + 1) & 1u ? exp2_fast(z.y) : 0.f;
               sum = add2(sum, make_float2(x, y));
@@ -649,12 +652,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             }
             tmem_st16(sbuf + c / 2, w);
           };
-          if (!edge) {
+          if (!edge && !__any_sync(0xffffffffu, fabsf(m) > 0x1p20f && m != -INFINITY)) {
 #pragma unroll
-            for (uint32_t c = 0; c < COLS; c += 32) weights(c, ~0u);
+            for (uint32_t c = 0; c < COLS; c += 32) weights(c, ~0u, false);
           } else {
 #pragma unroll 1
-            for (uint32_t c = 0; c < COLS; c += 32) weights(c, seen_word(bits, from + static_cast<int>(c)));
+            for (uint32_t c = 0; c < COLS; c += 32)
+              weights(c, edge ? seen_word(bits, from + static_cast<int>(c)) : ~0u, true);
           }
         }
         l += sum.x + sum.y;

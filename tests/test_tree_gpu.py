@@ -219,14 +219,21 @@ def test_extreme_magnitudes(kernels):
         c.layout.put(c.v, c.slot(0, p), np.full((1, 128), 1e-3 * (p + 1), np.float32))
     c.values = [np.stack([c.layout.get(c.v, c.slot(0, p)) for p in range(702)])]
     c.check(c.run(kernels))
-    # a weight of one: the value itself, whatever the scale of q
-    c = Case(ref.F16, 2, 1, 64, 16, [300], [1], seed=9)
+
+
+@pytest.mark.parametrize("type", [kb.TYPE_F32, kb.TYPE_BF16])
+@pytest.mark.parametrize("drafts", [1, 9])
+def test_one_position_takes_all(kernels, drafts, type):
+    """Logits of 1e30: a weight of one, the value itself, in both kernels."""
+    c = Case(ref.F16, 2, 1, 64, 16, [300], [drafts], type=type, seed=9)
     c.q *= 1e30
     got = c.run(kernels)
     qv = c.q.double().cpu().numpy()
-    for h in range(2):
-        best = int((c.keys[0][:, 0] @ qv[0, h]).argmax())
-        assert np.abs(got[0, h] - c.values[0][best, 0]).max() <= 2.0 ** -20 * 5
+    for t in range(drafts):
+        seen = [p for p in range(300 + drafts) if p < 300 or c.masks[0][t] >> (p - 300) & 1]
+        for h in range(2):
+            best = seen[int((c.keys[0][seen, 0] @ qv[t, h]).argmax())]
+            assert np.abs(got[t, h] - c.values[0][best, 0]).max() <= (2.0 ** -20 + STEP[type]) * 5
 
 
 def test_scale_strides_and_another_stream(kernels):
