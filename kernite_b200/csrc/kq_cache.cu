@@ -8,10 +8,12 @@
 #include <cmath>
 #include <cstring>
 #include <string>
+#include <type_traits>
 
 #include "kq_cache.cuh"
 #include "kq_device.cuh"
 #include "kq_internal.h"
+#include "kq_launch.h"
 
 namespace kq {
 namespace {
@@ -106,12 +108,17 @@ __device__ __forceinline__ void keep(const CacheView& c, uint8_t* record, uint32
   for (int o = 16 / VE; o; o >>= 1) most = max(most, __shfl_xor_sync(mask, most, o));
   const uint32_t byte = scale_byte(most, c.kind);
   const float scale = scale_value(byte), top = cache_top(c.kind);
+  const bool zero = byte == 0 || byte == kScaleNan;
+  const float inverse = zero ? 0.f : 1.f / scale;
   uint32_t u[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    // a correctly rounded quotient: which codes a value near a tie gets must not depend on how the
-    // division was made
-    const float code = byte == 0 || byte == kScaleNan ? 0.f : rintf(__fdiv_rn(y[i], scale));
+    // The code is the correctly rounded quotient's nearest integer, so that which of two a value near a tie
+    // gets does not depend on how it was divided: the product with the rounded reciprocal (off by 2^-15 at
+    // most) decides unless it is that near.
+    const float q = zero ? 0.f : y[i] * inverse;
+    float code = rintf(q);
+    if (fabsf(fabsf(q - code) - 0.5f) < 0x1p-12f) code = rintf(__fdiv_rn(y[i], scale));
     u[i] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(code, -top), top)) +
                                  (c.kind == KQ_CACHE_Q8 ? 128 : 8));
   }
@@ -140,13 +147,10 @@ __device__ __forceinline__ void keep(const CacheView& c, uint8_t* record, uint32
   if (e % 8 == 0) *reinterpret_cast<uint32_t*>(record + cache_offset(p, e / 2, c.row)) = word;
 }
 
-// Grid (tokens, shares of the rows). The angles of a token are taken once a CTA: position * turns in
-// f64 (position 100000 turns pair 0 by 16000 turns: f32 would leave 10 bits of the fraction), its
-// fraction exactly to f32, then sincospi of twice that.
-template <typename T, int VE>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
-  __shared__ float2 cs[128];
-  const uint32_t t = blockIdx.x;
+// The (gain cos, gain sin) of a token's pairs into shared memory: position * turns in f64 (position 100000
+// turns pair 0 by 16000 turns: f32 would leave 10 bits of the fraction), its fraction exactly to f32, then
+// sincospi of twice that.
+__device__ __forceinline__ void take_angles(const RopeArgs& a, uint32_t t, float2* cs) {
   for (uint32_t i = threadIdx.x; i < a.rot_half; i += kThreads) {
     const double turns = static_cast<double>(a.positions[t]) * a.rope.turns[i];
     const float part = static_cast<float>(turns - rint(turns));
@@ -154,15 +158,110 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     sincospif(2.f * part, &s, &c);
     cs[i] = make_float2(a.rope.gain * c, a.rope.gain * s);
   }
+}
+
+// Token t's slot, -1 where it is not kept (or out of the cache, which is recorded).
+__device__ __forceinline__ long long take_slot(const RopeArgs& a, uint32_t t) {
+  if (!a.slots) return -1;
+  const long long slot = a.slots[t];
+  if (slot < 0) return -1;
+  if (static_cast<uint64_t>(slot) >> a.cache.page_log2 < a.cache.n_pages) return slot;
+  if (threadIdx.x == 0) report_error(a.err, kErrCacheRange);
+  return -1;
+}
+
+// Heads of 64, 128 or 256 elements, every row on 16 bytes. A lane holds E consecutive elements of a row,
+// dim / E lanes a row, so that its place in a head, and with it its angles, are the same for every row
+// it takes: they stay in registers. A pair's other element is in the lane (pairs) or rot_half / E lanes
+// away (halves). A warp has AHEAD rows' loads in flight. Grid: (tokens, shares of the rows).
+template <typename T, int E>
+__global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4) rope_rows_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr uint32_t AHEAD = 2;
+  __shared__ float2 cs[128];
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t t = blockIdx.x;
+  take_angles(a, t, cs);
+  const long long slot = take_slot(a, t);
   __syncthreads();
-  long long slot = -1;
-  if (a.slots) {
-    slot = a.slots[t];
-    if (slot >= 0 && static_cast<uint64_t>(slot) >> a.cache.page_log2 >= a.cache.n_pages) {
-      if (threadIdx.x == 0) report_error(a.err, kErrCacheRange);
-      slot = -1;
+  const uint32_t rows = a.nq + (slot >= 0 ? 2 * a.cache.n_kv : 0);
+  const uint32_t page = static_cast<uint32_t>(slot >= 0 ? slot >> a.cache.page_log2 : 0);
+  const uint32_t p = static_cast<uint32_t>(slot) & (a.cache.page() - 1);
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t per_row = a.dim / E, e = lane % per_row * E, sub = lane / per_row;
+  const uint32_t at_once = 32 / per_row;  // rows a warp takes at once
+  const bool halves = a.rope.layout == KQ_ROPE_HALVES;
+  const uint32_t rot = 2 * a.rot_half;
+  // y = x * by + other * with; elements past rot as they are
+  float by[E], with[E];
+  uint32_t partner = lane;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    by[i] = 1.f;
+    with[i] = 0.f;
+    if (e + i < rot) {
+      const bool first = halves ? e < a.rot_half : (i & 1) == 0;
+      const float2 w = cs[halves ? (first ? e + i : e + i - a.rot_half) : (e + i) / 2];
+      by[i] = w.x;
+      with[i] = first ? -w.y : w.y;
     }
   }
+  if (halves && e < rot) partner = e < a.rot_half ? lane + a.rot_half / E : lane - a.rot_half / E;
+  const uint32_t step = gridDim.y * kWarps * at_once;
+  for (uint32_t r0 = (blockIdx.y * kWarps + warp) * at_once; r0 < rows; r0 += AHEAD * step) {
+    float x[AHEAD][E];
+#pragma unroll
+    for (uint32_t k = 0; k < AHEAD; ++k) {
+      const uint32_t row = r0 + k * step + sub;
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[k][i] = 0.f;
+      if (row >= rows) continue;
+      const T* from = row < a.nq ? static_cast<const T*>(a.q) + t * a.q_token + row * a.q_head
+                      : row < a.nq + a.cache.n_kv
+                          ? static_cast<const T*>(a.k) + t * a.k_token + (row - a.nq) * a.dim
+                          : static_cast<const T*>(a.v) + t * a.v_token + (row - a.nq - a.cache.n_kv) * a.dim;
+      load_wide<T, E>(from + e, x[k]);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < AHEAD; ++k) {
+      if (r0 + k * step >= rows) break;  // the warp's first row: all its lanes leave
+      const uint32_t row = r0 + k * step + sub;
+      const bool in = row < rows, turns = row < a.nq + a.cache.n_kv;
+      float y[E];
+      if (halves) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float other = __shfl_sync(0xffffffffu, x[k][i], partner);
+          y[i] = turns && e < rot ? fmaf(x[k][i], by[i], other * with[i]) : x[k][i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          y[i] = turns && e + i < rot ? fmaf(x[k][i], by[i], x[k][i ^ 1] * with[i]) : x[k][i];
+      }
+      const uint32_t mask = __ballot_sync(0xffffffffu, in && row >= a.nq);
+      if (!in) continue;
+      if (row < a.nq) {
+        store_wide<T, E>(static_cast<T*>(a.q_out) + t * a.out_token + row * a.out_head + e, y);
+      } else {
+        const uint32_t h = turns ? row - a.nq : row - a.nq - a.cache.n_kv;
+        keep<E>(a.cache, (turns ? a.cache.k : a.cache.v) + a.cache.at(page, h), p, e, y, mask);
+      }
+    }
+  }
+}
+
+// Any other head, stride or alignment: a warp takes the rows of `together` heads at once, VE consecutive
+// elements a lane. Grid (tokens, shares of the rows).
+template <typename T, int VE>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+  __shared__ float2 cs[128];
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t t = blockIdx.x;
+  take_angles(a, t, cs);
+  const long long slot = take_slot(a, t);
+  __syncthreads();
   const uint32_t rows = a.nq + (slot >= 0 ? 2 * a.cache.n_kv : 0);
   const uint32_t page = static_cast<uint32_t>(slot >= 0 ? slot >> a.cache.page_log2 : 0);
   const uint32_t p = static_cast<uint32_t>(slot) & (a.cache.page() - 1);
@@ -238,35 +337,38 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
   }
 }
 
-template <typename T, int VE>
-int launch_rope(const RopeArgs& a, uint32_t tokens, uint32_t rows, int sm_count, cudaStream_t s,
-                const char* call) {
+int launch_rope(void (*kernel)(RopeArgs), const RopeArgs& a, uint32_t tokens, uint32_t rows, int sm_count,
+                cudaStream_t s, const char* call) {
   // One CTA a token leaves most SMs idle below some hundred tokens: the rows are then shared by more
   // CTAs, each taking the token's angles again.
   const uint32_t groups = (rows + kWarps * a.together - 1) / (kWarps * a.together);
   const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(groups, 4u * sm_count / tokens));
-  rope_kernel<T, VE><<<dim3(tokens, shares), kThreads, 0, s>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", call);
+  const cudaError_t e = launch_pdl(kernel, dim3(tokens, shares), kThreads, 0, s, a);
+  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernelExC", call);
 }
 
-// The wide form wants every row it reads or writes on 16 bytes and, for halves, partners a whole lane
+// The wide forms want every row they read or write on 16 bytes and, for halves, partners a whole lane
 // apart; anything else is served one element a lane.
 template <typename T>
 int dispatch_rope(RopeArgs& a, bool aligned, uint32_t tokens, uint32_t rows, int sm_count, cudaStream_t s,
                   const char* call) {
   constexpr int VE = 16 / sizeof(T);
-  const bool wide = aligned && a.dim % VE == 0 &&
-                    (a.rope.layout == KQ_ROPE_PAIRS || a.rot_half % VE == 0);
-  if (wide) {
+  const uint32_t lane = sizeof(T) == 4 && a.dim == 256 ? 8 : VE;  // elements a lane
+  const bool wide = aligned && a.dim % VE == 0 && (a.rope.layout == KQ_ROPE_PAIRS || a.rot_half % lane == 0);
+  if (wide && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
+    a.together = 32 * lane / a.dim;
+    if (lane == VE) return launch_rope(rope_rows_kernel<T, VE>, a, tokens, rows, sm_count, s, call);
+    return launch_rope(rope_rows_kernel<T, 8>, a, tokens, rows, sm_count, s, call);
+  }
+  if (wide && (a.rope.layout == KQ_ROPE_PAIRS || a.rot_half % VE == 0)) {
     // narrow heads: a warp takes several at once, where the queries come out even
     const uint32_t width = a.slots ? a.cache.pitch : a.dim;
     const uint32_t n = std::max<uint32_t>(1, 32 * VE / width);
     a.together = a.nq % n == 0 ? n : 1;
-    return launch_rope<T, VE>(a, tokens, rows, sm_count, s, call);
+    return launch_rope(rope_kernel<T, VE>, a, tokens, rows, sm_count, s, call);
   }
   a.together = 1;
-  return launch_rope<T, 1>(a, tokens, rows, sm_count, s, call);
+  return launch_rope(rope_kernel<T, 1>, a, tokens, rows, sm_count, s, call);
 }
 
 uint32_t type_size(uint32_t type) {
@@ -288,60 +390,81 @@ bool on16(uint64_t bytes) { return bytes % 16 == 0; }
 
 // ---------------------------------------------------------------- reading back
 
-// Eight elements a thread, a grid over (rows of the output, K then V).
-template <typename T>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheView c, T* k_out, T* v_out,
-                                                              const long long* slots, uint64_t token_stride,
-                                                              uint32_t count, bool wide, unsigned* err) {
-  const bool value = blockIdx.y;
+// E elements (16 bytes of output) a thread, of ROWS rows at once so that their loads are in flight together.
+// Grid: (row groups, parts of a row, K then V).
+template <typename T, int KIND, int ROWS>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheView c, T* k_out, T* v_out, const long long* slots,
+                                                              uint64_t token_stride, uint32_t count,
+                                                              uint32_t per_head, uint32_t over_head, bool wide,
+                                                              unsigned* err) {
+  constexpr int E = 16 / sizeof(T);
+  constexpr int B = KIND == KQ_CACHE_F16 ? 2 * E : KIND == KQ_CACHE_Q8 ? E : 4;  // bytes of codes (Q4: a word)
+  pdl_wait();
+  pdl_launch_dependents();
+  const bool value = blockIdx.z;
   T* out = value ? v_out : k_out;
   const uint8_t* base = value ? c.v : c.k;
-  const uint32_t units = c.dim / 8;
-  const uint64_t total = uint64_t(count) * c.n_kv * units;
-  for (uint64_t i = blockIdx.x * uint64_t(kThreads) + threadIdx.x; i < total; i += uint64_t(gridDim.x) * kThreads) {
-    const uint32_t unit = i % units;
-    const uint32_t h = (i / units) % c.n_kv;
-    const uint64_t r = i / units / c.n_kv;
-    const long long slot = slots[r];
-    float y[8];
+  const uint32_t i = blockIdx.y * kThreads + threadIdx.x;
+  const uint32_t h = over_head ? __umulhi(i, over_head) : i, e = (i - h * per_head) * E;
+  if (h >= c.n_kv) return;
+  const uint32_t r0 = blockIdx.x * ROWS;
+  long long slot[ROWS];
+  uint32_t raw[ROWS][B / 4], scale[ROWS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = 0.f;
-    if (slot >= 0) {
-      if (static_cast<uint64_t>(slot) >> c.page_log2 >= c.n_pages) {
-        report_error(err, kErrCacheRange);
-        continue;
-      }
-      const uint8_t* rec = base + c.at(static_cast<uint32_t>(slot >> c.page_log2), h);
-      const uint32_t p = static_cast<uint32_t>(slot) & (c.page() - 1), e = 8 * unit;
-      if (c.kind == KQ_CACHE_F16) {
-        load_act<__half, 8>(reinterpret_cast<const __half*>(rec + cache_offset(p, 2 * e, c.row)), y);
+  for (int k = 0; k < ROWS; ++k) slot[k] = r0 + k < count ? slots[r0 + k] : -1;
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+#pragma unroll
+    for (int w = 0; w < B / 4; ++w) raw[k][w] = 0;
+    scale[k] = 0;
+    if (slot[k] < 0) continue;
+    if (static_cast<uint64_t>(slot[k]) >> c.page_log2 >= c.n_pages) {
+      report_error(err, kErrCacheRange);
+      slot[k] = -2;  // this row is left as it is
+      continue;
+    }
+    const uint8_t* rec = base + c.at(static_cast<uint32_t>(slot[k] >> c.page_log2), h);
+    const uint32_t p = static_cast<uint32_t>(slot[k]) & (c.page() - 1);
+    const uint8_t* from =
+        rec + cache_offset(p, KIND == KQ_CACHE_F16 ? 2 * e : KIND == KQ_CACHE_Q8 ? e : e / 8 * 4, c.row);
+    if constexpr (B == 16) {
+      const uint4 w = *reinterpret_cast<const uint4*>(from);
+      raw[k][0] = w.x;
+      raw[k][1] = w.y;
+      raw[k][2] = w.z;
+      raw[k][3] = w.w;
+    } else if constexpr (B == 8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(from);
+      raw[k][0] = w.x;
+      raw[k][1] = w.y;
+    } else {
+      raw[k][0] = *reinterpret_cast<const uint32_t*>(from);
+    }
+    if constexpr (KIND != KQ_CACHE_F16) scale[k] = rec[c.page() * c.row + p * c.scales + e / 32];
+  }
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    if (r0 + k >= count || slot[k] == -2) continue;
+    float y[E];
+    const float s = scale_value(scale[k]);
+    const bool zero = slot[k] < 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      if constexpr (KIND == KQ_CACHE_F16) {
+        y[j] = h2f(raw[k][j / 2] >> (16 * (j % 2)) & 0xffffu);
+      } else if constexpr (KIND == KQ_CACHE_Q8) {
+        y[j] = zero ? 0.f : (static_cast<float>(raw[k][j / 4] >> (8 * (j % 4)) & 255u) - 128.f) * s;
       } else {
-        const float s = scale_value(rec[c.page() * c.row + p * c.scales + e / 32]);
-        if (c.kind == KQ_CACHE_Q8) {
-          const uint2 w = *reinterpret_cast<const uint2*>(rec + cache_offset(p, e, c.row));
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            y[j] = (static_cast<float>(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u) - 128.f) * s;
-        } else {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + cache_offset(p, e / 2, c.row));
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            y[j] = (static_cast<float>((w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u) - 8.f) * s;
-        }
+        const uint32_t n = e % 8 + j;  // element of the word
+        y[j] = zero ? 0.f : (static_cast<float>(raw[k][0] >> (4 * (n / 2 + 4 * (n % 2))) & 15u) - 8.f) * s;
       }
     }
-    T* to = out + r * token_stride + h * c.dim + 8 * unit;
+    T* to = out + (r0 + k) * token_stride + h * c.dim + e;
     if (wide) {
-      if constexpr (sizeof(T) == 4) {
-        const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
-        store_act<T, 4>(to, lo);
-        store_act<T, 4>(to + 4, hi);
-      } else {
-        store_act<T, 8>(to, y);
-      }
+      store_act<T, E>(to, y);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) to[j] = act_from_f32<T>(y[j]);
+      for (int j = 0; j < E; ++j) to[j] = act_from_f32<T>(y[j]);
     }
   }
 }
@@ -358,6 +481,8 @@ __global__ void __launch_bounds__(kThreads) cache_move_kernel(CacheView c, const
   __shared__ uint8_t scales[kMaxMoves][8];
   uint8_t* base = blockIdx.z ? c.v : c.k;
   const uint32_t h = blockIdx.y;
+  pdl_wait();
+  pdl_launch_dependents();
   const int a = starts[blockIdx.x], b = starts[blockIdx.x + 1];
   if (a < 0 || b < a || static_cast<uint32_t>(b) > moves || b - a > static_cast<int>(kMaxMoves)) {
     if (threadIdx.x == 0) report_error(err, kErrCacheRange);
@@ -573,8 +698,6 @@ int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s) {
   if (d.k_out % size || d.v_out % size || d.slots % 8)
     return fail(KQ_E_INVALID, call, "k_out and v_out must be aligned to their elements, slots to 8 bytes");
   const bool wide = on16(d.k_out) && on16(d.v_out) && on16(stride * size);
-  const uint64_t total = uint64_t(d.count) * dense / 8;
-  const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>((total + kThreads - 1) / kThreads, 8u * ctx->sm_count));
   const auto slots = reinterpret_cast<const long long*>(d.slots);
   // a grid row for each output that is wanted
   const auto go = [&](auto* zero) {
@@ -590,13 +713,27 @@ int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s) {
     } else if (!v) {
       arrays = 1;
     }
-    cache_read_kernel<T><<<dim3(grid, arrays), kThreads, 0, s>>>(view, k, v, slots, stride, d.count, wide, ctx->err);
+    constexpr uint32_t E = 16 / sizeof(T);
+    const uint32_t per_head = c.dim / E, over_head = static_cast<uint32_t>(((1ull << 32) + per_head - 1) / per_head);
+    const uint32_t parts = (c.n_kv * per_head + kThreads - 1) / kThreads;
+    // four rows a thread hide the loads' latency (65536 rows of 1024: 128 -> TIME us); one where that would
+    // leave SMs idle
+    const bool many = uint64_t(d.count) * parts * arrays >= 32u * ctx->sm_count;
+    const auto run = [&](auto kind) {
+      constexpr int K = decltype(kind)::value;
+      return many ? launch_pdl(cache_read_kernel<T, K, 4>, dim3((d.count + 3) / 4, parts, arrays), kThreads, 0, s, view,
+                               k, v, slots, stride, d.count, per_head, over_head, wide, ctx->err)
+                  : launch_pdl(cache_read_kernel<T, K, 1>, dim3(d.count, parts, arrays), kThreads, 0, s, view, k, v,
+                               slots, stride, d.count, per_head, over_head, wide, ctx->err);
+    };
+    return c.kind == KQ_CACHE_F16  ? run(std::integral_constant<int, KQ_CACHE_F16>())
+           : c.kind == KQ_CACHE_Q8 ? run(std::integral_constant<int, KQ_CACHE_Q8>())
+                                   : run(std::integral_constant<int, KQ_CACHE_Q4>());
   };
-  if (d.type == KQ_TYPE_F32) go(static_cast<float*>(nullptr));
-  else if (d.type == KQ_TYPE_F16) go(static_cast<__half*>(nullptr));
-  else go(static_cast<__nv_bfloat16*>(nullptr));
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", call);
+  const cudaError_t e = d.type == KQ_TYPE_F32   ? go(static_cast<float*>(nullptr))
+                        : d.type == KQ_TYPE_F16 ? go(static_cast<__half*>(nullptr))
+                                                : go(static_cast<__nv_bfloat16*>(nullptr));
+  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernelExC", call);
 }
 
 int cache_move(kq_ctx* ctx, const kq_cache_move_desc& d, cudaStream_t s) {
@@ -609,11 +746,11 @@ int cache_move(kq_ctx* ctx, const kq_cache_move_desc& d, cudaStream_t s) {
   if (d.src % 8 || d.dst % 8 || d.starts % 4)
     return fail(KQ_E_INVALID, call, "src and dst must be 8-byte aligned, starts 4-byte aligned");
   if (d.groups > 0x7fffffffu || d.moves > 0x7fffffffu) return fail(KQ_E_INVALID, call, "too many moves");
-  cache_move_kernel<<<dim3(d.groups, c.n_kv, 2), kThreads, std::min(d.moves, kMaxMoves) * c.row, s>>>(
-      c, reinterpret_cast<const long long*>(d.src), reinterpret_cast<const long long*>(d.dst),
-      reinterpret_cast<const int*>(d.starts), d.moves, ctx->err);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernel", call);
+  const cudaError_t e = launch_pdl(cache_move_kernel, dim3(d.groups, c.n_kv, 2), kThreads,
+                                   std::min(d.moves, kMaxMoves) * c.row, s, c, reinterpret_cast<const long long*>(d.src),
+                                   reinterpret_cast<const long long*>(d.dst), reinterpret_cast<const int*>(d.starts),
+                                   d.moves, ctx->err);
+  return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernelExC", call);
 }
 
 }  // namespace kq

@@ -102,6 +102,23 @@ __device__ __forceinline__ void load_act(const T* p, float (&v)[N]) {
   }
 }
 
+// The same for up to 32 bytes (p aligned to 16).
+template <typename T, int N>
+__device__ __forceinline__ void load_wide(const T* p, float (&v)[N]) {
+  if constexpr (N * sizeof(T) <= 16) {
+    load_act<T, N>(p, v);
+  } else {
+    float lo[N / 2], hi[N / 2];
+    load_act<T, N / 2>(p, lo);
+    load_act<T, N / 2>(p + N / 2, hi);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      v[i] = lo[i];
+      v[N / 2 + i] = hi[i];
+    }
+  }
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_act(T* p, const float (&v)[N]) {
   if constexpr (N * sizeof(T) == 16) {
@@ -119,6 +136,22 @@ __device__ __forceinline__ void store_act(T* p, const float (&v)[N]) {
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = act_from_f32<T>(v[i]);
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_wide(T* p, const float (&v)[N]) {
+  if constexpr (N * sizeof(T) <= 16) {
+    store_act<T, N>(p, v);
+  } else {
+    float lo[N / 2], hi[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      lo[i] = v[i];
+      hi[i] = v[N / 2 + i];
+    }
+    store_act<T, N / 2>(p, lo);
+    store_act<T, N / 2>(p + N / 2, hi);
   }
 }
 

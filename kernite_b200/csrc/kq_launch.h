@@ -11,9 +11,14 @@
 
 namespace kq {
 
-template <typename... P, typename... A>
+template <typename T>
+struct SameType {
+  using Type = T;
+};
+
+template <typename... P>
 cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, uint32_t threads, size_t shared, cudaStream_t stream,
-                       const A&... args) {
+                       const typename SameType<P>::Type&... args) {
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -24,7 +29,8 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, uint32_t threads, size_t
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  void* list[] = {const_cast<void*>(static_cast<const void*>(&args))...};
+  return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), list);
 }
 
 }  // namespace kq
