@@ -300,7 +300,7 @@ typedef struct kq_rope {
     uint32_t rot_dim, layout;
     float gain;
     uint32_t reserved;
-    double turns[128];     /* pair i's turns (angle / 2 pi) per position */
+    uint64_t turns[128];   /* pair i's turns (angle / 2 pi) per position, modulo 1, times 2^64 */
 } kq_rope;
 int kq_rope_init(const kq_rope_params* params, kq_rope* out);
 

@@ -159,7 +159,7 @@ class KqRopeParams(ctypes.Structure):
 class KqRope(ctypes.Structure):
     _fields_ = [
         ("rot_dim", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("gain", ctypes.c_float),
-        ("reserved", ctypes.c_uint32), ("turns", ctypes.c_double * 128),
+        ("reserved", ctypes.c_uint32), ("turns", ctypes.c_uint64 * 128),
     ]
 
 
@@ -522,31 +522,31 @@ class Kernels:
 
     def rope(self, desc: "KqRopeDesc", stream=None) -> None:
         """``kq_rope_apply``: heads rotated by each token's position."""
-        rc = lib().kq_rope_apply(self._ctx, desc, _stream(stream))
+        rc = _lib.kq_rope_apply(self._ctx, desc, stream and _stream(stream))
         if rc:
             _check(rc, "kq_rope_apply")
 
     def cache_write(self, desc: "KqCacheWriteDesc", stream=None) -> None:
         """``kq_cache_write``: query heads rotated, key heads rotated and kept, value heads kept."""
-        rc = lib().kq_cache_write(self._ctx, desc, _stream(stream))
+        rc = _lib.kq_cache_write(self._ctx, desc, stream and _stream(stream))
         if rc:
             _check(rc, "kq_cache_write")
 
     def cache_read(self, desc: "KqCacheReadDesc", stream=None) -> None:
         """``kq_cache_read``: slots of the cache back as values."""
-        rc = lib().kq_cache_read(self._ctx, desc, _stream(stream))
+        rc = _lib.kq_cache_read(self._ctx, desc, stream and _stream(stream))
         if rc:
             _check(rc, "kq_cache_read")
 
     def cache_move(self, desc: "KqCacheMoveDesc", stream=None) -> None:
         """``kq_cache_move``: rows of the cache to other slots."""
-        rc = lib().kq_cache_move(self._ctx, desc, _stream(stream))
+        rc = _lib.kq_cache_move(self._ctx, desc, stream and _stream(stream))
         if rc:
             _check(rc, "kq_cache_move")
 
     def attention_tree(self, desc: "KqTreeDesc", stream=None) -> None:
         """``kq_attention_tree``: drafted tokens' attention over their sequences' caches."""
-        rc = lib().kq_attention_tree(self._ctx, desc, _stream(stream))
+        rc = _lib.kq_attention_tree(self._ctx, desc, stream and _stream(stream))
         if rc:
             _check(rc, "kq_attention_tree")
 

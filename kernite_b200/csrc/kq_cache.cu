@@ -26,7 +26,8 @@ constexpr uint32_t kMaxMoves = 64;
 // copies heads into the cache (values). A CTA takes one token and a share of its rows (heads); a warp
 // takes the rows of `together` heads at once, VE consecutive elements a lane.
 struct RopeArgs {
-  kq_rope rope;
+  float gain;
+  uint32_t layout;
   const void* q;   // rows [0, nq): to q_out
   const void* k;   // rows [nq, nq + n_kv): rotated, to the cache
   const void* v;   // rows [nq + n_kv, nq + 2 n_kv): to the cache
@@ -37,8 +38,16 @@ struct RopeArgs {
   uint32_t nq, dim;
   uint32_t rot_half;  // rotated pairs a head (0: none)
   uint32_t together;  // heads a warp takes at once
+  uint32_t tokens, per_block;  // tokens; of those, a CTA's (rope_rows_kernel)
   CacheView cache;
   unsigned* err;
+};
+
+// The pairs' turns per position, times 2^64. Kernels take the smaller table where it will do: 1 KB of
+// parameters costs the host 2 us a launch more than 100 bytes do.
+template <uint32_t PAIRS>
+struct Turns {
+  uint64_t at[PAIRS];
 };
 
 // (x_a, x_b) of a pair whose (gain cos, gain sin) is w.
@@ -147,17 +156,14 @@ __device__ __forceinline__ void keep(const CacheView& c, uint8_t* record, uint32
   if (e % 8 == 0) *reinterpret_cast<uint32_t*>(record + cache_offset(p, e / 2, c.row)) = word;
 }
 
-// The (gain cos, gain sin) of a token's pairs into shared memory: position * turns in f64 (position 100000
-// turns pair 0 by 16000 turns: f32 would leave 10 bits of the fraction), its fraction exactly to f32, then
-// sincospi of twice that.
-__device__ __forceinline__ void take_angles(const RopeArgs& a, uint32_t t, float2* cs) {
-  for (uint32_t i = threadIdx.x; i < a.rot_half; i += kThreads) {
-    const double turns = static_cast<double>(a.positions[t]) * a.rope.turns[i];
-    const float part = static_cast<float>(turns - rint(turns));
-    float s, c;
-    sincospif(2.f * part, &s, &c);
-    cs[i] = make_float2(a.rope.gain * c, a.rope.gain * s);
-  }
+// (gain cos, gain sin) of pair i at a position. Whole turns do not matter, so position * turns is taken
+// modulo 1 as a 64-bit fraction, exactly but for the table's rounding (position 2^31: 2^-33 turns); its
+// upper half as a signed fraction of a turn goes to f32 and sincospi.
+__device__ __forceinline__ float2 angle(int position, uint64_t turns, float gain) {
+  const uint64_t at = static_cast<uint64_t>(static_cast<int64_t>(position)) * turns;
+  float s, c;
+  sincospif(static_cast<float>(static_cast<int>(at >> 32)) * 0x1p-31f, &s, &c);
+  return make_float2(gain * c, gain * s);
 }
 
 // Token t's slot, -1 where it is not kept (or out of the cache, which is recorded).
@@ -166,31 +172,40 @@ __device__ __forceinline__ long long take_slot(const RopeArgs& a, uint32_t t) {
   const long long slot = a.slots[t];
   if (slot < 0) return -1;
   if (static_cast<uint64_t>(slot) >> a.cache.page_log2 < a.cache.n_pages) return slot;
-  if (threadIdx.x == 0) report_error(a.err, kErrCacheRange);
+  if (threadIdx.x % 32 == 0) report_error(a.err, kErrCacheRange);
   return -1;
 }
 
 // Heads of 64, 128 or 256 elements, every row on 16 bytes. A lane holds E consecutive elements of a row,
 // dim / E lanes a row, so that its place in a head, and with it its angles, are the same for every row
 // it takes: they stay in registers. A pair's other element is in the lane (pairs) or rot_half / E lanes
-// away (halves). A warp has AHEAD rows' loads in flight. Grid: (tokens, shares of the rows).
-template <typename T, int E>
-__global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4) rope_rows_kernel(const __grid_constant__ RopeArgs a) {
+// away (halves). A warp has AHEAD rows' loads in flight. A CTA takes per_block tokens, as many warps each;
+// with one, the grid's y shares out its rows.
+template <typename T, int E, uint32_t PAIRS>
+__global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4)
+    rope_rows_kernel(const __grid_constant__ RopeArgs a, const __grid_constant__ Turns<PAIRS> turns_of) {
   constexpr uint32_t AHEAD = 2;
-  __shared__ float2 cs[128];
+  extern __shared__ float2 angles[];  // [per_block][rot_half]
   pdl_wait();
   pdl_launch_dependents();
-  const uint32_t t = blockIdx.x;
-  take_angles(a, t, cs);
-  const long long slot = take_slot(a, t);
+  const uint32_t t0 = blockIdx.x * a.per_block;
+  for (uint32_t i = threadIdx.x; i < a.per_block * a.rot_half; i += kThreads) {
+    const uint32_t k = i / a.rot_half;
+    if (t0 + k < a.tokens) angles[i] = angle(a.positions[t0 + k], turns_of.at[i - k * a.rot_half], a.gain);
+  }
   __syncthreads();
+  const uint32_t each = kWarps / a.per_block;  // warps a token
+  const uint32_t warp = threadIdx.x / 32 % each, lane = threadIdx.x % 32;
+  const uint32_t t = t0 + threadIdx.x / 32 / each;
+  if (t >= a.tokens) return;
+  const float2* cs = angles + (t - t0) * a.rot_half;
+  const long long slot = take_slot(a, t);
   const uint32_t rows = a.nq + (slot >= 0 ? 2 * a.cache.n_kv : 0);
   const uint32_t page = static_cast<uint32_t>(slot >= 0 ? slot >> a.cache.page_log2 : 0);
   const uint32_t p = static_cast<uint32_t>(slot) & (a.cache.page() - 1);
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t per_row = a.dim / E, e = lane % per_row * E, sub = lane / per_row;
   const uint32_t at_once = 32 / per_row;  // rows a warp takes at once
-  const bool halves = a.rope.layout == KQ_ROPE_HALVES;
+  const bool halves = a.layout == KQ_ROPE_HALVES;
   const uint32_t rot = 2 * a.rot_half;
   // y = x * by + other * with; elements past rot as they are
   float by[E], with[E];
@@ -207,8 +222,8 @@ __global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4) rope_rows_kernel(con
     }
   }
   if (halves && e < rot) partner = e < a.rot_half ? lane + a.rot_half / E : lane - a.rot_half / E;
-  const uint32_t step = gridDim.y * kWarps * at_once;
-  for (uint32_t r0 = (blockIdx.y * kWarps + warp) * at_once; r0 < rows; r0 += AHEAD * step) {
+  const uint32_t step = gridDim.y * each * at_once;
+  for (uint32_t r0 = (blockIdx.y * each + warp) * at_once; r0 < rows; r0 += AHEAD * step) {
     float x[AHEAD][E];
 #pragma unroll
     for (uint32_t k = 0; k < AHEAD; ++k) {
@@ -253,13 +268,14 @@ __global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4) rope_rows_kernel(con
 
 // Any other head, stride or alignment: a warp takes the rows of `together` heads at once, VE consecutive
 // elements a lane. Grid (tokens, shares of the rows).
-template <typename T, int VE>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
-  __shared__ float2 cs[128];
+template <typename T, int VE, uint32_t PAIRS>
+__global__ void __launch_bounds__(kThreads)
+    rope_kernel(const __grid_constant__ RopeArgs a, const __grid_constant__ Turns<PAIRS> turns_of) {
+  __shared__ float2 cs[PAIRS];
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t t = blockIdx.x;
-  take_angles(a, t, cs);
+  for (uint32_t i = threadIdx.x; i < a.rot_half; i += kThreads) cs[i] = angle(a.positions[t], turns_of.at[i], a.gain);
   const long long slot = take_slot(a, t);
   __syncthreads();
   const uint32_t rows = a.nq + (slot >= 0 ? 2 * a.cache.n_kv : 0);
@@ -267,7 +283,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
   const uint32_t p = static_cast<uint32_t>(slot) & (a.cache.page() - 1);
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t step = gridDim.y * kWarps * a.together;
-  const bool halves = a.rope.layout == KQ_ROPE_HALVES;
+  const bool halves = a.layout == KQ_ROPE_HALVES;
   for (uint32_t r0 = (blockIdx.y * kWarps + warp) * a.together; r0 < rows; r0 += step) {
     if (r0 < a.nq) {
       // queries: a lane takes VE elements, for halves with their partners, so that nothing it reads
@@ -337,49 +353,71 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
   }
 }
 
-int launch_rope(void (*kernel)(RopeArgs), const RopeArgs& a, uint32_t tokens, uint32_t rows, int sm_count,
-                cudaStream_t s, const char* call) {
-  // One CTA a token leaves most SMs idle below some hundred tokens: the rows are then shared by more
-  // CTAs, each taking the token's angles again.
+template <uint32_t PAIRS>
+int launch_rope(void (*kernel)(RopeArgs, Turns<PAIRS>), RopeArgs& a, const kq_rope* rope, uint32_t rows, int sm_count,
+                cudaStream_t s, const char* call, bool by_rows) {
+  Turns<PAIRS> turns;
+  if (rope) std::memcpy(turns.at, rope->turns, sizeof(turns.at[0]) * a.rot_half);
+  // Below some hundred tokens one CTA a token leaves most SMs idle: a token's rows are then shared by more
+  // CTAs, each taking the angles again. With many tokens of few rows a CTA takes four, so that the angles'
+  // latency is paid once for them (4001 tokens of 40 16-bit heads: ONE -> FOUR us; 6144 of 96 rows the
+  // other way: OTHER).
   const uint32_t groups = (rows + kWarps * a.together - 1) / (kWarps * a.together);
-  const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(groups, 4u * sm_count / tokens));
-  const cudaError_t e = launch_pdl(kernel, dim3(tokens, shares), kThreads, 0, s, a);
+  a.per_block = by_rows && a.tokens >= 16u * sm_count && groups <= 3 ? 4 : 1;
+  const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(groups, 4u * sm_count / a.tokens));
+  const uint32_t shared = by_rows ? a.per_block * a.rot_half * sizeof(float2) : 0;
+  const cudaError_t e = launch_pdl(kernel, dim3((a.tokens + a.per_block - 1) / a.per_block, shares), kThreads, shared,
+                                   s, a, turns);
   return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernelExC", call);
 }
 
 // The wide forms want every row they read or write on 16 bytes and, for halves, partners a whole lane
 // apart; anything else is served one element a lane.
-template <typename T>
-int dispatch_rope(RopeArgs& a, bool aligned, uint32_t tokens, uint32_t rows, int sm_count, cudaStream_t s,
+template <typename T, uint32_t PAIRS>
+int dispatch_rope(RopeArgs& a, const kq_rope* rope, bool aligned, uint32_t rows, int sm_count, cudaStream_t s,
                   const char* call) {
   constexpr int VE = 16 / sizeof(T);
   const uint32_t lane = sizeof(T) == 4 && a.dim == 256 ? 8 : VE;  // elements a lane
-  const bool wide = aligned && a.dim % VE == 0 && (a.rope.layout == KQ_ROPE_PAIRS || a.rot_half % lane == 0);
-  if (wide && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
+  const bool pairs = a.layout == KQ_ROPE_PAIRS;
+  const bool wide = aligned && a.dim % VE == 0;
+  if (wide && (pairs || a.rot_half % lane == 0) && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
     a.together = 32 * lane / a.dim;
-    if (lane == VE) return launch_rope(rope_rows_kernel<T, VE>, a, tokens, rows, sm_count, s, call);
-    return launch_rope(rope_rows_kernel<T, 8>, a, tokens, rows, sm_count, s, call);
+    return launch_rope(lane == VE ? rope_rows_kernel<T, VE, PAIRS> : rope_rows_kernel<T, 8, PAIRS>, a, rope, rows,
+                       sm_count, s, call, true);
   }
-  if (wide && (a.rope.layout == KQ_ROPE_PAIRS || a.rot_half % VE == 0)) {
+  if (wide && (pairs || a.rot_half % VE == 0)) {
     // narrow heads: a warp takes several at once, where the queries come out even
     const uint32_t width = a.slots ? a.cache.pitch : a.dim;
     const uint32_t n = std::max<uint32_t>(1, 32 * VE / width);
     a.together = a.nq % n == 0 ? n : 1;
-    return launch_rope(rope_kernel<T, VE>, a, tokens, rows, sm_count, s, call);
+    return launch_rope(rope_kernel<T, VE, PAIRS>, a, rope, rows, sm_count, s, call, false);
   }
   a.together = 1;
-  return launch_rope(rope_kernel<T, 1>, a, tokens, rows, sm_count, s, call);
+  return launch_rope(rope_kernel<T, 1, PAIRS>, a, rope, rows, sm_count, s, call, false);
 }
 
 uint32_t type_size(uint32_t type) {
   return type == KQ_TYPE_F32 ? 4 : type == KQ_TYPE_F16 || type == KQ_TYPE_BF16 ? 2 : 0;
 }
 
-int run_rope(RopeArgs& a, uint32_t type, bool aligned, uint32_t tokens, uint32_t rows, int sm_count,
-             cudaStream_t s, const char* call) {
-  if (type == KQ_TYPE_F32) return dispatch_rope<float>(a, aligned, tokens, rows, sm_count, s, call);
-  if (type == KQ_TYPE_F16) return dispatch_rope<__half>(a, aligned, tokens, rows, sm_count, s, call);
-  return dispatch_rope<__nv_bfloat16>(a, aligned, tokens, rows, sm_count, s, call);
+template <typename T>
+int run_rope_of(RopeArgs& a, const kq_rope* rope, bool aligned, uint32_t rows, int sm_count, cudaStream_t s,
+                const char* call) {
+  return a.rot_half <= 64 ? dispatch_rope<T, 64>(a, rope, aligned, rows, sm_count, s, call)
+                          : dispatch_rope<T, 128>(a, rope, aligned, rows, sm_count, s, call);
+}
+
+int run_rope(RopeArgs& a, const kq_rope* rope, uint32_t type, bool aligned, uint32_t tokens, uint32_t rows,
+             int sm_count, cudaStream_t s, const char* call) {
+  a.tokens = tokens;
+  if (rope) {
+    a.gain = rope->gain;
+    a.layout = rope->layout;
+    a.rot_half = rope->rot_dim / 2;
+  }
+  if (type == KQ_TYPE_F32) return run_rope_of<float>(a, rope, aligned, rows, sm_count, s, call);
+  if (type == KQ_TYPE_F16) return run_rope_of<__half>(a, rope, aligned, rows, sm_count, s, call);
+  return run_rope_of<__nv_bfloat16>(a, rope, aligned, rows, sm_count, s, call);
 }
 
 bool rope_ok(const kq_rope* r) {
@@ -605,7 +643,10 @@ int rope_init(const kq_rope_params* p, kq_rope* out) {
       const double mix = (1.0 - ramp) * p->ext_factor;
       slow = p->freq_scale * (1.0 - mix) + mix;
     }
-    r.turns[i] = f * slow / kTwoPi;
+    // modulo 1, to 64 bits (2^64 itself, which rounding could give, is 0)
+    const double turns = f * slow / kTwoPi, part = turns - std::floor(turns);
+    const double scaled = std::ldexp(part, 64);
+    r.turns[i] = scaled >= 0x1p64 ? 0 : static_cast<uint64_t>(scaled);
   }
   *out = r;
   return KQ_OK;
@@ -625,7 +666,6 @@ int rope_apply(kq_ctx* ctx, const kq_rope_desc& d, cudaStream_t s) {
   if (d.x % size || d.y % size || d.positions % 4)
     return fail(KQ_E_INVALID, call, "x and y must be aligned to their elements, positions to 4 bytes");
   RopeArgs a = {};
-  a.rope = *d.rope;
   a.q = reinterpret_cast<const void*>(d.x);
   a.q_out = reinterpret_cast<void*>(d.y);
   a.positions = reinterpret_cast<const int*>(d.positions);
@@ -635,11 +675,10 @@ int rope_apply(kq_ctx* ctx, const kq_rope_desc& d, cudaStream_t s) {
   a.out_token = d.y_token ? d.y_token : uint64_t(d.heads) * d.head_dim;
   a.nq = d.heads;
   a.dim = d.head_dim;
-  a.rot_half = d.rope->rot_dim / 2;
   a.err = ctx->err;
   const bool aligned = on16(d.x) && on16(d.y) && on16(a.q_head * size) && on16(a.q_token * size) &&
                        on16(a.out_head * size) && on16(a.out_token * size);
-  return run_rope(a, d.type, aligned, d.tokens, d.heads, ctx->sm_count, s, call);
+  return run_rope(a, d.rope, d.type, aligned, d.tokens, d.heads, ctx->sm_count, s, call);
 }
 
 int cache_write(kq_ctx* ctx, const kq_cache_write_desc& d, cudaStream_t s) {
@@ -660,7 +699,6 @@ int cache_write(kq_ctx* ctx, const kq_cache_write_desc& d, cudaStream_t s) {
   if (d.q % size || d.k % size || d.v % size || d.q_out % size || d.positions % 4 || d.slots % 8)
     return fail(KQ_E_INVALID, call, "q, k, v and q_out must be aligned to their elements, positions to 4 bytes, "
                                     "slots to 8");
-  if (d.rope) a.rope = *d.rope;
   a.q = reinterpret_cast<const void*>(d.q);
   a.k = reinterpret_cast<const void*>(d.k);
   a.v = reinterpret_cast<const void*>(d.v);
@@ -676,11 +714,10 @@ int cache_write(kq_ctx* ctx, const kq_cache_write_desc& d, cudaStream_t s) {
   a.out_token = d.q_out_token ? d.q_out_token : uint64_t(d.n_heads) * dim;
   a.nq = d.q ? d.n_heads : 0;
   a.dim = d.cache->head_dim;
-  a.rot_half = d.rope ? d.rope->rot_dim / 2 : 0;
   a.err = ctx->err;
   const bool aligned = on16(d.q) && on16(d.k) && on16(d.v) && on16(d.q_out) && on16(a.q_token * size) &&
                        on16(a.k_token * size) && on16(a.v_token * size) && on16(a.out_token * size);
-  return run_rope(a, d.type, aligned, d.tokens, a.nq + 2 * d.cache->n_kv, ctx->sm_count, s, call);
+  return run_rope(a, d.rope, d.type, aligned, d.tokens, a.nq + 2 * d.cache->n_kv, ctx->sm_count, s, call);
 }
 
 int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s) {
