@@ -214,7 +214,7 @@ __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t
 // For few rows (8 an item). mma.sync.m16n8k16 (f16 in, f32 accumulated), operands from registers: the
 // positions are M of S^T = K Q^T, the head's elements M of O^T += V^T P^T, and the rows N = 8 of both, so
 // no part of an MMA is spent on rows that are not there; P^T comes from S^T by movmatrix. Seven warps take
-// 16 positions each in turn and keep separate maxima, sums and outputs, joined at an item's end; the
+// 32 positions each in turn and keep separate maxima, sums and outputs, joined at an item's end; the
 // eighth copies tiles of 128 positions into a ring, ahead over items' ends. For f32 activations Q and P are
 // sums of two f16 (about 22 bits): two MMAs into one sum.
 //
@@ -225,7 +225,8 @@ __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t
 
 constexpr uint32_t kReaders = 7;
 constexpr uint32_t kThreads = (kReaders + 1) * 32;
-constexpr uint32_t kPart = 16;                    // positions a warp takes at once
+constexpr uint32_t kSubs = 2;                     // times 16 positions a warp takes at once: two chains of
+constexpr uint32_t kPart = 16 * kSubs;            // latencies side by side
 constexpr uint32_t kParts = kTile / kPart;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -527,75 +528,81 @@ struct Lane {
   }
 };
 
-// Where 16 positions (number `part` of a tile) lie: the first one's row and scales. A segment (a page, or a
+// Where 16 positions (from p0 on, in a tile) lie: the first one's row and scales. A segment (a page, or a
 // tile's part of one) is its rows and then its scales; 16 rows are whole lines of 128 bytes, so the
 // permutation is that of the positions in them.
 template <class S>
 struct PartView {
   uint32_t code, scale;
 
-  __device__ PartView(uint32_t slot, uint32_t part, uint32_t seg_log2) {
-    const uint32_t p0 = part * kPart, in = p0 & ((1u << seg_log2) - 1);
+  __device__ PartView(uint32_t slot, uint32_t p0, uint32_t seg_log2) {
+    const uint32_t in = p0 & ((1u << seg_log2) - 1);
     const uint32_t seg = slot + (p0 - in) * (S::kRow + S::kScales);
     code = seg + in * S::kRow;
     scale = seg + (S::kRow << seg_log2) + in * S::kScales;
   }
 };
 
-// S^T of the warp's 16 positions: c = sum of K Q^T over the head, q the rows' operand B (hi, and lo).
+// S^T of the warp's positions, 16 at a time: c = sum of K Q^T over the head, q the rows' operand B (hi, lo).
 template <uint32_t KIND, uint32_t D, bool SPLIT, class Q>
-__device__ __forceinline__ void key_product(const PartView<Shape<KIND, D>>& part,
-                                            const Lane<Shape<KIND, D>>& at, const Q& q,
-                                            float (&c)[4]) {
+__device__ __forceinline__ void key_product(const PartView<Shape<KIND, D>> (&part)[kSubs],
+                                            const Lane<Shape<KIND, D>>& at, const Q& q, float (&c)[kSubs][4]) {
   using S = Shape<KIND, D>;
   constexpr uint32_t B = S::EK * S::kBits / 8;
-  float acc[2][4];  // two sums: an MMA's result is some 20 cycles away
+  float acc[kSubs][2][4];  // two sums each: an MMA's result is some 20 cycles away
 #pragma unroll
-  for (uint32_t i = 0; i < 2; ++i)
+  for (uint32_t s = 0; s < kSubs; ++s)
 #pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) acc[i][k] = 0.f;
+    for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) acc[s][i][k] = 0.f;
 #pragma unroll
   for (uint32_t j = 0; j < D / 4 / S::EK; ++j) {
-    uint32_t w[2][B / 4];
-    Scale2 s[2];
+    uint32_t w[kSubs][2][B / 4];
+    Scale2 scale[kSubs][2];
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-      lds_words<B>(part.code + at.key[j & 1] + h * 8 * S::kRow + (j >> 1) * 128, w[h]);
-      if constexpr (S::kScales != 0) {
-        const uint32_t b = lds_u8(part.scale + at.key_scale + h * 8 * S::kScales + j * (S::EK * 4 / 32));
-        s[h] = scale2<KIND>(b, b);
-      }
-    }
-#pragma unroll
-    for (uint32_t k = 0; k < S::EK / 4; ++k) {
-      uint32_t f[2][2];  // positions pi(g) and pi(g) + 8, the step's first and last two elements
+    for (uint32_t s = 0; s < kSubs; ++s)
 #pragma unroll
       for (uint32_t h = 0; h < 2; ++h) {
-        if constexpr (KIND == KQ_CACHE_F16) {
-          f[h][0] = w[h][2 * k];
-          f[h][1] = w[h][2 * k + 1];
-        } else if constexpr (KIND == KQ_CACHE_Q8) {
-          f[h][0] = decode2(prmt(w[h][k], kMagic, 0x4140), s[h]);
-          f[h][1] = decode2(prmt(w[h][k], kMagic, 0x4342), s[h]);
-        } else {
-          f[h][0] = decode2(nibbles(nibble_up(w[h][k / 2], 2 * (k % 2))), s[h]);
-          f[h][1] = decode2(nibbles(nibble_up(w[h][k / 2], 2 * (k % 2) + 1)), s[h]);
+        lds_words<B>(part[s].code + at.key[j & 1] + h * 8 * S::kRow + (j >> 1) * 128, w[s][h]);
+        if constexpr (S::kScales != 0) {
+          const uint32_t b = lds_u8(part[s].scale + at.key_scale + h * 8 * S::kScales + j * (S::EK * 4 / 32));
+          scale[s][h] = scale2<KIND>(b, b);
         }
       }
+#pragma unroll
+    for (uint32_t k = 0; k < S::EK / 4; ++k) {
       const uint32_t ks = j * (S::EK / 4) + k;
       uint32_t b[4];
       q(ks, b);
-      mma16816(acc[SPLIT ? 0 : ks & 1], f[0][0], f[1][0], f[0][1], f[1][1], b[0], b[1]);
-      if constexpr (SPLIT) mma16816(acc[1], f[0][0], f[1][0], f[0][1], f[1][1], b[2], b[3]);
+#pragma unroll
+      for (uint32_t s = 0; s < kSubs; ++s) {
+        uint32_t f[2][2];  // positions pi(g) and pi(g) + 8, the step's first and last two elements
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+          if constexpr (KIND == KQ_CACHE_F16) {
+            f[h][0] = w[s][h][2 * k];
+            f[h][1] = w[s][h][2 * k + 1];
+          } else if constexpr (KIND == KQ_CACHE_Q8) {
+            f[h][0] = decode2(prmt(w[s][h][k], kMagic, 0x4140), scale[s][h]);
+            f[h][1] = decode2(prmt(w[s][h][k], kMagic, 0x4342), scale[s][h]);
+          } else {
+            f[h][0] = decode2(nibbles(nibble_up(w[s][h][k / 2], 2 * (k % 2))), scale[s][h]);
+            f[h][1] = decode2(nibbles(nibble_up(w[s][h][k / 2], 2 * (k % 2) + 1)), scale[s][h]);
+          }
+        }
+        mma16816(acc[s][SPLIT ? 0 : ks & 1], f[0][0], f[1][0], f[0][1], f[1][1], b[0], b[1]);
+        if constexpr (SPLIT) mma16816(acc[s][1], f[0][0], f[1][0], f[0][1], f[1][1], b[2], b[3]);
+      }
     }
   }
 #pragma unroll
-  for (uint32_t k = 0; k < 4; ++k) {
-    c[k] = acc[0][k] + acc[1][k];
-  }
+  for (uint32_t s = 0; s < kSubs; ++s)
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) c[s][k] = acc[s][0][k] + acc[s][1][k];
 }
 
-// O^T += V^T P^T of the warp's 16 positions, b the weights as operand B (hi, and lo). EDGE: the tile
+// O^T += V^T P^T of 16 of the warp's positions, b the weights as operand B (hi, and lo). EDGE: the tile
 // reaches past the prefix, so rows past the end (left: positions the tile has) and values that are not
 // finite count as zero here (P is zero where a position is masked, and zero times those would not be);
 // the caller adds the latter where they are
@@ -661,13 +668,13 @@ __device__ __forceinline__ void value_product(const PartView<Shape<KIND, D>>& pa
   }
 }
 
-// Of the warp's positions p0 .. p0 + 15 below `left`, those with a value that is not finite, as bits.
+// Of the warp's positions p0 .. p0 + 31 below `left`, those with a value that is not finite, as bits.
 template <uint32_t KIND, uint32_t D>
 __device__ __noinline__ uint32_t special_positions(TileView<Shape<KIND, D>> tile, uint32_t p0, uint32_t left) {
   using S = Shape<KIND, D>;
   const uint32_t lane = threadIdx.x % 32;
   uint32_t found = 0;
-  for (uint32_t p = p0; p < p0 + 16 && p < left; ++p) {
+  for (uint32_t p = p0; p < p0 + kPart && p < left; ++p) {
     bool odd = false;
     if constexpr (KIND == KQ_CACHE_F16) {
       for (uint32_t u = lane; u < S::kRow / 16; u += 32) {
@@ -845,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
     const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
     const uint32_t here = min(tiles - first_tile, count - done);  // of the item's tiles, this CTA's
     for (uint32_t n = warp; n < here * kParts; n += kReaders) {
-      const uint32_t it = 2 * (done + n / kParts), part_no = n % kParts, p0 = part_no * kPart;
+      const uint32_t it = 2 * (done + n / kParts), p0 = n % kParts * kPart;
       const uint32_t base = (first_tile + n / kParts) * kTile, left = p.seq.length() - base;  // positions left
       const bool edge = base + kTile > p.seq.prefix;
       const uint32_t k_slot = it % NS, v_slot = (it + 1) % NS;
@@ -854,7 +861,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         live = false;
       }
       __syncwarp();
-      uint32_t pb[4];
+      uint32_t pb[kSubs][4];
       const auto row_bits = [&](unsigned long long (&bits)[2]) {  // of rows 2 t, 2 t + 1
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
@@ -863,32 +870,51 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         }
       };
       if (p0 < left) {
-        float c[4];
-        key_product<KIND, D, SPLIT>(PartView<S>(ring + k_slot * S::kSlot, part_no, seg_log2), place, q_at, c);
+        const uint32_t from = ring + k_slot * S::kSlot;
+        const PartView<S> keys[kSubs] = {{from, p0, seg_log2}, {from, p0 + 16, seg_log2}};
+        float c[kSubs][4];
+        key_product<KIND, D, SPLIT>(keys, place, q_at, c);
         // rows 2 t, 2 t + 1 at position pi(g), then at pi(g) + 8: logits in log2 units, to the reference
-        float2 z0 = fma2(make_float2(c[0], c[1]), unit2, minus), z1 = fma2(make_float2(c[2], c[3]), unit2, minus);
+        float2 z[kSubs][2];
+        float most = -INFINITY;
+#pragma unroll
+        for (uint32_t s = 0; s < kSubs; ++s) {
+          z[s][0] = fma2(make_float2(c[s][0], c[s][1]), unit2, minus);
+          z[s][1] = fma2(make_float2(c[s][2], c[s][3]), unit2, minus);
+        }
         if (edge) {
           unsigned long long bits[2];
           row_bits(bits);
-          const uint32_t pos = base + p0 + pi8(g);
-          if (!sees(bits[0], pos, p.seq)) z0.x = -INFINITY;
-          if (!sees(bits[1], pos, p.seq)) z0.y = -INFINITY;
-          if (!sees(bits[0], pos + 8, p.seq)) z1.x = -INFINITY;
-          if (!sees(bits[1], pos + 8, p.seq)) z1.y = -INFINITY;
+#pragma unroll
+          for (uint32_t s = 0; s < kSubs; ++s)
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+              const uint32_t pos = base + p0 + 16 * s + pi8(g) + 8 * h;
+              if (!sees(bits[0], pos, p.seq)) z[s][h].x = -INFINITY;
+              if (!sees(bits[1], pos, p.seq)) z[s][h].y = -INFINITY;
+            }
         }
-        if (__any_sync(0xffffffffu, max3(fmaxf(z0.x, z0.y), z1.x, z1.y) > limit)) {
-          // a new reference for the rows that want one (all rows have one after this, but those that see
-          // nothing yet, whose weights are zero whatever it is)
-          // The logits themselves, each one rounded: the largest is then exactly the reference, however
-          // large it is.
-          const float x[4] = {__fmul_rn(c[0], unit2.x), __fmul_rn(c[1], unit2.y), __fmul_rn(c[2], unit2.x),
-                              __fmul_rn(c[3], unit2.y)};
-          float* z[4] = {&z0.x, &z0.y, &z1.x, &z1.y};
+#pragma unroll
+        for (uint32_t s = 0; s < kSubs; ++s)
+          most = max3(max3(most, z[s][0].x, z[s][0].y), z[s][1].x, z[s][1].y);
+        if (__any_sync(0xffffffffu, most > limit)) {
+          // A new reference for the rows that want one (all rows have one after this, but those that see
+          // nothing yet, whose weights are zero whatever it is). It is of the logits themselves, each one
+          // rounded: the largest is then exactly the reference, however large it is.
           float f[2];
 #pragma unroll
           for (uint32_t i = 0; i < 2; ++i) {
-            float top = fmaxf(*z[i], *z[2 + i]);  // to the old reference
-            float now = fmaxf(*z[i] == -INFINITY ? -INFINITY : x[i], *z[2 + i] == -INFINITY ? -INFINITY : x[2 + i]);
+            float x[kSubs][2];
+            float top = -INFINITY, now = -INFINITY;  // to the old reference, and itself
+#pragma unroll
+            for (uint32_t s = 0; s < kSubs; ++s)
+#pragma unroll
+              for (uint32_t h = 0; h < 2; ++h) {
+                const float old = i ? z[s][h].y : z[s][h].x;
+                x[s][h] = old == -INFINITY ? -INFINITY : __fmul_rn(c[s][2 * h + i], i ? unit2.y : unit2.x);
+                top = fmaxf(top, old);
+                now = fmaxf(now, x[s][h]);
+              }
 #pragma unroll
             for (int s = 4; s < 32; s <<= 1) {
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
@@ -900,8 +926,10 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
             f[i] = fresh ? 0.f : exp2f(m[i] - now);
             m[i] = now;
             (i ? minus.y : minus.x) = next;
-            if (*z[i] != -INFINITY) *z[i] = x[i] + next;
-            if (*z[2 + i] != -INFINITY) *z[2 + i] = x[2 + i] + next;
+#pragma unroll
+            for (uint32_t s = 0; s < kSubs; ++s)
+#pragma unroll
+              for (uint32_t h = 0; h < 2; ++h) (i ? z[s][h].y : z[s][h].x) = x[s][h] + next;
           }
           l.x *= f[0];
           l.y *= f[1];
@@ -911,21 +939,24 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
             for (uint32_t i = 0; i < 4; ++i) o[j][i] *= f[i & 1];
           limit = __any_sync(0xffffffffu, m[0] == -INFINITY || m[1] == -INFINITY) ? -INFINITY : kSlack + kLift;
         }
-        const float2 w0 = make_float2(exp2_fast(z0.x), exp2_fast(z0.y));
-        const float2 w1 = make_float2(exp2_fast(z1.x), exp2_fast(z1.y));
-        l = add2(l, add2(w0, w1));
-        if constexpr (SPLIT) {
-          uint32_t hi0, lo0, hi1, lo1;
-          split2(w0.x, w0.y, hi0, lo0);
-          split2(w1.x, w1.y, hi1, lo1);
-          pb[0] = transpose8(hi0);
-          pb[1] = transpose8(hi1);
-          pb[2] = transpose8(lo0);
-          pb[3] = transpose8(lo1);
-        } else {
-          pb[0] = transpose8(h2(__floats2half2_rn(w0.x, w0.y)));
-          pb[1] = transpose8(h2(__floats2half2_rn(w1.x, w1.y)));
-          pb[2] = pb[3] = 0;
+#pragma unroll
+        for (uint32_t s = 0; s < kSubs; ++s) {
+          const float2 w0 = make_float2(exp2_fast(z[s][0].x), exp2_fast(z[s][0].y));
+          const float2 w1 = make_float2(exp2_fast(z[s][1].x), exp2_fast(z[s][1].y));
+          l = add2(l, add2(w0, w1));
+          if constexpr (SPLIT) {
+            uint32_t hi0, lo0, hi1, lo1;
+            split2(w0.x, w0.y, hi0, lo0);
+            split2(w1.x, w1.y, hi1, lo1);
+            pb[s][0] = transpose8(hi0);
+            pb[s][1] = transpose8(hi1);
+            pb[s][2] = transpose8(lo0);
+            pb[s][3] = transpose8(lo1);
+          } else {
+            pb[s][0] = transpose8(h2(__floats2half2_rn(w0.x, w0.y)));
+            pb[s][1] = transpose8(h2(__floats2half2_rn(w1.x, w1.y)));
+            pb[s][2] = pb[s][3] = 0;
+          }
         }
       }
       __syncwarp();
@@ -938,7 +969,10 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       if (p0 < left) {
         const uint32_t slot = ring + v_slot * S::kSlot;
         if (edge) {
-          value_product<KIND, D, SPLIT, true>(PartView<S>(slot, part_no, seg_log2), place, p0 + t, left, pb, o);
+#pragma unroll
+          for (uint32_t s = 0; s < kSubs; ++s)
+            value_product<KIND, D, SPLIT, true>(PartView<S>(slot, p0 + 16 * s, seg_log2), place, p0 + 16 * s + t, left,
+                                                pb[s], o);
           const TileView<S> values = {slot, seg_log2};
           // infinities and NaN reach the rows that see their position
           for (uint32_t odd = special_positions<KIND, D>(values, p0, left); odd; odd &= odd - 1) {
@@ -956,7 +990,10 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
               }
           }
         } else {
-          value_product<KIND, D, SPLIT, false>(PartView<S>(slot, part_no, seg_log2), place, p0 + t, left, pb, o);
+#pragma unroll
+          for (uint32_t s = 0; s < kSubs; ++s)
+            value_product<KIND, D, SPLIT, false>(PartView<S>(slot, p0 + 16 * s, seg_log2), place, p0 + 16 * s + t, left,
+                                                 pb[s], o);
         }
       }
       __syncwarp();
