@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < NS; ++i) {
       mbar_init(bars + 16 * i, 1);
-      mbar_init(bars + 16 * i + 8, kParts);
+      mbar_init(bars + 16 * i + 8, kReaders);
     }
     fence_mbar_init();
   }
@@ -851,10 +851,14 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
 
     const uint32_t tiles = position_tiles<kTile>(p.seq), first_tile = p.tile;
     const uint32_t here = min(tiles - first_tile, count - done);  // of the item's tiles, this CTA's
-    for (uint32_t n = warp; n < here * kParts; n += kReaders) {
-      const uint32_t it = 2 * (done + n / kParts), p0 = n % kParts * kPart;
-      const uint32_t base = (first_tile + n / kParts) * kTile, left = p.seq.length() - base;  // positions left
+    // The parts go round the warps; a warp also passes the tiles it has no part of, so that it sees every
+    // phase of every slot in turn (a parity it had skipped would be taken for the one before).
+    uint32_t turn = warp;  // (warp - parts so far) mod kReaders: the warp's part of the tile, if below kParts
+    for (uint32_t n = 0; n < here; ++n, turn = turn >= kParts ? turn - kParts : turn + kReaders - kParts) {
+      const uint32_t it = 2 * (done + n), p0 = turn * kPart;
+      const uint32_t base = (first_tile + n) * kTile, left = p.seq.length() - base;  // positions left
       const bool edge = base + kTile > p.seq.prefix;
+      const bool reads = turn < kParts && p0 < left;
       const uint32_t k_slot = it % NS, v_slot = (it + 1) % NS;
       if (live && !mbar_wait(bars + 16 * k_slot, (it / NS) & 1)) {
         report_error(a.err, kErrWaitFull);
@@ -869,7 +873,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
           bits[i] = r < rows ? mask_bits(a, p.seq, token_of(a, r)) : 0ull;
         }
       };
-      if (p0 < left) {
+      if (reads) {
         const uint32_t from = ring + k_slot * S::kSlot;
         const PartView<S> keys[kSubs] = {{from, p0, seg_log2}, {from, p0 + 16, seg_log2}};
         float c[kSubs][4];
@@ -966,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         live = false;
       }
       __syncwarp();
-      if (p0 < left) {
+      if (reads) {
         const uint32_t slot = ring + v_slot * S::kSlot;
         if (edge) {
 #pragma unroll

@@ -40,7 +40,9 @@ struct Wide {
   static constexpr uint32_t kRaw = TW * (S::kRow + S::kScales);
   static constexpr uint32_t kFixed = kOperands * kOperand + 4096;
   static constexpr uint32_t kFit = (227 * 1024 - kFixed) / kRaw;
-  static constexpr uint32_t kRaws = kFit > 8 ? 8 : kFit;
+  // keys and values in turn; even, so that a slot is always keys' or values' and the warps of one see every
+  // phase of their slots' barriers
+  static constexpr uint32_t kRaws = kFit > 8 ? 8 : kFit / 2 * 2;
   static constexpr uint32_t kBytes = kFixed + kRaws * kRaw;
   static_assert(kRaws >= 2 && kBytes <= 227 * 1024, "ring");
   // tensor memory columns: S (then P) buffers, O (one a softmax group where there is room), Q

@@ -236,6 +236,23 @@ def test_one_position_takes_all(kernels, drafts, type):
             assert np.abs(got[t, h] - c.values[0][best, 0]).max() <= (2.0 ** -20 + STEP[type]) * 5
 
 
+@pytest.mark.parametrize("case", [(ref.F16, 64, 8, 128, 64, [700] * 6, [1] * 6), (ref.Q8, 16, 2, 256, 32, [900] * 4, [3] * 4),
+                                  (ref.F16, 16, 2, 128, 16, [1500] * 3, [4] * 3), (ref.Q8, 8, 8, 128, 64, [1100] * 5, [1] * 5),
+                                  (ref.Q4, 8, 2, 64, 64, [3000], [1])], ids=str)
+def test_rings_go_round_many_times(kernels, case):
+    """Several tiles and items a CTA, forty calls one after another: the same bits every time, and right."""
+    c = Case(*case, seed=21)
+    d = c.desc(kernels)
+    first = None
+    for _ in range(40):
+        kernels.attention_tree(d)
+        got = c.out.clone()
+        first = got if first is None else first
+        assert torch.equal(got, first)
+    kernels.device_error()
+    c.check(first.double().cpu().numpy())
+
+
 def test_scale_strides_and_another_stream(kernels):
     c = Case(ref.Q8, 8, 2, 64, 32, [321], [6], seed=12)
     wide = 8 * 64 + 64
