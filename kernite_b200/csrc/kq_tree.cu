@@ -60,6 +60,10 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   const uint64_t tiles = (uint64_t(d.max_len) + p.tile - 1) / p.tile;
   const uint64_t items = uint64_t(d.n_seq) * c.n_kv * row_tiles;
   if (items > 0x7fffffffu) return fail(KQ_E_INVALID, call, "too many sequences, heads and drafts");
+  // kernels number the tiles of one sequence in 32 bits, up to the length that its pages hold
+  const uint64_t most = ((uint64_t(d.max_pages) << c.page_log2) + p.tile - 1) / p.tile;
+  if (most * c.n_kv * row_tiles > 0xffffffffu)
+    return fail(KQ_E_INVALID, call, "too many positions, heads and drafts in one sequence");
   p.ctas = static_cast<uint32_t>(std::min<uint64_t>(
       uint64_t(ctx->sm_count) * (p.wide ? 1 : tree::narrow_ctas(c.kind, c.pitch)), std::max<uint64_t>(1, items * tiles)));
   p.bytes = uint64_t(p.ctas) * 2 * tree::part_floats(p.rows, c.pitch) * 4;

@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
                  ? static_cast<uint32_t>(a.pages[uint64_t(p.s) * a.max_pages + (pos >> a.c.page_log2)])
                  : 0u;
     };
-    uint32_t page = page_of();
+    uint32_t page = page_of(), sent = 0;  // uses copied
     for (uint32_t i = 0; i < count; ++i) {
       const Place now = p;
       const uint32_t now_page = page;
@@ -764,9 +764,14 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
           live = false;
         }
         live = __all_sync(0xffffffffu, live);
-        if (live) copy_segments<S>(a, now, now_page, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
+        if (!live) continue;
+        copy_segments<S>(a, now, now_page, kv ? a.c.v : a.c.k, ring + slot * S::kSlot, bar);
+        sent = use + 1;
       }
     }
+    // no copy is in flight when the CTA ends, whatever gave up
+    for (uint32_t use = sent > NS ? sent - NS : 0; use < sent; ++use)
+      if (!mbar_wait(bars + 16 * (use % NS), (use / NS) & 1)) report_error(a.err, kErrWaitFull);
     return;
   }
 

@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       const uint8_t* src = kv ? a.c.v : a.c.k;
       PageIds<TW> ids;
       ids.load(a, p);
-      uint32_t it = kv;
+      uint32_t it = kv, sent = kv;  // the next use, and the one after the last copied
       while (at < end) {
         const uint32_t tiles = position_tiles<TW>(p.seq);
         while (p.tile < tiles && at < end) {
@@ -346,7 +346,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
             report_error(a.err, kErrWaitEmpty);
             live = false;
           }
-          if (live) copy_tile<S, TW>(a, now, these, src, raws + slot * W::kRaw, bar.raw_full(slot));
+          if (live) {
+            copy_tile<S, TW>(a, now, these, src, raws + slot * W::kRaw, bar.raw_full(slot));
+            sent = it + 2;
+          }
           it += 2;
         }
         if (at < end) {
@@ -354,6 +357,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
           ids.load(a, p);
         }
       }
+      // no copy is in flight when the CTA ends, whatever gave up
+      for (uint32_t use = sent > W::kRaws + kv ? sent - W::kRaws : kv; use < sent; use += 2)
+        if (!mbar_wait(bar.raw_full(use % W::kRaws), (use / W::kRaws) & 1)) report_error(a.err, kErrWaitFull);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -523,6 +529,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         const uint32_t base = p.tile * TW;
         const bool edge = base + TW > p.seq.prefix;
         const uint32_t buf = n % W::kBufs, sbuf = lanes + buf * W::kS;
+        // (of three buffers a group passes over every second phase; it cannot take the one before for
+        // this one: that was tile n - 3's, done before tile n - 2's, which the group has seen)
         wait_or_die(live, bar.s_full(buf), (n / W::kBufs) & 1, a.err, kErrWaitFull);
         tc_fence_after();
         // the lane's logits (times unit: log2 units), masked in tiles that reach past the prefix
