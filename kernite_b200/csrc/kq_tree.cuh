@@ -171,8 +171,13 @@ __device__ __forceinline__ void next_item(const TreeArgs& a, Place& p) {
   } while (p.seq.drafts == 0);
 }
 
-// CTA c of n <= total takes tiles [range_start(c), range_start(c + 1)) of `total`, at least one.
+// CTA c of n <= total takes tiles [range_start(c), range_start(c + 1)) of `total`, at least one (n < 2^16,
+// so that where total has 32 bits, all of this has: 64-bit divisions are calls of some 100 cycles).
 __device__ __forceinline__ uint64_t range_start(uint64_t total, uint32_t c, uint32_t n) {
+  if (total >> 32 == 0) {
+    const uint32_t whole = static_cast<uint32_t>(total) / n;
+    return uint64_t(whole) * c + (static_cast<uint32_t>(total) - whole * n) * c / n;
+  }
   return total / n * c + total % n * c / n;
 }
 
@@ -201,6 +206,58 @@ __device__ __forceinline__ uint32_t seen_word(unsigned long long bits, int from)
   if (from <= -32) return ~0u;
   if (from >= static_cast<int>(kMaxDrafts)) return 0u;
   return from < 0 ? static_cast<uint32_t>(bits << -from) | ((1u << -from) - 1u) : static_cast<uint32_t>(bits >> from);
+}
+
+__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+
+// Elements at(0), at(1), .. of q from element `row` on, N (4 or 8) each; zeros from element `dim` on and
+// where there is no row. All loads are issued before any is looked at, so that they are one latency: a
+// choice of type at each would wait for each (one token over 99 positions: BEFORE -> AFTER us).
+template <uint32_t COUNT, uint32_t N, class At>
+__device__ __forceinline__ void load_row(const TreeArgs& a, uint64_t row, bool have, const At& at,
+                                         float (&x)[COUNT][N]) {
+  const uint32_t dim = have ? a.c.dim : 0;
+  if (a.type == KQ_TYPE_F32) {
+    const float* q = static_cast<const float*>(a.q) + row;
+#pragma unroll
+    for (uint32_t j = 0; j < COUNT; ++j)
+#pragma unroll
+      for (uint32_t k = 0; k < N; k += 4) {
+        const float4 v = at(j) < dim ? *reinterpret_cast<const float4*>(q + at(j) + k) : make_float4(0, 0, 0, 0);
+        x[j][k] = v.x;
+        x[j][k + 1] = v.y;
+        x[j][k + 2] = v.z;
+        x[j][k + 3] = v.w;
+      }
+    return;
+  }
+  uint32_t w[COUNT][N / 2];
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + row;
+#pragma unroll
+  for (uint32_t j = 0; j < COUNT; ++j) {
+    if constexpr (N == 8) {
+      const uint4 v = at(j) < dim ? *reinterpret_cast<const uint4*>(q + at(j)) : make_uint4(0, 0, 0, 0);
+      w[j][0] = v.x;
+      w[j][1] = v.y;
+      w[j][2] = v.z;
+      w[j][3] = v.w;
+    } else {
+      const uint2 v = at(j) < dim ? *reinterpret_cast<const uint2*>(q + at(j)) : make_uint2(0, 0);
+      w[j][0] = v.x;
+      w[j][1] = v.y;
+    }
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < COUNT; ++j)
+#pragma unroll
+    for (uint32_t k = 0; k < N; k += 2) {
+      float2 v;
+      if (a.type == KQ_TYPE_F16) v = __half22float2(as_h2(w[j][k / 2]));
+      else v = make_float2(__uint_as_float(w[j][k / 2] << 16), __uint_as_float(w[j][k / 2] & 0xffff0000u));
+      x[j][k] = v.x;
+      x[j][k + 1] = v.y;
+    }
 }
 
 __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t type) {
@@ -245,9 +302,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
-
-__device__ __forceinline__ uint32_t h2(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-__device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
 // 2^x, to 2^-22 of it; results below f32's normal range are zero.
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -790,23 +844,12 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       const uint64_t row = have ? (p.seq.first + tok) * a.q_token +
                                       uint64_t(p.head * a.group + head_of(a, r, tok)) * a.c.dim
                                 : 0;
+      float x[S::kSteps][4];
+      load_row(a, row, have, [&](uint32_t ks) { return key_element<S>(ks, t); }, x);
       float most = 0.f;
-      constexpr uint32_t HOLD = D == 256 ? 1 : S::kSteps;  // steps held: all, where registers allow
-      float x[HOLD][4];
-      const auto load4 = [&](uint32_t ks, float (&x)[4]) {
-        const uint32_t e = key_element<S>(ks, t);
-        x[0] = x[1] = x[2] = x[3] = 0.f;
-        if (!have || e >= a.c.dim) return;
-        if (a.type == KQ_TYPE_F32) load_act<float, 4>(static_cast<const float*>(a.q) + row + e, x);
-        else if (a.type == KQ_TYPE_F16) load_act<__half, 4>(static_cast<const __half*>(a.q) + row + e, x);
-        else load_act<__nv_bfloat16, 4>(static_cast<const __nv_bfloat16*>(a.q) + row + e, x);
-      };
 #pragma unroll
-      for (uint32_t ks = 0; ks < S::kSteps; ++ks) {
-        float(&y)[4] = x[ks % HOLD];
-        load4(ks, y);
-        most = fmaxf(most, fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
-      }
+      for (uint32_t ks = 0; ks < S::kSteps; ++ks)
+        most = fmaxf(most, fmaxf(fmaxf(fabsf(x[ks][0]), fabsf(x[ks][1])), fmaxf(fabsf(x[ks][2]), fabsf(x[ks][3]))));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const RowScale scale = row_scale<SPLIT>(most, a.scale_log2);
@@ -815,8 +858,7 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
       unit2.y = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
 #pragma unroll
       for (uint32_t ks = 0; ks < S::kSteps; ++ks) {
-        float(&y)[4] = x[ks % HOLD];
-        if constexpr (HOLD == 1) load4(ks, y);
+        const float(&y)[4] = x[ks];
         uint32_t hi0, lo0, hi1, lo1;
         split2(y[0] * up, y[1] * up, hi0, lo0);
         split2(y[2] * up, y[3] * up, hi1, lo1);

@@ -252,23 +252,6 @@ __device__ __forceinline__ float value_at(const TreeArgs& a, const Place& p, uin
   return rec[a.c.page() * S::kRow + in * S::kScales + e / 32] >= 0xf8u ? __int_as_float(0x7fc00000) : 0.f;
 }
 
-// Eight activations from element i on.
-__device__ __forceinline__ void load_acts(const void* p, uint64_t i, uint32_t type, float (&x)[8]) {
-  if (type == KQ_TYPE_F32) {
-    float y[4];
-    load_act<float, 4>(static_cast<const float*>(p) + i, y);
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) x[k] = y[k];
-    load_act<float, 4>(static_cast<const float*>(p) + i + 4, y);
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) x[4 + k] = y[k];
-  } else if (type == KQ_TYPE_F16) {
-    load_act<__half, 8>(static_cast<const __half*>(p) + i, x);
-  } else {
-    load_act<__nv_bfloat16, 8>(static_cast<const __nv_bfloat16*>(p) + i, x);
-  }
-}
-
 template <uint32_t KIND, uint32_t D, bool SPLIT>
 __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_constant__ TreeArgs a) {
   using W = Wide<KIND, D>;
@@ -483,35 +466,41 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       const uint64_t q_row = (p.seq.first + token) * a.q_token + uint64_t(q_head) * a.c.dim;
       float unit;
       {
-        float x[D / 16][8];  // all of this thread's part, so that its loads are one latency
-#pragma unroll
-        for (uint32_t j = 0; j < D / 16; ++j) {
-          const uint32_t e = half * (D / 2) + 8 * j;
-#pragma unroll
-          for (uint32_t k = 0; k < 8; ++k) x[j][k] = 0.f;
-          if (have && e < a.c.dim) load_acts(a.q, q_row + e, a.type, x[j]);
-        }
+        // in chunks that registers hold: the last stays, one before it is read again
+        constexpr uint32_t CHUNK = D / 16 < 8 ? D / 16 : 8, CHUNKS = D / 16 / CHUNK;
+        float x[CHUNK][8];
         float most = 0.f;
+        const auto load = [&](uint32_t c) {
+          load_row(a, q_row, have, [&](uint32_t j) { return half * (D / 2) + 8 * (c * CHUNK + j); }, x);
+        };
 #pragma unroll
-        for (uint32_t j = 0; j < D / 16; ++j)
+        for (uint32_t c = 0; c < CHUNKS; ++c) {
+          load(c);
 #pragma unroll
-          for (uint32_t k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[j][k]));
+          for (uint32_t j = 0; j < CHUNK; ++j)
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x[j][k]));
+        }
         most = fmaxf(most, swap(swaps++ & 1, most));
         const RowScale scale = row_scale<SPLIT>(most, a.scale_log2);
         const float up = scale.up;
         unit = scale.unit;
 #pragma unroll
-        for (uint32_t j0 = 0; j0 < D / 16; j0 += 4) {
-          uint32_t w[16];
+        for (uint32_t c = CHUNKS; c-- > 0;) {
+          if (c + 1 < CHUNKS) load(c);
 #pragma unroll
-          for (uint32_t j = 0; j < 4; ++j)
+          for (uint32_t j0 = 0; j0 < CHUNK; j0 += 4) {
+            uint32_t w[16];
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-              uint32_t hi, lo;
-              split2(x[j0 + j][2 * k] * up, x[j0 + j][2 * k + 1] * up, hi, lo);
-              w[4 * j + k] = second ? lo : hi;
-            }
-          tmem_st16(lanes + W::kQ + half * (D / 4) + 4 * j0, w);
+            for (uint32_t j = 0; j < 4; ++j)
+#pragma unroll
+              for (uint32_t k = 0; k < 4; ++k) {
+                uint32_t hi, lo;
+                split2(x[j0 + j][2 * k] * up, x[j0 + j][2 * k + 1] * up, hi, lo);
+                w[4 * j + k] = second ? lo : hi;
+              }
+            tmem_st16(lanes + W::kQ + half * (D / 4) + 4 * (c * CHUNK + j0), w);
+          }
         }
       }
       tmem_wait_st();
