@@ -34,7 +34,9 @@ struct Plan {
   uint32_t rows;   // rows an item
   uint32_t tile;   // positions a tile
   uint32_t ctas;
-  uint64_t bytes;  // workspace
+  bool many;       // few rows of many parts each: join_kernel's SHARED
+  uint64_t parts;  // workspace: bytes of the parts, and all
+  uint64_t bytes;
 };
 
 // What does not depend on addresses: shapes, and the launch they give. KQ_OK or KQ_E_INVALID.
@@ -66,17 +68,19 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
     return fail(KQ_E_INVALID, call, "too many positions, heads and drafts in one sequence");
   p.ctas = static_cast<uint32_t>(std::min<uint64_t>(
       uint64_t(ctx->sm_count) * (p.wide ? 1 : tree::narrow_ctas(c.kind, c.pitch)), std::max<uint64_t>(1, items * tiles)));
-  p.bytes = uint64_t(p.ctas) * 2 * tree::part_floats(p.rows, c.pitch) * 4;
+  p.many = !p.wide && p.ctas > 8 * items;
+  p.parts = uint64_t(p.ctas) * 2 * tree::part_floats(p.rows, c.pitch) * 4;
+  p.bytes = p.parts + uint64_t(p.ctas) * 2 * sizeof(uint4);
   *out = p;
   return KQ_OK;
 }
 
-template <uint32_t ROWS, uint32_t TW>
+template <uint32_t ROWS, bool SHARED>
 cudaError_t launch_join(const tree::TreeArgs& a, uint32_t ctas, cudaStream_t s) {
-  return launch_pdl(a.c.pitch == 64    ? tree::join_kernel<ROWS, 64, TW>
-                    : a.c.pitch == 128 ? tree::join_kernel<ROWS, 128, TW>
-                                       : tree::join_kernel<ROWS, 256, TW>,
-                    dim3(ctas, ROWS / 8), 256, 0, s, a, ctas);
+  return launch_pdl(a.c.pitch == 64    ? tree::join_kernel<ROWS, 64, SHARED>
+                    : a.c.pitch == 128 ? tree::join_kernel<ROWS, 128, SHARED>
+                                       : tree::join_kernel<ROWS, 256, SHARED>,
+                    dim3(ctas, SHARED ? ROWS : ROWS / 8), 256, 0, s, a);
 }
 
 bool on16(uint64_t bytes) { return bytes % 16 == 0; }
@@ -132,6 +136,7 @@ int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {
   a.pages = reinterpret_cast<const int*>(d.pages);
   a.mask = reinterpret_cast<const unsigned long long*>(d.mask);
   a.part = reinterpret_cast<float*>(d.workspace);
+  a.splits = reinterpret_cast<uint4*>(d.workspace + p.parts);
   a.scale_log2 = static_cast<float>((d.scale > 0.f ? static_cast<double>(d.scale)
                                                    : 1.0 / std::sqrt(static_cast<double>(a.c.dim))) *
                                     1.4426950408889634);
@@ -150,9 +155,10 @@ int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {
   cudaError_t e = launch(a, p.split, p.wide, p.ctas, s);
   if (e != cudaSuccess) return cuda_fail(e, "cudaLaunchKernelExC", call);
   if (p.ctas == 1) return KQ_OK;  // nothing is split
-  e = p.rows == 8 ? launch_join<8, 128>(a, p.ctas, s)
-      : p.rows == 64 ? launch_join<64, 64>(a, p.ctas, s)
-                     : launch_join<128, 64>(a, p.ctas, s);
+  const auto join = p.rows == 8    ? (p.many ? launch_join<8, true> : launch_join<8, false>)
+                    : p.rows == 64 ? launch_join<64, false>
+                                   : launch_join<128, false>;
+  e = join(a, p.ctas, s);
   return e == cudaSuccess ? KQ_OK : cuda_fail(e, "cudaLaunchKernelExC", "tree attention join");
 }
 

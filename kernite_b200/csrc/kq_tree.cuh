@@ -38,6 +38,7 @@ struct TreeArgs {
   const int* pages;
   const unsigned long long* mask;
   float* part;
+  uint4* splits;  // two a CTA: Split
   float scale_log2;
   uint32_t n_seq, n_heads, group, tokens, max_drafts, max_pages;
   uint32_t per_group;  // ceil(2^32 / group); 0 for a group of one
@@ -58,10 +59,8 @@ struct Seq {
   __device__ uint32_t length() const { return prefix + drafts; }
 };
 
-// Read through L2: the join kernel looks before its pdl_wait(), when its SM's L1 may hold what an earlier
-// step had there.
 __device__ __forceinline__ Seq load_seq(const TreeArgs& a, uint32_t s) {
-  const int b = __ldcg(a.starts + s), e = __ldcg(a.starts + s + 1), p = __ldcg(a.prefix + s);
+  const int b = a.starts[s], e = a.starts[s + 1], p = a.prefix[s];
   Seq q = {static_cast<uint32_t>(b), static_cast<uint32_t>(e - b), static_cast<uint32_t>(p)};
   const bool ok = b >= 0 && e >= b && static_cast<uint32_t>(e) <= a.tokens && q.drafts <= a.max_drafts &&
                   p >= 0 && uint64_t(q.prefix) + q.drafts <= uint64_t(a.max_pages) << a.c.page_log2;
@@ -189,6 +188,29 @@ __device__ __forceinline__ uint32_t range_owner(uint64_t total, uint64_t at, uin
 // Floats of one slot of partial results: rows x pitch outputs, then rows maxima and rows sums.
 __host__ __device__ constexpr uint64_t part_floats(uint32_t rows, uint32_t pitch) {
   return uint64_t(rows) * (pitch + 2);
+}
+
+// What a CTA tells the join kernel of an item that it began and others went on with: the last of those,
+// the item. (CTA 0 is never the last, so 0 says that there is none.)
+struct Split {
+  uint32_t last, rows, head, drafts, first;
+  __device__ static Split load(const TreeArgs& a, uint32_t cta) {
+    const uint4 x = a.splits[2 * cta], y = a.splits[2 * cta + 1];
+    return {x.x, x.y, x.z, x.w, y.x};
+  }
+  __device__ void store(const TreeArgs& a, uint32_t cta) const {
+    a.splits[2 * cta] = make_uint4(last, rows, head, drafts);
+    a.splits[2 * cta + 1] = make_uint4(first, 0, 0, 0);
+  }
+};
+
+// By one thread of each CTA, once: after its last item p (end: one past its tiles, of n, of which it did the
+// item's first ones or not), or for a CTA without work.
+__device__ __forceinline__ void leave_split(const TreeArgs& a, const Place& p, bool began, bool whole, uint64_t total,
+                                            uint64_t end, uint32_t done, uint32_t tiles, uint32_t n) {
+  Split s = {0, 0, 0, 0, 0};
+  if (began && !whole) s = {range_owner(total, end - done + tiles - 1, n), p.rows, p.head, p.seq.drafts, p.seq.first};
+  s.store(a, blockIdx.x);
 }
 
 // Whether row token t (of the sequence) sees position pos.
@@ -787,7 +809,10 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
   const Work<ROWS, kTile> work(a);
   const uint64_t total = work.total;
   const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(gridDim.x), total));
-  if (blockIdx.x >= ctas) return;
+  if (blockIdx.x >= ctas) {
+    if (threadIdx.x == 0) Split{0, 0, 0, 0, 0}.store(a, blockIdx.x);
+    return;
+  }
   const uint64_t at = range_start(total, blockIdx.x, ctas);
   const uint32_t count = static_cast<uint32_t>(range_start(total, blockIdx.x + 1, ctas) - at);  // this CTA's tiles
   Place p = locate(a, work, at);
@@ -1137,6 +1162,8 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
         part[ROWS * (D + 1) + row] = den;
       }
     }
+    if (done == count && threadIdx.x == 0)
+      leave_split(a, p, first_tile == 0, whole, total, at + count, here, tiles, ctas);
     if (done < count) {
       next_item<ROWS>(a, p);
       named_barrier(1, kReaders * 32);  // read, before the next item's are written
@@ -1147,45 +1174,36 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
 // ---------------------------------------------------------------- the join of split items
 
 // out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over the parts of each item that more than one CTA
-// did, in the parts' order, with a running maximum M. Grid: (the CTAs that left parts, rows / 8): an item
-// is joined by the blocks of the CTA that began it (each began at most one that another went on with),
-// a warp a row, CB parts at a time so that their loads share L2's latency.
+// did, in an order that the lengths alone decide, with a running maximum M. Grid: (the CTAs that may have
+// left parts, shares of the rows): an item is joined by the blocks of the CTA that began it (each began at
+// most one that others went on with), which say so in the workspace. CB parts at a time, so that their
+// loads share L2's latency, and a warp a row; where items have many parts (SHARED) a block a row, its
+// warps the parts in turn, for then there are few rows: 8 items of 37 parts each WARP -> BLOCK us, but 256
+// of 2 or 3 the other way OTHER.
 //
-// Joining in the main kernel, by the CTA that leaves an item's last part, was slower (one token over
-// 131001 positions 94 us against 92, 25 drafts 56 against 49): that CTA joins alone, after the fences.
-template <uint32_t ROWS, uint32_t D, uint32_t TW>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeArgs a, uint32_t grid) {
-  // Where the parts are, while the main kernel is at work: the lengths were there before it (it lets this
-  // kernel start after its own pdl_wait).
-  const Work<ROWS, TW> work(a);
-  const uint64_t total = work.total;
-  const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(grid), total)), c0 = blockIdx.x;
-  const bool splits = c0 + 1 < ctas;
-  const uint64_t last = splits ? range_start(total, c0 + 1, ctas) - 1 : 0;  // the CTA's last tile
-  const Place p = locate(a, work, last);
-  const uint64_t item = last - p.tile;
-  const uint32_t tiles = position_tiles<TW>(p.seq);
-  const uint32_t row = blockIdx.y * 8 + threadIdx.x / 32, rr = p.rows * ROWS + row;
-  const bool mine = splits && item + tiles != last + 1 && item >= range_start(total, c0, ctas) &&
-                    rr < p.seq.drafts * a.group;
-  pdl_wait();  // in every block: a kernel after this one waits for this one alone
+// Finding the parts again from the lengths, as the main kernel does, cost each block some 2 us, and they
+// cannot do it early: they do not fit an SM beside the main kernel's CTAs. Joining in the main kernel, by the
+// CTA that leaves an item's last part, was slower (one token over 131001 positions 94 us against 92, 25
+// drafts 56 against 49): that CTA joins alone, after the fences.
+template <uint32_t ROWS, uint32_t D, bool SHARED>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeArgs a) {
+  pdl_wait();
   pdl_launch_dependents();
-  if (!mine) return;
-  const uint32_t c1 = range_owner(total, item + tiles - 1, ctas);
+  const uint32_t c0 = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const Split split = Split::load(a, c0);
+  const uint32_t row = SHARED ? blockIdx.y : blockIdx.y * 8 + warp, rr = split.rows * ROWS + row;
+  if (split.last == 0 || rr >= split.drafts * a.group) return;
   constexpr uint64_t stride = part_floats(ROWS, D);
-  constexpr uint32_t V = D / 32, CB = 8;
-  const uint32_t lane = threadIdx.x % 32;
-  const uint32_t tok = token_of(a, rr);
-  const uint64_t to = (p.seq.first + tok) * a.out_token + uint64_t(p.head * a.group + head_of(a, rr, tok)) * a.c.dim;
+  constexpr uint32_t V = D / 32, CB = 8, STEP = SHARED ? 8 : 1;
   float top = -INFINITY, den = 0.f, v[V] = {};
 #pragma unroll 1
-  for (uint32_t c = c0; c <= c1; c += CB) {
+  for (uint32_t c = c0 + (SHARED ? warp : 0); c <= split.last; c += CB * STEP) {
     float m[CB], l[CB], x[CB][V];
 #pragma unroll
     for (uint32_t j = 0; j < CB; ++j) {
-      const bool there = c + j <= c1;
+      const bool there = c + j * STEP <= split.last;
       // slot 1 of the CTA that began the item, slot 0 of those that went on
-      const float* part = a.part + (uint64_t(c + j) * 2 + (c + j == c0 ? 1 : 0)) * stride;
+      const float* part = a.part + (uint64_t(c + j * STEP) * 2 + (c + j * STEP == c0 ? 1 : 0)) * stride;
       m[j] = there ? part[ROWS * D + row] : -INFINITY;
       l[j] = there ? part[ROWS * (D + 1) + row] : 0.f;
 #pragma unroll
@@ -1211,10 +1229,37 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TreeA
       for (uint32_t i = 0; i < V; ++i) v[i] = fmaf(f, x[j][i], v[i]);
     }
   }
-  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const uint32_t tok = token_of(a, rr);
+  const uint64_t to = (split.first + tok) * a.out_token + uint64_t(split.head * a.group + head_of(a, rr, tok)) * a.c.dim;
+  if constexpr (!SHARED) {
+    const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
-  for (uint32_t i = 0; i < V; ++i)
-    if (lane * V + i < a.c.dim) store_one(a.out, to + lane * V + i, v[i] * inv, a.type);
+    for (uint32_t i = 0; i < V; ++i)
+      if (lane * V + i < a.c.dim) store_one(a.out, to + lane * V + i, v[i] * inv, a.type);
+  } else {
+    __shared__ float tops[8], dens[8], outs[8][D];
+    if (lane == 0) {
+      tops[warp] = top;
+      dens[warp] = den;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < V; ++i) outs[warp][lane * V + i] = v[i];
+    __syncthreads();
+    const uint32_t e = threadIdx.x;
+    if (e >= a.c.dim) return;
+    float mx = -INFINITY;
+#pragma unroll
+    for (uint32_t w = 0; w < 8; ++w) mx = fmaxf(mx, tops[w]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float y = 0.f, all = 0.f;
+#pragma unroll
+    for (uint32_t w = 0; w < 8; ++w) {
+      const float f = exp2f(tops[w] - ref);
+      all = fmaf(f, dens[w], all);
+      y = fmaf(f, outs[w][e], y);
+    }
+    store_one(a.out, to + e, all == 0.f ? 0.f : y / all, a.type);
+  }
 }
 
 // CTAs of the warp-MMA kernel a SM holds.

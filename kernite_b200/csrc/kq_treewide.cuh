@@ -292,7 +292,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   const Work<ROWS, TW> work(a);
   const uint64_t total = work.total;
   const uint32_t ctas = static_cast<uint32_t>(min(uint64_t(gridDim.x), total));
-  if (blockIdx.x >= ctas) return;
+  if (blockIdx.x >= ctas) {
+    if (threadIdx.x == 0) Split{0, 0, 0, 0, 0}.store(a, blockIdx.x);
+    return;
+  }
   if (warp == 0) {
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
     tmem_relinquish();
@@ -760,7 +763,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       }
       tc_fence_before();  // O is read before the next item's first product writes it
       named_barrier(1, kSoftWarps * 32);
-      if (threadIdx.x == 0) special[items & 1] = 0;
+      if (threadIdx.x == 0) {
+        special[items & 1] = 0;
+        if (at == end) leave_split(a, p, first_tile == 0, whole, total, end, p.tile - first_tile, tiles, ctas);
+      }
       ++items;
       if (at < end) next_item<ROWS>(a, p);
     }
