@@ -95,16 +95,28 @@ __device__ __forceinline__ void rotate_halves(const T* row, uint32_t e, uint32_t
   }
 }
 
-// VE values of elements e.. of position p into a head's record; the 32 / VE lanes of a block of 32
-// elements call this together (mask: the lanes that do).
+// 1 / x to a unit or two of the last place.
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// VE values of elements e.. of a head's row into the cache: their codes to `to`, their block's scale to
+// `scale_to`; the 32 / VE lanes of a block of 32 elements call this together (mask: the lanes that do).
+//
+// A code is the correctly rounded quotient's nearest integer, so that which of two a value near a tie gets
+// does not depend on how it was divided. The sum q + 1.5 2^23, q the product with the rounded reciprocal (off
+// by 2^-15 at most), has that integer in its low bits; what it left of q says whether q was so near a tie
+// that the quotient itself is needed. Rounding and conversion instructions would take the special
+// function unit, four lanes a cycle (6144 tokens of 32 + 32 heads written and read back: BEFORE -> AFTER us).
 template <int VE>
-__device__ __forceinline__ void keep(const CacheView& c, uint8_t* record, uint32_t p, uint32_t e,
-                                     const float (&y)[VE], uint32_t mask) {
-  if (c.kind == KQ_CACHE_F16) {
+__device__ __forceinline__ void keep(uint32_t kind, uint8_t* to, uint8_t* scale_to, uint32_t e, const float (&x)[VE],
+                                     uint32_t mask) {
+  if (kind == KQ_CACHE_F16) {
     __half h[VE];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) h[i] = __float2half_rn(y[i]);
-    uint8_t* to = record + cache_offset(p, 2 * e, c.row);
+    for (int i = 0; i < VE; ++i) h[i] = __float2half_rn(x[i]);
     if constexpr (VE == 8) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
     else if constexpr (VE == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(h);
     else *reinterpret_cast<__half*>(to) = h[0];
@@ -112,36 +124,45 @@ __device__ __forceinline__ void keep(const CacheView& c, uint8_t* record, uint32
   }
   uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < VE; ++i) most = max(most, __float_as_uint(y[i]) & 0x7fffffffu);
+  for (int i = 0; i < VE; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
   for (int o = 16 / VE; o; o >>= 1) most = max(most, __shfl_xor_sync(mask, most, o));
-  const uint32_t byte = scale_byte(most, c.kind);
-  const float scale = scale_value(byte), top = cache_top(c.kind);
-  const bool zero = byte == 0 || byte == kScaleNan;
-  const float inverse = zero ? 0.f : 1.f / scale;
-  uint32_t u[VE];
+  const uint32_t byte = scale_byte(most, kind);
+  const float scale = scale_value(byte);
+  float inverse = reciprocal(scale);
+  float y[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) y[i] = x[i];
+  if (byte == 0 || byte >= cache_last_scale(kind)) {
+    // nothing to hold (zeros, or a block that reads back as NaN), or magnitudes that may saturate
+    const float lim = byte == cache_last_scale(kind) ? cache_top(kind) * scale : 0.f;
+    if (lim == 0.f) inverse = 0.f;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) y[i] = lim == 0.f ? 0.f : fminf(fmaxf(y[i], -lim), lim);
+  }
+  const float magic = 12582912.f + (kind == KQ_CACHE_Q8 ? 128.f : 8.f);  // 1.5 2^23, and the code's offset
+  float sum[VE], near = 0.f;
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
-    // The code is the correctly rounded quotient's nearest integer, so that which of two a value near a tie
-    // gets does not depend on how it was divided: the product with the rounded reciprocal (off by 2^-15 at
-    // most) decides unless it is that near.
-    const float q = zero ? 0.f : y[i] * inverse;
-    float code = rintf(q);
-    if (fabsf(fabsf(q - code) - 0.5f) < 0x1p-12f) code = rintf(__fdiv_rn(y[i], scale));
-    u[i] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(code, -top), top)) +
-                                 (c.kind == KQ_CACHE_Q8 ? 128 : 8));
+    sum[i] = fmaf(y[i], inverse, magic);
+    near = fmaxf(near, fabsf(fmaf(y[i], inverse, magic - sum[i])));
   }
-  if (e % 32 == 0) record[c.page() * c.row + p * c.scales + e / 32] = static_cast<uint8_t>(byte);
-  if (c.kind == KQ_CACHE_Q8) {
-    uint8_t* to = record + cache_offset(p, e, c.row);
-    if constexpr (VE == 8) {
-      *reinterpret_cast<uint2*>(to) = make_uint2(u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24,
-                                                 u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24);
-    } else if constexpr (VE == 4) {
-      *reinterpret_cast<uint32_t*>(to) = u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24;
-    } else {
-      *to = static_cast<uint8_t>(u[0]);
-    }
+  if (near > 0.5f - 0x1p-12f) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) sum[i] = magic + rintf(__fdiv_rn(y[i], scale));
+  }
+  uint32_t u[VE];
+#pragma unroll
+  for (int i = 0; i < VE; ++i) u[i] = __float_as_uint(sum[i]);
+  if (e % 32 == 0) *scale_to = static_cast<uint8_t>(byte);
+  if (kind == KQ_CACHE_Q8) {
+    const auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+      return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    };
+    if constexpr (VE == 8)
+      *reinterpret_cast<uint2*>(to) = make_uint2(four(u[0], u[1], u[2], u[3]), four(u[4], u[5], u[6], u[7]));
+    else if constexpr (VE == 4) *reinterpret_cast<uint32_t*>(to) = four(u[0], u[1], u[2], u[3]);
+    else *to = static_cast<uint8_t>(u[0]);
     return;
   }
   // eight elements a word, element 2i at nibble i and 2i + 1 at nibble i + 4
@@ -149,11 +170,11 @@ __device__ __forceinline__ void keep(const CacheView& c, uint8_t* record, uint32
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     const uint32_t j = (e + i) & 7u;
-    word |= u[i] << (4 * ((j >> 1) + 4 * (j & 1)));
+    word |= (u[i] & 15u) << (4 * ((j >> 1) + 4 * (j & 1)));
   }
 #pragma unroll
   for (int o = 4 / VE; o; o >>= 1) word |= __shfl_xor_sync(mask, word, o);
-  if (e % 8 == 0) *reinterpret_cast<uint32_t*>(record + cache_offset(p, e / 2, c.row)) = word;
+  if (e % 8 == 0) *reinterpret_cast<uint32_t*>(to) = word;
 }
 
 // (gain cos, gain sin) of pair i at a position. Whole turns do not matter, so position * turns is taken
@@ -206,22 +227,33 @@ __global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4)
   const uint32_t per_row = a.dim / E, e = lane % per_row * E, sub = lane / per_row;
   const uint32_t at_once = 32 / per_row;  // rows a warp takes at once
   const bool halves = a.layout == KQ_ROPE_HALVES;
-  const uint32_t rot = 2 * a.rot_half;
-  // y = x * by + other * with; elements past rot as they are
+  // y = x * by + other * with, where the lane's elements turn (all of them or none)
+  const bool lane_turns = e < 2 * a.rot_half;
   float by[E], with[E];
   uint32_t partner = lane;
+  if (lane_turns) {
+    const bool first = e < a.rot_half;
+    const float2* w = cs + (halves ? (first ? e : e - a.rot_half) : e / 2);
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    by[i] = 1.f;
-    with[i] = 0.f;
-    if (e + i < rot) {
-      const bool first = halves ? e < a.rot_half : (i & 1) == 0;
-      const float2 w = cs[halves ? (first ? e + i : e + i - a.rot_half) : (e + i) / 2];
-      by[i] = w.x;
-      with[i] = first ? -w.y : w.y;
+    for (int i = 0; i < E; ++i) {
+      const float2 v = w[halves ? i : i / 2];
+      by[i] = v.x;
+      with[i] = (halves ? first : (i & 1) == 0) ? -v.y : v.y;
     }
+    if (halves) partner = first ? lane + a.rot_half / E : lane - a.rot_half / E;
   }
-  if (halves && e < rot) partner = e < a.rot_half ? lane + a.rot_half / E : lane - a.rot_half / E;
+  // where a row r is: queries first, then the keys, then the values, addressed by r throughout
+  const uint32_t keys_end = a.nq + a.cache.n_kv;
+  const T* q = static_cast<const T*>(a.q) + t * a.q_token + e;
+  const T* k_in = static_cast<const T*>(a.k) + t * a.k_token + e;
+  const T* v_in = static_cast<const T*>(a.v) + t * a.v_token + e;
+  T* q_out = static_cast<T*>(a.q_out) + t * a.out_token + e;
+  const uint32_t byte_at = a.cache.kind == KQ_CACHE_F16  ? 2 * e
+                           : a.cache.kind == KQ_CACHE_Q8 ? e
+                                                         : e / 8 * 4;  // of its word
+  const uint64_t page_at = a.cache.at(page, 0);
+  const uint32_t code_at = cache_offset(p, byte_at, a.cache.row);
+  const uint32_t scale_at = a.cache.page() * a.cache.row + p * a.cache.scales + e / 32;
   const uint32_t step = gridDim.y * each * at_once;
   for (uint32_t r0 = (blockIdx.y * each + warp) * at_once; r0 < rows; r0 += AHEAD * step) {
     float x[AHEAD][E];
@@ -231,36 +263,34 @@ __global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4)
 #pragma unroll
       for (int i = 0; i < E; ++i) x[k][i] = 0.f;
       if (row >= rows) continue;
-      const T* from = row < a.nq ? static_cast<const T*>(a.q) + t * a.q_token + row * a.q_head
-                      : row < a.nq + a.cache.n_kv
-                          ? static_cast<const T*>(a.k) + t * a.k_token + (row - a.nq) * a.dim
-                          : static_cast<const T*>(a.v) + t * a.v_token + (row - a.nq - a.cache.n_kv) * a.dim;
-      load_wide<T, E>(from + e, x[k]);
+      const T* from = row < a.nq       ? q + row * a.q_head
+                      : row < keys_end ? k_in + uint64_t(row - a.nq) * a.dim
+                                       : v_in + uint64_t(row - keys_end) * a.dim;
+      load_wide<T, E>(from, x[k]);
     }
 #pragma unroll
     for (uint32_t k = 0; k < AHEAD; ++k) {
       if (r0 + k * step >= rows) break;  // the warp's first row: all its lanes leave
       const uint32_t row = r0 + k * step + sub;
-      const bool in = row < rows, turns = row < a.nq + a.cache.n_kv;
+      const bool in = row < rows, turns = row < keys_end;
       float y[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = x[k][i ^ 1];
       if (halves) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const float other = __shfl_sync(0xffffffffu, x[k][i], partner);
-          y[i] = turns && e < rot ? fmaf(x[k][i], by[i], other * with[i]) : x[k][i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          y[i] = turns && e + i < rot ? fmaf(x[k][i], by[i], x[k][i ^ 1] * with[i]) : x[k][i];
+        for (int i = 0; i < E; ++i) y[i] = __shfl_sync(0xffffffffu, x[k][i], partner);
       }
+      const bool turned = turns && lane_turns;
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = turned ? fmaf(x[k][i], by[i], y[i] * with[i]) : x[k][i];
       const uint32_t mask = __ballot_sync(0xffffffffu, in && row >= a.nq);
       if (!in) continue;
       if (row < a.nq) {
-        store_wide<T, E>(static_cast<T*>(a.q_out) + t * a.out_token + row * a.out_head + e, y);
+        store_wide<T, E>(q_out + row * a.out_head, y);
       } else {
-        const uint32_t h = turns ? row - a.nq : row - a.nq - a.cache.n_kv;
-        keep<E>(a.cache, (turns ? a.cache.k : a.cache.v) + a.cache.at(page, h), p, e, y, mask);
+        uint8_t* record = (turns ? a.cache.k : a.cache.v) + page_at +
+                          uint64_t(row - (turns ? a.nq : keys_end)) * a.cache.record;
+        keep<E>(a.cache.kind, record + code_at, record + scale_at, e, y, mask);
       }
     }
   }
@@ -348,7 +378,12 @@ __global__ void __launch_bounds__(kThreads)
         rotate_pairs<T, VE>(x, e, a.rot_half, cs, y);
       }
       __syncwarp(mask);
-      keep<VE>(a.cache, (key ? a.cache.k : a.cache.v) + a.cache.at(page, h), p, e, y, mask);
+      uint8_t* record = (key ? a.cache.k : a.cache.v) + a.cache.at(page, h);
+      const uint32_t byte_at = a.cache.kind == KQ_CACHE_F16  ? 2 * e
+                               : a.cache.kind == KQ_CACHE_Q8 ? e
+                                                             : e / 8 * 4;  // of its word
+      keep<VE>(a.cache.kind, record + cache_offset(p, byte_at, a.cache.row),
+               record + a.cache.page() * a.cache.row + p * a.cache.scales + e / 32, e, y, mask);
     }
   }
 }
@@ -372,7 +407,8 @@ int launch_rope(void (*kernel)(RopeArgs, Turns<PAIRS>), RopeArgs& a, const kq_ro
 }
 
 // The wide forms want every row they read or write on 16 bytes and, for halves, partners a whole lane
-// apart; anything else is served one element a lane.
+// apart (rope_rows_kernel also, for pairs, whole lanes that turn); anything else is served one element a
+// lane.
 template <typename T, uint32_t PAIRS>
 int dispatch_rope(RopeArgs& a, const kq_rope* rope, bool aligned, uint32_t rows, int sm_count, cudaStream_t s,
                   const char* call) {
@@ -380,7 +416,7 @@ int dispatch_rope(RopeArgs& a, const kq_rope* rope, bool aligned, uint32_t rows,
   const uint32_t lane = sizeof(T) == 4 && a.dim == 256 ? 8 : VE;  // elements a lane
   const bool pairs = a.layout == KQ_ROPE_PAIRS;
   const bool wide = aligned && a.dim % VE == 0;
-  if (wide && (pairs || a.rot_half % lane == 0) && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
+  if (wide && (pairs ? 2 * a.rot_half : a.rot_half) % lane == 0 && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
     a.together = 32 * lane / a.dim;
     return launch_rope(lane == VE ? rope_rows_kernel<T, VE, PAIRS> : rope_rows_kernel<T, 8, PAIRS>, a, rope, rows,
                        sm_count, s, call, true);
@@ -428,28 +464,36 @@ bool on16(uint64_t bytes) { return bytes % 16 == 0; }
 
 // ---------------------------------------------------------------- reading back
 
-// E elements (16 bytes of output) a thread, of ROWS rows at once so that their loads are in flight together.
-// Grid: (row groups, parts of a row, K then V).
+// E elements (16 bytes of output) a thread, of ROWS rows at once so that their loads are in flight together;
+// a CTA has `subs` rows side by side where a row is less than its threads. Grid: (row groups, parts of a
+// row, K then V). What differs by rows alone is worked out once a thread, and codes become f32 by their
+// place in the low bits of 2^23 (conversions take the special function unit): the kernel was bound by its
+// instructions (65536 rows of 1024: BEFORE -> AFTER us).
 template <typename T, int KIND, int ROWS>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheView c, T* k_out, T* v_out, const long long* slots,
-                                                              uint64_t token_stride, uint32_t count,
-                                                              uint32_t per_head, uint32_t over_head, bool wide,
-                                                              unsigned* err) {
+__global__ void __launch_bounds__(kThreads)
+    cache_read_kernel(CacheView c, T* k_out, T* v_out, const long long* slots, uint64_t token_stride, uint32_t count,
+                      uint32_t units, uint32_t subs, uint32_t over_units, uint32_t per_head, uint32_t over_head,
+                      bool wide, unsigned* err) {
   constexpr int E = 16 / sizeof(T);
   constexpr int B = KIND == KQ_CACHE_F16 ? 2 * E : KIND == KQ_CACHE_Q8 ? E : 4;  // bytes of codes (Q4: a word)
   pdl_wait();
   pdl_launch_dependents();
   const bool value = blockIdx.z;
-  T* out = value ? v_out : k_out;
-  const uint8_t* base = value ? c.v : c.k;
-  const uint32_t i = blockIdx.y * kThreads + threadIdx.x;
+  const uint32_t thread = blockIdx.y * kThreads + threadIdx.x;
+  const uint32_t sub = subs > 1 ? __umulhi(thread, over_units) : 0, i = thread - sub * units;
   const uint32_t h = over_head ? __umulhi(i, over_head) : i, e = (i - h * per_head) * E;
-  if (h >= c.n_kv) return;
-  const uint32_t r0 = blockIdx.x * ROWS;
+  if (sub >= subs || h >= c.n_kv) return;
+  const uint32_t r0 = blockIdx.x * (ROWS * subs) + sub;
+  const uint8_t* base = (value ? c.v : c.k) + h * c.record;
+  const uint64_t page_bytes = c.n_kv * c.record;
+  const uint32_t byte = KIND == KQ_CACHE_F16 ? 2 * e : KIND == KQ_CACHE_Q8 ? e : e / 8 * 4;
+  const uint32_t scales = c.page() * c.row + e / 32;
+  const Swizzle swizzle(c.row);
+  T* to = (value ? v_out : k_out) + r0 * token_stride + h * c.dim + e;
   long long slot[ROWS];
   uint32_t raw[ROWS][B / 4], scale[ROWS];
 #pragma unroll
-  for (int k = 0; k < ROWS; ++k) slot[k] = r0 + k < count ? slots[r0 + k] : -1;
+  for (int k = 0; k < ROWS; ++k) slot[k] = r0 + k * subs < count ? slots[r0 + k * subs] : -1;
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
 #pragma unroll
@@ -461,10 +505,9 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheView c, T* k_
       slot[k] = -2;  // this row is left as it is
       continue;
     }
-    const uint8_t* rec = base + c.at(static_cast<uint32_t>(slot[k] >> c.page_log2), h);
+    const uint8_t* rec = base + static_cast<uint32_t>(slot[k] >> c.page_log2) * page_bytes;
     const uint32_t p = static_cast<uint32_t>(slot[k]) & (c.page() - 1);
-    const uint8_t* from =
-        rec + cache_offset(p, KIND == KQ_CACHE_F16 ? 2 * e : KIND == KQ_CACHE_Q8 ? e : e / 8 * 4, c.row);
+    const uint8_t* from = rec + ((p * c.row + byte) ^ swizzle.bytes(p));
     if constexpr (B == 16) {
       const uint4 w = *reinterpret_cast<const uint4*>(from);
       raw[k][0] = w.x;
@@ -478,31 +521,31 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheView c, T* k_
     } else {
       raw[k][0] = *reinterpret_cast<const uint32_t*>(from);
     }
-    if constexpr (KIND != KQ_CACHE_F16) scale[k] = rec[c.page() * c.row + p * c.scales + e / 32];
+    if constexpr (KIND != KQ_CACHE_F16) scale[k] = rec[scales + p * c.scales];
   }
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
-    if (r0 + k >= count || slot[k] == -2) continue;
+    const bool there = r0 + k * subs < count && slot[k] != -2;
     float y[E];
-    const float s = scale_value(scale[k]);
-    const bool zero = slot[k] < 0;
+    const float s = slot[k] < 0 ? 0.f : scale_value(scale[k]);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       if constexpr (KIND == KQ_CACHE_F16) {
         y[j] = h2f(raw[k][j / 2] >> (16 * (j % 2)) & 0xffffu);
       } else if constexpr (KIND == KQ_CACHE_Q8) {
-        y[j] = zero ? 0.f : (static_cast<float>(raw[k][j / 4] >> (8 * (j % 4)) & 255u) - 128.f) * s;
+        y[j] = (__uint_as_float(__byte_perm(raw[k][j / 4], 0x4b000000u, 0x7650 + j % 4)) - 8388736.f) * s;
       } else {
         const uint32_t n = e % 8 + j;  // element of the word
-        y[j] = zero ? 0.f : (static_cast<float>(raw[k][0] >> (4 * (n / 2 + 4 * (n % 2))) & 15u) - 8.f) * s;
+        y[j] = (__uint_as_float((raw[k][0] >> (4 * (n / 2 + 4 * (n % 2))) & 15u) | 0x4b000000u) - 8388616.f) * s;
       }
     }
-    T* to = out + (r0 + k) * token_stride + h * c.dim + e;
+    T* at = to + k * (subs * token_stride);
+    if (!there) continue;
     if (wide) {
-      store_act<T, E>(to, y);
+      store_act<T, E>(at, y);
     } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) to[j] = act_from_f32<T>(y[j]);
+      for (int j = 0; j < E; ++j) at[j] = act_from_f32<T>(y[j]);
     }
   }
 }
@@ -752,16 +795,18 @@ int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s) {
     }
     constexpr uint32_t E = 16 / sizeof(T);
     const uint32_t per_head = c.dim / E, over_head = static_cast<uint32_t>(((1ull << 32) + per_head - 1) / per_head);
-    const uint32_t parts = (c.n_kv * per_head + kThreads - 1) / kThreads;
-    // four rows a thread hide the loads' latency (65536 rows of 1024: 128 -> TIME us); one where that would
-    // leave SMs idle
-    const bool many = uint64_t(d.count) * parts * arrays >= 32u * ctx->sm_count;
+    const uint32_t units = c.n_kv * per_head, parts = (units + kThreads - 1) / kThreads;
+    const uint32_t subs = std::max<uint32_t>(1, kThreads / units);
+    const uint32_t over_units = static_cast<uint32_t>(((1ull << 32) + units - 1) / units);
+    // four rows a thread hide the loads' latency (65536 rows of 1024: ONE -> FOUR us); one where that would
+    // leave SMs idle (1001 rows: FOUR -> ONE us)
+    const bool many = uint64_t(d.count) / subs * parts * arrays >= 32u * ctx->sm_count;
     const auto run = [&](auto kind) {
       constexpr int K = decltype(kind)::value;
-      return many ? launch_pdl(cache_read_kernel<T, K, 4>, dim3((d.count + 3) / 4, parts, arrays), kThreads, 0, s, view,
-                               k, v, slots, stride, d.count, per_head, over_head, wide, ctx->err)
-                  : launch_pdl(cache_read_kernel<T, K, 1>, dim3(d.count, parts, arrays), kThreads, 0, s, view, k, v,
-                               slots, stride, d.count, per_head, over_head, wide, ctx->err);
+      const uint32_t rows = subs * (many ? 4 : 1);
+      return launch_pdl(many ? cache_read_kernel<T, K, 4> : cache_read_kernel<T, K, 1>,
+                        dim3((d.count + rows - 1) / rows, parts, arrays), kThreads, 0, s, view, k, v, slots, stride,
+                        d.count, units, subs, over_units, per_head, over_head, wide, ctx->err);
     };
     return c.kind == KQ_CACHE_F16  ? run(std::integral_constant<int, KQ_CACHE_F16>())
            : c.kind == KQ_CACHE_Q8 ? run(std::integral_constant<int, KQ_CACHE_Q8>())

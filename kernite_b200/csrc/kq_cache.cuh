@@ -32,6 +32,14 @@ __host__ __device__ __forceinline__ uint32_t cache_swizzle(uint32_t p, uint32_t 
   return row >= 128 ? (p & 7u) : row == 64 ? ((p >> 1) & 3u) << 1 : ((p >> 2) & 1u) << 2;
 }
 
+// The same for many positions of one row size: (p >> a & m) << b.
+struct Swizzle {
+  uint32_t a, m, b;  // b: of bytes
+  __device__ explicit Swizzle(uint32_t row)
+      : a(row >= 128 ? 0 : row == 64 ? 1 : 2), m(row >= 128 ? 7 : row == 64 ? 3 : 1), b(4 + a) {}
+  __device__ uint32_t bytes(uint32_t p) const { return (p >> a & m) << b; }
+};
+
 // Offset in a record's codes of byte `byte` of position p's row.
 __host__ __device__ __forceinline__ uint32_t cache_offset(uint32_t p, uint32_t byte, uint32_t row) {
   return (p * row + byte) ^ (cache_swizzle(p, row) << 4);
@@ -51,10 +59,15 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
 }
 
 // The scale byte of a block whose largest magnitude has the bits `most` (f32): the smallest value of
-// 4 significant bits not below most / top. Magnitudes compare as their bits do, NaN above infinity.
+// 4 significant bits not below most / top (the correctly rounded quotient). Magnitudes compare as their
+// bits do, NaN above infinity.
 __device__ __forceinline__ uint32_t scale_byte(uint32_t most, uint32_t kind) {
   if (most >= 0x7f800000u) return kScaleNan;
-  const float want = __fdiv_rn(__uint_as_float(most), cache_top(kind));
+  const float top = cache_top(kind);
+  // the product with 1 / top is off by two units at most: only near a value of 4 bits, where that would
+  // choose another one, and below f16's normal range is the quotient itself needed
+  float want = __uint_as_float(most) * (kind == KQ_CACHE_Q8 ? 1.f / 127.f : 1.f / 7.f);
+  if (want < 0x1p-13f || ((__float_as_uint(want) + 3u) & 0xFFFFFu) <= 6u) want = __fdiv_rn(__uint_as_float(most), top);
   // normal f16 range: round the fraction up to 3 bits and rebias the exponent (127 - 15); below
   // it the values are multiples of 2^-17
   const uint32_t b = want >= 0x1p-14f ? ((__float_as_uint(want) + 0xFFFFFu) >> 20) - (112u << 3)
