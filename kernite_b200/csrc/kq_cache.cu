@@ -413,7 +413,7 @@ template <typename T, uint32_t PAIRS>
 int dispatch_rope(RopeArgs& a, const kq_rope* rope, bool aligned, uint32_t rows, int sm_count, cudaStream_t s,
                   const char* call) {
   constexpr int VE = 16 / sizeof(T);
-  const uint32_t lane = sizeof(T) == 4 && a.dim == 256 ? 8 : VE;  // elements a lane
+  const uint32_t lane = 8;  // elements a lane
   const bool pairs = a.layout == KQ_ROPE_PAIRS;
   const bool wide = aligned && a.dim % VE == 0;
   if (wide && (pairs ? 2 * a.rot_half : a.rot_half) % lane == 0 && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
@@ -464,6 +464,8 @@ bool on16(uint64_t bytes) { return bytes % 16 == 0; }
 
 // ---------------------------------------------------------------- reading back
 
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+
 // E elements (16 bytes of output) a thread, of ROWS rows at once so that their loads are in flight together;
 // a CTA has `subs` rows side by side where a row is less than its threads. Grid: (row groups, parts of a
 // row, K then V). What differs by rows alone is worked out once a thread, and codes become f32 by their
@@ -490,6 +492,7 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t scales = c.page() * c.row + e / 32;
   const Swizzle swizzle(c.row);
   T* to = (value ? v_out : k_out) + r0 * token_stride + h * c.dim + e;
+  const uint64_t step = subs * token_stride, slots_end = uint64_t(c.n_pages) << c.page_log2;
   long long slot[ROWS];
   uint32_t raw[ROWS][B / 4], scale[ROWS];
 #pragma unroll
@@ -500,7 +503,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int w = 0; w < B / 4; ++w) raw[k][w] = 0;
     scale[k] = 0;
     if (slot[k] < 0) continue;
-    if (static_cast<uint64_t>(slot[k]) >> c.page_log2 >= c.n_pages) {
+    if (static_cast<uint64_t>(slot[k]) >= slots_end) {
       report_error(err, kErrCacheRange);
       slot[k] = -2;  // this row is left as it is
       continue;
@@ -525,9 +528,31 @@ __global__ void __launch_bounds__(kThreads)
   }
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
-    const bool there = r0 + k * subs < count && slot[k] != -2;
+    if (r0 + k * subs >= count || slot[k] == -2) continue;
+    T* at = to + k * step;
+    const uint32_t s16 = slot[k] < 0 ? 0u : scale[k] << 7;  // the scale as f16
+    if constexpr (KIND != KQ_CACHE_F16 && std::is_same_v<T, __half>) {
+      // 1024 + code, less 1024 + offset, times the scale: each exact
+      const __half2 by = as_half2(s16 | s16 << 16);
+      uint32_t w[E / 2];
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) {
+        const uint32_t x = KIND == KQ_CACHE_Q8 ? __byte_perm(raw[k][j / 2], 0x64646464u, j % 2 ? 0x4342 : 0x4140)
+                                               : ((raw[k][0] >> (4 * j)) & 0x000f000fu) | 0x64006400u;
+        const __half2 y = __hmul2(__hsub2(as_half2(x), __float2half2_rn(KIND == KQ_CACHE_Q8 ? 1152.f : 1032.f)), by);
+        w[j] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+      if (wide) {
+        *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          at[j] = __ushort_as_half(static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2))));
+      }
+      continue;
+    }
     float y[E];
-    const float s = slot[k] < 0 ? 0.f : scale_value(scale[k]);
+    const float s = h2f(s16);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       if constexpr (KIND == KQ_CACHE_F16) {
@@ -535,12 +560,11 @@ __global__ void __launch_bounds__(kThreads)
       } else if constexpr (KIND == KQ_CACHE_Q8) {
         y[j] = (__uint_as_float(__byte_perm(raw[k][j / 4], 0x4b000000u, 0x7650 + j % 4)) - 8388736.f) * s;
       } else {
-        const uint32_t n = e % 8 + j;  // element of the word
-        y[j] = (__uint_as_float((raw[k][0] >> (4 * (n / 2 + 4 * (n % 2))) & 15u) | 0x4b000000u) - 8388616.f) * s;
+        // elements 2 i at nibble i, 2 i + 1 at i + 4; the word's second four are 8 bits up
+        const uint32_t x = E == 4 ? raw[k][0] >> (2 * (e & 4u)) : raw[k][0];
+        y[j] = (__uint_as_float((x >> (4 * (j / 2 + 4 * (j % 2))) & 15u) | 0x4b000000u) - 8388616.f) * s;
       }
     }
-    T* at = to + k * (subs * token_stride);
-    if (!there) continue;
     if (wide) {
       store_act<T, E>(at, y);
     } else {

@@ -132,20 +132,30 @@ __device__ __forceinline__ void load_wide(const T* p, float (&v)[N]) {
   }
 }
 
+// A word of v[0] (and, 16-bit types, v[1]).
+template <typename T>
+__device__ __forceinline__ uint32_t act_word(const float* v);
+template <>
+__device__ __forceinline__ uint32_t act_word<float>(const float* v) { return __float_as_uint(v[0]); }
+template <>
+__device__ __forceinline__ uint32_t act_word<__half>(const float* v) {
+  const __half2 h = __floats2half2_rn(v[0], v[1]);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t act_word<__nv_bfloat16>(const float* v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_act(T* p, const float (&v)[N]) {
+  constexpr int W = 4 / sizeof(T);  // elements a word
   if constexpr (N * sizeof(T) == 16) {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = act_from_f32<T>(v[i]);
-    *reinterpret_cast<uint4*>(p) = raw;
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(act_word<T>(v), act_word<T>(v + W), act_word<T>(v + 2 * W), act_word<T>(v + 3 * W));
   } else if constexpr (N * sizeof(T) == 8) {
-    uint2 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = act_from_f32<T>(v[i]);
-    *reinterpret_cast<uint2*>(p) = raw;
+    *reinterpret_cast<uint2*>(p) = make_uint2(act_word<T>(v), act_word<T>(v + W));
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = act_from_f32<T>(v[i]);
