@@ -109,7 +109,7 @@ __device__ __forceinline__ float reciprocal(float x) {
 // does not depend on how it was divided. The sum q + 1.5 2^23, q the product with the rounded reciprocal (off
 // by 2^-15 at most), has that integer in its low bits; what it left of q says whether q was so near a tie
 // that the quotient itself is needed. Rounding and conversion instructions would take the special
-// function unit, four lanes a cycle (6144 tokens of 32 + 32 heads written and read back: BEFORE -> AFTER us).
+// function unit, four lanes a cycle.
 template <int VE>
 __device__ __forceinline__ void keep(uint32_t kind, uint8_t* to, uint8_t* scale_to, uint32_t e, const float (&x)[VE],
                                      uint32_t mask) {
@@ -197,15 +197,18 @@ __device__ __forceinline__ long long take_slot(const RopeArgs& a, uint32_t t) {
   return -1;
 }
 
+constexpr int kLane = 8;  // elements a lane of rope_rows_kernel has of a row
+
 // Heads of 64, 128 or 256 elements, every row on 16 bytes. A lane holds E consecutive elements of a row,
 // dim / E lanes a row, so that its place in a head, and with it its angles, are the same for every row
 // it takes: they stay in registers. A pair's other element is in the lane (pairs) or rot_half / E lanes
-// away (halves). A warp has AHEAD rows' loads in flight. A CTA takes per_block tokens, as many warps each;
+// away (halves). A CTA takes per_block tokens, as many warps each;
 // with one, the grid's y shares out its rows.
-template <typename T, int E, uint32_t PAIRS>
-__global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4)
+template <typename T, uint32_t PAIRS>
+__global__ void __launch_bounds__(kThreads, 4)
     rope_rows_kernel(const __grid_constant__ RopeArgs a, const __grid_constant__ Turns<PAIRS> turns_of) {
-  constexpr uint32_t AHEAD = 2;
+  constexpr int E = kLane, WORDS = E * sizeof(T) / 4;
+  constexpr uint32_t AHEAD = 16 / WORDS;  // rows whose loads are in flight
   extern __shared__ float2 angles[];  // [per_block][rot_half]
   pdl_wait();
   pdl_launch_dependents();
@@ -256,33 +259,42 @@ __global__ void __launch_bounds__(kThreads, E == 4 ? 5 : 4)
   const uint32_t scale_at = a.cache.page() * a.cache.row + p * a.cache.scales + e / 32;
   const uint32_t step = gridDim.y * each * at_once;
   for (uint32_t r0 = (blockIdx.y * each + warp) * at_once; r0 < rows; r0 += AHEAD * step) {
-    float x[AHEAD][E];
+    uint32_t raw[AHEAD][WORDS];
 #pragma unroll
     for (uint32_t k = 0; k < AHEAD; ++k) {
       const uint32_t row = r0 + k * step + sub;
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[k][i] = 0.f;
+      for (int i = 0; i < WORDS; ++i) raw[k][i] = 0;
       if (row >= rows) continue;
       const T* from = row < a.nq       ? q + row * a.q_head
                       : row < keys_end ? k_in + uint64_t(row - a.nq) * a.dim
                                        : v_in + uint64_t(row - keys_end) * a.dim;
-      load_wide<T, E>(from, x[k]);
+      load_words(from, raw[k]);
     }
 #pragma unroll
     for (uint32_t k = 0; k < AHEAD; ++k) {
-      if (r0 + k * step >= rows) break;  // the warp's first row: all its lanes leave
-      const uint32_t row = r0 + k * step + sub;
+      const uint32_t row0 = r0 + k * step, row = row0 + sub;
+      if (row0 >= rows) break;  // the warp's first row: all its lanes leave
       const bool in = row < rows, turns = row < keys_end;
-      float y[E];
+      float x[E], y[E];
+      words_to_f32<T>(raw[k], x);
+      if (row0 >= keys_end) {  // all values
 #pragma unroll
-      for (int i = 0; i < E; ++i) y[i] = x[k][i ^ 1];
-      if (halves) {
+        for (int i = 0; i < E; ++i) y[i] = x[i];
+      } else {
+        if (halves) {
+          uint32_t other[WORDS];
 #pragma unroll
-        for (int i = 0; i < E; ++i) y[i] = __shfl_sync(0xffffffffu, x[k][i], partner);
+          for (int i = 0; i < WORDS; ++i) other[i] = __shfl_sync(0xffffffffu, raw[k][i], partner);
+          words_to_f32<T>(other, y);
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; ++i) y[i] = x[i ^ 1];
+        }
+        const bool turned = turns && lane_turns;
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] = turned ? fmaf(x[i], by[i], y[i] * with[i]) : x[i];
       }
-      const bool turned = turns && lane_turns;
-#pragma unroll
-      for (int i = 0; i < E; ++i) y[i] = turned ? fmaf(x[k][i], by[i], y[i] * with[i]) : x[k][i];
       const uint32_t mask = __ballot_sync(0xffffffffu, in && row >= a.nq);
       if (!in) continue;
       if (row < a.nq) {
@@ -394,11 +406,10 @@ int launch_rope(void (*kernel)(RopeArgs, Turns<PAIRS>), RopeArgs& a, const kq_ro
   Turns<PAIRS> turns;
   if (rope) std::memcpy(turns.at, rope->turns, sizeof(turns.at[0]) * a.rot_half);
   // Below some hundred tokens one CTA a token leaves most SMs idle: a token's rows are then shared by more
-  // CTAs, each taking the angles again. With many tokens of few rows a CTA takes four, so that the angles'
-  // latency is paid once for them (4001 tokens of 40 16-bit heads: ONE -> FOUR us; 6144 of 96 rows the
-  // other way: OTHER).
+  // CTAs, each taking the angles again. With many tokens a CTA takes four, so that the angles' latency is
+  // paid once for them (4001 tokens of 40 16-bit heads: 29 -> 21 us; 6144 of 96 rows 131 -> 125).
   const uint32_t groups = (rows + kWarps * a.together - 1) / (kWarps * a.together);
-  a.per_block = by_rows && a.tokens >= 16u * sm_count && groups <= 3 ? 4 : 1;
+  a.per_block = by_rows && a.tokens >= 16u * sm_count ? 4 : 1;
   const uint32_t shares = std::max<uint32_t>(1, std::min<uint32_t>(groups, 4u * sm_count / a.tokens));
   const uint32_t shared = by_rows ? a.per_block * a.rot_half * sizeof(float2) : 0;
   const cudaError_t e = launch_pdl(kernel, dim3((a.tokens + a.per_block - 1) / a.per_block, shares), kThreads, shared,
@@ -413,13 +424,11 @@ template <typename T, uint32_t PAIRS>
 int dispatch_rope(RopeArgs& a, const kq_rope* rope, bool aligned, uint32_t rows, int sm_count, cudaStream_t s,
                   const char* call) {
   constexpr int VE = 16 / sizeof(T);
-  const uint32_t lane = 8;  // elements a lane
   const bool pairs = a.layout == KQ_ROPE_PAIRS;
   const bool wide = aligned && a.dim % VE == 0;
-  if (wide && (pairs ? 2 * a.rot_half : a.rot_half) % lane == 0 && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
-    a.together = 32 * lane / a.dim;
-    return launch_rope(lane == VE ? rope_rows_kernel<T, VE, PAIRS> : rope_rows_kernel<T, 8, PAIRS>, a, rope, rows,
-                       sm_count, s, call, true);
+  if (wide && (pairs ? 2 * a.rot_half : a.rot_half) % kLane == 0 && (a.dim == 64 || a.dim == 128 || a.dim == 256)) {
+    a.together = 32 * kLane / a.dim;
+    return launch_rope(rope_rows_kernel<T, PAIRS>, a, rope, rows, sm_count, s, call, true);
   }
   if (wide && (pairs || a.rot_half % VE == 0)) {
     // narrow heads: a warp takes several at once, where the queries come out even
@@ -470,7 +479,7 @@ __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_ca
 // a CTA has `subs` rows side by side where a row is less than its threads. Grid: (row groups, parts of a
 // row, K then V). What differs by rows alone is worked out once a thread, and codes become f32 by their
 // place in the low bits of 2^23 (conversions take the special function unit): the kernel was bound by its
-// instructions (65536 rows of 1024: BEFORE -> AFTER us).
+// instructions (65536 rows of 1024, 8 bits to f16: 75 -> 71 us, 89 % of the copy rate).
 template <typename T, int KIND, int ROWS>
 __global__ void __launch_bounds__(kThreads)
     cache_read_kernel(CacheView c, T* k_out, T* v_out, const long long* slots, uint64_t token_stride, uint32_t count,
@@ -822,8 +831,8 @@ int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s) {
     const uint32_t units = c.n_kv * per_head, parts = (units + kThreads - 1) / kThreads;
     const uint32_t subs = std::max<uint32_t>(1, kThreads / units);
     const uint32_t over_units = static_cast<uint32_t>(((1ull << 32) + units - 1) / units);
-    // four rows a thread hide the loads' latency (65536 rows of 1024: ONE -> FOUR us); one where that would
-    // leave SMs idle (1001 rows: FOUR -> ONE us)
+    // four rows a thread hide the loads' latency (65536 rows of 1024: 109 -> 71 us, 1001 rows 4.6 -> 4.3);
+    // one where that would leave SMs idle
     const bool many = uint64_t(d.count) / subs * parts * arrays >= 32u * ctx->sm_count;
     const auto run = [&](auto kind) {
       constexpr int K = decltype(kind)::value;

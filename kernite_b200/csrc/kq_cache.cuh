@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "kq.h"
 
 namespace kq {
@@ -115,19 +117,32 @@ __device__ __forceinline__ void load_act(const T* p, float (&v)[N]) {
   }
 }
 
-// The same for up to 32 bytes (p aligned to 16).
-template <typename T, int N>
-__device__ __forceinline__ void load_wide(const T* p, float (&v)[N]) {
-  if constexpr (N * sizeof(T) <= 16) {
-    load_act<T, N>(p, v);
-  } else {
-    float lo[N / 2], hi[N / 2];
-    load_act<T, N / 2>(p, lo);
-    load_act<T, N / 2>(p + N / 2, hi);
+// W words at p (16-byte aligned; W 4 or 8), and words as the values they hold.
+template <int W>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[W]) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      v[i] = lo[i];
-      v[N / 2 + i] = hi[i];
+  for (int i = 0; i < W; i += 4) {
+    const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
+    w[i] = v.x;
+    w[i + 1] = v.y;
+    w[i + 2] = v.z;
+    w[i + 3] = v.w;
+  }
+}
+template <typename T, int N, int W>
+__device__ __forceinline__ void words_to_f32(const uint32_t (&w)[W], float (&v)[N]) {
+  static_assert(N * sizeof(T) == W * 4);
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    } else {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
 }

@@ -235,7 +235,7 @@ __device__ __forceinline__ __half2 as_h2(uint32_t v) { return *reinterpret_cast<
 
 // Elements at(0), at(1), .. of q from element `row` on, N (4 or 8) each; zeros from element `dim` on and
 // where there is no row. All loads are issued before any is looked at, so that they are one latency: a
-// choice of type at each would wait for each (one token over 99 positions: BEFORE -> AFTER us).
+// choice of type at each would wait for each (4 sequences of 64 drafts: 138 -> 132 us).
 template <uint32_t COUNT, uint32_t N, class At>
 __device__ __forceinline__ void load_row(const TreeArgs& a, uint64_t row, bool have, const At& at,
                                          float (&x)[COUNT][N]) {
@@ -397,7 +397,7 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // `unit`. The power of two in `up` brings the row's largest magnitude (most) to [2^7, 2^8) (or, split,
 // near it), so that f16's range fits any q; it is 1 for a row of zeros or with infinities. 16-bit rows stay
 // exact; split ones take the softmax's scale along, so that `unit` is a power of two and a product's
-// largest logit is the maximum exactly, however large.
+// largest logit is the maximum exactly, however large. unit is never zero: masked logits are -inf times it.
 struct RowScale {
   float up, unit;
 };
@@ -412,9 +412,9 @@ __device__ __forceinline__ RowScale row_scale(float most, float scale_log2) {
     const uint32_t bits = __float_as_uint(scale_log2);
     const float part = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
     const float power = __uint_as_float(bits & 0x7f800000u);
-    return {up * part, down * power};
+    return {up * part, fmaxf(down * power, 0x1p-149f)};
   }
-  return {up, down * scale_log2};
+  return {up, fmaxf(down * scale_log2, 0x1p-149f)};
 }
 
 // How a head of pitch D lies in rows of codes, per kind: bytes of a row, EK elements of a thread's piece of
@@ -1178,11 +1178,12 @@ __global__ void __launch_bounds__(kThreads, Narrow<KIND, D>::kCtas) tree_kernel(
 // left parts, shares of the rows): an item is joined by the blocks of the CTA that began it (each began at
 // most one that others went on with), which say so in the workspace. CB parts at a time, so that their
 // loads share L2's latency, and a warp a row; where items have many parts (SHARED) a block a row, its
-// warps the parts in turn, for then there are few rows: 8 items of 37 parts each WARP -> BLOCK us, but 256
-// of 2 or 3 the other way OTHER.
+// warps the parts in turn, for then there are few rows: 8 items of 37 parts each 66.7 -> 64.0 us with
+// their attention, but 256 of 2 or 3 74.0 -> 78.1.
 //
-// Finding the parts again from the lengths, as the main kernel does, cost each block some 2 us, and they
-// cannot do it early: they do not fit an SM beside the main kernel's CTAs. Joining in the main kernel, by the
+// Finding the parts again from the lengths, as the main kernel does, cost each block some 2 us (4 sequences
+// of 64 drafts 132 us against 125), and they cannot do it early: they do not fit an SM beside the main
+// kernel's CTAs. Joining in the main kernel, by the
 // CTA that leaves an item's last part, was slower (one token over 131001 positions 94 us against 92, 25
 // drafts 56 against 49): that CTA joins alone, after the fences.
 template <uint32_t ROWS, uint32_t D, bool SHARED>
