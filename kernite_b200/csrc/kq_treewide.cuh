@@ -19,6 +19,14 @@
 // and three or four S buffers are under way at once. Each softmax group has its own maxima, sums and,
 // up to a pitch of 128, its own O, joined at an item's end; at 256 there is room for one O, and a tile's
 // maximum is passed on to the group that has the next tile.
+//
+// What bounds it. A tile of 64 positions x 128 elements takes the tensor core 520 cycles (M = 128) and the
+// special function unit 512 for its exponentials; it takes 1300, whatever number of rows is real: a softmax
+// group's way through its tile (read S, maximum, exponentials, P back) is some 2450 cycles of latencies, and
+// there is room for two groups. 4 sequences of 64 drafts x 64 / 8 heads over 6000 to 16000 positions of 8-bit
+// keys and values, bf16: 127 us, 0.73 PFLOP/s; 25 f32 drafts over 8191: 45 us. Holding all of S in
+// registers instead of reading it twice spilled (149 us), and with registers moved from the other warps was
+// no faster (127). MMAs issued by lane 0 instead of an elected thread took 573 us, two S buffers 200.
 #pragma once
 
 #include "kq_tc.cuh"
@@ -308,7 +316,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   const uint64_t end = range_start(total, blockIdx.x + 1, ctas);
   Place p = locate(a, work, at);
   bool live = true;
-  const uint32_t seg_log2 = min(a.c.page_log2, TW == 128 ? 7u : 6u);
+  const uint32_t seg_log2 = min(a.c.page_log2, 6u);
 
   if (warp >= kCopyWarp) {
     // ---- copies, from one thread: raw tiles of keys (use 2 i of the ring) or of values (2 i + 1)
