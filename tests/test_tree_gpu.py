@@ -236,6 +236,16 @@ def test_one_position_takes_all(kernels, drafts, type):
             assert np.abs(got[t, h] - c.values[0][best, 0]).max() <= (2.0 ** -20 + STEP[type]) * 5
 
 
+@pytest.mark.parametrize("type", [kb.TYPE_F32, kb.TYPE_F16])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 256])
+@pytest.mark.parametrize("kind", [ref.F16, ref.Q8, ref.Q4])
+@pytest.mark.parametrize("drafts", [[1, 0, 1, 2], [5, 0, 12, 3]], ids=["few", "many"])
+def test_every_kind_and_head_size(kernels, kind, dim, drafts, type):
+    """Single tokens and small trees of ragged sequences, one of them empty, one without a context."""
+    c = Case(kind, 8, 2, dim, 32, [333, 40, 0, 129], drafts, seed=31, type=type)
+    c.check(c.run(kernels))
+
+
 @pytest.mark.parametrize("case", [(ref.F16, 64, 8, 128, 64, [700] * 6, [1] * 6), (ref.Q8, 16, 2, 256, 32, [900] * 4, [3] * 4),
                                   (ref.F16, 16, 2, 128, 16, [1500] * 3, [4] * 3), (ref.Q8, 8, 8, 128, 64, [1100] * 5, [1] * 5),
                                   (ref.Q4, 8, 2, 64, 64, [3000], [1])], ids=str)
