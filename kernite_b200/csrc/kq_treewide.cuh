@@ -53,6 +53,11 @@ struct Wide {
   static constexpr uint32_t kRaws = kFit > 8 ? 8 : kFit / 2 * 2;
   static constexpr uint32_t kBytes = kFixed + kRaws * kRaw;
   static_assert(kRaws >= 2 && kBytes <= 227 * 1024, "ring");
+  // Flag words (decoder to softmax, a word an item in turn). Values are decoded as far ahead as their operand
+  // slots let them, which in items of one tile is that many items: none may come back to the word of the item
+  // that is being finished.
+  static constexpr uint32_t kFlags = 8;
+  static_assert(kFlags > kOperands / 2 && (kFlags & (kFlags - 1)) == 0, "flag words");
   // tensor memory columns: S (then P) buffers, O (one a softmax group where there is room), Q
   static constexpr bool kOwnO = D <= 128;
   static constexpr uint32_t kBufs = D == 256 ? 2 : D == 128 ? 3 : 4;
@@ -271,7 +276,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
   const uint32_t tail = W::kOperands * W::kOperand + W::kRaws * W::kRaw;
   const WideBars bar = {ops + tail};
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + tail + 384);
-  unsigned long long* special = reinterpret_cast<unsigned long long*>(smem + tail + 392);  // of the item's drafts
+  // drafts whose values are not finite, as bits; [W::kFlags]
+  unsigned long long* special = reinterpret_cast<unsigned long long*>(smem + tail + 392);
   // what the two softmax groups tell each other
   float* exchange = reinterpret_cast<float*>(smem + tail + 512);
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
     mbar_init(bar.q_full(), kSoftWarps);
     mbar_init(bar.drained(), 1);
     fence_mbar_init();
-    special[0] = special[1] = 0;
+    for (uint32_t i = 0; i < W::kFlags; ++i) special[i] = 0;
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -436,7 +442,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
         const uint32_t from = raws + raw * W::kRaw, to = ops + slot * W::kOperand;
         if (kv && drafts_at < static_cast<int>(TW)) {
           const unsigned long long odd = decoder.template run<true>(from, to, left, drafts_at);
-          if (odd) atomicOr(special + (items & 1), odd);
+          if (odd) atomicOr(special + items % W::kFlags, odd);
         } else {
           decoder.template run<false>(from, to, left, drafts_at);
         }
@@ -702,9 +708,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       const uint32_t o_other = lanes + W::kO + (1 - last_half) * D;
       const float f_last = W::kOwnO ? (last_half == half ? mine : theirs) : 1.f;
       const float f_other = last_half == half ? theirs : mine;
-      // every tile's values were decoded before their product: the flags are complete, and the next
-      // item's go to the other word
-      const unsigned long long odd = *reinterpret_cast<volatile unsigned long long*>(special + (items & 1)) & bits;
+      // every tile's values were decoded before their product: the flags are complete, and the items decoded
+      // meanwhile have other words
+      const unsigned long long odd =
+          *reinterpret_cast<volatile unsigned long long*>(special + items % W::kFlags) & bits;
       const uint64_t to = (p.seq.first + token) * a.out_token + uint64_t(q_head) * a.c.dim;
       constexpr uint32_t WIDE = SPLIT ? D / 4 : D / 2;
       const uint32_t o0 = half * (D / 2), e0 = o0 + (second ? WIDE : 0);
@@ -772,7 +779,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(const __grid_cons
       tc_fence_before();  // O is read before the next item's first product writes it
       named_barrier(1, kSoftWarps * 32);
       if (threadIdx.x == 0) {
-        special[items & 1] = 0;
+        special[items % W::kFlags] = 0;
         if (at == end) leave_split(a, p, first_tile == 0, whole, total, end, p.tile - first_tile, tiles, ctas);
       }
       ++items;

@@ -207,6 +207,53 @@ def test_infinities_and_nan_in_masked_places(kernels, kind, dim, type):
         assert np.isnan(got[3][:, block]).all() and np.isfinite(got[3][:, :32]).all()
 
 
+@pytest.mark.parametrize("type", [kb.TYPE_F32, kb.TYPE_BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kind", [ref.F16, ref.Q8, ref.Q4])
+def test_infinities_and_nan_in_many_short_contexts(kernels, kind, dim, type):
+    """Four short contexts, each seen by twenty sequences (the same pages), so that a CTA has several items of
+    one or two tiles: every row that sees a draft whose value is infinite or NaN says so, and no other."""
+    prefixes, drafts = [20, 70, 20, 70], [5, 25, 25, 9]
+    c = Case(kind, 16, 8, dim, 16, prefixes, drafts, type=type, seed=17)
+    heads, rng = c.q.shape[1], np.random.default_rng(18)
+    for s, t in enumerate(drafts):
+        nan, inf = (int(p) for p in rng.permutation(t)[:2])
+        for draft, odd, e in ((nan, np.nan, 3), (inf, np.inf, 41), (inf, -np.inf, dim - 1)):
+            p = prefixes[s] + draft
+            vv = c.values[s][p].astype(np.float32)
+            vv[:, e] = odd
+            c.layout.put(c.v, c.slot(s, p), vv)
+            c.values[s][p] = c.layout.get(c.v, c.slot(s, p))
+    with np.errstate(invalid="ignore"):
+        rows = np.cumsum([0] + drafts)
+        each = [ref.tree_attention(c.q[rows[s]: rows[s + 1]].double().cpu().numpy(), c.keys[s], c.values[s],
+                                   prefixes[s], c.masks[s], dim ** -0.5) for s in range(4)]
+    many = [s for s in range(4) for _ in range(20)]
+    c.table = c.table[many]
+    c.q = torch.cat([c.q[rows[s]: rows[s + 1]] for s in many])
+    c.prefixes, c.drafts, c.masks = [prefixes[s] for s in many], [drafts[s] for s in many], [c.masks[s] for s in many]
+    d = c.desc(kernels)
+    first = None
+    for _ in range(40):
+        c.out.fill_(5.0)
+        kernels.attention_tree(d)
+        got = c.out.clone()
+        first = got if first is None else first
+        assert torch.equal(got.nan_to_num(nan=1e4), first.nan_to_num(nan=1e4))
+    kernels.device_error()
+    got, at = first.double().cpu().numpy(), 0
+    for s in many:
+        want, weight, reach = each[s]
+        mine = got[at: at + drafts[s]]
+        at += drafts[s]
+        fine = np.isfinite(want)
+        assert np.array_equal(np.where(fine, 0.0, want), np.where(fine, 0.0, mine), equal_nan=True)
+        bound = 2.0 ** -12 * (1 + 2.0 ** -5 * reach[..., None]) * weight + (
+            0 if type == kb.TYPE_F32 else 2.0 ** -10 * weight + STEP[type] * 1.02 * np.abs(want))
+        assert (np.abs(mine[fine] - want[fine]) <= bound[fine] + 1e-30).all()
+    assert at == len(got) and not np.isfinite(got).all()
+
+
 def test_extreme_magnitudes(kernels):
     """q of 1e-30 and 1e30 (logits near zero, or one position taking all), rows of zeros, values of very
     different sizes, and keys that give large logits."""
