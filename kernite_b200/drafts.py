@@ -18,6 +18,7 @@ kernite has no decode stack; the layers are those of kernite_b200.stack, with th
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 from .stack import CudaBackend, StackConfig, plan
@@ -50,7 +51,9 @@ def accepted(tokens, parents, root: int, choices) -> tuple[list[int], int]:
 
 class DraftStack:
     """One sequence's stack and caches on one GPU. ``cache``: CACHE_F16, CACHE_Q8 or CACHE_Q4;
-    ``cfg.max_pos`` positions fit, drafts among them."""
+    ``cfg.max_pos`` positions fit, drafts among them. The work of a call goes to ``stream`` (None: torch's
+    current one at the call), after what the caller's current stream was given before the call, and what
+    it is given afterwards waits for it."""
 
     def __init__(self, cfg: StackConfig, kernels, *, cache: int | None = None, page_size: int = 64,
                  max_drafts: int = MAX_DRAFTS, stream=None):
@@ -64,10 +67,11 @@ class DraftStack:
             raise ValueError("attention needs whole heads and whole query groups")
         self.kb, self.torch, self.cfg, self.k, self.stream = kb, torch, cfg, kernels, stream
         self.max_drafts, self.page, self.kept, self.drafts = max_drafts, page_size, 0, 0
-        backend = CudaBackend(kernels, stream=stream)
+        self.done = torch.cuda.Event()  # the last call's work
         self.shards = plan(cfg, 0, 1)
         load = lambda name, layer: backend.weights(self.shards[name], cfg.seed, cfg.tensor_id(layer, name))
-        with torch.cuda.stream(stream):
+        with self._ordered() as now:
+            backend = CudaBackend(kernels, stream=now)
             self.weights = [{n: load(n, layer) for n in ("qkv", "o", "gate_up", "down")} for layer in range(cfg.layers)]
             self.head = load("head", cfg.layers)
             t, h = max_drafts, cfg.hidden
@@ -89,6 +93,24 @@ class DraftStack:
             self.workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
         self.descs = {}
 
+    @contextlib.contextmanager
+    def _ordered(self):
+        """The stream that a call's work goes to, made torch's current one. It waits for the call before (whose
+        stream may have been another) and for the caller's stream, which then waits for it."""
+        cuda = self.torch.cuda
+        caller = cuda.current_stream()
+        stream = caller if self.stream is None else self.stream
+        stream.wait_event(self.done)
+        if stream != caller:
+            stream.wait_stream(caller)
+        try:
+            with cuda.stream(stream):
+                yield stream
+        finally:
+            self.done.record(stream)
+            if stream != caller:
+                caller.wait_event(self.done)
+
     def _tree(self, cache, drafts: int, workspace, nbytes: int):
         return self.kb.tree_desc(cache, self.att, self.q, self.cfg.n_heads, self.starts, self.prefix, self.pages,
                                  self.n_pages, 1, drafts, drafts, self.cfg.max_pos, mask=self.masks,
@@ -108,7 +130,8 @@ class DraftStack:
 
     def check(self, x, parents):
         """Logits [T, vocab] after each of T drafts, whose input vectors are x [T, hidden] (f32, on the
-        GPU). The drafts' rows are in the caches until the next call; keep() makes them the context's."""
+        GPU). The drafts' rows are in the caches, and the logits in their buffer, until the next call; keep()
+        makes the rows the context's."""
         cfg, kb, k, n = self.cfg, self.kb, self.k, len(parents)
         if not 1 <= n <= self.max_drafts:
             raise ValueError(f"1..{self.max_drafts} drafts a step")
@@ -117,7 +140,7 @@ class DraftStack:
         if self.kept + n > cfg.max_pos:
             raise ValueError(f"the caches hold {cfg.max_pos} positions")
         words, depths = tree_words(parents)
-        with self.torch.cuda.stream(self.stream):
+        with self._ordered() as stream:
             self.x[:n].copy_(x)
             self._put(self.positions, [self.kept + d for d in depths])
             self._put(self.slots, [self.kept + i for i in range(n)])
@@ -126,24 +149,25 @@ class DraftStack:
             self._put(self.prefix, [self.kept])
             at = self.x
             for layer, (w, (write, attend)) in enumerate(zip(self.weights, self._step_descs(n))):
-                self._matvec(w, "qkv", self.qkv, at, n, rmsnorm=layer > 0)
-                k.cache_write(write, stream=self.stream)
-                k.attention_tree(attend, stream=self.stream)
-                self._matvec(w, "o", self.o, self.att, n)
-                self._matvec(w, "gate_up", self.a, self.o, n, pair_scale=1.0 / math.sqrt(cfg.ffn))
-                self._matvec(w, "down", self.xd, self.a, n)
+                self._matvec(stream, w, "qkv", self.qkv, at, n, rmsnorm=layer > 0)
+                k.cache_write(write, stream=stream)
+                k.attention_tree(attend, stream=stream)
+                self._matvec(stream, w, "o", self.o, self.att, n)
+                self._matvec(stream, w, "gate_up", self.a, self.o, n, pair_scale=1.0 / math.sqrt(cfg.ffn))
+                self._matvec(stream, w, "down", self.xd, self.a, n)
                 at = self.xd
-            self._matvec({"head": self.head}, "head", self.logits, at, n, rmsnorm=True)
+            self._matvec(stream, {"head": self.head}, "head", self.logits, at, n, rmsnorm=True)
         self.drafts = n
         return self.logits[:n]
 
-    def _matvec(self, weights, name: str, y, x, batch: int, rmsnorm: bool = False, pair_scale: float | None = None):
+    def _matvec(self, stream, weights, name: str, y, x, batch: int, rmsnorm: bool = False,
+                pair_scale: float | None = None):
         kb, s = self.kb, self.shards[name]
         self.k.matvec(s.qtype, y, weights[name], x, s.rows, s.k, batch,
                       prologue=kb.PROLOGUE_RMSNORM if rmsnorm else kb.PROLOGUE_NONE, eps=self.cfg.eps,
                       epilogue=kb.EPILOGUE_NONE if pair_scale is None else kb.EPILOGUE_PAIR_PRODUCT,
                       pair_scale=1.0 if pair_scale is None else pair_scale, flags=kb.FLAG_WEIGHTS_STATIC,
-                      stream=self.stream)
+                      stream=stream)
 
     def keep(self, path) -> None:
         """The last step's drafts ``path`` (in order, each after its parent) become the context's end."""
@@ -151,12 +175,12 @@ class DraftStack:
             raise ValueError("path must be drafts of the last step, in order")
         moves = [(self.kept + i, self.kept + j) for j, i in enumerate(path) if i != j]
         if moves:
-            with self.torch.cuda.stream(self.stream):
+            with self._ordered() as stream:
                 self._put(self.src, [a for a, _ in moves])
                 self._put(self.dst, [b for _, b in moves])
                 self._put(self.starts, [0, len(moves)])
                 for c in self.caches:
                     self.k.cache_move(self.kb.cache_move_desc(c, self.src, self.dst, self.starts, 1, len(moves)),
-                                      stream=self.stream)
+                                      stream=stream)
         self.kept += len(path)
         self.drafts = 0

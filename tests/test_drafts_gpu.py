@@ -115,6 +115,40 @@ def test_greedy_decoding_with_drafts_equals_one_token_at_a_time(kernels, table, 
     assert steps < 20  # some drafts were kept
 
 
+@pytest.mark.parametrize("own", [False, True], ids=["the caller's stream", "its own"])
+@pytest.mark.parametrize("side", [False, True], ids=["default", "side"])
+def test_calls_are_ordered_with_the_callers_stream(kernels, table, own, side):
+    """x made late on the caller's stream and overwritten right after the call, logits read there at once,
+    calls from changing streams: the bits of a run that waits for the GPU after every call."""
+    steps = [([3, 900, 17, 44], [-1, 0, 1, 2], [0, 1, 2, 3]), ([5, 6, 7, 8, 9], [-1, -1, 0, 1, 3], [1, 3, 4]),
+             ([11, 12], [-1, 0], [0, 1]), ([1, 2, 3], [-1, -1, 1], [1, 2])]
+    xs = [vectors(table, tokens) for tokens, _, _ in steps]
+    waits = DraftStack(CFG, kernels, page_size=16)
+    want = []
+    for x, (_, parents, path) in zip(xs, steps):
+        want.append(waits.check(x, parents).clone())
+        waits.keep(path)
+        torch.cuda.synchronize()
+    callers = [torch.cuda.Stream() if side else torch.cuda.default_stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(callers[0]):
+        stack = DraftStack(CFG, kernels, page_size=16, stream=torch.cuda.Stream() if own else None)
+    got = []
+    for i, (x, (_, parents, path)) in enumerate(zip(xs, steps)):
+        with torch.cuda.stream(callers[i % 2]):
+            late = torch.zeros_like(x)
+            torch.cuda._sleep(20_000_000)  # some 10 ms
+            late.copy_(x)
+            out = stack.check(late, parents)
+            late.fill_(float("nan"))
+            got.append(out.clone())
+            stack.keep(path)
+    torch.cuda.synchronize()
+    kernels.device_error()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 def test_refusals(kernels):
     for bad in (dict(max_drafts=0), dict(max_drafts=9)):
         with pytest.raises(ValueError):
