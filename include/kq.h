@@ -345,7 +345,8 @@ uint64_t kq_cache_bytes(const kq_cache* cache);
  * rotated and its value heads. Slot = page * page_size + position in the page; a negative slot writes
  * nothing (q_out is still written). No two tokens may have the same slot. Heads of a token are dense
  * (head_dim apart); token strides in elements, 0 = (n_heads + 2 n_kv) * head_dim for q, k, v (one
- * q|k|v row) and n_heads * head_dim for q_out. q, k, v, q_out have one type; q_out may be q. q == 0:
+ * q|k|v row) and n_heads * head_dim for q_out, or q's own where q_out is q: that rotates in place, and
+ * wants equal strides; other overlaps are not allowed. q, k, v, q_out have one type. q == 0:
  * no queries; rope == NULL: no rotation (positions unused). The rotation is rounded once, to f32,
  * before a key is quantised. */
 typedef struct kq_cache_write_desc {

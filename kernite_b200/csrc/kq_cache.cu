@@ -792,7 +792,11 @@ int cache_write(kq_ctx* ctx, const kq_cache_write_desc& d, cudaStream_t s) {
   a.q_token = d.q_token ? d.q_token : packed;
   a.k_token = d.k_token ? d.k_token : packed;
   a.v_token = d.v_token ? d.v_token : packed;
-  a.out_token = d.q_out_token ? d.q_out_token : uint64_t(d.n_heads) * dim;
+  // in place by default where q_out is q: rows of another stride would be written over tokens not yet read
+  const bool in_place = d.q && d.q_out == d.q;
+  a.out_token = d.q_out_token ? d.q_out_token : in_place ? a.q_token : uint64_t(d.n_heads) * dim;
+  if (in_place && d.tokens > 1 && a.out_token != a.q_token)
+    return fail(KQ_E_INVALID, call, "q_out may be q with q's own token stride only");
   a.nq = d.q ? d.n_heads : 0;
   a.dim = d.cache->head_dim;
   a.err = ctx->err;

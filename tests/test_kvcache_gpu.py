@@ -182,6 +182,40 @@ def test_cache_write(kernels, type, kind, heads, n_kv, dim, rot, halves, page, t
     assert np.array_equal(k, k2)  # nothing else changed
 
 
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("type", [kb.TYPE_F32, kb.TYPE_BF16])
+@pytest.mark.parametrize("dim,rot,pad", [(128, 128, 0), (128, 64, 1), (96, 48, 0), (64, 20, 0), (160, 160, 3)])
+def test_queries_in_place(kernels, dim, rot, pad, type, halves):
+    """q_out is q, many tokens, the strides' defaults (or q's own, padded): the bits that a separate q_out gets,
+    the cache's too, and k and v as they were. Another stride is refused."""
+    tokens, heads, n_kv = 203, 6, 2
+    layout = ref.Layout(ref.Q8, n_kv, dim, 32, 8)
+    wide = (heads + 2 * n_kv) * dim + pad
+    qkv, _ = _act(np.random.default_rng(dim), type, tokens, wide)
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda") * 37
+    slots = torch.arange(tokens, device="cuda")
+    rope = kb.Rope(rot, kb.ROPE_HALVES if halves else kb.ROPE_PAIRS)
+    _, _, kd, vd, cache = _cache(layout)
+    apart = torch.empty(tokens, heads * dim, device="cuda", dtype=TORCH[type])
+    more = dict(type=type, token_stride=wide if pad else 0)
+    kernels.cache_write(kb.cache_write_desc(cache, rope, qkv, apart, pos, slots, tokens, heads, **more))
+    k, v, before = kd.clone(), vd.clone(), qkv.clone()
+    for stride in (0, wide):
+        _, _, kd, vd, cache = _cache(layout)
+        qkv.copy_(before)
+        kernels.cache_write(kb.cache_write_desc(cache, rope, qkv, qkv, pos, slots, tokens, heads, q_out_token=stride,
+                                                **more))
+        assert torch.equal(qkv[:, : heads * dim], apart)
+        assert torch.equal(qkv[:, heads * dim:], before[:, heads * dim:])
+        assert torch.equal(kd, k) and torch.equal(vd, v)
+    for stride in (heads * dim, wide + 8):
+        with pytest.raises(kb.Error) as e:
+            kernels.cache_write(kb.cache_write_desc(cache, rope, qkv, qkv, pos, slots, tokens, heads, q_out_token=stride,
+                                                    **more))
+        assert e.value.code == kb.KQ_E_INVALID
+    kernels.device_error()
+
+
 @pytest.mark.parametrize("kind", [ref.Q8, ref.Q4])
 def test_quantised_blocks_at_the_edges(kernels, kind):
     """Bytes of blocks of zeros, tiny, huge, infinite and NaN values, of exact ties and of magnitudes on
