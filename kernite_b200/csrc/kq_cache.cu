@@ -754,6 +754,8 @@ int rope_apply(kq_ctx* ctx, const kq_rope_desc& d, cudaStream_t s) {
   a.q_token = d.x_token ? d.x_token : uint64_t(d.heads) * d.head_dim;
   a.out_head = d.y_head ? d.y_head : d.head_dim;
   a.out_token = d.y_token ? d.y_token : uint64_t(d.heads) * d.head_dim;
+  if (d.y == d.x && ((d.tokens > 1 && a.out_token != a.q_token) || (d.heads > 1 && a.out_head != a.q_head)))
+    return fail(KQ_E_INVALID, call, "y may be x with the same strides only");
   a.nq = d.heads;
   a.dim = d.head_dim;
   a.err = ctx->err;

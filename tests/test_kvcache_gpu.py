@@ -216,6 +216,18 @@ def test_queries_in_place(kernels, dim, rot, pad, type, halves):
     kernels.device_error()
 
 
+def test_rope_in_place_with_unlike_strides_is_refused(kernels):
+    t = torch.zeros(1 << 10, device="cuda")
+    p = torch.zeros(2, dtype=torch.int32, device="cuda")
+    args = (kb.Rope(64), t, t, p, 2, 2, 64)
+    for strides in (dict(x_token=256), dict(y_token=192), dict(x_head=128, x_token=256, y_token=256)):
+        with pytest.raises(kb.Error) as e:
+            kernels.rope(kb.rope_desc(*args, **strides))
+        assert e.value.code == kb.KQ_E_INVALID
+    kernels.rope(kb.rope_desc(kb.Rope(64), t, t, p, 1, 2, 64, x_token=256))  # of one token they do not matter
+    kernels.device_error()
+
+
 @pytest.mark.parametrize("kind", [ref.Q8, ref.Q4])
 def test_quantised_blocks_at_the_edges(kernels, kind):
     """Bytes of blocks of zeros, tiny, huge, infinite and NaN values, of exact ties and of magnitudes on
