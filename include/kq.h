@@ -411,7 +411,8 @@ typedef struct kq_tree_desc {
 } kq_tree_desc;
 int kq_attention_tree(kq_ctx* ctx, const kq_tree_desc* desc, kq_stream stream);
 /* The workspace a call with this descriptor needs (its addresses are not looked at; 0 when it is
- * not a valid one). It does not grow with the contexts' lengths. */
+ * not a valid one). It depends on the cache's shape, type, n_heads and max_drafts alone: one made for
+ * the most drafts serves contexts of any length, any number of sequences, and fewer drafts. */
 uint64_t kq_tree_workspace(kq_ctx* ctx, const kq_tree_desc* desc);
 
 /* ---- Row-sharded stacks: a matvec whose epilogue also pushes its outputs to other GPUs ----

@@ -37,6 +37,7 @@ struct Plan {
   bool many;       // few rows of many parts each: join_kernel's SHARED
   uint64_t parts;  // workspace: bytes of the parts, and all
   uint64_t bytes;
+  uint64_t most;   // all, whatever max_len and n_seq are
 };
 
 // What does not depend on addresses: shapes, and the launch they give. KQ_OK or KQ_E_INVALID.
@@ -69,11 +70,13 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   const uint64_t most = ((uint64_t(d.max_pages) << c.page_log2) + p.tile - 1) / p.tile;
   if (most * c.n_kv * row_tiles > 0xffffffffu)
     return fail(KQ_E_INVALID, call, "too many positions, heads and drafts in one sequence");
-  p.ctas = static_cast<uint32_t>(std::min<uint64_t>(
-      uint64_t(ctx->sm_count) * (p.wide ? 1 : tree::narrow_ctas(c.kind, c.pitch)), std::max<uint64_t>(1, items * tiles)));
+  const uint64_t full = uint64_t(ctx->sm_count) * (p.wide ? 1 : tree::narrow_ctas(c.kind, c.pitch));
+  p.ctas = static_cast<uint32_t>(std::min<uint64_t>(full, std::max<uint64_t>(1, items * tiles)));
   p.many = !p.wide && p.ctas > 8 * items;  // more parts than a warp loads at once
-  p.parts = uint64_t(p.ctas) * 2 * tree::part_floats(p.rows, c.pitch) * 4;
-  p.bytes = p.parts + uint64_t(p.ctas) * 2 * sizeof(uint4);
+  const uint64_t part = 2 * tree::part_floats(p.rows, c.pitch) * 4;  // a CTA's
+  p.parts = p.ctas * part;
+  p.bytes = p.ctas * (part + 2 * sizeof(uint4));
+  p.most = full * (part + 2 * sizeof(uint4));
   *out = p;
   return KQ_OK;
 }
@@ -105,7 +108,7 @@ uint64_t tree_workspace_bytes(kq_ctx* ctx, const kq_tree_desc& d) {
     fail(KQ_E_INVALID, call, "not a valid cache");
     return 0;
   }
-  return plan(ctx, d, c, call, &p) == KQ_OK ? p.bytes : 0;
+  return plan(ctx, d, c, call, &p) == KQ_OK ? p.most : 0;
 }
 
 int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {

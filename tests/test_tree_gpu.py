@@ -376,6 +376,26 @@ def test_bad_lengths_and_pages_are_recorded_not_followed(kernels):
     c.check(c.run(kernels))  # the next call is fine
 
 
+@pytest.mark.parametrize("drafts", [1, 9])
+def test_a_workspace_serves_any_length(kernels, drafts):
+    """Its size does not depend on max_len, n_seq or tokens, and one for many drafts is enough for one."""
+    c = Case(ref.Q8, 8, 1, 64, 16, [700, 5], [drafts, 1], seed=5)
+    d = c.desc(kernels, max_len=1)
+    for fields in (dict(max_len=1 << 20), dict(n_seq=1), dict(n_seq=1 << 16), dict(tokens=1 << 16), dict(max_len=702)):
+        for name, value in fields.items():
+            was = getattr(d, name)
+            setattr(d, name, value)
+            assert kernels.tree_workspace(d) == d.workspace_bytes
+            setattr(d, name, was)
+    d.max_len = 709
+    kernels.attention_tree(d)
+    kernels.device_error()
+    c.check(c.out.double().cpu().numpy())
+    for n in range(1, drafts):
+        d.max_drafts = n
+        assert kernels.tree_workspace(d) <= d.workspace_bytes
+
+
 def test_refusals(kernels):
     c = Case(ref.Q8, 4, 2, 64, 16, [40], [2], seed=3)
     good = c.desc(kernels)
