@@ -695,13 +695,15 @@ int rope_init(const kq_rope_params* p, kq_rope* out) {
   if (p->ext_factor > 0.0 && (p->orig_ctx == 0 || !(p->beta_fast > 0.0) || !(p->beta_slow > 0.0) ||
                               !std::isfinite(p->beta_fast) || !std::isfinite(p->beta_slow)))
     return fail(KQ_E_INVALID, call, "ext_factor needs orig_ctx, beta_fast and beta_slow");
-  constexpr double kTwoPi = 6.283185307179586476925;
+  // The turns in 64-bit significands (long double of x86-64, more elsewhere): a position multiplies their error.
+  using Long = long double;
+  constexpr Long kTwoPi = 6.283185307179586476925286766559L;
   const double rot = p->rot_dim;
   double low = 0, high = 0;
   if (p->ext_factor > 0.0) {
     // the pair that turns beta times in orig_ctx positions
     const auto pair = [&](double beta) {
-      return rot * std::log(p->orig_ctx / (beta * kTwoPi)) / (2 * std::log(p->base));
+      return rot * std::log(p->orig_ctx / (beta * static_cast<double>(kTwoPi))) / (2 * std::log(p->base));
     };
     low = std::max(0.0, std::floor(pair(p->beta_fast)));
     high = std::min(rot - 1, std::ceil(pair(p->beta_slow)));
@@ -712,22 +714,22 @@ int rope_init(const kq_rope_params* p, kq_rope* out) {
   r.gain = static_cast<float>(p->attn_factor *
                               (p->ext_factor > 0.0 ? 1.0 + 0.1 * std::log(1.0 / p->freq_scale) : 1.0));
   for (uint32_t i = 0; i < p->rot_dim / 2; ++i) {
-    double f = std::pow(p->base, -2.0 * i / rot);
+    Long f = std::pow(static_cast<Long>(p->base), static_cast<Long>(-2.0 * i) / p->rot_dim);
     if (p->freq_factors) {
       if (!(p->freq_factors[i] > 0.f) || !std::isfinite(p->freq_factors[i]))
         return fail(KQ_E_INVALID, call, "freq_factors must be above 0");
       f /= p->freq_factors[i];
     }
-    double slow = p->freq_scale;
+    Long slow = p->freq_scale;
     if (p->ext_factor > 0.0) {
-      const double ramp = std::min(1.0, std::max(0.0, (i - low) / std::max(0.001, high - low)));
-      const double mix = (1.0 - ramp) * p->ext_factor;
-      slow = p->freq_scale * (1.0 - mix) + mix;
+      const Long ramp = std::min<Long>(1, std::max<Long>(0, (i - low) / std::max<Long>(0.001, high - low)));
+      const Long mix = (1 - ramp) * p->ext_factor;
+      slow = p->freq_scale * (1 - mix) + mix;
     }
-    // modulo 1, to 64 bits (2^64 itself, which rounding could give, is 0)
-    const double turns = f * slow / kTwoPi, part = turns - std::floor(turns);
-    const double scaled = std::ldexp(part, 64);
-    r.turns[i] = scaled >= 0x1p64 ? 0 : static_cast<uint64_t>(scaled);
+    // modulo 1, to the nearest 2^-64 (2^64 itself is 0)
+    const Long turns = f * slow / kTwoPi, part = turns - std::floor(turns);
+    const Long scaled = std::floor(std::ldexp(part, 64) + 0.5L);
+    r.turns[i] = scaled >= 0x1p64L ? 0 : static_cast<uint64_t>(scaled);
   }
   *out = r;
   return KQ_OK;

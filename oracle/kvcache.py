@@ -4,6 +4,7 @@ definitions in include/kq.h, one element at a time where it matters; test infras
 from __future__ import annotations
 
 import math
+from decimal import Decimal, localcontext
 
 import numpy as np
 
@@ -46,6 +47,29 @@ def rope_angles(rot: int, base: float, freq_scale: float = 1.0, ext_factor: floa
         out.append(f)
     gain = attn_factor * (1 + 0.1 * math.log(1 / freq_scale) if ext_factor else 1.0)
     return np.array(out), gain
+
+
+def rope_turns(rot: int, base: float, freq_scale: float = 1.0, ext_factor: float = 0.0, beta_fast: float = 32.0,
+               beta_slow: float = 1.0, orig_ctx: int = 0, freq_factors=None) -> list:
+    """Turns per position of each pair, to 50 digits."""
+    with localcontext() as ctx:
+        ctx.prec = 60
+        two_pi = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+        big = Decimal(base)
+        out = []
+        for i in range(rot // 2):
+            f = big ** (Decimal(-2 * i) / rot)
+            if freq_factors is not None:
+                f /= Decimal(float(np.float32(freq_factors[i])))
+            slow = Decimal(freq_scale)
+            if ext_factor:
+                edge = [rot * (orig_ctx / (two_pi * Decimal(b))).ln() / (2 * big.ln()) for b in (beta_fast, beta_slow)]
+                low, high = max(0, math.floor(edge[0])), min(rot - 1, math.ceil(edge[1]))
+                ramp = min(Decimal(1), max(Decimal(0), (i - low) / max(Decimal(0.001), Decimal(high - low))))
+                mix = (1 - ramp) * Decimal(ext_factor)
+                slow = slow * (1 - mix) + mix
+            out.append(f * slow / two_pi)
+        return out
 
 
 def rope(x, positions, rot: int, halves: bool, angles, gain: float) -> np.ndarray:

@@ -61,6 +61,21 @@ def test_rope_table(rot, kw):
         assert min(off, 1 - off) <= Fraction(1, 2 ** 48)
 
 
+@pytest.mark.parametrize("rot,kw", [(2, {}), (256, {}), (128, dict(base=500000.0)), (96, dict(base=1e8)),
+                                    (64, dict(base=10000.0, freq_scale=0.3)),
+                                    (96, dict(base=500000.0, freq_scale=0.25, ext_factor=0.7, orig_ctx=8192)),
+                                    (16, dict(freq_factors=[1, 2, 3.7, 4, 5, 6, 7, 8]))], ids=str)
+def test_rope_table_to_its_last_bits(rot, kw):
+    """The table against 50 digits: the nearest 2^-64 is 2^-65 away at most, and 64-bit significands add a few
+    2^-67 (turns are below 1/6, each of five operations errs by 2^-65 of the result), 2^-63 in all; so a position
+    of 2^31 is 2^-32 turns off at most."""
+    table = kb.Rope(rot, **kw).c
+    for i, want in enumerate(ref.rope_turns(rot, kw.get("base", 10000.0),
+                                            **{k: v for k, v in kw.items() if k != "base"})):
+        off = abs(Fraction(table.turns[i], 2 ** 64) - Fraction(want) % 1)
+        assert min(off, 1 - off) <= Fraction(1, 2 ** 63), i
+
+
 @pytest.mark.parametrize("rot,kw", [(0, {}), (3, {}), (258, {}), (64, dict(layout=7)), (64, dict(base=1.0)),
                                     (64, dict(base=float("nan"))), (64, dict(freq_scale=0.0)),
                                     (64, dict(freq_scale=float("inf"))), (64, dict(ext_factor=1.0)),

@@ -9,6 +9,8 @@ covers them. Narrowing to f16 or bf16 adds half a step of the result (2^-11, 2^-
 for rotated keys, which differ by the above, a code may move by one where the quotient is that near a
 tie, and a scale by one step where the largest magnitude is that near a scale's bound, so a key is held
 to one scale step plus the rotation's error."""
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
@@ -214,6 +216,25 @@ def test_queries_in_place(kernels, dim, rot, pad, type, halves):
                                                     **more))
         assert e.value.code == kb.KQ_E_INVALID
     kernels.device_error()
+
+
+@pytest.mark.parametrize("base", [10000.0, 500000.0])
+@pytest.mark.parametrize("halves", [False, True])
+def test_rope_at_the_last_positions(kernels, halves, base):
+    """Positions up to 2^31, against turns of 50 digits: the same tolerance as at small ones (the table's error
+    times the position is 2^-32 turns)."""
+    rot, heads = 128, 3
+    pos = [2 ** 31 - 1, -2 ** 31, 2 ** 30 + 7, 10 ** 9, 123456789, -(10 ** 8 + 1)]
+    x, xv = _act(np.random.default_rng(6), kb.TYPE_F32, len(pos), heads, rot)
+    turns = [Fraction(t) for t in ref.rope_turns(rot, base)]
+    y = torch.empty_like(x)
+    rope = kb.Rope(rot, kb.ROPE_HALVES if halves else kb.ROPE_PAIRS, base)
+    kernels.rope(kb.rope_desc(rope, y, x, torch.tensor(pos, dtype=torch.int32, device="cuda"), len(pos), heads, rot))
+    got = y.double().cpu().numpy()
+    for i, p in enumerate(pos):
+        angles = np.array([float(p * t % 1) * 2 * np.pi for t in turns])
+        want = ref.rope(xv[i: i + 1], [1], rot, halves, angles, 1.0)
+        assert (np.abs(got[i] - want[0]) <= _rope_bound(xv[i], rot, halves, 1.0, want[0], kb.TYPE_F32)).all()
 
 
 def test_rope_in_place_with_unlike_strides_is_refused(kernels):
