@@ -66,7 +66,7 @@ class DraftStack:
         if cfg.hidden % cfg.head_dim or cfg.kv % cfg.head_dim or cfg.n_heads % cfg.n_kv:
             raise ValueError("attention needs whole heads and whole query groups")
         self.kb, self.torch, self.cfg, self.k, self.stream = kb, torch, cfg, kernels, stream
-        self.max_drafts, self.page, self.kept, self.drafts = max_drafts, page_size, 0, 0
+        self.max_drafts, self.page, self.kept, self.parents = max_drafts, page_size, 0, ()
         self.done = torch.cuda.Event()  # the last call's work
         self.shards = plan(cfg, 0, 1)
         load = lambda name, layer: backend.weights(self.shards[name], cfg.seed, cfg.tensor_id(layer, name))
@@ -140,6 +140,7 @@ class DraftStack:
         if self.kept + n > cfg.max_pos:
             raise ValueError(f"the caches hold {cfg.max_pos} positions")
         words, depths = tree_words(parents)
+        self.parents = ()  # nothing to keep until this step is whole
         with self._ordered() as stream:
             self.x[:n].copy_(x)
             self._put(self.positions, [self.kept + d for d in depths])
@@ -157,7 +158,7 @@ class DraftStack:
                 self._matvec(stream, w, "down", self.xd, self.a, n)
                 at = self.xd
             self._matvec(stream, {"head": self.head}, "head", self.logits, at, n, rmsnorm=True)
-        self.drafts = n
+        self.parents = tuple(parents)
         return self.logits[:n]
 
     def _matvec(self, stream, weights, name: str, y, x, batch: int, rmsnorm: bool = False,
@@ -170,9 +171,13 @@ class DraftStack:
                       stream=stream)
 
     def keep(self, path) -> None:
-        """The last step's drafts ``path`` (in order, each after its parent) become the context's end."""
-        if any(not 0 <= i < self.drafts for i in path) or any(b <= a for a, b in zip(path, path[1:])):
-            raise ValueError("path must be drafts of the last step, in order")
+        """The last step's drafts ``path`` (from one that continues the context on, each the child of the one
+        before) become the context's end."""
+        path, at = list(path), -1
+        for i in path:
+            if not 0 <= i < len(self.parents) or self.parents[i] != at:
+                raise ValueError("path must go down the last step's tree, from a draft that continues the context")
+            at = i
         moves = [(self.kept + i, self.kept + j) for j, i in enumerate(path) if i != j]
         if moves:
             with self._ordered() as stream:
@@ -183,4 +188,4 @@ class DraftStack:
                     self.k.cache_move(self.kb.cache_move_desc(c, self.src, self.dst, self.starts, 1, len(moves)),
                                       stream=stream)
         self.kept += len(path)
-        self.drafts = 0
+        self.parents = ()

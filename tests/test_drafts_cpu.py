@@ -1,7 +1,7 @@
 """Trees of drafts on the host: masks, depths, which drafts are kept."""
 import pytest
 
-from kernite_b200.drafts import accepted, tree_words
+from kernite_b200.drafts import DraftStack, accepted, tree_words
 
 
 def test_tree_words():
@@ -11,6 +11,20 @@ def test_tree_words():
     for bad in ([0], [-1, 1], [-2], [-1, 2, 0]):
         with pytest.raises(ValueError):
             tree_words(bad)
+
+
+@pytest.mark.parametrize("path", [[0, 1], [1], [0, 3], [2, 4], [0, 2, 3], [0, 0], [-1], [0, 9], [4]], ids=str)
+def test_only_paths_of_the_tree_are_kept(path):
+    """Drafts 0 and 3 continue the context, 1 and 2 draft 0, 4 draft 3."""
+    stack = DraftStack.__new__(DraftStack)  # what keep() looks at before it moves anything
+    stack.kept, stack.parents = 7, (-1, 0, 0, -1, 3)
+    if path == [0, 1]:
+        stack.keep(iter(path))
+        assert stack.kept == 9 and stack.parents == ()
+    else:
+        with pytest.raises(ValueError):
+            stack.keep(path)
+        assert stack.kept == 7
 
 
 def test_accepted():
