@@ -508,13 +508,15 @@ __global__ void __launch_bounds__(kThreads)
   T* to = (value ? v_out : k_out) + r0 * token_stride + h * c.dim + e;
   const uint64_t step = subs * token_stride, slots_end = uint64_t(c.n_pages) << c.page_log2;
   long long slot[ROWS];
+  // codes of a row that is not there: zeros, with the kind's offset
+  constexpr uint32_t kNone = KIND == KQ_CACHE_F16 ? 0u : KIND == KQ_CACHE_Q8 ? 0x80808080u : 0x88888888u;
   uint32_t raw[ROWS][B / 4], scale[ROWS];
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) slot[k] = r0 + k * subs < count ? slots[r0 + k * subs] : -1;
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
 #pragma unroll
-    for (int w = 0; w < B / 4; ++w) raw[k][w] = 0;
+    for (int w = 0; w < B / 4; ++w) raw[k][w] = kNone;
     scale[k] = 0;
     if (slot[k] < 0) continue;
     if (static_cast<uint64_t>(slot[k]) >= slots_end) {

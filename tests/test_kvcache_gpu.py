@@ -317,6 +317,18 @@ def test_cache_read(kernels, type, kind, n_kv, dim, page, count, stride):
     assert torch.equal(only[:, : n_kv * dim].nan_to_num(), v_out[:, : n_kv * dim].nan_to_num())
 
 
+@pytest.mark.parametrize("type", [kb.TYPE_F32, kb.TYPE_F16, kb.TYPE_BF16])
+@pytest.mark.parametrize("kind", [ref.F16, ref.Q8, ref.Q4])
+def test_rows_of_negative_slots_have_no_sign(kernels, kind, type):
+    layout = ref.Layout(kind, 2, 64, 16, 1)
+    _, _, _, _, cache = _cache(layout)
+    out = torch.full((3, 2 * 64), -1.0, device="cuda", dtype=TORCH[type])
+    slots = torch.tensor([-1, -(1 << 40), -7], device="cuda")
+    kernels.cache_read(kb.cache_read_desc(cache, out, None, slots, 3, type=type))
+    kernels.device_error()
+    assert (out == 0).all() and not torch.signbit(out).any()
+
+
 @pytest.mark.parametrize("kind,n_kv,dim,page", [(ref.Q8, 2, 128, 16), (ref.Q4, 3, 64, 32), (ref.F16, 1, 256, 16),
                                                 (ref.Q4, 1, 128, 64), (ref.Q8, 1, 96, 16)])
 def test_cache_move(kernels, kind, n_kv, dim, page):
