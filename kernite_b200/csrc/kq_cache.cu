@@ -820,6 +820,7 @@ int cache_read(kq_ctx* ctx, const kq_cache_read_desc& d, cudaStream_t s) {
   if (!size) return fail(KQ_E_INVALID, call, "type must be F32, F16 or BF16");
   if (d.count == 0 || (!d.k_out && !d.v_out)) return KQ_OK;
   if (!d.slots) return fail(KQ_E_INVALID, call, "null slots");
+  if (d.count > 0x7fffffffu) return fail(KQ_E_INVALID, call, "too many rows");
   const uint64_t dense = uint64_t(c.n_kv) * c.dim;
   const uint64_t stride = d.token_stride ? d.token_stride : dense;
   if (stride < dense) return fail(KQ_E_INVALID, call, "token_stride must be at least n_kv * head_dim");

@@ -317,6 +317,24 @@ def test_cache_read(kernels, type, kind, n_kv, dim, page, count, stride):
     assert torch.equal(only[:, : n_kv * dim].nan_to_num(), v_out[:, : n_kv * dim].nan_to_num())
 
 
+def test_counts_past_31_bits_are_refused(kernels):
+    """Before anything is launched, by every call."""
+    t = torch.zeros(1 << 14, device="cuda")
+    i = torch.zeros(64, dtype=torch.int64, device="cuda")
+    cache, many = kb.KvCache(kb.CACHE_Q8, 1, 64, 16, 4, t, t), 1 << 31
+    calls = [lambda n: kernels.rope(kb.rope_desc(kb.Rope(64), t, t, i, n, 1, 64)),
+             lambda n: kernels.cache_write(kb.cache_write_desc(cache, None, t, None, None, i, n, 0)),
+             lambda n: kernels.cache_read(kb.cache_read_desc(cache, t, t, i, n)),
+             lambda n: kernels.cache_move(kb.cache_move_desc(cache, i, i, i, n, 1)),
+             lambda n: kernels.cache_move(kb.cache_move_desc(cache, i, i, i, 1, n))]
+    for call in calls:
+        for n in (many, many + 1, (1 << 32) - 1):
+            with pytest.raises(kb.Error) as e:
+                call(n)
+            assert e.value.code == kb.KQ_E_INVALID
+    kernels.device_error()
+
+
 @pytest.mark.parametrize("type", [kb.TYPE_F32, kb.TYPE_F16, kb.TYPE_BF16])
 @pytest.mark.parametrize("kind", [ref.F16, ref.Q8, ref.Q4])
 def test_rows_of_negative_slots_have_no_sign(kernels, kind, type):
