@@ -40,6 +40,12 @@ struct Plan {
   uint64_t most;   // all, whatever max_len and n_seq are
 };
 
+// The logits' scale in log2 units.
+float scale_log2(const kq_tree_desc& d, const CacheView& c) {
+  const double scale = d.scale > 0.f ? static_cast<double>(d.scale) : 1.0 / std::sqrt(static_cast<double>(c.dim));
+  return static_cast<float>(scale * 1.4426950408889634);
+}
+
 // What does not depend on addresses: shapes, and the launch they give. KQ_OK or KQ_E_INVALID.
 int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const char* call, Plan* out) {
   if (d.type != KQ_TYPE_F32 && d.type != KQ_TYPE_F16 && d.type != KQ_TYPE_BF16)
@@ -52,7 +58,9 @@ int plan(const kq_ctx* ctx, const kq_tree_desc& d, const CacheView& c, const cha
   if ((uint64_t(d.max_pages) << c.page_log2) > 0x7fffffffu)
     return fail(KQ_E_INVALID, call, "max_pages pages must hold fewer than 2^31 positions");
   if (d.n_seq > 0x7fffffffu || d.tokens > 0x7fffffffu) return fail(KQ_E_INVALID, call, "too many sequences or tokens");
-  if (!std::isfinite(d.scale) || d.scale < 0.f) return fail(KQ_E_INVALID, call, "scale must be finite and not negative");
+  // (in log2 units it has to be an f32 too)
+  if (!(d.scale >= 0.f) || !std::isfinite(scale_log2(d, c)))
+    return fail(KQ_E_INVALID, call, "scale must be 0 to 2^127 and not NaN");
   Plan p = {};
   p.split = d.type == KQ_TYPE_F32;
   const uint32_t group = d.n_heads / c.n_kv;
@@ -143,9 +151,7 @@ int attention_tree(kq_ctx* ctx, const kq_tree_desc& d, cudaStream_t s) {
   a.mask = reinterpret_cast<const unsigned long long*>(d.mask);
   a.part = reinterpret_cast<float*>(d.workspace);
   a.splits = reinterpret_cast<uint4*>(d.workspace + p.parts);
-  a.scale_log2 = static_cast<float>((d.scale > 0.f ? static_cast<double>(d.scale)
-                                                   : 1.0 / std::sqrt(static_cast<double>(a.c.dim))) *
-                                    1.4426950408889634);
+  a.scale_log2 = scale_log2(d, a.c);
   a.n_seq = d.n_seq;
   a.n_heads = d.n_heads;
   a.group = d.n_heads / a.c.n_kv;

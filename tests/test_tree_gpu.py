@@ -396,6 +396,17 @@ def test_a_workspace_serves_any_length(kernels, drafts):
         assert kernels.tree_workspace(d) <= d.workspace_bytes
 
 
+def test_scales_past_the_range_are_refused(kernels):
+    """Up to 2^127 they are taken: queries of zeros then still give the mean of the values."""
+    c = Case(ref.Q8, 4, 2, 64, 16, [40], [1], seed=3)
+    c.q.zero_()
+    for scale in (3e38, float("inf"), float("-inf"), float("nan")):
+        with pytest.raises(kb.Error) as e:
+            kernels.attention_tree(c.desc(kernels, scale=scale, workspace=1 << 40, workspace_bytes=1 << 40))
+        assert e.value.code == kb.KQ_E_INVALID
+    c.check(c.run(kernels, scale=2.0 ** 127))
+
+
 def test_refusals(kernels):
     c = Case(ref.Q8, 4, 2, 64, 16, [40], [2], seed=3)
     good = c.desc(kernels)
