@@ -376,6 +376,111 @@ def test_bad_lengths_and_pages_are_recorded_not_followed(kernels):
     c.check(c.run(kernels))  # the next call is fine
 
 
+# ---------------------------------------------------------------- errors on the mean square
+#
+# The bounds above add up worst cases; these are for the relative error of a whole output in the mean square,
+# |got - want| / |want|, of standard normal queries, keys and values. An error of a weight relative to itself,
+# independent of the values, becomes the same relative error of the output, as both add up in squares. f32
+# activations: logits are sums of 2 dim / 16 <= 32 products of the tensor core, each cut at 2^-23 (2^-24 in the mean)
+# of a partial sum near 0.7: 1.4e-6; exp2's argument (below 16) is rounded at 2^-21: 7e-7; exp2 itself
+# 2^-22, the weights' two f16 2^-23: in all below 2^-18 (3.8e-6). The output is a sum of n / 16 products at most, each
+# cut at 2^-23 of the sum so far: n / 16 2^-23 at most. What leaving out a second f16 costs is a rounding
+# of 2^-11 at most of every weight or query element, 2^-12.3 in the mean (f16's steps are 2^-10 to 2^-11 of a number,
+# a rounding is 1 / sqrt(12) of a step): 2e-4, which the bound notices up to 20000 positions.
+# f16 activations have that rounding of the weights, and the output's, 2^-11 with both: together below 2^-11 + 2^-18.
+
+def mean_square(got, want):
+    return np.sqrt(((got - want) ** 2).sum() / (want ** 2).sum())
+
+
+def one_f16(c, which):
+    """c's first sequence in 64 bits, with the weights or the queries (or both) rounded to f16 once."""
+    q, out = c.q.double().cpu().numpy()[: c.drafts[0]], []
+    dim, group = c.args[3], c.args[1] // c.args[2]
+    for t, row in enumerate(q):
+        seen = [p for p in range(c.prefixes[0] + c.drafts[0])
+                if p < c.prefixes[0] or c.masks[0][t] >> (p - c.prefixes[0]) & 1]
+        for h, x in enumerate(row):
+            x = x.astype(np.float16).astype(np.float64) if "q" in which else x
+            z = c.keys[0][seen, h // group] @ x * dim ** -0.5
+            w = 4 * np.exp(z - z.max())
+            v = w.astype(np.float16).astype(np.float64) if "p" in which else w
+            out.append(v @ c.values[0][seen, h // group] / w.sum())
+    return np.array(out).reshape(q.shape)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kind", [ref.F16, ref.Q8, ref.Q4])
+@pytest.mark.parametrize("length,heads,drafts", [(99, 8, 1), (700, 2, 3), (260, 6, 3), (1500, 4, 11)])
+def test_f32_activations_have_more_than_16_bits(kernels, kind, dim, length, heads, drafts):
+    c = Case(kind, heads, 1, dim, 64, [length], [drafts], masks="chain", seed=41)
+    want = ref.tree_attention(c.q.double().cpu().numpy(), c.keys[0], c.values[0], length, c.masks[0], dim ** -0.5)[0]
+    bound = 2.0 ** -18 + (length + drafts) / 16 * 2.0 ** -23
+    for which in ("p", "q", "pq"):
+        assert mean_square(one_f16(c, which), want) > 2 * bound, which
+    assert mean_square(c.run(kernels), want) <= bound
+
+
+@pytest.mark.parametrize("kind", [ref.F16, ref.Q8, ref.Q4])
+@pytest.mark.parametrize("heads,drafts", [(8, 1), (4, 11)])
+def test_f16_activations_in_the_mean_square(kernels, kind, heads, drafts):
+    c = Case(kind, heads, 1, 128, 64, [900], [drafts], masks="chain", type=kb.TYPE_F16, seed=42)
+    want = ref.tree_attention(c.q.double().cpu().numpy(), c.keys[0], c.values[0], 900, c.masks[0], 128 ** -0.5)[0]
+    assert mean_square(c.run(kernels), want) <= 2.0 ** -11 + 2.0 ** -18 + 911 / 16 * 2.0 ** -23
+
+
+def copied(c, n):
+    """c's only sequence n times over the same pages, with the same queries: so many items that a CTA does
+    whole ones. The expected rows, and the reference's other results, of one."""
+    t = c.drafts[0]
+    each = ref.tree_attention(c.q.double().cpu().numpy(), c.keys[0], c.values[0], c.prefixes[0], c.masks[0],
+                              c.args[3] ** -0.5)
+    c.table, c.q = np.repeat(c.table, n, axis=0), c.q.repeat(n, 1, 1)
+    c.prefixes, c.drafts, c.masks = c.prefixes * n, [t] * n, c.masks * n
+    return each
+
+
+@pytest.mark.parametrize("heads,drafts", [(2, 3), (2, 9)])
+def test_a_long_context_by_one_cta(kernels, heads, drafts):
+    """Some 8100 positions added up by one CTA (the warp-MMA kernel's are 296), in the mean square and at the worst."""
+    c = Case(ref.Q8, heads, 1, 64, 64, [8100], [drafts], masks="chain", seed=43)
+    n = 320 if drafts == 3 else 160
+    want, weight, reach = copied(c, n)
+    got = c.run(kernels).reshape(n, drafts, heads, 64)
+    bound = 2.0 ** -18 + 8111 / 16 * 2.0 ** -23
+    assert all(mean_square(g, want) <= bound for g in got)
+    assert (np.abs(got - want) <= 2.0 ** -12 * (1 + 2.0 ** -5 * reach[..., None]) * weight).all()
+
+
+@pytest.mark.parametrize("type", [kb.TYPE_F32, kb.TYPE_BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kind", [ref.F16, ref.Q8, ref.Q4])
+@pytest.mark.parametrize("heads,drafts", [(2, 2), (3, 5)], ids=["few", "many"])
+def test_logits_that_rise_along_the_context(kernels, kind, dim, type, heads, drafts):
+    """Three stretches of a context, the logits of each some 15 log2 units above those before, and values the
+    smaller for it (2^10, 2^-5, 2^-17: the smallest a quantised cache holds), so that the first two are a tenth of the
+    output each: a maximum is replaced (the kernels rescale what they have by factors near 2^-15) twice in an
+    item, and the rescaled part shows."""
+    stretches = [(0, 212), (212, 333), (333, 700)]
+    c = Case(kind, heads, 1, dim, 32, [700], [drafts], masks="chain", type=type, seed=44)
+    c.q[..., 0] = dim ** 0.5
+    rng = np.random.default_rng(45)
+    kk, vv = (rng.standard_normal((700 + drafts, 1, dim)).astype(np.float32) for _ in range(2))
+    for i, (a, b) in enumerate(stretches):
+        b = len(kk) if i == 2 else b
+        kk[a:b, :, 0] = 15 * np.log(2) * i
+        vv[a:b] = vv[a:b] * 2.0 ** (10 - 15 * i) if i < 2 else rng.integers(-1, 2, vv[a:b].shape) * 2.0 ** -17
+    c.keys, c.values = [], []
+    c.fill(0, kk, vv)
+    n = 320 if drafts * heads <= 8 else 160
+    want, weight, reach = copied(c, n)
+    got = c.run(kernels).reshape(n, drafts, heads, dim)
+    bound = 2.0 ** -12 * (1 + 2.0 ** -5 * reach[..., None]) * weight + STEP[type] * np.abs(want) * (1 + 2.0 ** -6)
+    if type != kb.TYPE_F32:
+        bound += 2.0 ** -10 * weight
+    assert (np.abs(got - want) <= bound + 1e-30).all()
+
+
 @pytest.mark.parametrize("drafts", [1, 9])
 def test_a_workspace_serves_any_length(kernels, drafts):
     """Its size does not depend on max_len, n_seq or tokens, and one for many drafts is enough for one."""
