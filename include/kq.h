@@ -267,8 +267,10 @@ uint64_t kq_attention_workspace(kq_ctx* ctx, uint32_t n_heads, uint32_t n_kv, ui
  * kernite has no rotary embedding, no cache and no drafted tokens; the attention itself follows its
  * microgpt example (examples/microgpt/src/gpu.rs:130-230). Positions, slots and lengths are read on
  * the device (a captured graph serves every step). What the host cannot check there, the kernels
- * do: a slot, page or length out of range is skipped and recorded in the ctx's device error word
- * (kq_device_error), never followed. */
+ * do: a slot out of range is skipped, a sequence whose lengths do not fit gets no output, the positions
+ * of a page that is not there are page 0's, and each is recorded in the ctx's device error word
+ * (kq_device_error): what is out of range is never followed, and outputs of a call that recorded an
+ * error are not to be used. */
 
 /* Element types of activations (GGML's type numbers). */
 enum { KQ_TYPE_F32 = 0, KQ_TYPE_F16 = 1, KQ_TYPE_BF16 = 30 };
@@ -390,11 +392,12 @@ int kq_cache_move(kq_ctx* ctx, const kq_cache_move_desc* desc, kq_stream stream)
  * head h reads key/value head h / (n_heads / n_kv):
  *   out[t][h] = sum_p w_p v_p, w = softmax_p(q[t][h] . k_p * scale).
  * A token that sees no position gets zeros. A masked position's key and value are not looked at,
- * infinities and NaNs included. q and out: `type`, heads dense, tokens q_token / out_token elements
- * apart (0: n_heads * head_dim); q and out 16-byte aligned, strides multiples of 16 bytes; out may
- * not overlap q. scale 0: 1 / sqrt(head_dim). Products: q and the weights enter the tensor cores as
- * f16 (f32 activations: as the sum of two f16, about 22 bits), sums and softmax in f32; the order of
- * the sums depends on the lengths and the GPU alone, so equal calls give equal bits.
+ * infinities and NaNs included; an infinite value that is seen gives infinity or NaN. q and out:
+ * `type`, heads dense, tokens q_token / out_token elements apart (0: n_heads * head_dim); q and out
+ * 16-byte aligned, strides multiples of 16 bytes; out may not overlap q. scale 0: 1 / sqrt(head_dim).
+ * Products: q and the weights enter the tensor cores as f16 (f32 activations: as the sum of two f16,
+ * about 22 bits), sums and softmax in f32; the order of the sums depends on the lengths and the GPU
+ * alone, so equal calls give equal bits.
  * max_drafts, max_len: no sequence has more drafts, or prefix + drafts positions (max_len sizes the
  * launch; a longer sequence is still served). n_heads / n_kv 1..64. */
 typedef struct kq_tree_desc {

@@ -303,10 +303,12 @@ __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t
 // then meet no bank twice.
 //
 // What bounds it. Read once, 8-bit keys and values come at the memory's rate: 32 sequences of 64 / 8 heads of
-// 128, one f32 token each, take 62 us at 4096 positions and 104 us at 8192, so the second half at 6.5 TB/s; the
-// first 20 us are launches, the lengths' and pages' latencies, the items' ends and the join. In 4 bits
-// decoding two codes takes three instructions for half the bytes, and the instructions are the bound: one
-// token over 131001 positions 64 us, 2.6 TB/s. Parts of 16 positions a warp, one chain of latencies, took 69.
+// 128, one f32 token each, take 63 us at 4096 positions and 106 us at 8192, so the second half at 6.5 TB/s; the
+// first 20 us are launches, the lengths' and pages' latencies, the items' ends and the join. 16-bit ones take
+// 90 us at 4096 (85 at the copy rate). In 4 bits there are half the bytes and as many instructions: one token
+// over 131001 positions takes 64 us, 2.2 TB/s, and 57600 instructions a scheduler, 56 % of its issue slots (of
+// the integer pipe 50 %, of the tensor pipe 27 %). No pipe is full: the rest is latency, with 3.5 warps a
+// scheduler. Parts of 16 positions a warp, one chain of latencies, took 69 us.
 // Why seven readers and one copier: a warp that copies in its turn makes its tile late (77 us against 68).
 // Why one pass: a maximum that only ever grows costs a rescaling of O when it does, which kSlack makes rare.
 
@@ -411,10 +413,11 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 }
 
 // How a row of q becomes an f16 operand: times `up`; and the logits (in log2 units) of the product: times
-// `unit`. The power of two in `up` brings the row's largest magnitude (most) to [2^7, 2^8) (or, split,
-// near it), so that f16's range fits any q; it is 1 for a row of zeros or with infinities. 16-bit rows stay
-// exact; split ones take the softmax's scale along, so that `unit` is a power of two and a product's
-// largest logit is the maximum exactly, however large. unit is never zero: masked logits are -inf times it.
+// `unit`. The power of two in `up` brings the row's largest magnitude (most) to [2^7, 2^8) (or, split, near
+// it), so that f16's range fits any q; it is 1 for a row of zeros or with infinities. 16-bit rows stay exact
+// but for elements below 2^-21 of the row's largest, which are rounded at 2^-32 of it; split ones take the
+// softmax's scale along, so that `unit` is a power of two and a product's largest logit is the maximum exactly,
+// however large. unit is never zero: masked logits are -inf times it.
 struct RowScale {
   float up, unit;
 };
@@ -816,7 +819,9 @@ __device__ __forceinline__ float special_value(const TileView<Shape<KIND, D>>& t
 // Weights are kept times 2^kLift of the reference they were taken to, and outputs are rescaled to a new
 // reference only when a logit is more than 2^kSlack above it, which after an item's first tile hardly
 // happens: the largest weight is below 2^15, in f16's range, and what f16 loses of a small one (2^-25) is
-// 2^-27 of the reference's own weight at most.
+// 2^-27 of the reference's own weight at most. 16-bit activations leave it at that one f16, 2^-11 of a weight
+// at most: a second one would double the products of P V for less than their type's own rounding (4 sequences of
+// 64 bf16 drafts: relative error 1.670e-3, of f32 weights 1.657e-3).
 constexpr float kLift = 2.f;
 constexpr float kSlack = 13.f;
 

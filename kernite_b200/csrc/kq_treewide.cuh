@@ -21,11 +21,12 @@
 // maximum is passed on to the group that has the next tile.
 //
 // What bounds it. A tile of 64 positions x 128 elements takes the tensor core 520 cycles (M = 128) and the
-// special function unit 512 for its exponentials; it takes 1300, whatever number of rows is real: a softmax
-// group's way through its tile (read S, maximum, exponentials, P back) is some 2450 cycles of latencies, and
-// there is room for two groups. 4 sequences of 64 drafts x 64 / 8 heads over 6000 to 16000 positions of 8-bit
-// keys and values, bf16: 127 us, 0.73 PFLOP/s; 25 f32 drafts over 8191: 45 us. Holding all of S in
-// registers instead of reading it twice spilled (149 us), and with registers moved from the other warps was
+// special function unit 512 for its exponentials; it takes 1300 to 1390, whatever number of rows is real: a
+// softmax group's way through its tile (read S, maximum, exponentials, P back) is some 2450 cycles of
+// latencies, and there is room for two groups (tensor pipe 37 %, issue slots 56 %, 760 instructions a tile and
+// scheduler). 4 sequences of 64 drafts x 64 / 8 heads over 11000 positions each of 8-bit keys and values, bf16:
+// 128 us, 0.72 PFLOP/s, of 16-bit ones 158 us; 25 f32 drafts over 8191: 46 us. Holding all of S in registers
+// instead of reading it twice spilled (149 us against 127), and with registers moved from the other warps was
 // no faster (127). MMAs issued by lane 0 instead of an elected thread took 573 us, two S buffers 200.
 #pragma once
 
