@@ -218,6 +218,49 @@ def test_queries_in_place(kernels, dim, rot, pad, type, halves):
     kernels.device_error()
 
 
+@pytest.mark.parametrize("halves", [False, True])
+def test_rope_in_the_mean_square(kernels, halves):
+    """f32 heads. A rounding to f32 errs by 2.53e-8 of a number in the mean square (half a step of 2^-23 to 2^-24 of
+    it, uniform). A rotated pair has one in the cosine or sine (one step more is allowed for below, as sincospi is
+    not the nearest number), half of one in the one product that is rounded, one in the sum: sqrt(2.5) 2.53e-8 =
+    4.0e-8; an angle of at most an eighth of a turn adds 1e-8 (its steps are 2^-27 half turns and less, uniform),
+    4.1e-8 with it. A tenth more for sincospi: 4.5e-8. An angle of up to half a turn in f32 adds 3.9e-8: 5.6e-8."""
+    rng = np.random.default_rng(12)
+    tokens, heads, rot = 300, 8, 128
+    x, xv = _act(rng, kb.TYPE_F32, tokens, heads, rot)
+    pos = rng.integers(0, 131072, tokens).astype(np.int32)
+    turns = [Fraction(t) for t in ref.rope_turns(rot, 500000.0)]
+    y = torch.empty_like(x)
+    rope = kb.Rope(rot, kb.ROPE_HALVES if halves else kb.ROPE_PAIRS, 500000.0)
+    kernels.rope(kb.rope_desc(rope, y, x, torch.from_numpy(pos).cuda(), tokens, heads, rot))
+    got, off, all_ = y.double().cpu().numpy(), 0.0, 0.0
+    for i, p in enumerate(pos):
+        angles = np.array([float(int(p) * t % 1) * 2 * np.pi for t in turns])
+        want = ref.rope(xv[i: i + 1], [1], rot, halves, angles, 1.0)[0]
+        off += ((got[i] - want) ** 2).sum()
+        all_ += (want ** 2).sum()
+    assert np.sqrt(off / all_) <= 4.5e-8
+
+
+@pytest.mark.parametrize("halves", [False, True])
+def test_rope_of_quarter_turns(kernels, halves):
+    """Turns of whole quarters and next to them, by a table made by hand: signs and exchanged parts, exactly."""
+    rope = kb.Rope(2, kb.ROPE_HALVES if halves else kb.ROPE_PAIRS)
+    rope.c.turns[0] = 1 << 62
+    pos = [0, 1, 2, 3, 4, -1, -2, -3, 2 ** 31 - 1]
+    x = torch.tensor([[3.0, 5.0]], device="cuda").repeat(len(pos), 1)
+    y = torch.empty_like(x)
+    kernels.rope(kb.rope_desc(rope, y, x, torch.tensor(pos, dtype=torch.int32, device="cuda"), len(pos), 1, 2))
+    turned = [[3.0, 5.0], [-5.0, 3.0], [-3.0, -5.0], [5.0, -3.0]]
+    assert y.tolist() == [turned[p % 4] for p in pos]
+    for eighth in range(8):  # the edges between quarters
+        rope.c.turns[0] = (eighth << 61) + 1
+        angle = 2 * np.pi * ((eighth << 61) + 1) / 2 ** 64
+        kernels.rope(kb.rope_desc(rope, y, x, torch.ones(len(pos), dtype=torch.int32, device="cuda"), len(pos), 1, 2))
+        want = [3 * np.cos(angle) - 5 * np.sin(angle), 3 * np.sin(angle) + 5 * np.cos(angle)]
+        assert np.abs(np.array(y[0].tolist()) - want).max() <= 2.0 ** -20 * 8
+
+
 @pytest.mark.parametrize("base", [10000.0, 500000.0])
 @pytest.mark.parametrize("halves", [False, True])
 def test_rope_at_the_last_positions(kernels, halves, base):
