@@ -207,7 +207,7 @@ constexpr int kLane = 8;  // elements a lane of rope_rows_kernel has of a row
 // Heads of 64, 128 or 256 elements, every row on 16 bytes. A lane holds E consecutive elements of a row, dim /
 // E lanes a row, so that its place in a head, and with it its angles, are the same for every row it takes: they
 // stay in registers. A pair's other element is in the lane (pairs) or rot_half / E lanes away (halves). Bound
-// by memory in principle (4001 tokens of 40 16-bit heads: 12.7 us of copying, 21 taken; 6144 tokens of 32 + 32
+// by memory in principle (4001 tokens of 40 16-bit heads: 12.7 us of copying, 22 taken; 6144 tokens of 32 + 32
 // + 32 f32 heads written to 8 bits: 70 us of copying, 96 taken) and by instructions and latencies in fact: the
 // quantisation of a block, the exchange of halves. A CTA takes per_block tokens, as many warps each; with one,
 // the grid's y shares out its rows.

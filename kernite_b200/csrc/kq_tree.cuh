@@ -305,7 +305,7 @@ __device__ __forceinline__ void store_one(void* p, uint64_t i, float v, uint32_t
 // What bounds it. Read once, 8-bit keys and values come at the memory's rate: 32 sequences of 64 / 8 heads of
 // 128, one f32 token each, take 63 us at 4096 positions and 106 us at 8192, so the second half at 6.5 TB/s; the
 // first 20 us are launches, the lengths' and pages' latencies, the items' ends and the join. 16-bit ones take
-// 90 us at 4096 (85 at the copy rate). In 4 bits there are half the bytes and as many instructions: one token
+// 90 us at 4096 (85 at the copy rate). In 4 bits there are half the bytes and an eighth more instructions: one token
 // over 131001 positions takes 64 us, 2.2 TB/s, and 57600 instructions a scheduler, 56 % of its issue slots (of
 // the integer pipe 50 %, of the tensor pipe 27 %). No pipe is full: the rest is latency, with 3.5 warps a
 // scheduler. Parts of 16 positions a warp, one chain of latencies, took 69 us.
